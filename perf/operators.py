@@ -232,10 +232,11 @@ def _append(st):
     past, new = st["n_past"].long(), st["n_new"].long()
     n, width = tables.shape
     have = (past + page - 1) // page
-    need = (past + new + page - 1) // page - have
-    off = torch.cumsum(need, 0) - need
     end = torch.cumsum(new, 0)
-    ok = (off + need <= st["n_free"]) & (past + new <= width * page) & (end <= m)
+    fits = (past + new <= width * page) & (end <= m)
+    need = torch.where(fits, (past + new + page - 1) // page - have, torch.zeros_like(have))
+    off = torch.cumsum(need, 0) - need
+    ok = fits & (off + need <= st["n_free"])
     i = torch.arange(width, device="cuda")[None]
     fresh = ok[:, None] & (i >= have[:, None]) & (i < (have + need)[:, None])
     at = (st["n_free"].long() - 1 - off[:, None] - (i - have[:, None])).clamp(0, st["free"].numel() - 1)
