@@ -236,7 +236,7 @@ def _append(st):
     fits = (past + new <= width * page) & (end <= m)
     need = torch.where(fits, (past + new + page - 1) // page - have, torch.zeros_like(have))
     off = torch.cumsum(need, 0) - need
-    ok = fits & (off + need <= st["n_free"])
+    ok = fits & ((need == 0) | (off + need <= st["n_free"]))
     i = torch.arange(width, device="cuda")[None]
     fresh = ok[:, None] & (i >= have[:, None]) & (i < (have + need)[:, None])
     at = (st["n_free"].long() - 1 - off[:, None] - (i - have[:, None])).clamp(0, st["free"].numel() - 1)
