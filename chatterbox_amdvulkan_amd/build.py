@@ -28,6 +28,7 @@ SOURCES = [
     "cbx_api.cpp",
     "cbx_gguf.cpp",
     "cbx_graph.cpp",
+    "cbx_paged.cpp",
     "k_rows.hip",
     "k_norm.hip",
     "k_group_norm.hip",
@@ -41,6 +42,10 @@ SOURCES = [
     "k_batch.hip",
     "k_group.hip",
     "k_binary.hip",
+    "k_paged_plan.hip",
+    "k_qk.hip",
+    "k_paged_attn.hip",
+    "k_logprob.hip",
 ]
 HEADERS = ["cbx_internal.h", "cbx_device.h", "cbx_rowops.h", os.path.join("..", "..", "include", "cbxops.h")]
 

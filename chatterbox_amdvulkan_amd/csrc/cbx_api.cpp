@@ -193,6 +193,10 @@ struct cbx_rope_cache {
 // handle from a new one at the same address.
 static std::atomic<uint64_t> g_handle_serial{1};
 
+cbx::RopeTable cbx::rope_table(const cbx_rope_cache* c) {
+    return RopeTable{c->device, c->p, c->n_pos, c->table, c->freq_factors};
+}
+
 uint64_t cbx::rope_cache_serial(const cbx_rope_cache* c) { return c ? c->serial : 0; }
 uint64_t cbx::conv1d_weights_serial(const cbx_conv1d_weights* w) { return w ? w->serial : 0; }
 

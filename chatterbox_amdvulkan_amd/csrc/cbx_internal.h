@@ -60,6 +60,7 @@ struct DeviceState {
 enum : uint32_t {
     DEV_ERR_ROW_INDEX = 1u,   // a get_rows index was out of range (row zeroed)
     DEV_ERR_RESERVED1 = 2u,   // no longer raised (in-place GroupNorm never takes the split)
+    DEV_ERR_PAGE = 4u,        // a page number, slot or length of the paged cache was out of range (left out)
 };
 
 // ---- host helpers implemented in cbx_api.cpp ----------------------------
@@ -266,6 +267,62 @@ struct RopeParams {
 int launch_rope(const cbx_tensor* x, const cbx_tensor* pos, const RopeParams& p,
                 const float2* table, int32_t n_pos, const float* freq_factors_dev,
                 cbx_tensor* y, DeviceState* st, hipStream_t s);
+// What a rope cache holds, for entry points outside cbx_api.cpp.
+struct RopeTable {
+    int           device;
+    RopeParams    p;
+    int32_t       n_pos;
+    const float2* table;
+    const float*  ff;
+};
+RopeTable rope_table(const cbx_rope_cache* c);
+// ---- the paged key-value cache (cbx_paged.cpp checks the arguments) ---------
+constexpr int kPagedMaxSeq = 4096;   // requests of an append or release: their scans are held in LDS
+struct AppendArgs {
+    const int32_t *n_past, *n_new, *free_pages, *n_free;
+    int32_t *seq_lens, *n_free_out, *tok_start, *slots, *positions;
+    char* tables;
+    int64_t tables_nb1;
+    int32_t n_seq, max_pages, page, pool, n_slots;
+};
+int launch_paged_append(const AppendArgs& a, DeviceState* st, hipStream_t s);
+struct ReleaseArgs {
+    const int32_t *seq_lens, *release, *n_free;
+    int32_t *free_pages, *seq_lens_out, *n_free_out;
+    char* tables;
+    int64_t tables_nb1;
+    int32_t n_seq, max_pages, page, pool;
+};
+int launch_paged_release(const ReleaseArgs& a, DeviceState* st, hipStream_t s);
+// q (with gq, yq), k and v may each be null; k goes to yk or to k_cache, v to
+// v_cache; norm: the norm and the rotation, else rows are copied.
+struct QkCall {
+    const cbx_tensor *q, *gq, *k, *gk, *v, *pos, *slots;
+    cbx_tensor *yq, *yk, *k_cache, *v_cache;
+    float eps;
+    RopeTable rope;
+    bool norm;
+};
+int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s);
+struct PagedAttnCall {
+    const cbx_tensor *q, *k, *v, *tables, *lens;
+    cbx_tensor* y;
+    float scale, softcap;
+    int32_t window;
+    void* ws;
+};
+size_t paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
+int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s);
+struct LogProbCall {
+    const cbx_tensor *x, *ids;
+    cbx_tensor *logp, *entropy, *top_ids, *top_logp;
+    float scale;
+    int n_top;
+    void* ws;
+};
+constexpr int kLogProbTop = 64;
+size_t token_log_probs_workspace(const cbx_tensor* x, int n_top, const DeviceState* st);
+int launch_token_log_probs(const LogProbCall& c, DeviceState* st, hipStream_t s);
 // b: the second score term added in front (x's shape), or null
 int launch_soft_max(const cbx_tensor* x, const cbx_tensor* b, float s, int64_t n_past, cbx_tensor* y,
                     DeviceState* st, hipStream_t strm);

@@ -1,0 +1,169 @@
+// k_qk.hip -- RMS norm of query and key heads with the rotation in the same
+// pass, keys and values rounded into their cache pages on the way.
+//
+// A head row of D elements: y = rope(x * (1 / sqrt(mean(x^2) + eps)) * g), the
+// arithmetic of cbx_rms_norm_mul (f32 squares summed in f64, one rounding a
+// product) and of cbx_rope_ext (cos and sin from the position's table row,
+// or the same recurrence on the device past the table), the value between
+// the two kept in f32.
+//
+// One wave a head row; rows number tokens, then query, key and value heads.
+#include "cbx_rowops.h"
+
+namespace cbx {
+namespace {
+
+constexpr int kQkThreads = 256;
+constexpr int kQkMax = 512;   // elements of a head
+
+struct QkArgs {
+    const char *q, *k, *v;
+    const float *gq, *gk;
+    const int32_t *pos, *slots;
+    char *yq, *yk, *kc, *vc;          // yk, or kc and vc with slots
+    const float2* table;
+    const float* ff;
+    int64_t q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2, yq_nb1, yq_nb2, yk_nb1, yk_nb2;
+    int64_t kc_nb1, kc_nb2, kc_nb3, vc_nb1, vc_nb2, vc_nb3;
+    uint32_t hq, hkv, heads, rows, D;   // heads: hq + hkv (+ hkv value rows)
+    uint32_t page, n_slot;              // page size, slots of the cache
+    int32_t n_pos;
+    float eps;
+    int32_t norm;
+    RopeParams rp;
+    uint32_t* err;
+};
+
+template <typename T, typename TC>
+__global__ __launch_bounds__(kQkThreads) void k_qk(QkArgs a) {
+    __shared__ float rows[kQkThreads / 64][kQkMax];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const uint32_t row = blockIdx.x * (kQkThreads / 64) + wid;
+    float* r = rows[wid];
+    const bool live = row < a.rows;
+    const uint32_t tok = live ? row / a.heads : 0, h = live ? row - tok * a.heads : 0;
+    const int kind = h < a.hq ? 0 : (h < a.hq + a.hkv ? 1 : 2);   // q, k, v
+    const uint32_t hh = h - (kind == 0 ? 0 : (kind == 1 ? a.hq : a.hq + a.hkv));
+    const char* x = kind == 0 ? a.q + tok * a.q_nb2 + hh * a.q_nb1
+                  : kind == 1 ? a.k + tok * a.k_nb2 + hh * a.k_nb1 : a.v + tok * a.v_nb2 + hh * a.v_nb1;
+    const uint32_t D = a.D;
+    constexpr int N = kQkMax / 64;
+    float v[N];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t e = lane + 64 * i;
+        v[i] = live && e < D ? Elt<T>::load1(x + e * Elt<T>::size) : 0.0f;
+        sum += static_cast<double>(v[i] * v[i]);
+    }
+    if (a.norm) {
+        const float ms = static_cast<float>(wave_sum(sum) / static_cast<double>(D));
+        const float sc = 1.0f / sqrtf(ms + a.eps);
+        const float* g = kind == 0 ? a.gq : a.gk;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t e = lane + 64 * i;
+            float y = kind == 2 ? v[i] : v[i] * sc;
+            if (kind != 2 && g && e < D) y = y * g[e];
+            if (e < D) r[e] = y;
+        }
+        __syncthreads();
+        if (kind != 2) {
+            const int32_t p = live ? a.pos[tok] : 0;
+            const uint32_t nd = static_cast<uint32_t>(a.rp.n_dims), half = nd / 2;
+            const bool in_tab = p >= 0 && p < a.n_pos;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const uint32_t e = lane + 64 * i;
+                if (e >= D) continue;
+                v[i] = r[e];
+                if (e >= nd) continue;
+                const bool second = a.rp.mode == 2 ? e >= half : (e & 1);
+                const uint32_t pair = a.rp.mode == 2 ? (second ? e - half : e) : e >> 1;
+                const float other = r[a.rp.mode == 2 ? (second ? e - half : e + half) : e ^ 1];
+                float2 c;
+                if (in_tab) c = a.table[static_cast<int64_t>(p) * half + pair];
+                else rope_cos_sin_dev(p, static_cast<int>(pair), a.rp, a.ff, &c.x, &c.y);
+                v[i] = second ? other * c.y + v[i] * c.x : v[i] * c.x - other * c.y;
+            }
+        }
+    }
+    if (!live) return;
+    if (kind == 0 || (kind == 1 && !a.slots)) {
+        char* y = kind == 0 ? a.yq + tok * a.yq_nb2 + hh * a.yq_nb1 : a.yk + tok * a.yk_nb2 + hh * a.yk_nb1;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t e = lane + 64 * i;
+            if (e < D) Elt<T>::store1(y + e * Elt<T>::size, v[i]);
+        }
+        return;
+    }
+    const int32_t slot = a.slots[tok];
+    if (slot < 0) return;
+    if (static_cast<uint32_t>(slot) >= a.n_slot) {
+        if (lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
+        return;
+    }
+    const uint32_t pg = static_cast<uint32_t>(slot) / a.page, at = static_cast<uint32_t>(slot) - pg * a.page;
+    char* y = kind == 1 ? a.kc + pg * a.kc_nb3 + hh * a.kc_nb2 + at * a.kc_nb1
+                        : a.vc + pg * a.vc_nb3 + hh * a.vc_nb2 + at * a.vc_nb1;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t e = lane + 64 * i;
+        if (e < D) Elt<TC>::store1(y + e * Elt<TC>::size, v[i]);
+    }
+}
+
+int64_t nb(const cbx_tensor* t, int i) { return t ? static_cast<int64_t>(t->nb[i]) : 0; }
+
+}  // namespace
+
+int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
+    const cbx_tensor* k = c.k;
+    QkArgs a{};
+    auto in = [](const cbx_tensor* t) { return t ? static_cast<const char*>(t->data) : nullptr; };
+    auto out = [](cbx_tensor* t) { return t ? static_cast<char*>(t->data) : nullptr; };
+    a.q = in(c.q);
+    a.k = in(k);
+    a.v = in(c.v);
+    a.gq = reinterpret_cast<const float*>(in(c.gq));
+    a.gk = reinterpret_cast<const float*>(in(c.gk));
+    a.pos = reinterpret_cast<const int32_t*>(in(c.pos));
+    a.slots = reinterpret_cast<const int32_t*>(in(c.slots));
+    a.yq = out(c.yq);
+    a.yk = out(c.yk);
+    a.kc = out(c.k_cache);
+    a.vc = out(c.v_cache);
+    a.table = c.rope.table;
+    a.ff = c.rope.ff;
+    a.n_pos = c.rope.n_pos;
+    a.rp = c.rope.p;
+    a.q_nb1 = nb(c.q, 1); a.q_nb2 = nb(c.q, 2);
+    a.k_nb1 = nb(k, 1); a.k_nb2 = nb(k, 2);
+    a.v_nb1 = nb(c.v, 1); a.v_nb2 = nb(c.v, 2);
+    a.yq_nb1 = nb(c.yq, 1); a.yq_nb2 = nb(c.yq, 2);
+    a.yk_nb1 = nb(c.yk, 1); a.yk_nb2 = nb(c.yk, 2);
+    a.kc_nb1 = nb(c.k_cache, 1); a.kc_nb2 = nb(c.k_cache, 2); a.kc_nb3 = nb(c.k_cache, 3);
+    a.vc_nb1 = nb(c.v_cache, 1); a.vc_nb2 = nb(c.v_cache, 2); a.vc_nb3 = nb(c.v_cache, 3);
+    a.hq = c.q ? static_cast<uint32_t>(c.q->ne[1]) : 0;
+    a.hkv = static_cast<uint32_t>(k->ne[1]);
+    a.heads = a.hq + a.hkv * (c.v ? 2 : 1);
+    const int64_t rows = k->ne[2] * a.heads;
+    a.rows = static_cast<uint32_t>(rows);
+    a.D = static_cast<uint32_t>(k->ne[0]);
+    a.page = c.k_cache ? static_cast<uint32_t>(c.k_cache->ne[1]) : 1;
+    a.n_slot = c.k_cache ? static_cast<uint32_t>(c.k_cache->ne[1] * c.k_cache->ne[3]) : 0;
+    a.eps = c.eps;
+    a.norm = c.norm;
+    a.err = st->err_word;
+    if (rows == 0 || a.D == 0) return CBX_OK;
+    const dim3 grid(static_cast<unsigned>(cdiv(rows, kQkThreads / 64))), block(kQkThreads);
+    const bool t16 = k->type == CBX_TYPE_F16, c16 = c.k_cache ? c.k_cache->type == CBX_TYPE_F16 : t16;
+    if (t16 && c16) hipLaunchKernelGGL((k_qk<uint16_t, uint16_t>), grid, block, 0, s, a);
+    else if (t16) hipLaunchKernelGGL((k_qk<uint16_t, float>), grid, block, 0, s, a);
+    else if (c16) hipLaunchKernelGGL((k_qk<float, uint16_t>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_qk<float, float>), grid, block, 0, s, a);
+    return check_launch("cbx_qk_norm_rope");
+}
+
+}  // namespace cbx

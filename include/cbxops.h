@@ -84,7 +84,8 @@ const char* cbx_version(void);
  * synchronising the device first.  Bit 0: a get_rows index was out of
  * range (ggml aborts there; this library writes zeros to that row).
  * Bit 1: reserved, never raised (in-place GroupNorm calls do not take the
- * split reduction, the only path that raised it).                          */
+ * split reduction, the only path that raised it).  Bit 2: a page number,
+ * slot or length of the paged cache lay outside its tensor (left out).     */
 int  cbx_device_errors(int device, uint32_t* flags_out, int clear);
 
 /* ---- gather and conversion ---------------------------------------------- */
@@ -513,6 +514,148 @@ int cbx_conv_transpose1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
 int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
                       const cbx_tensor* mask, const cbx_tensor* bias,
                       cbx_tensor* y, cbx_stream stream);
+
+/* ---- decoding many streams over a paged key-value cache ---------------------- */
+
+/* The reference keeps one stream's keys and values in one tensor a layer
+ * (t3.cpp:238-262) and runs softmax(K q) V over a view of it
+ * (t3.cpp:488-522).  These entry points are the same step for many streams
+ * at once: the cache is a pool of pages that requests take as they grow.
+ *
+ *   page      page_size consecutive keys (values) of one request, all heads
+ *   k_cache, v_cache
+ *             F32 or F16 (both one type), ne = (head_dim, page_size,
+ *             n_head_kv, n_pages), any strides past nb[0]
+ *   block_tables
+ *             I32 (max_pages, n_seq): entry i of request s is the page that
+ *             holds its keys [i * page_size, (i + 1) * page_size)
+ *   slot      page * page_size + place in the page; a negative slot belongs
+ *             to no request (the padding of a batch)
+ *   free_pages, n_free
+ *             I32: a stack of free page numbers, n_free[0] of them, the top
+ *             last
+ * All of it lives on the device: no call reads a length on the host, so a
+ * captured step replays as its requests grow.  Page numbers, slots and
+ * lengths that lie outside their tensors are left out by the kernels that
+ * meet them, which raise bit 2 of the device error word
+ * (cbx_device_errors).                                                     */
+
+/* One step's bookkeeping: n_new[s] tokens follow the n_past[s] cached ones
+ * of every request s (0: it sits this step out).
+ *   tok_start  I32 (n_seq + 1): the step's tokens are numbered request after
+ *              request, those of s from tok_start[s]; the total is last
+ *   positions, slots
+ *              I32 (n_slots): of token tok_start[s] + j, n_past[s] + j and
+ *              the slot of its key; from the total on, 0 and -1
+ *   block_tables
+ *              gets the pages newly taken, popped from the stack in the
+ *              order of the requests; other entries stay as they are
+ *   seq_lens   I32 (n_seq): n_past + n_new, the keys to attend over
+ *   n_free_out I32 (1): what is left on the stack
+ * A request is refused as a whole when its table row cannot hold
+ * n_past + n_new keys, when its tokens do not all lie below n_slots, or when
+ * the stack runs out (then also every later one that needs a page): it takes
+ * no page, its slots are -1 and its seq_lens entry is n_past[s].  Nothing is
+ * kept: the same arguments give the same results, and outputs overlap no
+ * input.  n_seq <= 4096; max_pages * page_size < 2^31.                      */
+int cbx_paged_append(const cbx_tensor* n_past, const cbx_tensor* n_new,
+                     const cbx_tensor* free_pages, const cbx_tensor* n_free,
+                     cbx_tensor* block_tables, int32_t page_size,
+                     cbx_tensor* seq_lens, cbx_tensor* n_free_out,
+                     cbx_tensor* tok_start, cbx_tensor* slots,
+                     cbx_tensor* positions, cbx_stream stream);
+
+/* Gives back the pages of every request s with release[s] != 0: pushed on
+ * the stack in the order of the requests and of their tables, their table
+ * entries set to -1, seq_lens_out[s] = 0; the other requests' lengths are
+ * copied.  Pages past the stack's end (more given back than were taken) are
+ * dropped and raise the error bit.                                         */
+int cbx_paged_release(const cbx_tensor* seq_lens, const cbx_tensor* release,
+                      cbx_tensor* block_tables, int32_t page_size,
+                      cbx_tensor* free_pages, const cbx_tensor* n_free,
+                      cbx_tensor* seq_lens_out, cbx_tensor* n_free_out,
+                      cbx_stream stream);
+
+/* Writes key and value rows into their pages (t3.cpp:488-489's cpy into the
+ * cache view): row t of k and v, F32 or F16 (head_dim, n_head_kv, n_tok),
+ * goes to slot slots[t], rounded to the cache's type; negative slots are
+ * skipped.  The non-negative slots of a call are distinct; a slot given
+ * twice gets each head's row from one of its tokens.                       */
+int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v,
+                    const cbx_tensor* slots, cbx_tensor* k_cache,
+                    cbx_tensor* v_cache, cbx_stream stream);
+
+/* RMS norm of every query and key head, then the rotation, in one pass:
+ *   yq = ggml_rope_ext(ggml_mul(ggml_rms_norm(q, eps), gq), pos, ...)
+ *   yk = ggml_rope_ext(ggml_mul(ggml_rms_norm(k, eps), gk), pos, ...)
+ * q: F32 or F16 (head_dim, n_head, n_tok), k: the same type (head_dim,
+ * n_head_kv, n_tok), any strides past nb[0] (views of one projection's
+ * output); gq, gk: F32 (head_dim) or NULL; pos: I32 (n_tok); the rotation is
+ * `rope`'s (both pairings, a part of the head, scaled).  F32: the bits of
+ * cbx_rms_norm_mul, then cbx_rope_ext; F16: the same without the rounding
+ * between the two.  head_dim % 8 == 0, head_dim <= 512, n_dims % 8 == 0.
+ * yq may be q and yk k; outputs overlap nothing else.                      */
+int cbx_qk_norm_rope(const cbx_tensor* q, const cbx_tensor* gq,
+                     const cbx_tensor* k, const cbx_tensor* gk, float eps,
+                     const cbx_tensor* pos, const cbx_rope_cache* rope,
+                     cbx_tensor* yq, cbx_tensor* yk, cbx_stream stream);
+
+/* The same with the keys rounded straight into the cache and the values
+ * beside them, as cbx_paged_store: k is not stored elsewhere.              */
+int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
+                           const cbx_tensor* k, const cbx_tensor* gk,
+                           const cbx_tensor* v, float eps,
+                           const cbx_tensor* pos, const cbx_rope_cache* rope,
+                           const cbx_tensor* slots, cbx_tensor* yq,
+                           cbx_tensor* k_cache, cbx_tensor* v_cache,
+                           cbx_stream stream);
+
+/* Attention of one new token a request over its cached keys
+ * (t3.cpp:494-522 with N_new = 1, for every request at once):
+ *   s_i = scale * q . k_i, softcap > 0: s_i = softcap * tanh(s_i / softcap)
+ *   y   = sum_i softmax(s)_i v_i over 0 <= i < seq_lens[s], window > 0: over
+ *         the last `window` of them
+ * q, y: F32 or F16 (head_dim, n_head, n_seq), one type; n_head a multiple of
+ * n_head_kv, query head h reads key head h / (n_head / n_head_kv).  A request
+ * without keys gets zeros; keys past its length are never looked at, whatever
+ * the page holds there.  head_dim <= 512.  Scores, sums and products are
+ * held in f32, also between the parts that a long request is split into;
+ * where the parts begin depends on all of the call's lengths.
+ * ws: 16-byte aligned scratch of at least the bytes that
+ * cbx_paged_attention_workspace gives for these shapes (it may be 0), used by
+ * this call only: nothing in it needs to be set or kept, and calls that may
+ * run at the same time need one each.                                      */
+int cbx_paged_attention_workspace(const cbx_tensor* q,
+                                  const cbx_tensor* k_cache,
+                                  const cbx_tensor* block_tables,
+                                  size_t* bytes);
+int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
+                        const cbx_tensor* v_cache,
+                        const cbx_tensor* block_tables,
+                        const cbx_tensor* seq_lens, float scale,
+                        float softcap, int32_t window, cbx_tensor* y,
+                        void* ws, size_t ws_bytes, cbx_stream stream);
+
+/* What a step answers with: of each row of logits x, F32 or F16
+ * (n_vocab, n_tok), with p = softmax(scale * x) (scale > 0: one over the
+ * temperature),
+ *   logp[t]        F32 (n_tok): log p of token ids[t]
+ *   entropy[t]     F32 (n_tok): -sum p log p
+ *   top_ids, top_logp
+ *                  I32 and F32 (n_top, n_tok): the n_top largest logits'
+ *                  tokens, largest first, equal ones by number, and their
+ *                  log p; n_top <= 64, n_top <= n_vocab
+ * ids with logp, entropy, and top_ids with top_logp may each be NULL.
+ * Logits of -inf have p = 0; a row of nothing else has logp and top_logp
+ * -inf and entropy 0.  A NaN makes its row's numbers NaN and counts as the
+ * largest.  An id outside [0, n_vocab) gets logp 0 and raises bit 0 of the
+ * device error word.  ws as for cbx_paged_attention.                       */
+int cbx_token_log_probs_workspace(const cbx_tensor* logits, int32_t n_top,
+                                  size_t* bytes);
+int cbx_token_log_probs(const cbx_tensor* logits, const cbx_tensor* ids,
+                        float scale, cbx_tensor* logp, cbx_tensor* entropy,
+                        cbx_tensor* top_ids, cbx_tensor* top_logp, void* ws,
+                        size_t ws_bytes, cbx_stream stream);
 
 /* ---- model tables from a GGUF file ---------------------------------------- */
 
