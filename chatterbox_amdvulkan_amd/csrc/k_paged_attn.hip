@@ -5,8 +5,21 @@
 // exp(s_i - m) v_i, both rescaled by exp(m - m') when the maximum rises to m',
 // and y = o / l at the end.  f32 throughout.
 //
-// A workgroup a request and query head; its waves take keys in turn, a key's
-// D elements over the lanes, and their (m, l, o) are joined in LDS.
+// Bound by the read of the keys and values, each of which the heads of a
+// group share: the group's products run on the matrix cores (16 heads wide;
+// a group of one fills a 16th of them, which is still several times what the
+// reads feed), so that no group size pays for its arithmetic.
+//
+// k_attn_tiles: the requests' keys are cut into tiles of 4 waves x NK keys and
+// all tiles of the call (request after request, key head after key head) are
+// dealt to a fixed grid in equal runs, so that one long request or a thousand
+// short ones fill the chip alike.  The lengths are on the device: every
+// workgroup finds its run from a scan over them.  A key head whose tiles fall
+// into one run is written to y; the parts of one that spans runs go to the
+// workspace as (m, l, o) and k_attn_join adds them up in order.
+//
+// k_attn_rows: head sizes, strides and alignments that the tiles do not take,
+// a workgroup a request and query head, a key's elements over the lanes.
 #include "cbx_device.h"
 
 namespace cbx {
@@ -14,7 +27,8 @@ namespace {
 
 constexpr int kAttnThreads = 256;
 constexpr int kAttnMaxD = 512;
-constexpr float kLowest = -3.0e38f;   // below every finite score that matters; finite, so that m - m is 0
+constexpr float kLowest = -3.0e38f;   // below every score that matters; finite, so that m - m is 0
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct AttnArgs {
     const char *q, *k, *v, *tables;
@@ -25,6 +39,12 @@ struct AttnArgs {
     int32_t window;
     float scale, softcap;
     uint32_t* err;
+    // k_attn_tiles and k_attn_join
+    uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
+    uint32_t gc, ngr, H;             // heads a run holds (<= 16), runs of heads a group, hkv * ngr
+    uint32_t W;                      // workgroups
+    float* part_o;                   // [W][2][gc][D]
+    float2* part_ml;                 // [W][2][gc]
 };
 
 __device__ __forceinline__ float wave_sum_f32(float v) {
@@ -110,11 +130,661 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
     }
 }
 
+
+// ---- tiles ------------------------------------------------------------------
+
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t page_of(const AttnArgs& a, uint32_t key) {
+    return static_cast<uint32_t>((static_cast<uint64_t>(key) * a.page_mul) >> a.page_shift);
+}
+
+// A request's keys: [first, len), and the tiles of KT keys they lie in; a
+// request without keys has one tile all the same, which writes its zeros.
+struct Span {
+    uint32_t first, len, tile0, tiles;
+    bool wrong;
+};
+template <int KT>
+__device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
+    const uint32_t cap = a.max_pages * a.page;
+    const int32_t n = a.lens[s];
+    Span r;
+    r.wrong = n < 0 || static_cast<uint32_t>(n) > cap;
+    r.len = n < 0 ? 0 : min(static_cast<uint32_t>(n), cap);
+    r.first = a.window > 0 && r.len > static_cast<uint32_t>(a.window) ? r.len - a.window : 0;
+    r.tile0 = r.first / KT;
+    r.tiles = max(1u, (r.len + KT - 1) / KT - r.tile0);
+    return r;
+}
+
+// The exclusive prefix over the requests of their tiles, as every workgroup
+// needs it: each thread sums c neighbouring requests.  *total the sum.
+template <int KT>
+__device__ __forceinline__ uint32_t tiles_before(const AttnArgs& a, uint32_t c, uint32_t* lds, uint32_t* mine, uint32_t* total) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    uint32_t sum = 0;
+    for (uint32_t s = tid * c; s < min(a.n_seq, (tid + 1) * c); s++) sum += span_of<KT>(a, s).tiles;
+    uint32_t x = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t u = __shfl_up(x, d);
+        if (lane >= static_cast<uint32_t>(d)) x += u;
+    }
+    if (lane == 63) lds[wid] = x;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kAttnThreads / 64; w++) {
+        if (w < wid) before += lds[w];
+        all += lds[w];
+    }
+    *mine = sum;
+    *total = all;
+    return before + x - sum;
+}
+
+// First tile of workgroup w's run of the call's T tiles, W <= T.
+__device__ __forceinline__ uint32_t run_start(uint32_t w, uint32_t W, uint32_t T) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(w) * T / W);
+}
+// The workgroup whose run holds tile t: the last w with run_start(w) <= t.
+__device__ __forceinline__ uint32_t run_of(uint32_t t, uint32_t W, uint32_t T) {
+    return static_cast<uint32_t>(((static_cast<uint64_t>(t) + 1) * W - 1) / T);
+}
+
+// A matrix core's view of NK keys and 16 heads.  S^T = K Q^T: the A operand's
+// row is the key (lane % 16), the B operand's column the head (lane % 16),
+// both hold for the lane group lane / 16 the same dims; the result's lane has
+// head lane % 16 and keys 4 (lane / 16) + r.  O^T = V^T P^T: the B operand is
+// then what the lane already holds (the sum over the keys may take them in
+// any order, as long as V's rows come in the same one), the A operand's row
+// m is dim m * DP/16 + d of product d: a lane reads DP/16 neighbouring dims of
+// its keys.  The result's lane has head lane % 16 and dims
+// (4 (lane / 16) + r) * DP/16 + d.
+template <typename TC, int DP> struct Core;
+
+// f16 pages: 16x16x32 products, f32 sums.  An f32 query is scaled by a power
+// of two to below 2^15 and split into two f16 (22 bits); so is every
+// probability, times 2^14 (the smallest that keep their bits are then 2^-28
+// of the largest).
+template <int DP> struct Core<uint16_t, DP> {
+    static constexpr int NK = 32, NH = 2, NE = 8;   // keys a step, halves of 16, keys whose values a lane holds
+    static constexpr int CD = DP / 32;
+    h8v qh[CD], ql[CD], kf[NH][CD];
+    uint32_t vr[NE][CD];
+    f4v acc[DP / 16];
+    float qmul;        // what the query's power of two leaves to multiply scores by
+    bool two;          // ql is not zero
+
+    __device__ __forceinline__ void load_q(const float (&x)[CD * 8], bool f32) {
+        two = f32;
+        qmul = 1.0f;
+        float m = 0.0f;
+        if (f32) {
+#pragma unroll
+            for (int i = 0; i < CD * 8; i++) m = fmaxf(m, fabsf(x[i]));
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            // 2^e <= m < 2^(e + 1) goes to [2^14, 2^15)
+            int e = m > 0.0f && m < INFINITY ? static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23) - 127 : 14;
+            e = e < -100 ? -100 : e;
+            qmul = ldexpf(1.0f, e - 14);
+            const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+            for (int i = 0; i < CD * 8; i++) {
+                const float t = x[i] * up;
+                const _Float16 h = static_cast<_Float16>(t);
+                qh[i / 8][i % 8] = h;
+                ql[i / 8][i % 8] = static_cast<_Float16>(t - static_cast<float>(h));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CD * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(x[i]);
+        }
+    }
+    // dims the lane holds of its query and keys: 8 at 32 c + 8 grp
+    static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 32 * c + 8 * grp; }
+    static constexpr int QC = CD, QN = 8;
+
+    __device__ __forceinline__ void load_k(int h, const char* p, uint32_t grp, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+            const uint32_t d = dim_of(c, grp);
+            kf[h][c] = *reinterpret_cast<const h8v*>(p + (D == DP || d < D ? d * 2 : 0));
+        }
+    }
+    __device__ __forceinline__ void trim_k(uint32_t grp, uint32_t D) {   // dims past D: 0
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+            if (dim_of(c, grp) >= D) {
+#pragma unroll
+                for (int h = 0; h < NH; h++) kf[h][c] = h8v{};
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(int e, const char* p, uint32_t n, uint32_t D) {
+        const uint32_t d = n * (DP / 16);
+        if constexpr (CD == 2) {
+            const u2v t = *reinterpret_cast<const u2v*>(p + (D == DP || d < D ? d * 2 : 0));
+            vr[e][0] = t.x;
+            vr[e][1] = t.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < CD; c += 4) {
+                const u4v t = *reinterpret_cast<const u4v*>(p + (D == DP || d + 2 * c < D ? (d + 2 * c) * 2 : 0));
+                vr[e][c] = t.x;
+                vr[e][c + 1] = t.y;
+                vr[e][c + 2] = t.z;
+                vr[e][c + 3] = t.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void drop_v(int e) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) vr[e][c] = 0;
+    }
+    // keys of the lane's NE scores and values: h half, r in it
+    static __device__ __forceinline__ uint32_t key_of(int e, uint32_t grp) { return 16 * (e >> 2) + 4 * grp + (e & 3); }
+    static constexpr int half_of(int e) { return e >> 2; }
+
+    __device__ __forceinline__ void scores(float (&s)[NE]) {
+#pragma unroll
+        for (int h = 0; h < NH; h++) {
+            f4v t = {};
+            if (two) {
+#pragma unroll
+                for (int c = 0; c < CD; c++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][c], ql[c], t, 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < CD; c++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][c], qh[c], t, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * h + r] = t[r];
+        }
+    }
+    static constexpr float kBias = 14.0f;   // probabilities times 2^14
+    __device__ __forceinline__ void add_values(const float (&p)[NE]) {
+        h8v ph, pl;
+#pragma unroll
+        for (int e = 0; e < NE; e++) {
+            const _Float16 h = static_cast<_Float16>(p[e]);
+            ph[e] = h;
+            pl[e] = static_cast<_Float16>(p[e] - static_cast<float>(h));
+        }
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+            u4v lo, hi;   // dims 2c and 2c + 1 of the lane's eight keys
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                lo[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x05040100u);
+                hi[i] = __builtin_amdgcn_perm(vr[2 * i + 1][c], vr[2 * i][c], 0x07060302u);
+            }
+            const h8v a0 = __builtin_bit_cast(h8v, lo), a1 = __builtin_bit_cast(h8v, hi);
+            acc[2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pl, acc[2 * c], 0, 0, 0);
+            acc[2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pl, acc[2 * c + 1], 0, 0, 0);
+            acc[2 * c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ph, acc[2 * c], 0, 0, 0);
+            acc[2 * c + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ph, acc[2 * c + 1], 0, 0, 0);
+        }
+    }
+};
+
+// f32 pages: 16x16x4 products of f32.
+template <int DP> struct Core<float, DP> {
+    static constexpr int NK = 16, NH = 1, NE = 4;
+    static constexpr int CD = DP / 16, CV = DP / 64;
+    f4v qf[CD], kf[NH][CD], vr[NE][CV];
+    f4v acc[DP / 16];
+    float qmul;
+    static constexpr int QC = CD, QN = 4;
+    __device__ __forceinline__ void load_q(const float (&x)[CD * 4], bool) {
+        qmul = 1.0f;
+#pragma unroll
+        for (int i = 0; i < CD * 4; i++) qf[i / 4][i % 4] = x[i];
+    }
+    static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 16 * c + 4 * grp; }
+    __device__ __forceinline__ void load_k(int h, const char* p, uint32_t grp, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+            const uint32_t d = dim_of(c, grp);
+            kf[h][c] = *reinterpret_cast<const f4v*>(p + (D == DP || d < D ? d * 4 : 0));
+        }
+    }
+    __device__ __forceinline__ void trim_k(uint32_t grp, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+            if (dim_of(c, grp) >= D) kf[0][c] = f4v{};
+        }
+    }
+    __device__ __forceinline__ void load_v(int e, const char* p, uint32_t n, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CV; c++) {
+            const uint32_t d = n * (DP / 16) + 4 * c;
+            vr[e][c] = *reinterpret_cast<const f4v*>(p + (D == DP || d < D ? d * 4 : 0));
+        }
+    }
+    __device__ __forceinline__ void drop_v(int e) {
+#pragma unroll
+        for (int c = 0; c < CV; c++) vr[e][c] = f4v{};
+    }
+    static __device__ __forceinline__ uint32_t key_of(int e, uint32_t grp) { return 4 * grp + e; }
+    static constexpr int half_of(int) { return 0; }
+    __device__ __forceinline__ void scores(float (&s)[NE]) {
+        f4v t = {};
+#pragma unroll
+        for (int c = 0; c < CD; c++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) t = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[0][c][i], qf[c][i], t, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[r] = t[r];
+    }
+    static constexpr float kBias = 0.0f;
+    __device__ __forceinline__ void add_values(const float (&p)[NE]) {
+#pragma unroll
+        for (int r = 0; r < NE; r++) {
+#pragma unroll
+            for (int d = 0; d < DP / 16; d++) {
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[r][d / 4][d % 4], p[r], acc[d], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// Workgroups of a tile kernel that a CU holds, which their registers are limited to.
+constexpr int per_cu(int dp) { return dp <= 64 ? 4 : dp <= 128 ? 2 : 1; }
+
+// UNI: a page holds whole runs of 16 keys, looked up once a wave and half;
+// else every lane looks its key up and passes the page on.
+template <typename TQ, typename TC, int DP, bool UNI>
+__global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArgs a) {
+    using C = Core<TC, DP>;
+    constexpr int NK = C::NK, NH = C::NH, NE = C::NE, W4 = kAttnThreads / 64, KT = NK * W4;
+    extern __shared__ float lds_o[];                 // [4][gc][DP + 4]
+    __shared__ float lds_m[W4][16], lds_l[W4][16];
+    __shared__ uint32_t lds_scan[W4], lds_at[2];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 15, grp = lane >> 4;
+    const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    bool wrong = false;
+
+    // this workgroup's run of tiles, and the request that its first lies in
+    const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
+    uint32_t mine, total;
+    uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
+    const uint32_t T = total * a.H;
+    const uint32_t W = min(a.W, T);                  // runs, each of a tile at least
+    if (blockIdx.x >= W) return;
+    uint32_t at = run_start(blockIdx.x, W, T);
+    const uint32_t end = run_start(blockIdx.x + 1, W, T);
+    if (before * a.H <= at && at < (before + mine) * a.H) {
+        uint32_t s = tid * c;
+        for (;; s++) {
+            const uint32_t t = span_of<KT>(a, s).tiles;
+            if (at < (before + t) * a.H) break;
+            before += t;
+        }
+        lds_at[0] = s;
+        lds_at[1] = before * a.H;
+    }
+    __syncthreads();
+    uint32_t s = __builtin_amdgcn_readfirstlane(lds_at[0]), base = __builtin_amdgcn_readfirstlane(lds_at[1]);
+
+    C core;
+    while (at < end) {
+        const Span sp = span_of<KT>(a, s);
+        wrong |= sp.wrong;
+        const uint32_t h = (at - base) / sp.tiles, t0 = at - base - h * sp.tiles;
+        const uint32_t n_tiles = min(end - at, sp.tiles - t0);
+        const uint32_t hk = h / a.ngr, h0 = (h - hk * a.ngr) * a.gc;     // key head, first of the group's heads
+        const uint32_t heads = min(a.gc, a.g - h0);
+        const uint32_t hq0 = hk * a.g + h0;
+        const int32_t* row = reinterpret_cast<const int32_t*>(a.tables + s * a.t_nb1);
+        {
+            float x[C::QC * C::QN];
+            const char* qr = a.q + s * a.q_nb2 + (hq0 + (n < heads ? n : 0)) * a.q_nb1;
+#pragma unroll
+            for (int i = 0; i < C::QC; i++) {
+#pragma unroll
+                for (int j = 0; j < C::QN; j++) {
+                    const uint32_t d = C::dim_of(i, grp) + j;
+                    const bool in = n < heads && d < a.D;
+                    const float v = Elt<TQ>::load1(qr + (in ? d : 0) * Elt<TQ>::size);
+                    x[i * C::QN + j] = in ? v : 0.0f;
+                }
+            }
+            core.load_q(x, sizeof(TQ) == 4);
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 16; d++) core.acc[d] = f4v{};
+        float m = kLowest, l = 0.0f;
+        const float scale = core.qmul * a.scale;
+
+        // the wave's own steps: [tb, te) tiles, NK keys of each from kb on
+        uint32_t tb = sp.tile0 + t0, te = tb + n_tiles;
+        if (tb * KT + wid * NK + NK <= sp.first) tb++;
+        if (te > tb && (te - 1) * KT + wid * NK >= sp.len) te--;
+
+        const char* kb0 = a.k + hk * a.k_nb2;
+        const char* vb0 = a.v + hk * a.v_nb2;
+        int32_t pg[NH];           // UNI: pages of the halves; else pg[0] the page of key `lane` of the step
+        bool ok[NH];
+        auto look_up = [&](uint32_t kb) {
+            if constexpr (UNI) {
+#pragma unroll
+                for (int i = 0; i < NH; i++) {
+                    const uint32_t key = kb + 16 * i;
+                    ok[i] = key < sp.len && key + 16 > sp.first;
+                    pg[i] = __builtin_amdgcn_readfirstlane(row[ok[i] ? page_of(a, key) : 0]);
+                }
+            } else {
+                const uint32_t key = kb + (lane & (NK - 1));
+                const bool in = key < sp.len && key >= sp.first;
+                pg[0] = row[in ? page_of(a, key) : 0];
+                if (!in) pg[0] = -2;
+            }
+        };
+        // a looked-up page that is none: left out
+        auto settle = [&]() {
+            if constexpr (UNI) {
+#pragma unroll
+                for (int i = 0; i < NH; i++) {
+                    const bool good = static_cast<uint32_t>(pg[i]) < a.n_pages;
+                    wrong |= ok[i] && !good;
+                    ok[i] = ok[i] && good;
+                    if (!good) pg[i] = 0;
+                }
+            } else {
+                if (static_cast<uint32_t>(pg[0]) >= a.n_pages) {
+                    wrong |= pg[0] != -2;
+                    pg[0] = -1;
+                }
+            }
+        };
+        auto fetch_k = [&](uint32_t kb) {
+#pragma unroll
+            for (int i = 0; i < NH; i++) {
+                const char* p;
+                if constexpr (UNI) {
+                    const uint32_t key = kb + 16 * i, in = ok[i] ? key - page_of(a, key) * a.page : 0;
+                    p = kb0 + pg[i] * a.k_nb3 + in * a.k_nb1 + n * static_cast<uint32_t>(a.k_nb1);
+                } else {
+                    const uint32_t key = kb + 16 * i + n;
+                    const int32_t g = __shfl(pg[0], 16 * i + n);
+                    p = kb0 + (g < 0 ? 0 : g * a.k_nb3 + (key - page_of(a, key) * a.page) * a.k_nb1);
+                }
+                core.load_k(i, p, grp, a.D);
+            }
+        };
+        auto fetch_v = [&](uint32_t kb, bool (&live)[NE]) {
+#pragma unroll
+            for (int e = 0; e < NE; e++) {
+                const uint32_t key = kb + C::key_of(e, grp);
+                const char* p;
+                if constexpr (UNI) {
+                    const int i = C::half_of(e);
+                    const uint32_t k0 = kb + 16 * i, in = ok[i] ? k0 - page_of(a, k0) * a.page : 0;
+                    p = vb0 + pg[i] * a.v_nb3 + in * a.v_nb1 + (key - k0) * static_cast<uint32_t>(a.v_nb1);
+                    live[e] = ok[i] && key < sp.len && key >= sp.first;
+                } else {
+                    const int32_t g = __shfl(pg[0], C::key_of(e, grp));
+                    p = vb0 + (g < 0 ? 0 : g * a.v_nb3 + (key - page_of(a, key) * a.page) * a.v_nb1);
+                    live[e] = g >= 0;
+                }
+                core.load_v(e, p, n, a.D);
+            }
+        };
+        if (tb < te) {
+            uint32_t kb = tb * KT + wid * NK;
+            look_up(kb);
+            settle();
+            fetch_k(kb);
+            for (uint32_t t = tb; t < te; t++, kb += KT) {
+                bool live[NE];
+                fetch_v(kb, live);
+                bool whole = kb >= sp.first && kb + NK <= sp.len;
+                if constexpr (UNI) {
+#pragma unroll
+                    for (int i = 0; i < NH; i++) whole = whole && ok[i];
+                } else {
+                    whole = whole && __all(pg[0] >= 0);
+                }
+                const bool more = t + 1 < te;
+                if (more) look_up(kb + KT);
+                if (a.D != DP) core.trim_k(grp, a.D);
+                float sc[NE];
+                core.scores(sc);
+                if (more) {
+                    settle();
+                    fetch_k(kb + KT);
+                }
+                if (a.softcap > 0.0f) {
+#pragma unroll
+                    for (int e = 0; e < NE; e++) sc[e] = a.softcap * tanhf(sc[e] * scale / a.softcap) * kLog2e;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < NE; e++) sc[e] = sc[e] * (scale * kLog2e);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < NE; e++) {
+                        if (!live[e]) {
+                            sc[e] = -INFINITY;
+                            core.drop_v(e);
+                        }
+                    }
+                }
+                float mx = sc[0];
+#pragma unroll
+                for (int e = 1; e < NE; e++) mx = fmaxf(mx, sc[e]);
+                if (__any(mx > m)) {   // rare after the first steps: the sums are rescaled
+                    mx = fmaxf(mx, __shfl_xor(mx, 16));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32));
+                    const float m2 = fmaxf(m, mx), keep = __builtin_amdgcn_exp2f(m - m2);
+                    m = m2;
+                    l *= keep;
+#pragma unroll
+                    for (int d = 0; d < DP / 16; d++) core.acc[d] *= keep;
+                }
+                float p[NE];
+#pragma unroll
+                for (int e = 0; e < NE; e++) {
+                    p[e] = __builtin_amdgcn_exp2f(sc[e] - (m - C::kBias));
+                    l += p[e];
+                }
+                core.add_values(p);
+            }
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+
+        // the four waves' parts, joined through LDS
+        const uint32_t ld = DP + 4;
+        if (n < heads) {
+            float* o = lds_o + (wid * a.gc + n) * ld + grp * (DP / 4);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+#pragma unroll
+                for (int d = 0; d < DP / 16; d++) o[r * (DP / 16) + d] = core.acc[d][r];
+            }
+            if (grp == 0) {
+                lds_m[wid][n] = m;
+                lds_l[wid][n] = l;
+            }
+        }
+        __syncthreads();
+        const bool entire = n_tiles == sp.tiles;
+        const uint64_t slot = (static_cast<uint64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * a.gc;
+        for (uint32_t i = tid; i < heads * a.D; i += kAttnThreads) {
+            const uint32_t hh = i / a.D, d = i - hh * a.D;
+            float mm = lds_m[0][hh];
+#pragma unroll
+            for (int w = 1; w < W4; w++) mm = fmaxf(mm, lds_m[w][hh]);
+            float ll = 0.0f, oo = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W4; w++) {
+                const float f = __builtin_amdgcn_exp2f(lds_m[w][hh] - mm);
+                ll = fmaf(lds_l[w][hh], f, ll);
+                oo = fmaf(lds_o[(w * a.gc + hh) * ld + d], f, oo);
+            }
+            if (entire) {
+                Elt<TQ>::store1(a.y + s * a.y_nb2 + (hq0 + hh) * a.y_nb1 + d * Elt<TQ>::size, ll == 0.0f ? 0.0f : oo / ll);
+            } else {
+                a.part_o[(slot + hh) * a.D + d] = oo;
+                if (d == 0) a.part_ml[slot + hh] = make_float2(mm, ll);
+            }
+        }
+        __syncthreads();
+        at += n_tiles;
+        if (at == base + sp.tiles * a.H) {
+            s++;
+            base = at;
+        }
+    }
+    if (wrong && n == 0) atomicOr(a.err, DEV_ERR_PAGE);
+}
+
+// Adds up the parts of the key heads that several runs hold, in the order of
+// the runs: a workgroup a request and query head.  Part 0 lies in its run's
+// second place (the run ends with it), the others in the first.
+template <typename TQ, int KT>
+__global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
+    __shared__ uint32_t lds_scan[kAttnThreads / 64], lds_before;
+    __shared__ float lds_f[kAttnThreads], lds_w[kAttnThreads / 64];
+    __shared__ float lds_o[kAttnThreads];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t s = blockIdx.x / a.hq, hq = blockIdx.x - s * a.hq;
+    const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
+    uint32_t mine, total;
+    uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
+    if (tid == s / c) {
+        for (uint32_t i = tid * c; i < s; i++) before += span_of<KT>(a, i).tiles;
+        lds_before = before;
+    }
+    __syncthreads();
+    const uint32_t T = total * a.H, tiles = span_of<KT>(a, s).tiles;
+    const uint32_t hk = hq / a.g, in_g = hq - hk * a.g, run = in_g / a.gc, hh = in_g - run * a.gc;
+    const uint32_t t0 = lds_before * a.H + (hk * a.ngr + run) * tiles;
+    const uint32_t W = min(a.W, T);
+    const uint32_t w0 = run_of(t0, W, T), w1 = run_of(t0 + tiles - 1, W, T);
+    if (w0 == w1) return;
+    const uint32_t parts = w1 - w0 + 1;
+    auto slot = [&](uint32_t i) { return (static_cast<uint64_t>(w0 + i) * 2 + (i == 0 ? 1 : 0)) * a.gc + hh; };
+    float m = kLowest;
+    for (uint32_t i = tid; i < parts; i += kAttnThreads) m = fmaxf(m, a.part_ml[slot(i)].x);
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if ((tid & 63) == 0) lds_w[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(lds_w[0], lds_w[1]), fmaxf(lds_w[2], lds_w[3]));
+    // dims over 64-lane columns, parts over the four waves, 256 parts a turn
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t lane = tid & 63, wid = tid >> 6;
+    for (uint32_t i0 = 0; i0 < parts; i0 += kAttnThreads) {
+        __syncthreads();
+        if (i0 + tid < parts) {
+            const float2 ml = a.part_ml[slot(i0 + tid)];
+            const float f = __builtin_amdgcn_exp2f(ml.x - m);
+            lds_f[tid] = f;
+            l = fmaf(ml.y, f, l);
+        }
+        __syncthreads();
+        const uint32_t k = min(parts - i0, static_cast<uint32_t>(kAttnThreads));
+#pragma unroll 4
+        for (uint32_t i = wid; i < k; i += 4) {
+            const float* p = a.part_o + slot(i0 + i) * a.D;
+            const float f = lds_f[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t d = lane + 64 * j;
+                if (d < a.D) o[j] = fmaf(p[d], f, o[j]);
+            }
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
+    __syncthreads();
+    if (lane == 0) lds_w[wid] = l;
+    __syncthreads();
+    l = ((lds_w[0] + lds_w[1]) + lds_w[2]) + lds_w[3];
+    char* yr = a.y + s * a.y_nb2 + hq * a.y_nb1;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (64 * j >= static_cast<int>(a.D)) break;
+        __syncthreads();
+        lds_o[tid] = o[j];
+        __syncthreads();
+        const uint32_t d = lane + 64 * j;
+        if (wid == 0 && d < a.D) {
+            const float t = ((lds_o[lane] + lds_o[lane + 64]) + lds_o[lane + 128]) + lds_o[lane + 192];
+            Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
+        }
+    }
+}
+
+// ---- what runs where ------------------------------------------------------------
+
+struct AttnPlan {
+    bool tiles;            // k_attn_tiles, else k_attn_rows
+    int dp, kt;
+    uint32_t gc, ngr, H, W;
+    bool join;             // a key head's tiles may fall into several runs
+    size_t o_bytes, bytes; // of the workspace
+};
+
+// Everything but addresses, which the workspace's size may not depend on.
+AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
+    AttnPlan p{};
+    const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0;
+    const int64_t cap = tables->ne[0] * k->ne[1];
+    p.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    p.kt = (k->type == CBX_TYPE_F16 ? 32 : 16) * (kAttnThreads / 64);
+    p.ngr = static_cast<uint32_t>(cdiv(g, 16));
+    p.gc = static_cast<uint32_t>(cdiv(g, p.ngr));
+    p.H = static_cast<uint32_t>(hkv) * p.ngr;
+    const int64_t cap_tiles = std::max<int64_t>(1, cdiv(cap, p.kt));
+    const int64_t most = q->ne[2] * p.H * cap_tiles;
+    p.tiles = D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
+    if (!p.tiles) return p;
+    p.W = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(per_cu(p.dp)) * st->n_cu, most));
+    p.join = cap_tiles > 1;
+    if (p.join) {
+        p.o_bytes = static_cast<size_t>(cdiv(static_cast<int64_t>(p.W) * 2 * p.gc * D * 4, 16) * 16);
+        p.bytes = p.o_bytes + static_cast<size_t>(p.W) * 2 * p.gc * 8;
+    }
+    return p;
+}
+
+bool vector_rows(const cbx_tensor* t) {
+    if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
+    for (int i = 1; i < 4; i++) if (t->ne[i] > 1 && t->nb[i] % 16) return false;
+    return t->nb[1] < (size_t{1} << 26);
+}
+
+template <typename TQ, typename TC, int DP>
+void tiles_uni(bool uni, dim3 grid, size_t lds, hipStream_t s, const AttnArgs& a) {
+    if (uni) hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, true>), grid, dim3(kAttnThreads), lds, s, a);
+    else hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, false>), grid, dim3(kAttnThreads), lds, s, a);
+}
+
+template <typename TQ, typename TC>
+void launch_tiles(const AttnPlan& p, AttnArgs& a, hipStream_t s) {
+    const dim3 grid(p.W);
+    const size_t lds = static_cast<size_t>(kAttnThreads / 64) * p.gc * (p.dp + 4) * sizeof(float);
+    const bool uni = a.page % 16 == 0;
+    if (p.dp == 64) tiles_uni<TQ, TC, 64>(uni, grid, lds, s, a);
+    else if (p.dp == 128) tiles_uni<TQ, TC, 128>(uni, grid, lds, s, a);
+    else tiles_uni<TQ, TC, 256>(uni, grid, lds, s, a);
+    if (p.join) {
+        hipLaunchKernelGGL((k_attn_join<TQ, Core<TC, 64>::NK * (kAttnThreads / 64)>), dim3(a.n_seq * a.hq), dim3(kAttnThreads), 0,
+                           s, a);
+    }
+}
+
 }  // namespace
 
 size_t paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
-    (void)q; (void)k; (void)tables; (void)st;
-    return 0;
+    return attn_plan(q, k, tables, st).bytes;
 }
 
 int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
@@ -142,6 +812,25 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
     a.scale = c.scale;
     a.softcap = c.softcap;
     a.err = st->err_word;
+    const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
+    if (p.tiles && vector_rows(c.k) && vector_rows(c.v)) {
+        uint32_t l = 0;
+        while ((uint64_t{1} << l) < a.page) l++;
+        a.page_shift = 31 + l;
+        a.page_mul = static_cast<uint32_t>((uint64_t{1} << a.page_shift) / a.page + 1);
+        a.gc = p.gc;
+        a.ngr = p.ngr;
+        a.H = p.H;
+        a.W = p.W;
+        a.part_o = static_cast<float*>(c.ws);
+        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
+        const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
+        if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, a, s);
+        else if (t16) launch_tiles<uint16_t, float>(p, a, s);
+        else if (c16) launch_tiles<float, uint16_t>(p, a, s);
+        else launch_tiles<float, float>(p, a, s);
+        return check_launch("cbx_paged_attention");
+    }
     const dim3 grid(static_cast<unsigned>(c.q->ne[1] * c.q->ne[2])), block(kAttnThreads);
     const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
     if (t16 && c16) hipLaunchKernelGGL((k_attn_rows<uint16_t, uint16_t>), grid, block, 0, s, a);

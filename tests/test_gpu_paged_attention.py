@@ -273,6 +273,18 @@ def test_captured_step_follows_the_lengths(cbx):
             assert torch.equal(t, outs[0]), f"step {step}"
 
 
+@pytest.mark.parametrize("lens", [LENS, [1], [129], [4000, 1], [0, 0, 300]])
+def test_workspace_needs_no_preparation(cbx, lens):
+    """Scratch full of NaN and of ones: nothing in it is read before it is
+    written, also where there are fewer tiles than workgroups."""
+    q, kc, vc, tables = make(lens, 2, 2, 64, 16, F32, F16, 845)
+    need = cbx.paged_attention_workspace(q, kc, tables)
+    ref, bound = attention_ref(q, kc, vc, tables, lens, 0.125)
+    for fill in (float("nan"), 1.0):
+        ws = torch.full((need // 4 + 4,), fill, device="cuda")
+        assert_within(cbx.paged_attention(q, kc, vc, tables, ints(lens), 0.125, ws=ws), ref, bound, f"ws of {fill}")
+
+
 def test_same_call_same_bits(cbx):
     lens = [3000, 5, 1234, 0, 777]
     q, kc, vc, tables = make(lens, 2, 4, 128, 32, F16, F16, 850)
