@@ -1,17 +1,34 @@
 // k_logprob.hip -- log probabilities of given tokens, entropy and the largest
 // alternatives from a row of logits.
 //
-// With z_i = scale x_i - max scale x, T = sum exp(z_i):
+// With z_i = scale (x_i - max x), T = sum exp(z_i):
 //   log p_i = z_i - log T,  H = log T - (sum exp(z_i) z_i) / T
 // (both terms of H are >= 0: nothing cancels).  Order: 64-bit keys of the
 // logit's bits made monotone and the complement of its index, all distinct,
 // so that the alternatives do not depend on who finds them.
+//
+// Bound by the read of the logits, made once: a workgroup holds a chunk of a
+// row in registers (up to 16384 logits), reduces it to its maximum, T and
+// sum, and picks its alternatives.  A row of several chunks is joined by a
+// second kernel from the chunks' (maximum, T, sum) and their alternatives.
+//
+// The N largest without a sort: the 64 lanes' own maxima (over all waves)
+// are ranked; at least N keys are not below the N-th of them, and with
+// logits in any usual order few more (20 of 8194: some 24), so these are
+// collected in LDS and each is ranked among them.  When they do not fit
+// there (the largest all in a few lanes), or the row holds a NaN, the N
+// maxima are searched one after the other.
 #include "cbx_device.h"
 
 namespace cbx {
 namespace {
 
 constexpr int kLpThreads = 256;
+constexpr int kLpWaves = kLpThreads / 64;
+constexpr uint32_t kLpChunk = 16384;    // most logits of a workgroup: 64 a thread
+constexpr uint32_t kLpFew = 4096;       // of a chunk when there are few rows
+constexpr uint32_t kLpMost = 1024;      // keys collected in LDS
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct LpArgs {
     const char* x;
@@ -19,99 +36,337 @@ struct LpArgs {
     float *logp, *entropy;
     char *top_ids, *top_logp;
     int64_t x_nb1, ti_nb1, tl_nb1;
-    uint32_t V, rows;
+    uint32_t V, rows, chunk, chunks;
     int32_t n_top;
     float scale;
     uint32_t* err;
+    float4* sums;         // [rows][chunks]: maximum, T, sum, 1 when the chunk holds a NaN
+    uint64_t* keys;       // [rows][chunks][n_top]
 };
 
 // Larger logits have larger keys; NaN the largest, -0 as +0, of equal ones the first index.
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
+__device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-    const uint32_t o = x != x ? 0xfffffffeu : ((b & 0x80000000u) ? ~b : b | 0x80000000u);
-    return (static_cast<uint64_t>(o) << 32) | (0xffffffffu - i);
+    return x != x ? 0xfffffffeu : ((b & 0x80000000u) ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t i) {
+    return (static_cast<uint64_t>(order_of(x)) << 32) | (0xffffffffu - i);
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+__device__ __forceinline__ float logit_of(uint64_t k) {
+    const uint32_t o = static_cast<uint32_t>(k >> 32);
+    return o == 0xfffffffeu ? __builtin_nanf("") : __builtin_bit_cast(float, (o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+}
+
+__device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+struct LpShared {
+    float f[3][kLpWaves];
+    uint64_t lane[kLpWaves][64];
+    uint64_t kept[kLpMost];
+    uint64_t best[kLpWaves];
+    uint32_t count;
+};
+
+__device__ __forceinline__ float block_max(float v, float* lds) {
+    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) v = fmaxf(v, lds[w]);
+    return v;
+}
+__device__ __forceinline__ void block_sum2(float& a, float& b, float* la, float* lb) {
+    for (int d = 32; d > 0; d >>= 1) {
+        a += __shfl_xor(a, d);
+        b += __shfl_xor(b, d);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        la[threadIdx.x >> 6] = a;
+        lb[threadIdx.x >> 6] = b;
+    }
+    __syncthreads();
+    a = la[0];
+    b = lb[0];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) {
+        a += la[w];
+        b += lb[w];
+    }
+}
+
+// The n <= 64 largest of the block's keys (all, if fewer), put(rank, key) for
+// each by some thread.
+// best: the thread's largest key (0: none); each(f): f(key) for every key of
+// the thread that is not below `floor`, which it is told; all distinct.
+// search: one after the other from the start (then n of them at least).
+template <typename Each, typename Put>
+__device__ __forceinline__ void largest(LpShared& sh, int n, uint64_t best, bool search, Each each, Put put) {
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    uint32_t found = kLpMost + 1;
+    if (!search) {
+        sh.lane[wid][lane] = best;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        uint64_t mine = sh.lane[0][lane];
+#pragma unroll
+        for (int w = 1; w < kLpWaves; w++) mine = max64(mine, sh.lane[w][lane]);
+        // the n-th largest of the 64 (keys of 0, lanes without any, rank last)
+        uint32_t above = 0;
+#pragma unroll 8
+        for (int i = 0; i < 64; i++) {
+            const uint64_t other = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), i)) << 32 |
+                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), i));
+            above += other > mine || (other == mine && i < static_cast<int>(lane));
+        }
+        const uint64_t at = __ballot(above == static_cast<uint32_t>(n - 1));
+        const int src = __builtin_ctzll(at);
+        const uint64_t floor = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), src))) << 32 |
+                               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), src));
+        if (best >= floor) {
+            each(floor, [&](uint64_t k) {
+                const uint32_t i = atomicAdd(&sh.count, 1u);
+                if (i < kLpMost) sh.kept[i] = k;
+            });
+        }
+        __syncthreads();
+        found = sh.count;
+    }
+    if (found <= kLpMost) {
+        for (uint32_t i = tid; i < found; i += kLpThreads) {
+            const uint64_t k = sh.kept[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < found; j++) rank += sh.kept[j] > k;
+            if (rank < static_cast<uint32_t>(n)) put(rank, k);
+        }
+        return;
+    }
+    uint64_t last = ~uint64_t{0};
+    for (int r = 0; r < n; r++) {
+        uint64_t b = 0;
+        each(0, [&](uint64_t k) {
+            if (k < last && k > b) b = k;
+        });
+        for (int d = 32; d > 0; d >>= 1) b = max64(b, __shfl_xor(static_cast<unsigned long long>(b), d));
+        __syncthreads();
+        if (lane == 0) sh.best[wid] = b;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kLpWaves; w++) b = max64(b, sh.best[w]);
+        last = b;
+        if (tid == 0) put(r, b);
+    }
+}
+
+// A row's results from its maximum, T and sum (in powers of 2).
+struct RowSums {
+    float m, T, u;
+    bool nan;
+    __device__ __forceinline__ bool empty() const { return m == -INFINITY && !nan; }
+    __device__ __forceinline__ float log_p(float x, float scale) const {
+        if (nan || m == INFINITY) return __builtin_nanf("");
+        if (x == -INFINITY) return x;
+        return (x - m) * scale - logf(T);
+    }
+    __device__ __forceinline__ float entropy() const {
+        if (nan || m == INFINITY) return __builtin_nanf("");
+        return empty() ? 0.0f : logf(T) - kLn2 * (u / T);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void write_row(const LpArgs& a, uint32_t row, const RowSums& rs) {
+    if (threadIdx.x != 0) return;
+    if (a.logp) {
+        const int32_t id = a.ids[row];
+        float r = 0.0f;
+        if (id < 0 || static_cast<uint32_t>(id) >= a.V) {
+            atomicOr(a.err, DEV_ERR_ROW_INDEX);
+        } else {
+            r = rs.log_p(Elt<T>::load1(a.x + row * a.x_nb1 + static_cast<int64_t>(id) * Elt<T>::size), a.scale);
+        }
+        a.logp[row] = r;
+    }
+    if (a.entropy) a.entropy[row] = rs.entropy();
+}
+
+__device__ __forceinline__ void write_top(const LpArgs& a, uint32_t row, uint32_t rank, uint64_t k, const RowSums& rs) {
+    reinterpret_cast<int32_t*>(a.top_ids + row * a.ti_nb1)[rank] = static_cast<int32_t>(index_of(k));
+    reinterpret_cast<float*>(a.top_logp + row * a.tl_nb1)[rank] = rs.log_p(logit_of(k), a.scale);
+}
+
+// Four neighbouring logits at any element alignment.
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load4u(const float* p, float* v) {
+    const f4u t = *reinterpret_cast<const f4u*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = t[e];
+}
+__device__ __forceinline__ void load4u(const _Float16* p, float* v) {
+    const h4u t = *reinterpret_cast<const h4u*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = static_cast<float>(t[e]);
+}
+template <typename T> struct Raw { typedef float type; };
+template <> struct Raw<uint16_t> { typedef _Float16 type; };
+
+// A chunk of a row in registers: NV vectors of 4 a thread, thread t holding
+// logits 4 (256 j + t) + e of the chunk.
+template <typename T, int NV>
+__global__ __launch_bounds__(kLpThreads) void k_logprob(LpArgs a) {
+    __shared__ LpShared sh;
+    typedef typename Raw<T>::type R;
+    const uint32_t row = blockIdx.x / a.chunks, ch = blockIdx.x - row * a.chunks, tid = threadIdx.x;
+    const uint32_t i0 = ch * a.chunk, n = min(a.chunk, a.V - i0);
+    const R* x = reinterpret_cast<const R*>(a.x + row * a.x_nb1) + i0;
+    float v[NV][4];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const uint32_t i = 4 * (kLpThreads * j + tid);
+        if (i + 4 <= n) {
+            load4u(x + i, v[j]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[j][e] = i + e < n ? static_cast<float>(x[i + e]) : -INFINITY;
+        }
+    }
+    // the thread's first largest
+    float m = v[0][0];
+    uint32_t at = 0;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            nan |= v[j][e] != v[j][e];
+            if (v[j][e] > m) {
+                m = v[j][e];
+                at = 4 * j + e;
+            }
+        }
+    }
+    const uint32_t first = 4 * (kLpThreads * (at >> 2) + tid) + (at & 3);
+    const uint64_t best = first < n ? key_of(m, i0 + first) : 0;
+    RowSums rs;
+    rs.m = block_max(m, sh.f[0]);
+    const float sl = a.scale * kLog2e, off = rs.m == -INFINITY ? 0.0f : rs.m;
+    rs.T = rs.u = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float z = (v[j][e] - off) * sl, p = __builtin_amdgcn_exp2f(z);
+            rs.T += p;
+            rs.u += p > 0.0f ? p * z : 0.0f;
+        }
+    }
+    block_sum2(rs.T, rs.u, sh.f[1], sh.f[2]);
+    rs.nan = __syncthreads_or(nan);
+    if (a.chunks == 1) {
+        write_row<T>(a, row, rs);
+    } else if (tid == 0) {
+        a.sums[blockIdx.x] = make_float4(rs.m, rs.T, rs.u, rs.nan ? 1.0f : 0.0f);
+    }
+    if (a.n_top == 0) return;
+    auto each = [&](uint64_t floor, auto f) {
+        const uint32_t lo = static_cast<uint32_t>(floor >> 32);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t i = 4 * (kLpThreads * j + tid) + e, o = order_of(v[j][e]);
+                if (o >= lo && i < n) {
+                    const uint64_t k = static_cast<uint64_t>(o) << 32 | (0xffffffffu - (i0 + i));
+                    if (k >= floor) f(k);
+                }
+            }
+        }
+    };
+    uint64_t* out = a.keys + static_cast<uint64_t>(blockIdx.x) * a.n_top;
+    if (a.chunks > 1 && tid >= n && tid < static_cast<uint32_t>(a.n_top)) out[tid] = 0;   // a last chunk shorter than n_top
+    largest(sh, a.n_top, best, rs.nan, each, [&](uint32_t rank, uint64_t k) {
+        if (a.chunks == 1) write_top(a, row, rank, k, rs);
+        else out[rank] = k;
+    });
+}
+
+// A row of several chunks: their sums under the row's maximum, their
+// alternatives' best.
+template <typename T>
+__global__ __launch_bounds__(kLpThreads) void k_logprob_join(LpArgs a) {
+    __shared__ LpShared sh;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const float4* sums = a.sums + static_cast<uint64_t>(row) * a.chunks;
+    const uint64_t* keys = a.keys + static_cast<uint64_t>(row) * a.chunks * a.n_top;
+    const uint32_t n = a.chunks * a.n_top;
+    uint64_t best = 0;
+    for (uint32_t i = tid; i < n; i += kLpThreads) best = max64(best, keys[i]);
+    float m = -INFINITY;
+    bool nan = false;
+    for (uint32_t c = tid; c < a.chunks; c += kLpThreads) {
+        m = fmaxf(m, sums[c].x);
+        nan |= sums[c].w != 0.0f;
+    }
+    RowSums rs;
+    rs.m = block_max(m, sh.f[0]);
+    const float sl = a.scale * kLog2e;
+    rs.T = rs.u = 0.0f;
+    for (uint32_t c = tid; c < a.chunks; c += kLpThreads) {
+        const float4 s = sums[c];
+        if (s.x == -INFINITY) continue;
+        const float z = (s.x - rs.m) * sl, p = __builtin_amdgcn_exp2f(z);
+        rs.T = fmaf(s.y, p, rs.T);
+        if (p > 0.0f) rs.u = fmaf(p, fmaf(s.y, z, s.z), rs.u);
+    }
+    block_sum2(rs.T, rs.u, sh.f[1], sh.f[2]);
+    rs.nan = __syncthreads_or(nan);
+    write_row<T>(a, row, rs);
+    if (a.n_top == 0) return;
+    auto each = [&](uint64_t floor, auto f) {
+        for (uint32_t i = tid; i < n; i += kLpThreads) {
+            const uint64_t k = keys[i];
+            if (k >= floor) f(k);
+        }
+    };
+    largest(sh, a.n_top, best, false, each, [&](uint32_t rank, uint64_t k) { write_top(a, row, rank, k, rs); });
+}
+
+struct LpPlan {
+    uint32_t chunk, chunks;
+    size_t sums_bytes, bytes;
+};
+
+LpPlan lp_plan(const cbx_tensor* x, int n_top, const DeviceState* st) {
+    LpPlan p{};
+    const int64_t V = x->ne[0], rows = x->ne[1];
+    const int64_t most = rows * cdiv(V, kLpChunk) < st->n_cu ? kLpFew : kLpChunk;
+    const int64_t chunks = V <= kLpChunk ? 1 : cdiv(V, most);
+    p.chunk = static_cast<uint32_t>(chunks == 1 ? V : cdiv(cdiv(V, chunks), 4) * 4);
+    p.chunks = static_cast<uint32_t>(cdiv(V, p.chunk));
+    if (p.chunks > 1) {
+        p.sums_bytes = static_cast<size_t>(rows) * p.chunks * sizeof(float4);
+        p.bytes = p.sums_bytes + static_cast<size_t>(rows) * p.chunks * static_cast<size_t>(n_top) * sizeof(uint64_t);
+    }
+    return p;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kLpThreads) void k_logprob(LpArgs a) {
-    __shared__ float ldsf[kLpThreads / 64];
-    __shared__ unsigned long long lds64[kLpThreads / 64];
-    const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    const char* x = a.x + row * a.x_nb1;
-    auto at = [&](uint32_t i) { return Elt<T>::load1(x + static_cast<int64_t>(i) * Elt<T>::size); };
-    float m = -INFINITY;
-    for (uint32_t i = tid; i < a.V; i += kLpThreads) m = fmaxf(m, at(i));
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((tid & 63) == 0) ldsf[tid >> 6] = m;
-    __syncthreads();
-    m = ldsf[0];
-    for (int w = 1; w < kLpThreads / 64; w++) m = fmaxf(m, ldsf[w]);
-    __syncthreads();
-    const float ms = m * a.scale;
-    const bool none = m == -INFINITY;   // no logit above -inf (or NaN alone)
-    float total = 0.0f, u = 0.0f;
-    for (uint32_t i = tid; i < a.V; i += kLpThreads) {
-        const float v = at(i);
-        if (v == -INFINITY) continue;
-        const float z = v * a.scale - ms;
-        const float e = expf(z);
-        total += e;
-        u += e > 0.0f ? e * z : 0.0f;
-        if (e != e) u = e;
-    }
-    for (int pass = 0; pass < 2; pass++) {
-        float& t = pass ? u : total;
-        for (int d = 32; d > 0; d >>= 1) t += __shfl_xor(t, d);
-        if ((tid & 63) == 0) ldsf[tid >> 6] = t;
-        __syncthreads();
-        t = ldsf[0];
-        for (int w = 1; w < kLpThreads / 64; w++) t += ldsf[w];
-        __syncthreads();
-    }
-    const bool empty = none && total == 0.0f;
-    const float lse = empty ? 0.0f : logf(total);
-    auto log_p = [&](float v) { return v == -INFINITY && total == total ? v : v * a.scale - ms - lse; };
-    if (tid == 0) {
-        if (a.logp) {
-            const int32_t id = a.ids[row];
-            float r = 0.0f;
-            if (id < 0 || static_cast<uint32_t>(id) >= a.V) atomicOr(a.err, DEV_ERR_ROW_INDEX);
-            else r = log_p(at(static_cast<uint32_t>(id)));
-            a.logp[row] = r;
-        }
-        if (a.entropy) a.entropy[row] = empty ? 0.0f : lse - u / total;
-    }
-    uint64_t last = ~uint64_t{0};
-    for (int r = 0; r < a.n_top; r++) {
-        uint64_t best = 0;
-        for (uint32_t i = tid; i < a.V; i += kLpThreads) {
-            const uint64_t k = key_of(at(i), i);
-            if (k < last && k > best) best = k;
-        }
-        for (int d = 32; d > 0; d >>= 1) {
-            const uint64_t o = __shfl_xor(static_cast<unsigned long long>(best), d);
-            best = o > best ? o : best;
-        }
-        if ((tid & 63) == 0) lds64[tid >> 6] = best;
-        __syncthreads();
-        best = lds64[0];
-        for (int w = 1; w < kLpThreads / 64; w++) best = lds64[w] > best ? lds64[w] : best;
-        __syncthreads();
-        last = best;
-        if (tid == 0) {
-            const uint32_t i = 0xffffffffu - static_cast<uint32_t>(best);
-            reinterpret_cast<int32_t*>(a.top_ids + row * a.ti_nb1)[r] = static_cast<int32_t>(i);
-            reinterpret_cast<float*>(a.top_logp + row * a.tl_nb1)[r] = log_p(at(i));
-        }
-    }
+void launch_lp(const LpArgs& a, hipStream_t s) {
+    const dim3 grid(a.rows * a.chunks), block(kLpThreads);
+    const uint32_t nv = (a.chunk + 4 * kLpThreads - 1) / (4 * kLpThreads);
+    if (nv <= 1) hipLaunchKernelGGL((k_logprob<T, 1>), grid, block, 0, s, a);
+    else if (nv <= 2) hipLaunchKernelGGL((k_logprob<T, 2>), grid, block, 0, s, a);
+    else if (nv <= 4) hipLaunchKernelGGL((k_logprob<T, 4>), grid, block, 0, s, a);
+    else if (nv <= 9) hipLaunchKernelGGL((k_logprob<T, 9>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_logprob<T, 16>), grid, block, 0, s, a);
+    if (a.chunks > 1) hipLaunchKernelGGL((k_logprob_join<T>), dim3(a.rows), block, 0, s, a);
 }
 
 }  // namespace
 
-size_t token_log_probs_workspace(const cbx_tensor* x, int n_top, const DeviceState* st) {
-    (void)x; (void)n_top; (void)st;
-    return 0;
-}
+size_t token_log_probs_workspace(const cbx_tensor* x, int n_top, const DeviceState* st) { return lp_plan(x, n_top, st).bytes; }
 
 int launch_token_log_probs(const LogProbCall& c, DeviceState* st, hipStream_t s) {
     LpArgs a{};
@@ -129,9 +384,16 @@ int launch_token_log_probs(const LogProbCall& c, DeviceState* st, hipStream_t s)
     a.n_top = c.n_top;
     a.scale = c.scale;
     a.err = st->err_word;
-    const dim3 grid(a.rows), block(kLpThreads);
-    if (c.x->type == CBX_TYPE_F16) hipLaunchKernelGGL((k_logprob<uint16_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_logprob<float>), grid, block, 0, s, a);
+    const LpPlan p = lp_plan(c.x, c.n_top, st);
+    a.chunk = p.chunk;
+    a.chunks = p.chunks;
+    a.sums = static_cast<float4*>(c.ws);
+    a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(c.ws) + p.sums_bytes);
+    if (static_cast<uint64_t>(a.rows) * a.chunks * (a.n_top + 1) >= (uint64_t{1} << 31)) {
+        return set_error(CBX_ERR_UNSUPPORTED, "cbx_token_log_probs: too many logits");
+    }
+    if (c.x->type == CBX_TYPE_F16) launch_lp<uint16_t>(a, s);
+    else launch_lp<float>(a, s);
     return check_launch("cbx_token_log_probs");
 }
 

@@ -61,6 +61,14 @@ def test_sizes(cbx, dt, rows, vocab):
         check(cbx, x, ids, top, 1.0 if top else 0.7)
 
 
+def test_last_chunk_of_one(cbx):
+    """A row so long that its parts' rounding leaves one logit to the last."""
+    x = torch.randn(1, 4096 * 1500 + 1, device="cuda", generator=gen(2))
+    for last in (-50.0, 50.0):
+        x[0, -1] = last
+        check(cbx, x, torch.tensor([4096 * 1500], dtype=torch.int32, device="cuda"), 64)
+
+
 @pytest.mark.parametrize("vocab", [100, 8194, 40000])
 def test_equal_logits_go_by_number(cbx, vocab):
     """All equal; a few levels only; -0 and +0 equal."""
