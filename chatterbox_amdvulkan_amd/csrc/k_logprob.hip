@@ -13,11 +13,12 @@
 // second kernel from the chunks' (maximum, T, sum) and their alternatives.
 //
 // The N largest without a sort: the 64 lanes' own maxima (over all waves)
-// are ranked; at least N keys are not below the N-th of them, and with
+// are ranked; at least N logits are not below the N-th of them, and with
 // logits in any usual order few more (20 of 8194: some 24), so these are
 // collected in LDS and each is ranked among them.  When they do not fit
-// there (the largest all in a few lanes), or the row holds a NaN, the N
-// maxima are searched one after the other.
+// there (rows of equal or masked logits), the same is done with keys instead
+// of values; when those do not fit either (the largest all in a few lanes),
+// or the row holds a NaN, the N maxima are searched one after the other.
 #include "cbx_device.h"
 
 namespace cbx {
@@ -62,14 +63,37 @@ __device__ __forceinline__ uint64_t max64(uint64_t a, uint64_t b) { return a > b
 
 struct LpShared {
     float f[3][kLpWaves];
-    uint64_t lane[kLpWaves][64];
+    union {
+        float lanef[kLpWaves][64];
+        uint64_t lane[kLpWaves][64];
+    };
+    uint32_t above[kLpWaves][64];
     uint64_t kept[kLpMost];
     uint64_t best[kLpWaves];
-    uint32_t count;
+    uint32_t count[2];
 };
 
+// One float of the lane that a DPP control pairs this one with.
+template <int CTRL> __device__ __forceinline__ float dpp_f32(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_f32(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+// Over the 64 lanes, in the pairing order of wave_sum, the same in every lane.
+template <typename F> __device__ __forceinline__ float wave_f32(F f, float v) {
+    v = f(v, dpp_f32<0xB1>(v));
+    v = f(v, dpp_f32<0x4E>(v));
+    v = f(v, dpp_f32<0x141>(v));
+    v = f(v, dpp_f32<0x140>(v));
+    return f(f(lane_f32(v, 0), lane_f32(v, 16)), f(lane_f32(v, 32), lane_f32(v, 48)));
+}
+struct MaxOf { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct MinOf { __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); } };
+struct SumOf { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
+
 __device__ __forceinline__ float block_max(float v, float* lds) {
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    v = wave_f32(MaxOf(), v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lds[0];
@@ -78,10 +102,8 @@ __device__ __forceinline__ float block_max(float v, float* lds) {
     return v;
 }
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* la, float* lb) {
-    for (int d = 32; d > 0; d >>= 1) {
-        a += __shfl_xor(a, d);
-        b += __shfl_xor(b, d);
-    }
+    a = wave_f32(SumOf(), a);
+    b = wave_f32(SumOf(), b);
     if ((threadIdx.x & 63) == 0) {
         la[threadIdx.x >> 6] = a;
         lb[threadIdx.x >> 6] = b;
@@ -96,67 +118,89 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* la, float*
     }
 }
 
-// The n <= 64 largest of the block's keys (all, if fewer), put(rank, key) for
-// each by some thread.
-// best: the thread's largest key (0: none); each(f): f(key) for every key of
-// the thread that is not below `floor`, which it is told; all distinct.
-// search: one after the other from the start (then n of them at least).
-template <typename Each, typename Put>
-__device__ __forceinline__ void largest(LpShared& sh, int n, uint64_t best, bool search, Each each, Put put) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    uint32_t found = kLpMost + 1;
-    if (!search) {
-        sh.lane[wid][lane] = best;
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        uint64_t mine = sh.lane[0][lane];
+// put(rank, key) of the n largest of the keys collected in sh.kept.
+template <typename Put>
+__device__ __forceinline__ void rank_kept(const LpShared& sh, uint32_t found, int n, Put put) {
+    for (uint32_t i = threadIdx.x; i < found; i += kLpThreads) {
+        const uint64_t k = sh.kept[i];
+        uint32_t rank = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < found; j++) rank += sh.kept[j] > k;
+        if (rank < static_cast<uint32_t>(n)) put(rank, k);
+    }
+}
+
+// A value that at least n of the block's values are not below: the n-th
+// largest of the 64 lanes' maxima over the waves (m: the thread's maximum, no
+// NaN).  Each wave ranks the 64 against 16 of them.
+__device__ __forceinline__ float value_floor(LpShared& sh, int n, float m) {
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    sh.lanef[wid][lane] = m;
+    if (threadIdx.x == 0) sh.count[0] = sh.count[1] = 0;
+    __syncthreads();
+    float v = sh.lanef[0][lane];
 #pragma unroll
-        for (int w = 1; w < kLpWaves; w++) mine = max64(mine, sh.lane[w][lane]);
-        // the n-th largest of the 64 (keys of 0, lanes without any, rank last)
-        uint32_t above = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; i++) {
-            const uint64_t other = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), i)) << 32 |
-                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), i));
-            above += other > mine || (other == mine && i < static_cast<int>(lane));
-        }
-        const uint64_t at = __ballot(above == static_cast<uint32_t>(n - 1));
-        const int src = __builtin_ctzll(at);
-        const uint64_t floor = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), src))) << 32 |
-                               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), src));
-        if (best >= floor) {
-            each(floor, [&](uint64_t k) {
-                const uint32_t i = atomicAdd(&sh.count, 1u);
-                if (i < kLpMost) sh.kept[i] = k;
-            });
-        }
+    for (int w = 1; w < kLpWaves; w++) v = fmaxf(v, sh.lanef[w][lane]);
+    uint32_t above = 0;
+    if (n > 1) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) above += lane_f32(v, __builtin_amdgcn_readfirstlane(wid) * 16 + i) > v;
+        sh.above[wid][lane] = above;
         __syncthreads();
-        found = sh.count;
+        above = sh.above[0][lane];
+#pragma unroll
+        for (int w = 1; w < kLpWaves; w++) above += sh.above[w][lane];
+        return wave_f32(MinOf(), above < static_cast<uint32_t>(n) ? v : INFINITY);
     }
-    if (found <= kLpMost) {
-        for (uint32_t i = tid; i < found; i += kLpThreads) {
-            const uint64_t k = sh.kept[i];
-            uint32_t rank = 0;
-            for (uint32_t j = 0; j < found; j++) rank += sh.kept[j] > k;
-            if (rank < static_cast<uint32_t>(n)) put(rank, k);
-        }
-        return;
+    return wave_f32(MaxOf(), v);
+}
+
+// The same of 64-bit keys (best: the thread's largest, 0: none): the n-th
+// largest of the lanes' keys, those of 0 last.
+__device__ __forceinline__ uint64_t key_floor(LpShared& sh, int n, uint64_t best) {
+    const uint32_t lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    sh.lane[wid][lane] = best;
+    __syncthreads();
+    uint64_t mine = sh.lane[0][lane];
+#pragma unroll
+    for (int w = 1; w < kLpWaves; w++) mine = max64(mine, sh.lane[w][lane]);
+    auto of = [&](int i) {
+        return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine >> 32), i))) << 32 |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), i));
+    };
+    uint32_t above = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; i++) {
+        const uint64_t other = of(i);
+        above += other > mine || (other == mine && i < static_cast<int>(lane));
     }
+    return of(__builtin_ctzll(__ballot(above == static_cast<uint32_t>(n - 1))));
+}
+
+// The n largest keys one after the other.  each(f): f(key) for every key of
+// the thread, all of them distinct, n in the block at least.
+template <typename Each, typename Put>
+__device__ __forceinline__ void search_largest(LpShared& sh, int n, Each each, Put put) {
     uint64_t last = ~uint64_t{0};
     for (int r = 0; r < n; r++) {
         uint64_t b = 0;
-        each(0, [&](uint64_t k) {
+        each([&](uint64_t k) {
             if (k < last && k > b) b = k;
         });
         for (int d = 32; d > 0; d >>= 1) b = max64(b, __shfl_xor(static_cast<unsigned long long>(b), d));
         __syncthreads();
-        if (lane == 0) sh.best[wid] = b;
+        if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = b;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kLpWaves; w++) b = max64(b, sh.best[w]);
         last = b;
-        if (tid == 0) put(r, b);
+        if (threadIdx.x == 0) put(r, b);
     }
+}
+
+__device__ __forceinline__ void keep(LpShared& sh, int which, uint64_t k) {
+    const uint32_t i = atomicAdd(&sh.count[which], 1u);
+    if (i < kLpMost) sh.kept[i] = k;
 }
 
 // A row's results from its maximum, T and sum (in powers of 2).
@@ -215,7 +259,7 @@ template <> struct Raw<uint16_t> { typedef _Float16 type; };
 // A chunk of a row in registers: NV vectors of 4 a thread, thread t holding
 // logits 4 (256 j + t) + e of the chunk.
 template <typename T, int NV>
-__global__ __launch_bounds__(kLpThreads) void k_logprob(LpArgs a) {
+__global__ __launch_bounds__(kLpThreads, NV <= 4 ? 8 : NV <= 9 ? 6 : 4) void k_logprob(LpArgs a) {
     __shared__ LpShared sh;
     typedef typename Raw<T>::type R;
     const uint32_t row = blockIdx.x / a.chunks, ch = blockIdx.x - row * a.chunks, tid = threadIdx.x;
@@ -232,23 +276,13 @@ __global__ __launch_bounds__(kLpThreads) void k_logprob(LpArgs a) {
             for (int e = 0; e < 4; e++) v[j][e] = i + e < n ? static_cast<float>(x[i + e]) : -INFINITY;
         }
     }
-    // the thread's first largest
-    float m = v[0][0];
-    uint32_t at = 0;
-    bool nan = false;
+    float vm[NV];          // each vector's maximum
+    float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            nan |= v[j][e] != v[j][e];
-            if (v[j][e] > m) {
-                m = v[j][e];
-                at = 4 * j + e;
-            }
-        }
+        vm[j] = fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3]));
+        m = fmaxf(m, vm[j]);
     }
-    const uint32_t first = 4 * (kLpThreads * (at >> 2) + tid) + (at & 3);
-    const uint64_t best = first < n ? key_of(m, i0 + first) : 0;
     RowSums rs;
     rs.m = block_max(m, sh.f[0]);
     const float sl = a.scale * kLog2e, off = rs.m == -INFINITY ? 0.0f : rs.m;
@@ -259,37 +293,58 @@ __global__ __launch_bounds__(kLpThreads) void k_logprob(LpArgs a) {
         for (int e = 0; e < 4; e++) {
             const float z = (v[j][e] - off) * sl, p = __builtin_amdgcn_exp2f(z);
             rs.T += p;
-            rs.u += p > 0.0f ? p * z : 0.0f;
+            rs.u = fmaf(p, fmaxf(z, -200.0f), rs.u);   // exp2(-200) is 0: 0, not 0 * -inf
         }
     }
     block_sum2(rs.T, rs.u, sh.f[1], sh.f[2]);
-    rs.nan = __syncthreads_or(nan);
+    rs.nan = rs.T != rs.T;
     if (a.chunks == 1) {
         write_row<T>(a, row, rs);
     } else if (tid == 0) {
         a.sums[blockIdx.x] = make_float4(rs.m, rs.T, rs.u, rs.nan ? 1.0f : 0.0f);
     }
     if (a.n_top == 0) return;
-    auto each = [&](uint64_t floor, auto f) {
-        const uint32_t lo = static_cast<uint32_t>(floor >> 32);
+    uint64_t* out = a.keys + static_cast<uint64_t>(blockIdx.x) * a.n_top;
+    if (a.chunks > 1 && tid >= n && tid < static_cast<uint32_t>(a.n_top)) out[tid] = 0;   // a last chunk shorter than n_top
+    auto put = [&](uint32_t rank, uint64_t k) {
+        if (a.chunks == 1) write_top(a, row, rank, k, rs);
+        else out[rank] = k;
+    };
+    auto index = [&](int j, int e) { return 4 * (kLpThreads * j + tid) + e; };
+    // the rare ways read the row again: keys of every register would be held for them
+    auto each = [&](auto f) {
+        for (uint32_t i = tid; i < n; i += kLpThreads) f(key_of(static_cast<float>(x[i]), i0 + i));
+    };
+    if (rs.nan) {
+        search_largest(sh, min(a.n_top, static_cast<int>(n)), each, put);
+        return;
+    }
+    const float fl = value_floor(sh, a.n_top, m);
+    if (m >= fl) {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
+            if (vm[j] >= fl) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t i = 4 * (kLpThreads * j + tid) + e, o = order_of(v[j][e]);
-                if (o >= lo && i < n) {
-                    const uint64_t k = static_cast<uint64_t>(o) << 32 | (0xffffffffu - (i0 + i));
-                    if (k >= floor) f(k);
+                for (int e = 0; e < 4; e++) {
+                    if (v[j][e] >= fl && index(j, e) < n) keep(sh, 0, key_of(v[j][e], i0 + index(j, e)));
                 }
             }
         }
-    };
-    uint64_t* out = a.keys + static_cast<uint64_t>(blockIdx.x) * a.n_top;
-    if (a.chunks > 1 && tid >= n && tid < static_cast<uint32_t>(a.n_top)) out[tid] = 0;   // a last chunk shorter than n_top
-    largest(sh, a.n_top, best, rs.nan, each, [&](uint32_t rank, uint64_t k) {
-        if (a.chunks == 1) write_top(a, row, rank, k, rs);
-        else out[rank] = k;
-    });
+    }
+    __syncthreads();
+    uint32_t found = sh.count[0];
+    if (found > kLpMost) {      // too many that are equal: by key
+        uint64_t best = 0;
+        each([&](uint64_t k) { best = max64(best, k); });
+        const uint64_t kfl = key_floor(sh, a.n_top, best);
+        each([&](uint64_t k) {
+            if (k >= kfl) keep(sh, 1, k);
+        });
+        __syncthreads();
+        found = sh.count[1];
+    }
+    if (found <= kLpMost) rank_kept(sh, found, a.n_top, put);
+    else search_largest(sh, min(a.n_top, static_cast<int>(n)), each, put);
 }
 
 // A row of several chunks: their sums under the row's maximum, their
@@ -324,13 +379,19 @@ __global__ __launch_bounds__(kLpThreads) void k_logprob_join(LpArgs a) {
     rs.nan = __syncthreads_or(nan);
     write_row<T>(a, row, rs);
     if (a.n_top == 0) return;
-    auto each = [&](uint64_t floor, auto f) {
-        for (uint32_t i = tid; i < n; i += kLpThreads) {
-            const uint64_t k = keys[i];
-            if (k >= floor) f(k);
-        }
+    auto each = [&](auto f) {
+        for (uint32_t i = tid; i < n; i += kLpThreads) f(keys[i]);
     };
-    largest(sh, a.n_top, best, false, each, [&](uint32_t rank, uint64_t k) { write_top(a, row, rank, k, rs); });
+    if (tid == 0) sh.count[1] = 0;
+    const uint64_t fl = key_floor(sh, a.n_top, best);
+    each([&](uint64_t k) {
+        if (k >= fl) keep(sh, 1, k);
+    });
+    __syncthreads();
+    const uint32_t found = sh.count[1];
+    auto put = [&](uint32_t rank, uint64_t k) { write_top(a, row, rank, k, rs); };
+    if (found <= kLpMost) rank_kept(sh, found, a.n_top, put);
+    else search_largest(sh, a.n_top, each, put);
 }
 
 struct LpPlan {
