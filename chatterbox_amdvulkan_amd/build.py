@@ -1,4 +1,5 @@
-"""Builds libcbxops.so (gfx950) in-tree with hipcc.
+"""Builds libcbxops.so (gfx950) in-tree with hipcc, and _cbxtorch (the Python
+front end's calls on torch tensors, host code over the C ABI) with g++.
 
     python -m chatterbox_amdvulkan_amd.build [--jobs N] [--verbose]
 
@@ -23,6 +24,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libcbxops.so")
+TORCH_EXT = os.path.join(PKG, "_cbxtorch.so")
 
 SOURCES = [
     "cbx_api.cpp",
@@ -85,8 +87,32 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_torch_ext(verbose: bool) -> None:
+    """_cbxtorch.so: a CPython module linked to the libcbxops.so beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = TORCH_EXT + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           os.path.join(CSRC, "cbx_torch.cpp"), "-o", tmp]
+    cmd += ["-isystem" + p for p in cpp_extension.include_paths()] + ["-I" + sysconfig.get_paths()["include"]]
+    cmd += ["-L" + PKG, "-l:libcbxops.so", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch_python", "-ltorch_cpu", "-lc10",
+            "-Wl,-rpath," + lib]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: cbx_torch.cpp\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, TORCH_EXT)
+
+
 def build(jobs: int = 0, verbose: bool = False) -> str:
-    """Compiles every source for gfx950 and links libcbxops.so; returns its path."""
+    """Compiles every source for gfx950 and links libcbxops.so, then the torch
+    module over it; returns the library's path."""
     os.makedirs(BUILD, exist_ok=True)
     jobs = jobs or min(len(SOURCES), os.cpu_count() or 4, 8)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
@@ -99,6 +125,7 @@ def build(jobs: int = 0, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_torch_ext(verbose)
     return LIB
 
 

@@ -868,37 +868,45 @@ def snake(x, alpha, alpha_inv, out=None):
 
 # ---- decoding many streams over a paged key-value cache ------------------------
 
-def _together(*tensors) -> torch.device:
-    """The one device all of them live on, which the call is then made on."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if dev is None:
-            _ready(t)
-            dev = t.device
-        elif t.device != dev:
-            raise CbxError(ERR_INVALID_ARG, f"tensors on {dev} and {t.device}")
-    return dev
+# These calls go through _cbxtorch, which fills their descriptors and
+# allocates their outputs in C++ (attention over 9 tensors: 16 us of host time
+# when each descriptor was filled here).
+_native = None
 
 
-class _on:
-    """Makes the tensors' device the current one for a call (a no-op when it is)."""
+def _load_native():
+    """The _cbxtorch module (no GPU needed)."""
+    global _native
+    if _native is None:
+        load()
+        try:
+            from . import _cbxtorch
+        except ImportError as e:
+            raise CbxError(ERR_UNSUPPORTED, f"_cbxtorch is not built ({e}); run python -m chatterbox_amdvulkan_amd.build")
+        _cbxtorch.setup(CbxError)
+        _native = _cbxtorch
+    return _native
 
-    def __init__(self, dev: torch.device):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _opt(t):
-    return _ref(desc(t)) if t is not None else None
+def _call(name: str, *args):
+    """One _cbxtorch function on the tensors' device and that device's current
+    stream, the library set up for it first."""
+    fn = getattr(_native or _load_native(), name)
+    while True:
+        dev, stream = -1, 0
+        if torch.cuda.is_initialized():
+            dev = torch.cuda.current_device() if _raw_device is None else _raw_device()
+            stream = torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(dev)
+        r = fn(*args, dev, stream)
+        if r.__class__ is not int:
+            return r
+        if r == 1:
+            if dev in _initialised:
+                raise CbxError(ERR_NOT_INITIALIZED, f"device {dev} was shut down")
+            init(dev)
+        else:
+            with torch.cuda.device(-1000 - r):
+                return _call(name, *args)
 
 
 def paged_append(n_past, n_new, free_pages, n_free, block_tables, page_size, n_slots, out=None):
@@ -910,35 +918,16 @@ def paged_append(n_past, n_new, free_pages, n_free, block_tables, page_size, n_s
     [n_seq + 1], and each token's slot and position [n_slots] (-1 and 0 past
     the last token).  A request that does not fit keeps its length and gets
     slots of -1.  out: the five tensors to write to."""
-    dev = _together(n_past, n_new, free_pages, n_free, block_tables)
-    if out is None:
-        n = n_past.shape[0]
-        buf = torch.empty(2 * n + 2 + 2 * n_slots, dtype=torch.int32, device=dev)
-        out = buf.split([n, 1, n + 1, n_slots, n_slots])
-    lens, left, start, slots, pos = out
-    _together(n_past, *out)
-    with _on(dev):
-        _check(load().cbx_paged_append(_ref(desc(n_past)), _ref(desc(n_new)), _ref(desc(free_pages)),
-                                       _ref(desc(n_free)), _ref(desc(block_tables)), page_size, _ref(desc(lens)),
-                                       _ref(desc(left)), _ref(desc(start)), _ref(desc(slots)), _ref(desc(pos)),
-                                       _stream()))
-    return lens, left, start, slots, pos
+    a, b, c, d, e = out or (None,) * 5
+    return _call("paged_append", n_past, n_new, free_pages, n_free, block_tables, page_size, n_slots, a, b, c, d, e)
 
 
 def paged_release(seq_lens, release, block_tables, page_size, free_pages, n_free, out=None):
     """Pushes the pages of the requests with release[s] != 0 back on the stack
     (block_tables and free_pages in place); returns (seq_lens, n_free), the
     released requests' lengths 0."""
-    dev = _together(seq_lens, release, block_tables, free_pages, n_free)
-    if out is None:
-        out = torch.empty_like(seq_lens), torch.empty_like(n_free)
-    lens, left = out
-    _together(seq_lens, lens, left)
-    with _on(dev):
-        _check(load().cbx_paged_release(_ref(desc(seq_lens)), _ref(desc(release)), _ref(desc(block_tables)),
-                                        page_size, _ref(desc(free_pages)), _ref(desc(n_free)), _ref(desc(lens)),
-                                        _ref(desc(left)), _stream()))
-    return lens, left
+    a, b = out or (None, None)
+    return _call("paged_release", seq_lens, release, block_tables, page_size, free_pages, n_free, a, b)
 
 
 def paged_store(k, v, slots, k_cache, v_cache):
@@ -946,56 +935,27 @@ def paged_store(k, v, slots, k_cache, v_cache):
     caches [n_pages, n_head_kv, page_size, head_dim] (any strides, so a
     permuted [n_pages, page_size, n_head_kv, head_dim] too), rounded to the
     caches' type; negative slots are skipped."""
-    with _on(_together(k, v, slots, k_cache, v_cache)):
-        _check(load().cbx_paged_store(_ref(desc(k)), _ref(desc(v)), _ref(desc(slots)), _ref(desc(k_cache)),
-                                      _ref(desc(v_cache)), _stream()))
+    _call("paged_store", k, v, slots, k_cache, v_cache)
 
 
 def qk_norm_rope(q, k, gq, gk, eps, pos, cache: RopeCache, out_q=None, out_k=None):
     """RMS norm of each head of q [n_tok, n_head, head_dim] and k [n_tok,
     n_head_kv, head_dim] (gq, gk [head_dim] or None), then the rotation at
     pos[token], in one pass.  Returns (q, k)."""
-    dev = _together(q, k, gq, gk, pos, out_q, out_k)
-    if out_q is None:
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if out_k is None:
-        out_k = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    with _on(dev):
-        _check(load().cbx_qk_norm_rope(_ref(desc(q)), _opt(gq), _ref(desc(k)), _opt(gk), eps, _ref(desc(pos)),
-                                       cache.handle, _ref(desc(out_q)), _ref(desc(out_k)), _stream()))
-    return out_q, out_k
+    return _call("qk_norm_rope", q, k, gq, gk, eps, pos, cache.handle.value or 0, out_q, out_k)
 
 
 def qk_norm_rope_store(q, k, v, gq, gk, eps, pos, cache: RopeCache, slots, k_cache, v_cache, out_q=None):
     """qk_norm_rope with the keys, and v beside them, written into the caches
     as paged_store does.  Returns q."""
-    dev = _together(q, k, v, gq, gk, pos, slots, k_cache, v_cache, out_q)
-    if out_q is None:
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    with _on(dev):
-        _check(load().cbx_qk_norm_rope_store(_ref(desc(q)), _opt(gq), _ref(desc(k)), _opt(gk), _ref(desc(v)), eps,
-                                             _ref(desc(pos)), cache.handle, _ref(desc(slots)), _ref(desc(out_q)),
-                                             _ref(desc(k_cache)), _ref(desc(v_cache)), _stream()))
-    return out_q
-
-
-def _workspace(nbytes: int, ws, dev):
-    """(address, bytes, keeper) of a call's scratch: the caller's tensor, or
-    one of torch's allocator on the current stream (under capture: of the
-    graph's own pool)."""
-    if ws is None and nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    if ws is None:
-        return None, 0, None
-    if ws.device != dev or not ws.is_contiguous():
-        raise CbxError(ERR_INVALID_ARG, "ws must be a contiguous tensor on the call's device")
-    return ctypes.c_void_p(ws.data_ptr()), ws.numel() * ws.element_size(), ws
+    return _call("qk_norm_rope_store", q, k, v, gq, gk, eps, pos, cache.handle.value or 0, slots, k_cache, v_cache, out_q)
 
 
 def paged_attention_workspace(q, k_cache, block_tables) -> int:
     """Bytes of scratch that paged_attention needs for these shapes."""
+    _ready(q)
     n = ctypes.c_size_t(0)
-    with _on(_together(q, k_cache, block_tables)):
+    with torch.cuda.device(q.device):
         _check(load().cbx_paged_attention_workspace(_ref(desc(q)), _ref(desc(k_cache)), _ref(desc(block_tables)),
                                                     ctypes.byref(n)))
     return n.value
@@ -1007,26 +967,16 @@ def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap=
     n_head_kv, page_size, head_dim]; softcap > 0: scores softcap * tanh(s /
     softcap); window > 0: the last `window` keys only.  ws: scratch of
     paged_attention_workspace bytes that no other call uses meanwhile
-    (default: taken from torch for this call)."""
-    dev = _together(q, k_cache, v_cache, block_tables, seq_lens, out)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    with _on(dev):
-        L = load()
-        dq, dk, dt = desc(q), desc(k_cache), desc(block_tables)
-        n = ctypes.c_size_t(0)
-        if ws is None:
-            _check(L.cbx_paged_attention_workspace(_ref(dq), _ref(dk), _ref(dt), ctypes.byref(n)))
-        p, size, keep = _workspace(n.value, ws, dev)
-        _check(L.cbx_paged_attention(_ref(dq), _ref(dk), _ref(desc(v_cache)), _ref(dt), _ref(desc(seq_lens)), scale,
-                                     softcap, window, _ref(desc(out)), p, size, _stream()))
-    return out
+    (default: taken from torch for this call; under capture, of the graph's
+    own pool)."""
+    return _call("paged_attention", q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window, out, ws)
 
 
 def token_log_probs_workspace(logits, top_n) -> int:
     """Bytes of scratch that token_log_probs needs for these shapes."""
+    _ready(logits)
     n = ctypes.c_size_t(0)
-    with _on(_together(logits)):
+    with torch.cuda.device(logits.device):
         _check(load().cbx_token_log_probs_workspace(_ref(desc(logits)), top_n, ctypes.byref(n)))
     return n.value
 
@@ -1035,25 +985,9 @@ def token_log_probs(logits, ids=None, top_n=0, scale=1.0, entropy=True, ws=None)
     """(logp, entropy, top_ids, top_logp) of logits [n_tok, n_vocab] under
     softmax(scale * logits): the log probability of ids[t] (None without
     ids), the entropy (None when not asked for), and the top_n largest logits'
-    tokens and log probabilities [n_tok, top_n], equal logits by number."""
-    dev = _together(logits, ids)
-    n = logits.shape[0]
-    f32 = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)  # noqa: E731
-    logp = f32(n) if ids is not None else None
-    ent = f32(n) if entropy else None
-    top_logp = f32(n, top_n)
-    top_ids = torch.empty((n, top_n), dtype=torch.int32, device=dev)
-    asked = top_n != 0
-    with _on(dev):
-        L = load()
-        dx = desc(logits)
-        need = ctypes.c_size_t(0)
-        if ws is None:
-            _check(L.cbx_token_log_probs_workspace(_ref(dx), top_n, ctypes.byref(need)))
-        p, size, keep = _workspace(need.value, ws, dev)
-        _check(L.cbx_token_log_probs(_ref(dx), _opt(ids), scale, _opt(logp), _opt(ent), _opt(top_ids if asked else None),
-                                     _opt(top_logp if asked else None), p, size, _stream()))
-    return logp, ent, top_ids, top_logp
+    tokens and log probabilities [n_tok, top_n], equal logits by number.  ws as
+    for paged_attention."""
+    return _call("token_log_probs", logits, ids, top_n, scale, entropy, ws)
 
 
 # ---- one launch for several independent ops -----------------------------------
