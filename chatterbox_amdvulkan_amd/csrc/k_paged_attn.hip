@@ -42,9 +42,11 @@ struct AttnArgs {
     // k_attn_tiles and k_attn_join
     uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
     uint32_t gc, ngr, H;             // heads a run holds (<= 16), runs of heads a group, hkv * ngr
-    uint32_t W;                      // workgroups
+    uint32_t W;                      // runs; 0: a run a request and key head, none of them split
     float* part_o;                   // [W][2][gc][D]
     float2* part_ml;                 // [W][2][gc]
+    uint4* split;                    // [W]: request, first query head, heads and parts of the key head that begins
+                                     // in the run and ends in a later one; no parts: none does
 };
 
 __device__ __forceinline__ float wave_sum_f32(float v) {
@@ -135,9 +137,55 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
 
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef const int32_t __attribute__((address_space(4))) const_i32;
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u2w __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u4w __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u3v __attribute__((ext_vector_type(3)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+// Four neighbouring elements at any element alignment.
+__device__ __forceinline__ void load4u(const char* p, float* v, float) {
+    const f4u t = *reinterpret_cast<const f4u*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = t[j];
+}
+__device__ __forceinline__ void load4u(const char* p, float* v, uint16_t) {
+    const h4u t = *reinterpret_cast<const h4u*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = static_cast<float>(t[j]);
+}
+
+// Where a lane reads a row: behind a base of the wave's at the lane's offset
+// (a buffer load, whose base and step stay in scalar registers), or behind a
+// pointer of its own.
+struct WaveRows {
+    __amdgpu_buffer_rsrc_t base;
+    uint32_t off, step;     // the lane's, the wave's
+    __device__ __forceinline__ WaveRows(const char* p, uint32_t o, uint32_t s)
+        : base(__builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, -1, 0x00027000)), off(o), step(s) {}
+    __device__ __forceinline__ u4v load16(uint32_t o) const {
+        return __builtin_amdgcn_raw_buffer_load_b128(base, static_cast<int>(off + o), static_cast<int>(step), 0);
+    }
+    __device__ __forceinline__ u3v load12(uint32_t o) const {
+        return __builtin_amdgcn_raw_buffer_load_b96(base, static_cast<int>(off + o), static_cast<int>(step), 0);
+    }
+    __device__ __forceinline__ u2v load8(uint32_t o) const {
+        return __builtin_amdgcn_raw_buffer_load_b64(base, static_cast<int>(off + o), static_cast<int>(step), 0);
+    }
+};
+struct LaneRow {
+    const char* p;
+    __device__ __forceinline__ u4v load16(uint32_t o) const { return *reinterpret_cast<const u4w*>(p + o); }
+    __device__ __forceinline__ u3v load12(uint32_t o) const {
+        const u2v t = load8(o);
+        return u3v{t.x, t.y, *reinterpret_cast<const uint32_t*>(p + o + 8)};
+    }
+    __device__ __forceinline__ u2v load8(uint32_t o) const { return *reinterpret_cast<const u2w*>(p + o); }
+};
 
 __device__ __forceinline__ uint32_t page_of(const AttnArgs& a, uint32_t key) {
     return static_cast<uint32_t>((static_cast<uint64_t>(key) * a.page_mul) >> a.page_shift);
@@ -162,6 +210,20 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     return r;
 }
 
+// Inclusive prefix sum over the wave: within rows of 16 lanes by shifts, then
+// each row's last to the rows behind it.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t x) {
+    return x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x = dpp_add<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
+    x = dpp_add<0x112, 0xf>(x);
+    x = dpp_add<0x114, 0xf>(x);
+    x = dpp_add<0x118, 0xf>(x);
+    x = dpp_add<0x142, 0xa>(x);   // row_bcast 15 to rows 1 and 3
+    return dpp_add<0x143, 0xc>(x);   // row_bcast 31 to rows 2 and 3
+}
+
 // The exclusive prefix over the requests of their tiles, as every workgroup
 // needs it: each thread sums c neighbouring requests.  *total the sum.
 template <int KT>
@@ -169,12 +231,7 @@ __device__ __forceinline__ uint32_t tiles_before(const AttnArgs& a, uint32_t c, 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     uint32_t sum = 0;
     for (uint32_t s = tid * c; s < min(a.n_seq, (tid + 1) * c); s++) sum += span_of<KT>(a, s).tiles;
-    uint32_t x = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t u = __shfl_up(x, d);
-        if (lane >= static_cast<uint32_t>(d)) x += u;
-    }
+    const uint32_t x = wave_scan(sum);
     if (lane == 63) lds[wid] = x;
     __syncthreads();
     uint32_t before = 0, all = 0;
@@ -188,14 +245,42 @@ __device__ __forceinline__ uint32_t tiles_before(const AttnArgs& a, uint32_t c, 
     return before + x - sum;
 }
 
-// First tile of workgroup w's run of the call's T tiles, W <= T.
-__device__ __forceinline__ uint32_t run_start(uint32_t w, uint32_t W, uint32_t T) {
-    return static_cast<uint32_t>(static_cast<uint64_t>(w) * T / W);
+// T tiles in W <= T runs, the first T % W of them a tile longer.
+struct Runs {
+    uint32_t q, r;
+    __device__ __forceinline__ Runs(uint32_t T, uint32_t W) : q(T / W), r(T - T / W * W) {}
+    __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * q + min(w, r); }
+    __device__ __forceinline__ uint32_t of(uint32_t t) const {     // the run that holds tile t
+        const uint32_t longer = r * (q + 1);
+        return t < longer ? t / (q + 1) : r + (t - longer) / q;
+    }
+};
+
+// N dwords (a multiple of 4, or 2, 3 or 6) of a row from byte offset o on.
+template <int N, typename Row> __device__ __forceinline__ void load_dwords(const Row& r, uint32_t o, uint32_t (&v)[N]) {
+    if constexpr (N == 3) {
+        const u3v t = r.load12(o);
+        v[0] = t.x;
+        v[1] = t.y;
+        v[2] = t.z;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i + 4 <= N; i += 4) {
+        const u4v t = r.load16(o + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[i + j] = t[j];
+    }
+    if constexpr (N % 4 == 2) {
+        const u2v t = r.load8(o + 4 * (N - 2));
+        v[N - 2] = t.x;
+        v[N - 1] = t.y;
+    }
 }
-// The workgroup whose run holds tile t: the last w with run_start(w) <= t.
-__device__ __forceinline__ uint32_t run_of(uint32_t t, uint32_t W, uint32_t T) {
-    return static_cast<uint32_t>(((static_cast<uint64_t>(t) + 1) * W - 1) / T);
-}
+
+// The first of the PER dims that row m of O^T stands for.  The rows past D's
+// end stand for its last dims again, and make the same sums of them.
+template <int PER> __device__ __forceinline__ uint32_t value_dim(uint32_t m, uint32_t D) { return min(m * PER, D - PER); }
 
 // A matrix core's view of NK keys and 16 heads.  S^T = K Q^T: the A operand's
 // row is the key (lane % 16), the B operand's column the head (lane % 16),
@@ -203,9 +288,9 @@ __device__ __forceinline__ uint32_t run_of(uint32_t t, uint32_t W, uint32_t T) {
 // head lane % 16 and keys 4 (lane / 16) + r.  O^T = V^T P^T: the B operand is
 // then what the lane already holds (the sum over the keys may take them in
 // any order, as long as V's rows come in the same one), the A operand's row
-// m is dim m * DP/16 + d of product d: a lane reads DP/16 neighbouring dims of
-// its keys.  The result's lane has head lane % 16 and dims
-// (4 (lane / 16) + r) * DP/16 + d.
+// m is dim value_dim(m) + d of product d: a lane reads DP/16 neighbouring dims
+// of its keys.  The result's lane has head lane % 16 and dims
+// value_dim(4 (lane / 16) + r) + d.
 template <typename TC, int DP> struct Core;
 
 // f16 pages: 16x16x32 products, f32 sums.  An f32 query is scaled by a power
@@ -214,7 +299,7 @@ template <typename TC, int DP> struct Core;
 // of the largest).
 template <int DP> struct Core<uint16_t, DP> {
     static constexpr int NK = 32, NH = 2, NE = 8;   // keys a step, halves of 16, keys whose values a lane holds
-    static constexpr int CD = DP / 32;
+    static constexpr int CD = DP / 32, PER = DP / 16;
     h8v qh[CD], ql[CD], kf[NH][CD];
     uint32_t vr[NE][CD];
     f4v acc[DP / 16];
@@ -251,12 +336,17 @@ template <int DP> struct Core<uint16_t, DP> {
     static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 32 * c + 8 * grp; }
     static constexpr int QC = CD, QN = 8;
 
-    __device__ __forceinline__ void load_k(int h, const char* p, uint32_t grp, uint32_t D) {
+    // byte offsets of the lane's dims in a key's row (of dims past D: the
+    // row's first) and in a value's
+    uint32_t ko[CD], vo;
+    __device__ __forceinline__ void offsets(uint32_t n, uint32_t grp, uint32_t D) {
 #pragma unroll
-        for (int c = 0; c < CD; c++) {
-            const uint32_t d = dim_of(c, grp);
-            kf[h][c] = *reinterpret_cast<const h8v*>(p + (D == DP || d < D ? d * 2 : 0));
-        }
+        for (int c = 0; c < CD; c++) ko[c] = dim_of(c, grp) < D ? 2 * dim_of(c, grp) : 0;
+        vo = 2 * value_dim<PER>(n, D);
+    }
+    template <typename Row> __device__ __forceinline__ void load_k(int h, const Row& r) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) kf[h][c] = __builtin_bit_cast(h8v, r.load16(ko[c]));
     }
     __device__ __forceinline__ void trim_k(uint32_t grp, uint32_t D) {   // dims past D: 0
 #pragma unroll
@@ -267,23 +357,7 @@ template <int DP> struct Core<uint16_t, DP> {
             }
         }
     }
-    __device__ __forceinline__ void load_v(int e, const char* p, uint32_t n, uint32_t D) {
-        const uint32_t d = n * (DP / 16);
-        if constexpr (CD == 2) {
-            const u2v t = *reinterpret_cast<const u2v*>(p + (D == DP || d < D ? d * 2 : 0));
-            vr[e][0] = t.x;
-            vr[e][1] = t.y;
-        } else {
-#pragma unroll
-            for (int c = 0; c < CD; c += 4) {
-                const u4v t = *reinterpret_cast<const u4v*>(p + (D == DP || d + 2 * c < D ? (d + 2 * c) * 2 : 0));
-                vr[e][c] = t.x;
-                vr[e][c + 1] = t.y;
-                vr[e][c + 2] = t.z;
-                vr[e][c + 3] = t.w;
-            }
-        }
-    }
+    template <typename Row> __device__ __forceinline__ void load_v(int e, const Row& r) { load_dwords<CD>(r, vo, vr[e]); }
     __device__ __forceinline__ void drop_v(int e) {
 #pragma unroll
         for (int c = 0; c < CD; c++) vr[e][c] = 0;
@@ -335,8 +409,9 @@ template <int DP> struct Core<uint16_t, DP> {
 // f32 pages: 16x16x4 products of f32.
 template <int DP> struct Core<float, DP> {
     static constexpr int NK = 16, NH = 1, NE = 4;
-    static constexpr int CD = DP / 16, CV = DP / 64;
-    f4v qf[CD], kf[NH][CD], vr[NE][CV];
+    static constexpr int CD = DP / 16, PER = DP / 16;
+    f4v qf[CD], kf[NH][CD];
+    uint32_t vr[NE][PER];
     f4v acc[DP / 16];
     float qmul;
     static constexpr int QC = CD, QN = 4;
@@ -346,12 +421,15 @@ template <int DP> struct Core<float, DP> {
         for (int i = 0; i < CD * 4; i++) qf[i / 4][i % 4] = x[i];
     }
     static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 16 * c + 4 * grp; }
-    __device__ __forceinline__ void load_k(int h, const char* p, uint32_t grp, uint32_t D) {
+    uint32_t ko[CD], vo;
+    __device__ __forceinline__ void offsets(uint32_t n, uint32_t grp, uint32_t D) {
 #pragma unroll
-        for (int c = 0; c < CD; c++) {
-            const uint32_t d = dim_of(c, grp);
-            kf[h][c] = *reinterpret_cast<const f4v*>(p + (D == DP || d < D ? d * 4 : 0));
-        }
+        for (int c = 0; c < CD; c++) ko[c] = dim_of(c, grp) < D ? 4 * dim_of(c, grp) : 0;
+        vo = 4 * value_dim<PER>(n, D);
+    }
+    template <typename Row> __device__ __forceinline__ void load_k(int h, const Row& r) {
+#pragma unroll
+        for (int c = 0; c < CD; c++) kf[h][c] = __builtin_bit_cast(f4v, r.load16(ko[c]));
     }
     __device__ __forceinline__ void trim_k(uint32_t grp, uint32_t D) {
 #pragma unroll
@@ -359,16 +437,10 @@ template <int DP> struct Core<float, DP> {
             if (dim_of(c, grp) >= D) kf[0][c] = f4v{};
         }
     }
-    __device__ __forceinline__ void load_v(int e, const char* p, uint32_t n, uint32_t D) {
-#pragma unroll
-        for (int c = 0; c < CV; c++) {
-            const uint32_t d = n * (DP / 16) + 4 * c;
-            vr[e][c] = *reinterpret_cast<const f4v*>(p + (D == DP || d < D ? d * 4 : 0));
-        }
-    }
+    template <typename Row> __device__ __forceinline__ void load_v(int e, const Row& r) { load_dwords<PER>(r, vo, vr[e]); }
     __device__ __forceinline__ void drop_v(int e) {
 #pragma unroll
-        for (int c = 0; c < CV; c++) vr[e][c] = f4v{};
+        for (int c = 0; c < PER; c++) vr[e][c] = 0;
     }
     static __device__ __forceinline__ uint32_t key_of(int e, uint32_t grp) { return 4 * grp + e; }
     static constexpr int half_of(int) { return 0; }
@@ -388,19 +460,19 @@ template <int DP> struct Core<float, DP> {
         for (int r = 0; r < NE; r++) {
 #pragma unroll
             for (int d = 0; d < DP / 16; d++) {
-                acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[r][d / 4][d % 4], p[r], acc[d], 0, 0, 0);
+                acc[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vr[r][d]), p[r], acc[d], 0, 0, 0);
             }
         }
     }
 };
 
 // Workgroups of a tile kernel that a CU holds, which their registers are limited to.
-constexpr int per_cu(int dp) { return dp <= 64 ? 4 : dp <= 128 ? 2 : 1; }
+constexpr int per_cu(int dp, bool uni) { return dp <= 64 ? (uni ? 4 : 3) : dp <= 96 ? (uni ? 3 : 2) : dp <= 128 ? 2 : 1; }
 
 // UNI: a page holds whole runs of 16 keys, looked up once a wave and half;
 // else every lane looks its key up and passes the page on.
 template <typename TQ, typename TC, int DP, bool UNI>
-__global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(AttnArgs a) {
     using C = Core<TC, DP>;
     constexpr int NK = C::NK, NH = C::NH, NE = C::NE, W4 = kAttnThreads / 64, KT = NK * W4;
     extern __shared__ float lds_o[];                 // [4][gc][DP + 4]
@@ -411,28 +483,44 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
     bool wrong = false;
 
     // this workgroup's run of tiles, and the request that its first lies in
-    const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
-    uint32_t mine, total;
-    uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
-    const uint32_t T = total * a.H;
-    const uint32_t W = min(a.W, T);                  // runs, each of a tile at least
-    if (blockIdx.x >= W) return;
-    uint32_t at = run_start(blockIdx.x, W, T);
-    const uint32_t end = run_start(blockIdx.x + 1, W, T);
-    if (before * a.H <= at && at < (before + mine) * a.H) {
-        uint32_t s = tid * c;
-        for (;; s++) {
-            const uint32_t t = span_of<KT>(a, s).tiles;
-            if (at < (before + t) * a.H) break;
-            before += t;
+    uint32_t s, base, at, end, W = 1, T = 1;
+    uint4 split = make_uint4(0, 0, 0, 0);
+    if (a.W == 0) {
+        s = blockIdx.x / a.H;
+        base = 0;
+        const uint32_t tiles = span_of<KT>(a, s).tiles;
+        at = (blockIdx.x - s * a.H) * tiles;
+        end = at + tiles;
+    } else {
+        const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
+        uint32_t mine, total;
+        uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
+        T = total * a.H;
+        W = min(a.W, T);                                 // runs, each of a tile at least
+        if (blockIdx.x >= W) {
+            if (tid == 0) a.split[blockIdx.x] = make_uint4(0, 0, 0, 0);
+            return;
         }
-        lds_at[0] = s;
-        lds_at[1] = before * a.H;
+        const Runs runs(T, W);
+        at = runs.start(blockIdx.x);
+        end = runs.start(blockIdx.x + 1);
+        if (before * a.H <= at && at < (before + mine) * a.H) {
+            uint32_t i = tid * c;
+            for (;; i++) {
+                const uint32_t t = span_of<KT>(a, i).tiles;
+                if (at < (before + t) * a.H) break;
+                before += t;
+            }
+            lds_at[0] = i;
+            lds_at[1] = before * a.H;
+        }
+        __syncthreads();
+        s = __builtin_amdgcn_readfirstlane(lds_at[0]);
+        base = __builtin_amdgcn_readfirstlane(lds_at[1]);
     }
-    __syncthreads();
-    uint32_t s = __builtin_amdgcn_readfirstlane(lds_at[0]), base = __builtin_amdgcn_readfirstlane(lds_at[1]);
 
     C core;
+    core.offsets(n, grp, a.D);
     while (at < end) {
         const Span sp = span_of<KT>(a, s);
         wrong |= sp.wrong;
@@ -446,14 +534,13 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
             float x[C::QC * C::QN];
             const char* qr = a.q + s * a.q_nb2 + (hq0 + (n < heads ? n : 0)) * a.q_nb1;
 #pragma unroll
-            for (int i = 0; i < C::QC; i++) {
+            for (int i = 0; i < C::QC * C::QN; i += 4) {      // D % 8 == 0: four dims are all in or none
+                const uint32_t d = C::dim_of(i / C::QN, grp) + i % C::QN;
+                const bool in = n < heads && d < a.D;
+                float t[4];
+                load4u(qr + (in ? d : 0) * Elt<TQ>::size, t, TQ());
 #pragma unroll
-                for (int j = 0; j < C::QN; j++) {
-                    const uint32_t d = C::dim_of(i, grp) + j;
-                    const bool in = n < heads && d < a.D;
-                    const float v = Elt<TQ>::load1(qr + (in ? d : 0) * Elt<TQ>::size);
-                    x[i * C::QN + j] = in ? v : 0.0f;
-                }
+                for (int j = 0; j < 4; j++) x[i + j] = in ? t[j] : 0.0f;
             }
             core.load_q(x, sizeof(TQ) == 4);
         }
@@ -469,96 +556,95 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
 
         const char* kb0 = a.k + hk * a.k_nb2;
         const char* vb0 = a.v + hk * a.v_nb2;
-        int32_t pg[NH];           // UNI: pages of the halves; else pg[0] the page of key `lane` of the step
-        bool ok[NH];
+        // The pages of a step's keys.  UNI: one a half of 16 keys, read by scalar
+        // loads (their own counter: nothing of the keys in flight is waited
+        // for); else of key `lane` of the step.  Entries past the request's
+        // keys are not used, those that are no page are left out.
+        struct Pages {
+            int32_t pg[NH];
+            uint32_t ok;          // UNI: bit i: half i has keys
+        };
         auto look_up = [&](uint32_t kb) {
+            Pages r;
+            r.ok = 0;
+            if constexpr (UNI) {
+#pragma unroll
+                for (int i = 0; i < NH; i++) {
+                    r.pg[i] = reinterpret_cast<const_i32*>(reinterpret_cast<uintptr_t>(row))[min(page_of(a, kb + 16 * i), a.max_pages - 1)];
+                }
+            } else {
+                r.pg[0] = row[min(page_of(a, kb + (lane & (NK - 1))), a.max_pages - 1)];
+            }
+            return r;
+        };
+        auto settle = [&](Pages& r, uint32_t kb) {
             if constexpr (UNI) {
 #pragma unroll
                 for (int i = 0; i < NH; i++) {
                     const uint32_t key = kb + 16 * i;
-                    ok[i] = key < sp.len && key + 16 > sp.first;
-                    pg[i] = __builtin_amdgcn_readfirstlane(row[ok[i] ? page_of(a, key) : 0]);
+                    const bool in = key < sp.len && key + 16 > sp.first, good = static_cast<uint32_t>(r.pg[i]) < a.n_pages;
+                    wrong |= in && !good;
+                    r.ok |= (in && good ? 1u : 0u) << i;
+                    if (!good) r.pg[i] = 0;
                 }
             } else {
                 const uint32_t key = kb + (lane & (NK - 1));
-                const bool in = key < sp.len && key >= sp.first;
-                pg[0] = row[in ? page_of(a, key) : 0];
-                if (!in) pg[0] = -2;
+                const bool in = key < sp.len && key >= sp.first, good = static_cast<uint32_t>(r.pg[0]) < a.n_pages;
+                wrong |= in && !good;
+                if (!in || !good) r.pg[0] = -1;
             }
         };
-        // a looked-up page that is none: left out
-        auto settle = [&]() {
+        // UNI: the half's first row is the wave's, the key's place in it the lane's
+        auto fetch_k = [&](const Pages& r, uint32_t kb) {
+#pragma unroll
+            for (int i = 0; i < NH; i++) {
+                if constexpr (UNI) {
+                    const uint32_t key = kb + 16 * i, in = key - page_of(a, key) * a.page;
+                    core.load_k(i, WaveRows(kb0 + (r.pg[i] * a.k_nb3 + in * a.k_nb1), n * static_cast<uint32_t>(a.k_nb1), 0));
+                } else {
+                    const uint32_t key = kb + 16 * i + n;
+                    const int32_t g = __shfl(r.pg[0], 16 * i + n);
+                    core.load_k(i, LaneRow{kb0 + (g < 0 ? 0 : g * a.k_nb3 + (key - page_of(a, key) * a.page) * a.k_nb1)});
+                }
+            }
+        };
+        auto fetch_v = [&](const Pages& r, uint32_t kb) {
             if constexpr (UNI) {
 #pragma unroll
                 for (int i = 0; i < NH; i++) {
-                    const bool good = static_cast<uint32_t>(pg[i]) < a.n_pages;
-                    wrong |= ok[i] && !good;
-                    ok[i] = ok[i] && good;
-                    if (!good) pg[i] = 0;
+                    const uint32_t key = kb + 16 * i, in = key - page_of(a, key) * a.page;
+                    const char* p = vb0 + (r.pg[i] * a.v_nb3 + in * a.v_nb1);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        core.load_v(4 * i + e, WaveRows(p, 4 * grp * static_cast<uint32_t>(a.v_nb1), e * static_cast<uint32_t>(a.v_nb1)));
+                    }
                 }
             } else {
-                if (static_cast<uint32_t>(pg[0]) >= a.n_pages) {
-                    wrong |= pg[0] != -2;
-                    pg[0] = -1;
-                }
-            }
-        };
-        auto fetch_k = [&](uint32_t kb) {
 #pragma unroll
-            for (int i = 0; i < NH; i++) {
-                const char* p;
-                if constexpr (UNI) {
-                    const uint32_t key = kb + 16 * i, in = ok[i] ? key - page_of(a, key) * a.page : 0;
-                    p = kb0 + pg[i] * a.k_nb3 + in * a.k_nb1 + n * static_cast<uint32_t>(a.k_nb1);
-                } else {
-                    const uint32_t key = kb + 16 * i + n;
-                    const int32_t g = __shfl(pg[0], 16 * i + n);
-                    p = kb0 + (g < 0 ? 0 : g * a.k_nb3 + (key - page_of(a, key) * a.page) * a.k_nb1);
+                for (int e = 0; e < NE; e++) {
+                    const uint32_t key = kb + C::key_of(e, grp);
+                    const int32_t g = __shfl(r.pg[0], C::key_of(e, grp));
+                    core.load_v(e, LaneRow{vb0 + (g < 0 ? 0 : g * a.v_nb3 + (key - page_of(a, key) * a.page) * a.v_nb1)});
                 }
-                core.load_k(i, p, grp, a.D);
             }
         };
-        auto fetch_v = [&](uint32_t kb, bool (&live)[NE]) {
-#pragma unroll
-            for (int e = 0; e < NE; e++) {
-                const uint32_t key = kb + C::key_of(e, grp);
-                const char* p;
-                if constexpr (UNI) {
-                    const int i = C::half_of(e);
-                    const uint32_t k0 = kb + 16 * i, in = ok[i] ? k0 - page_of(a, k0) * a.page : 0;
-                    p = vb0 + pg[i] * a.v_nb3 + in * a.v_nb1 + (key - k0) * static_cast<uint32_t>(a.v_nb1);
-                    live[e] = ok[i] && key < sp.len && key >= sp.first;
-                } else {
-                    const int32_t g = __shfl(pg[0], C::key_of(e, grp));
-                    p = vb0 + (g < 0 ? 0 : g * a.v_nb3 + (key - page_of(a, key) * a.page) * a.v_nb1);
-                    live[e] = g >= 0;
-                }
-                core.load_v(e, p, n, a.D);
-            }
-        };
+        // Keys of a step arrive while the values before them are used, values
+        // while the next scores are made, pages a step before both.
         if (tb < te) {
             uint32_t kb = tb * KT + wid * NK;
-            look_up(kb);
-            settle();
-            fetch_k(kb);
+            Pages cur = look_up(kb), next = look_up(kb + KT);
+            settle(cur, kb);
+            fetch_k(cur, kb);
+            fetch_v(cur, kb);
             for (uint32_t t = tb; t < te; t++, kb += KT) {
-                bool live[NE];
-                fetch_v(kb, live);
-                bool whole = kb >= sp.first && kb + NK <= sp.len;
-                if constexpr (UNI) {
-#pragma unroll
-                    for (int i = 0; i < NH; i++) whole = whole && ok[i];
-                } else {
-                    whole = whole && __all(pg[0] >= 0);
-                }
                 const bool more = t + 1 < te;
-                if (more) look_up(kb + KT);
+                const Pages after = look_up(kb + 2 * KT);
                 if (a.D != DP) core.trim_k(grp, a.D);
                 float sc[NE];
                 core.scores(sc);
                 if (more) {
-                    settle();
-                    fetch_k(kb + KT);
+                    settle(next, kb + KT);
+                    fetch_k(next, kb + KT);
                 }
                 if (a.softcap > 0.0f) {
 #pragma unroll
@@ -567,10 +653,17 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
 #pragma unroll
                     for (int e = 0; e < NE; e++) sc[e] = sc[e] * (scale * kLog2e);
                 }
+                bool whole = kb >= sp.first && kb + NK <= sp.len;
+                if constexpr (UNI) whole = whole && cur.ok == (1u << NH) - 1;
+                else whole = whole && __all(cur.pg[0] >= 0);
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < NE; e++) {
-                        if (!live[e]) {
+                        const uint32_t key = kb + C::key_of(e, grp);
+                        bool live = key < sp.len && key >= sp.first;
+                        if constexpr (UNI) live = live && (cur.ok >> C::half_of(e) & 1);
+                        else live = __shfl(cur.pg[0], C::key_of(e, grp)) >= 0;
+                        if (!live) {
                             sc[e] = -INFINITY;
                             core.drop_v(e);
                         }
@@ -595,6 +688,9 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
                     l += p[e];
                 }
                 core.add_values(p);
+                if (more) fetch_v(next, kb + KT);
+                cur = next;
+                next = after;
             }
         }
         l += __shfl_xor(l, 16);
@@ -603,11 +699,12 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
         // the four waves' parts, joined through LDS
         const uint32_t ld = DP + 4;
         if (n < heads) {
-            float* o = lds_o + (wid * a.gc + n) * ld + grp * (DP / 4);
+            float* o = lds_o + (wid * a.gc + n) * ld;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
+                const uint32_t d0 = value_dim<DP / 16>(4 * grp + r, a.D);
 #pragma unroll
-                for (int d = 0; d < DP / 16; d++) o[r * (DP / 16) + d] = core.acc[d][r];
+                for (int d = 0; d < DP / 16; d++) o[d0 + d] = core.acc[d][r];
             }
             if (grp == 0) {
                 lds_m[wid][n] = m;
@@ -616,6 +713,9 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
         }
         __syncthreads();
         const bool entire = n_tiles == sp.tiles;
+        if (t0 == 0 && !entire) {
+            split = make_uint4(s, hq0, heads, Runs(T, W).of(at + sp.tiles - 1) - blockIdx.x + 1);
+        }
         const uint64_t slot = (static_cast<uint64_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1)) * a.gc;
         for (uint32_t i = tid; i < heads * a.D; i += kAttnThreads) {
             const uint32_t hh = i / a.D, d = i - hh * a.D;
@@ -643,93 +743,90 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP)) void k_attn_tiles(AttnArg
             base = at;
         }
     }
+    if (a.W != 0 && tid == 0) a.split[blockIdx.x] = split;
     if (wrong && n == 0) atomicOr(a.err, DEV_ERR_PAGE);
 }
 
 // Adds up the parts of the key heads that several runs hold, in the order of
-// the runs: a workgroup a request and query head.  Part 0 lies in its run's
-// second place (the run ends with it), the others in the first.
-template <typename TQ, int KT>
+// the runs: a workgroup a run that such a key head begins in and a head of it.
+// Part 0 lies in its run's second place (the run ends with it), the others in
+// the first.  A wave adds every fourth part, a part's dims over its lanes, 8
+// parts in flight (of the first 32 already while their maxima are read).
+template <typename TQ, int DP>
 __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
-    __shared__ uint32_t lds_scan[kAttnThreads / 64], lds_before;
-    __shared__ float lds_f[kAttnThreads], lds_w[kAttnThreads / 64];
-    __shared__ float lds_o[kAttnThreads];
-    const uint32_t tid = threadIdx.x;
-    const uint32_t s = blockIdx.x / a.hq, hq = blockIdx.x - s * a.hq;
-    const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
-    uint32_t mine, total;
-    uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
-    if (tid == s / c) {
-        for (uint32_t i = tid * c; i < s; i++) before += span_of<KT>(a, i).tiles;
-        lds_before = before;
-    }
-    __syncthreads();
-    const uint32_t T = total * a.H, tiles = span_of<KT>(a, s).tiles;
-    const uint32_t hk = hq / a.g, in_g = hq - hk * a.g, run = in_g / a.gc, hh = in_g - run * a.gc;
-    const uint32_t t0 = lds_before * a.H + (hk * a.ngr + run) * tiles;
-    const uint32_t W = min(a.W, T);
-    const uint32_t w0 = run_of(t0, W, T), w1 = run_of(t0 + tiles - 1, W, T);
-    if (w0 == w1) return;
-    const uint32_t parts = w1 - w0 + 1;
-    auto slot = [&](uint32_t i) { return (static_cast<uint64_t>(w0 + i) * 2 + (i == 0 ? 1 : 0)) * a.gc + hh; };
+    constexpr int N = DP / 64, U = 8;
+    __shared__ float lds_m[kAttnThreads / 64], lds_l[kAttnThreads / 64], lds_f[kAttnThreads];
+    __shared__ float lds_o[kAttnThreads / 64][DP];
+    const uint32_t run = blockIdx.x / a.gc, hh = blockIdx.x - run * a.gc;
+    const uint4 sp = a.split[run];
+    const uint32_t parts = sp.w;
+    if (parts == 0 || hh >= sp.z) return;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    auto slot = [&](uint32_t i) { return (static_cast<uint64_t>(run + i) * 2 + (i == 0 ? 1 : 0)) * a.gc + hh; };
+    float o[N], x[U][N];
+    auto fetch = [&](uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + 4 * u < parts ? i0 + 4 * u : 0;
+            const float* p = a.part_o + slot(i) * a.D;
+#pragma unroll
+            for (int j = 0; j < N; j++) x[u][j] = p[lane + 64 * j < a.D ? lane + 64 * j : 0];
+        }
+    };
+    fetch(wid);
     float m = kLowest;
     for (uint32_t i = tid; i < parts; i += kAttnThreads) m = fmaxf(m, a.part_ml[slot(i)].x);
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-    if ((tid & 63) == 0) lds_w[tid >> 6] = m;
+    if (lane == 0) lds_m[wid] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(lds_w[0], lds_w[1]), fmaxf(lds_w[2], lds_w[3]));
-    // dims over 64-lane columns, parts over the four waves, 256 parts a turn
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t lane = tid & 63, wid = tid >> 6;
-    for (uint32_t i0 = 0; i0 < parts; i0 += kAttnThreads) {
+    m = fmaxf(fmaxf(lds_m[0], lds_m[1]), fmaxf(lds_m[2], lds_m[3]));
+    float l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; j++) o[j] = 0.0f;
+    for (uint32_t t = 0; t < parts; t += kAttnThreads) {      // 256 parts a turn
         __syncthreads();
-        if (i0 + tid < parts) {
-            const float2 ml = a.part_ml[slot(i0 + tid)];
-            const float f = __builtin_amdgcn_exp2f(ml.x - m);
-            lds_f[tid] = f;
+        float f = 0.0f;
+        if (t + tid < parts) {
+            const float2 ml = a.part_ml[slot(t + tid)];
+            f = __builtin_amdgcn_exp2f(ml.x - m);
             l = fmaf(ml.y, f, l);
         }
+        lds_f[tid] = f;                                       // 0 past the last part
         __syncthreads();
-        const uint32_t k = min(parts - i0, static_cast<uint32_t>(kAttnThreads));
-#pragma unroll 4
-        for (uint32_t i = wid; i < k; i += 4) {
-            const float* p = a.part_o + slot(i0 + i) * a.D;
-            const float f = lds_f[i];
+        for (uint32_t i = wid; i < min(parts - t, static_cast<uint32_t>(kAttnThreads)); i += 4 * U) {
+            if (t + i != wid) fetch(t + i);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t d = lane + 64 * j;
-                if (d < a.D) o[j] = fmaf(p[d], f, o[j]);
+            for (int u = 0; u < U; u++) {
+                const float g = i + 4 * u < kAttnThreads ? lds_f[i + 4 * u] : 0.0f;
+                if (g == 0.0f) continue;                      // also no part: what is read for it is another's
+#pragma unroll
+                for (int j = 0; j < N; j++) o[j] = fmaf(x[u][j], g, o[j]);
             }
         }
     }
     for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
-    __syncthreads();
-    if (lane == 0) lds_w[wid] = l;
-    __syncthreads();
-    l = ((lds_w[0] + lds_w[1]) + lds_w[2]) + lds_w[3];
-    char* yr = a.y + s * a.y_nb2 + hq * a.y_nb1;
+    if (lane == 0) lds_l[wid] = l;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (64 * j >= static_cast<int>(a.D)) break;
-        __syncthreads();
-        lds_o[tid] = o[j];
-        __syncthreads();
-        const uint32_t d = lane + 64 * j;
-        if (wid == 0 && d < a.D) {
-            const float t = ((lds_o[lane] + lds_o[lane + 64]) + lds_o[lane + 128]) + lds_o[lane + 192];
-            Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
-        }
+    for (int j = 0; j < N; j++) lds_o[wid][lane + 64 * j] = o[j];
+    __syncthreads();
+    l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
+    char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
+    for (uint32_t d = tid; d < a.D; d += kAttnThreads) {
+        const float t = ((lds_o[0][d] + lds_o[1][d]) + lds_o[2][d]) + lds_o[3][d];
+        Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
     }
 }
 
 // ---- what runs where ------------------------------------------------------------
+
+bool uniform_pages(const cbx_tensor* k) { return k->ne[1] % 16 == 0; }
 
 struct AttnPlan {
     bool tiles;            // k_attn_tiles, else k_attn_rows
     int dp, kt;
     uint32_t gc, ngr, H, W;
     bool join;             // a key head's tiles may fall into several runs
-    size_t o_bytes, bytes; // of the workspace
+    size_t o_bytes, ml_bytes, bytes;   // of the workspace
 };
 
 // Everything but addresses, which the workspace's size may not depend on.
@@ -737,7 +834,7 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     AttnPlan p{};
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0;
     const int64_t cap = tables->ne[0] * k->ne[1];
-    p.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
     p.kt = (k->type == CBX_TYPE_F16 ? 32 : 16) * (kAttnThreads / 64);
     p.ngr = static_cast<uint32_t>(cdiv(g, 16));
     p.gc = static_cast<uint32_t>(cdiv(g, p.ngr));
@@ -746,11 +843,21 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     const int64_t most = q->ne[2] * p.H * cap_tiles;
     p.tiles = D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
     if (!p.tiles) return p;
-    p.W = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(per_cu(p.dp)) * st->n_cu, most));
-    p.join = cap_tiles > 1;
+    p.W = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(per_cu(p.dp, uniform_pages(k))) * st->n_cu, most));
+    // A run a key head, without a join, while the longest a table can hold ends
+    // about with the rest: 0.8 us a tile of one key head after another, against
+    // 4 us for the join and two key heads a run.  Both sides measured with
+    // lengths from 1 to the table's, S key heads: S 16, 3 tiles 6.9 us against
+    // 9.3, 8 tiles 10.4 against 9.3; S 64, 8 tiles 11.2 / 11.5, 16 tiles 19.7 /
+    // 14.0; S 256, 16 tiles 20.7 / 21.4 (head_dim 128: 35 / 41), 32 tiles 43 / 35;
+    // S 512, 16 tiles 64 / 73, 32 tiles 123 / 117; S 1024, 32 tiles 114 / 114, 64
+    // tiles 221 / 204: they cross near the square root of S.
+    const int64_t S = std::min<int64_t>(q->ne[2] * p.H, 1024);
+    p.join = cap_tiles > 7 && cap_tiles * cap_tiles > S;
     if (p.join) {
         p.o_bytes = static_cast<size_t>(cdiv(static_cast<int64_t>(p.W) * 2 * p.gc * D * 4, 16) * 16);
-        p.bytes = p.o_bytes + static_cast<size_t>(p.W) * 2 * p.gc * 8;
+        p.ml_bytes = static_cast<size_t>(p.W) * 2 * p.gc * 8;
+        p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(p.W) * sizeof(uint4);
     }
     return p;
 }
@@ -768,17 +875,19 @@ void tiles_uni(bool uni, dim3 grid, size_t lds, hipStream_t s, const AttnArgs& a
 }
 
 template <typename TQ, typename TC>
-void launch_tiles(const AttnPlan& p, AttnArgs& a, hipStream_t s) {
-    const dim3 grid(p.W);
+void launch_tiles(const AttnPlan& p, bool uni, AttnArgs& a, hipStream_t s) {
+    if (!p.join) a.W = 0;
+    const dim3 grid(p.join ? p.W : a.n_seq * a.H);
     const size_t lds = static_cast<size_t>(kAttnThreads / 64) * p.gc * (p.dp + 4) * sizeof(float);
-    const bool uni = a.page % 16 == 0;
     if (p.dp == 64) tiles_uni<TQ, TC, 64>(uni, grid, lds, s, a);
+    else if (p.dp == 96) tiles_uni<TQ, TC, 96>(uni, grid, lds, s, a);
     else if (p.dp == 128) tiles_uni<TQ, TC, 128>(uni, grid, lds, s, a);
     else tiles_uni<TQ, TC, 256>(uni, grid, lds, s, a);
-    if (p.join) {
-        hipLaunchKernelGGL((k_attn_join<TQ, Core<TC, 64>::NK * (kAttnThreads / 64)>), dim3(a.n_seq * a.hq), dim3(kAttnThreads), 0,
-                           s, a);
-    }
+    if (!p.join) return;
+    const dim3 parts(p.W * p.gc);
+    if (p.dp == 64) hipLaunchKernelGGL((k_attn_join<TQ, 64>), parts, dim3(kAttnThreads), 0, s, a);
+    else if (p.dp <= 128) hipLaunchKernelGGL((k_attn_join<TQ, 128>), parts, dim3(kAttnThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join<TQ, 256>), parts, dim3(kAttnThreads), 0, s, a);
 }
 
 }  // namespace
@@ -824,11 +933,12 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
         a.W = p.W;
         a.part_o = static_cast<float*>(c.ws);
         a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
+        a.split = reinterpret_cast<uint4*>(static_cast<char*>(c.ws) + p.o_bytes + p.ml_bytes);
         const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
-        if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, a, s);
-        else if (t16) launch_tiles<uint16_t, float>(p, a, s);
-        else if (c16) launch_tiles<float, uint16_t>(p, a, s);
-        else launch_tiles<float, float>(p, a, s);
+        if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, uniform_pages(c.k), a, s);
+        else if (t16) launch_tiles<uint16_t, float>(p, uniform_pages(c.k), a, s);
+        else if (c16) launch_tiles<float, uint16_t>(p, uniform_pages(c.k), a, s);
+        else launch_tiles<float, float>(p, uniform_pages(c.k), a, s);
         return check_launch("cbx_paged_attention");
     }
     const dim3 grid(static_cast<unsigned>(c.q->ne[1] * c.q->ne[2])), block(kAttnThreads);
