@@ -11,10 +11,10 @@
 // the stack without gaps.
 //
 // A few KB of data: latency is everything.  Every workgroup makes the two
-// scans for itself in LDS (a few requests a lane, a wave scan, four wave
-// totals), so one launch does without a second pass or a
-// message between workgroups, and then fills its part of the tokens and
-// pages, finding the request of each by a search over the scan.
+// scans for itself in LDS (a few requests a lane, a wave scan by DPP, four wave
+// totals), so one launch does without a second pass or a message between
+// workgroups, and then fills its part of the tokens and pages, finding the
+// request of every fourth token by a search over the scan.
 #include "cbx_device.h"
 
 namespace cbx {
@@ -22,29 +22,38 @@ namespace {
 
 constexpr int kPlanThreads = 256;
 
+// Sums of token and page counts stop at 2^31 - 1 (still associative for what
+// is not negative): a request behind that many is refused all the same.
+constexpr uint32_t kMostCount = 0x7fffffffu;
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, kMostCount); }
+
 // Exclusive scan of one value a thread over the block; *total the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int64_t* total) {
+// Within rows of 16 lanes by shifts, then each row's last to the rows behind.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_sat_add(uint32_t x) {
+    return sat_add(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    int64_t x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t u = __shfl_up(x, d);
-        if (lane >= d) x += u;
-    }
+    uint32_t x = v;
+    x = dpp_sat_add<0x111, 0xf>(x);
+    x = dpp_sat_add<0x112, 0xf>(x);
+    x = dpp_sat_add<0x114, 0xf>(x);
+    x = dpp_sat_add<0x118, 0xf>(x);
+    x = dpp_sat_add<0x142, 0xa>(x);
+    x = dpp_sat_add<0x143, 0xc>(x);
+    // the lane before; the wave's first has nothing before it
+    uint32_t before = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x138, 0xf, 0xf, false));
     if (lane == 63) lds[wid] = x;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    uint32_t all = 0;
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 64; w++) {
-        if (w < wid) before += lds[w];
-        all += lds[w];
+        if (w < wid) before = sat_add(before, lds[w]);
+        all = sat_add(all, lds[w]);
     }
-    __syncthreads();
     *total = all;
-    return before + x - v;
+    return before;
 }
-
-__device__ __forceinline__ int32_t sat32(int64_t v) { return v > 0x7fffffff ? 0x7fffffff : static_cast<int32_t>(v); }
 
 // The last s of [0, n) with start[s] <= i (start ascending, start[0] = 0).
 __device__ __forceinline__ int last_at_most(const int32_t* start, int n, int32_t i) {
@@ -61,111 +70,141 @@ __device__ __forceinline__ int32_t* table_row(char* tables, int64_t nb1, int s) 
     return reinterpret_cast<int32_t*>(tables + s * nb1);
 }
 
-// LDS: tok[n], off[n], have[n] (have -1: refused), each 32-bit.
+constexpr int kPlanTokens = 4;   // neighbouring tokens of a thread
+constexpr int kPlanHeld = 4;     // requests a thread reads at once
+
+// LDS: tok[n], off[n], have[n] (have -1: refused), past[n], each 32-bit.
 __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t* err) {
     extern __shared__ int32_t lds32[];
-    __shared__ int64_t part[kPlanThreads / 64];
+    __shared__ uint32_t part[2][kPlanThreads / 64];
     __shared__ int32_t took;
-    int32_t *tok = lds32, *off = lds32 + a.n_seq, *have = lds32 + 2 * a.n_seq;
     const int tid = threadIdx.x, n = a.n_seq;
-    const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
+    int32_t *tok = lds32, *off = lds32 + n, *have = lds32 + 2 * n, *had = lds32 + 3 * n;
+    const int32_t cap = a.max_pages * a.page;      // below 2^31
     int32_t free_n = *a.n_free;
     bool wrong = free_n < 0 || free_n > a.pool;
-    free_n = free_n < 0 ? 0 : (free_n > a.pool ? a.pool : free_n);
+    free_n = free_n < 0 ? 0 : min(free_n, a.pool);
     if (tid == 0) took = 0;
     // a lane's requests are neighbours: c of them from c * tid on
     const int c = (n + kPlanThreads - 1) / kPlanThreads;
-    const int s0 = tid * c, s1 = s0 + c < n ? s0 + c : n;
-    int64_t toks = 0, pages = 0;
-    for (int s = s0; s < s1; s++) toks += a.n_new[s] > 0 ? a.n_new[s] : 0;
-    int64_t n_tok;
-    int64_t t = block_scan(toks, part, &n_tok);
-    for (int s = s0; s < s1; s++) {
-        const int64_t past = a.n_past[s], nw = a.n_new[s] > 0 ? a.n_new[s] : 0;
-        const bool sane = past >= 0 && past <= cap && a.n_new[s] >= 0;
-        wrong |= !sane;
-        const bool fits = sane && past + nw <= cap && t + nw <= a.n_slots;
-        const int64_t hv = fits ? (past + a.page - 1) / a.page : -1;
-        if (fits) pages += (past + nw + a.page - 1) / a.page - hv;
-        tok[s] = sat32(t);
-        have[s] = static_cast<int32_t>(hv);
-        t += nw;
+    const int s0 = min(tid * c, n), s1 = min(s0 + c, n);
+    uint32_t toks = 0;
+    for (int b = s0; b < s1; b += kPlanHeld) {
+        int32_t past[kPlanHeld], nw[kPlanHeld];
+#pragma unroll
+        for (int k = 0; k < kPlanHeld; k++) {
+            past[k] = a.n_past[min(b + k, s1 - 1)];
+            nw[k] = a.n_new[min(b + k, s1 - 1)];
+        }
+#pragma unroll
+        for (int k = 0; k < kPlanHeld; k++) {
+            if (b + k >= s1) break;
+            wrong |= past[k] < 0 || past[k] > cap || nw[k] < 0;
+            had[b + k] = past[k];
+            off[b + k] = nw[k];                    // until its pages are known
+            toks = sat_add(toks, max(nw[k], 0));
+        }
     }
-    int64_t n_pages;
-    int64_t o = block_scan(pages, part, &n_pages);
+    uint32_t n_tok, n_pages;
+    uint32_t t = block_scan(toks, part[0], &n_tok), pages = 0;
+    auto pages_of = [&](int32_t len) { return static_cast<int32_t>((static_cast<uint32_t>(len) + a.page - 1) / a.page); };
     for (int s = s0; s < s1; s++) {
-        off[s] = sat32(o);
-        if (have[s] < 0) continue;
-        const int64_t need = (static_cast<int64_t>(a.n_past[s]) + a.n_new[s] + a.page - 1) / a.page - have[s];
-        if (need > 0 && o + need > free_n) have[s] = -1;
-        else if (need > 0) atomicMax(&took, static_cast<int32_t>(o + need));   // LDS; the maximum, in any order
-        o += need;
+        const int32_t past = had[s], nw = off[s];
+        const uint32_t end = sat_add(t, max(nw, 0));
+        const bool fits = past >= 0 && nw >= 0 && past <= cap && nw <= cap - past && end <= static_cast<uint32_t>(a.n_slots) &&
+                          end < kMostCount;
+        const int32_t hv = fits ? pages_of(past) : -1;
+        const uint32_t need = fits ? static_cast<uint32_t>(pages_of(past + nw) - hv) : 0;
+        tok[s] = static_cast<int32_t>(t);
+        have[s] = hv;
+        off[s] = static_cast<int32_t>(need);
+        pages = sat_add(pages, need);
+        t = end;
+    }
+    uint32_t o = block_scan(pages, part[1], &n_pages);
+    for (int s = s0; s < s1; s++) {
+        const uint32_t need = static_cast<uint32_t>(off[s]), end = sat_add(o, need);
+        off[s] = static_cast<int32_t>(o);
+        if (need > 0) {
+            if (end > static_cast<uint32_t>(free_n)) have[s] = -1;
+            else atomicMax(&took, static_cast<int32_t>(end));   // in LDS; the largest, in any order
+        }
+        o = end;
     }
     __syncthreads();
     if (blockIdx.x == 0) {
         for (int s = tid; s < n; s += kPlanThreads) {
-            a.seq_lens[s] = have[s] < 0 ? a.n_past[s] : a.n_past[s] + a.n_new[s];
+            a.seq_lens[s] = have[s] < 0 ? had[s] : had[s] + a.n_new[s];
             a.tok_start[s] = tok[s];
         }
         if (tid == 0) {
-            a.tok_start[n] = sat32(n_tok);
+            a.tok_start[n] = static_cast<int32_t>(n_tok);
             *a.n_free_out = free_n - took;
         }
     }
-    if (wrong) atomicOr(err, DEV_ERR_PAGE);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kPlanThreads;
     const int64_t first = static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid;
+    for (int64_t i0 = first * kPlanTokens; i0 < a.n_slots; i0 += step * kPlanTokens) {
+        int32_t slot[kPlanTokens], pos[kPlanTokens], page[kPlanTokens];
+        int s = i0 < n_tok ? last_at_most(tok, n, static_cast<int32_t>(i0)) : 0;
+#pragma unroll
+        for (int k = 0; k < kPlanTokens; k++) {     // the pages' loads first, together
+            const int64_t i = i0 + k;
+            page[k] = -1;
+            pos[k] = slot[k] = 0;
+            if (i >= n_tok || i >= a.n_slots) continue;
+            while (s + 1 < n && tok[s + 1] <= i) s++;
+            pos[k] = had[s] + static_cast<int32_t>(i - tok[s]);
+            if (have[s] < 0) continue;
+            slot[k] = 1;
+            const int32_t pi = static_cast<int32_t>(static_cast<uint32_t>(pos[k]) / static_cast<uint32_t>(a.page));
+            page[k] = pi < have[s] ? table_row(a.tables, a.tables_nb1, s)[pi] : a.free_pages[free_n - 1 - off[s] - (pi - have[s])];
+        }
+#pragma unroll
+        for (int k = 0; k < kPlanTokens; k++) {
+            if (i0 + k >= a.n_slots) break;
+            const int64_t p = static_cast<int64_t>(page[k]) * a.page + static_cast<uint32_t>(pos[k]) % static_cast<uint32_t>(a.page);
+            const bool good = page[k] >= 0 && p < kMostCount;
+            wrong |= slot[k] && !good;
+            a.slots[i0 + k] = slot[k] && good ? static_cast<int32_t>(p) : -1;
+            a.positions[i0 + k] = pos[k];
+        }
+    }
     // the pages newly taken: took of them, in the order of the requests
     for (int64_t i = first; i < took; i += step) {
         const int s = last_at_most(off, n, static_cast<int32_t>(i));
         table_row(a.tables, a.tables_nb1, s)[have[s] + (i - off[s])] = a.free_pages[free_n - 1 - i];
     }
-    for (int64_t i = first; i < a.n_slots; i += step) {
-        int32_t slot = -1, pos = 0;
-        if (i < n_tok) {
-            const int s = last_at_most(tok, n, static_cast<int32_t>(i));
-            pos = static_cast<int32_t>(a.n_past[s] + (i - tok[s]));
-            if (have[s] >= 0) {
-                const int32_t pi = pos / a.page;
-                const int32_t page = pi < have[s] ? table_row(a.tables, a.tables_nb1, s)[pi]
-                                                  : a.free_pages[free_n - 1 - off[s] - (pi - have[s])];
-                const int64_t p = static_cast<int64_t>(page) * a.page + pos % a.page;
-                if (page >= 0 && p <= 0x7fffffff) slot = static_cast<int32_t>(p);
-                else atomicOr(err, DEV_ERR_PAGE);
-            }
-        }
-        a.slots[i] = slot;
-        a.positions[i] = pos;
-    }
+    if (wrong) atomicOr(err, DEV_ERR_PAGE);
 }
 
 // LDS: off[n], the place above the stack of each released request's first page.
 __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_t* err) {
     extern __shared__ int32_t off[];
-    __shared__ int64_t part[kPlanThreads / 64];
+    __shared__ uint32_t part[kPlanThreads / 64];
     const int tid = threadIdx.x, n = a.n_seq;
-    const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
+    const int32_t cap = a.max_pages * a.page;
     int32_t free_n = *a.n_free;
     bool wrong = free_n < 0 || free_n > a.pool;
-    free_n = free_n < 0 ? 0 : (free_n > a.pool ? a.pool : free_n);
-    auto pages_of = [&](int s) -> int64_t {
-        const int64_t len = a.seq_lens[s];
+    free_n = free_n < 0 ? 0 : min(free_n, a.pool);
+    auto pages_of = [&](int s) -> uint32_t {
+        const int32_t len = a.seq_lens[s];
         if (a.release[s] == 0) return 0;
         if (len < 0 || len > cap) {
             wrong = true;
             return 0;
         }
-        return (len + a.page - 1) / a.page;
+        return (static_cast<uint32_t>(len) + a.page - 1) / a.page;
     };
     const int c = (n + kPlanThreads - 1) / kPlanThreads;
-    const int s0 = tid * c, s1 = s0 + c < n ? s0 + c : n;
-    int64_t sum = 0;
-    for (int s = s0; s < s1; s++) sum += pages_of(s);
-    int64_t total;
-    int64_t at = block_scan(sum, part, &total);
+    const int s0 = min(tid * c, n), s1 = min(s0 + c, n);
+    uint32_t sum = 0;
+    for (int s = s0; s < s1; s++) sum = sat_add(sum, pages_of(s));
+    uint32_t total;
+    uint32_t at = block_scan(sum, part, &total);
     for (int s = s0; s < s1; s++) {
-        off[s] = sat32(at);
-        at += pages_of(s);
+        off[s] = static_cast<int32_t>(at);
+        at = sat_add(at, pages_of(s));
     }
     __syncthreads();
     const int64_t room = a.pool - free_n;
@@ -176,12 +215,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_
     }
     if (wrong) atomicOr(err, DEV_ERR_PAGE);
     for (int s = blockIdx.x; s < n; s += gridDim.x) {
-        const int64_t pages = pages_of(s);
+        const uint32_t pages = pages_of(s);
         int32_t* row = table_row(a.tables, a.tables_nb1, s);
-        for (int64_t i = tid; i < pages; i += kPlanThreads) {
+        for (uint32_t i = tid; i < pages; i += kPlanThreads) {
             const int32_t page = row[i];
             row[i] = -1;
-            if (off[s] + i < room) a.free_pages[free_n + off[s] + i] = page;
+            if (static_cast<int64_t>(off[s]) + i < room) a.free_pages[free_n + off[s] + i] = page;
         }
     }
 }
@@ -189,8 +228,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_
 }  // namespace
 
 int launch_paged_append(const AppendArgs& a, DeviceState* st, hipStream_t s) {
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(cdiv(a.n_slots, kPlanThreads), 2 * st->n_cu));
-    hipLaunchKernelGGL(k_append, dim3(static_cast<unsigned>(grid)), dim3(kPlanThreads), 12 * static_cast<size_t>(a.n_seq), s,
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(cdiv(a.n_slots, kPlanThreads * kPlanTokens), 4 * st->n_cu));
+    hipLaunchKernelGGL(k_append, dim3(static_cast<unsigned>(grid)), dim3(kPlanThreads), 16 * static_cast<size_t>(a.n_seq), s,
                        a, st->err_word);
     return check_launch("cbx_paged_append");
 }
