@@ -277,6 +277,15 @@ struct RopeTable {
 };
 RopeTable rope_table(const cbx_rope_cache* c);
 // ---- the paged key-value cache (cbx_paged.cpp checks the arguments) ---------
+// key / page = (key * mul) >> shift in 64 bits, for 0 <= key < 2^31: mul =
+// floor(2^(31 + l) / page) + 1 with 2^l the first power of two not below page
+// is off by a fraction of at most 2^l / 2^(31 + l), less than 1 / key.
+inline void page_division(uint32_t page, uint32_t* mul, uint32_t* shift) {
+    uint32_t l = 0;
+    while ((uint64_t{1} << l) < page) l++;
+    *shift = 31 + l;
+    *mul = static_cast<uint32_t>((uint64_t{1} << *shift) / page + 1);
+}
 constexpr int kPagedMaxSeq = 4096;   // requests of an append or release: their scans are held in LDS
 struct AppendArgs {
     const int32_t *n_past, *n_new, *free_pages, *n_free;
@@ -284,6 +293,7 @@ struct AppendArgs {
     char* tables;
     int64_t tables_nb1;
     int32_t n_seq, max_pages, page, pool, n_slots;
+    uint32_t page_mul, page_shift;   // set by the launcher
 };
 int launch_paged_append(const AppendArgs& a, DeviceState* st, hipStream_t s);
 struct ReleaseArgs {

@@ -923,10 +923,7 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
     a.err = st->err_word;
     const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
     if (p.tiles && vector_rows(c.k) && vector_rows(c.v)) {
-        uint32_t l = 0;
-        while ((uint64_t{1} << l) < a.page) l++;
-        a.page_shift = 31 + l;
-        a.page_mul = static_cast<uint32_t>((uint64_t{1} << a.page_shift) / a.page + 1);
+        page_division(a.page, &a.page_mul, &a.page_shift);
         a.gc = p.gc;
         a.ngr = p.ngr;
         a.H = p.H;

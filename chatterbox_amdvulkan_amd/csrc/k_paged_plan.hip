@@ -6,15 +6,16 @@
 //   tok_s = sum_{r < s} new_r,    off_s = sum_{r < s} need_r
 // (requests refused for another reason than an empty pool add no need):
 // page i of the new ones of s is free[n_free - 1 - off_s - i], and token j of
-// s has position past_s + j in page (past_s + j) / P.  Granted requests that
+// s has position past_s + j in page (past_s + j) / P (the first key of a new
+// page is one of the tokens, which notes it in the table).  Granted requests that
 // need a page are a prefix of all that do, so what they take is the top of
 // the stack without gaps.
 //
 // A few KB of data: latency is everything.  Every workgroup makes the two
 // scans for itself in LDS (a few requests a lane, a wave scan by DPP, four wave
 // totals), so one launch does without a second pass or a message between
-// workgroups, and then fills its part of the tokens and pages, finding the
-// request of every fourth token by a search over the scan.
+// workgroups, and then fills its part of the tokens, finding the request of
+// every fourth by a search over the scan.
 #include "cbx_device.h"
 
 namespace cbx {
@@ -31,6 +32,18 @@ __device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min
 // Within rows of 16 lanes by shifts, then each row's last to the rows behind.
 template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_sat_add(uint32_t x) {
     return sat_add(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false)));
+}
+// The largest of the wave's values, in lane 63.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+    return max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = dpp_max<0x111, 0xf>(x);
+    x = dpp_max<0x112, 0xf>(x);
+    x = dpp_max<0x114, 0xf>(x);
+    x = dpp_max<0x118, 0xf>(x);
+    x = dpp_max<0x142, 0xa>(x);
+    return dpp_max<0x143, 0xc>(x);
 }
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
@@ -72,19 +85,18 @@ __device__ __forceinline__ int32_t* table_row(char* tables, int64_t nb1, int s) 
 
 constexpr int kPlanTokens = 4;   // neighbouring tokens of a thread
 constexpr int kPlanHeld = 4;     // requests a thread reads at once
+typedef int32_t i4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // LDS: tok[n], off[n], have[n] (have -1: refused), past[n], each 32-bit.
 __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t* err) {
     extern __shared__ int32_t lds32[];
     __shared__ uint32_t part[2][kPlanThreads / 64];
-    __shared__ int32_t took;
     const int tid = threadIdx.x, n = a.n_seq;
     int32_t *tok = lds32, *off = lds32 + n, *have = lds32 + 2 * n, *had = lds32 + 3 * n;
     const int32_t cap = a.max_pages * a.page;      // below 2^31
     int32_t free_n = *a.n_free;
     bool wrong = free_n < 0 || free_n > a.pool;
     free_n = free_n < 0 ? 0 : min(free_n, a.pool);
-    if (tid == 0) took = 0;
     // a lane's requests are neighbours: c of them from c * tid on
     const int c = (n + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(tid * c, n), s1 = min(s0 + c, n);
@@ -107,7 +119,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t*
     }
     uint32_t n_tok, n_pages;
     uint32_t t = block_scan(toks, part[0], &n_tok), pages = 0;
-    auto pages_of = [&](int32_t len) { return static_cast<int32_t>((static_cast<uint32_t>(len) + a.page - 1) / a.page); };
+    // for lengths and positions up to max_pages * page_size
+    auto page_of = [&](int32_t pos) {
+        return static_cast<int32_t>((static_cast<uint64_t>(static_cast<uint32_t>(pos)) * a.page_mul) >> a.page_shift);
+    };
+    auto pages_of = [&](int32_t len) { return len > 0 ? page_of(len - 1) + 1 : 0; };
     for (int s = s0; s < s1; s++) {
         const int32_t past = had[s], nw = off[s];
         const uint32_t end = sat_add(t, max(nw, 0));
@@ -121,17 +137,22 @@ __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t*
         pages = sat_add(pages, need);
         t = end;
     }
-    uint32_t o = block_scan(pages, part[1], &n_pages);
+    uint32_t o = block_scan(pages, part[1], &n_pages), granted = 0;
     for (int s = s0; s < s1; s++) {
         const uint32_t need = static_cast<uint32_t>(off[s]), end = sat_add(o, need);
         off[s] = static_cast<int32_t>(o);
         if (need > 0) {
             if (end > static_cast<uint32_t>(free_n)) have[s] = -1;
-            else atomicMax(&took, static_cast<int32_t>(end));   // in LDS; the largest, in any order
+            else granted = end;
         }
         o = end;
     }
+    granted = wave_max(granted);
+    if ((tid & 63) == 63) part[0][tid >> 6] = granted;
     __syncthreads();
+    uint32_t took = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; w++) took = max(took, part[0][w]);
     if (blockIdx.x == 0) {
         for (int s = tid; s < n; s += kPlanThreads) {
             a.seq_lens[s] = have[s] < 0 ? had[s] : had[s] + a.n_new[s];
@@ -139,41 +160,49 @@ __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t*
         }
         if (tid == 0) {
             a.tok_start[n] = static_cast<int32_t>(n_tok);
-            *a.n_free_out = free_n - took;
+            *a.n_free_out = free_n - static_cast<int32_t>(took);
         }
     }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kPlanThreads;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid;
-    for (int64_t i0 = first * kPlanTokens; i0 < a.n_slots; i0 += step * kPlanTokens) {
-        int32_t slot[kPlanTokens], pos[kPlanTokens], page[kPlanTokens];
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kPlanThreads * kPlanTokens;
+    for (int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kPlanThreads + tid) * kPlanTokens; i0 < a.n_slots; i0 += step) {
+        int32_t slot[kPlanTokens], pos[kPlanTokens], page[kPlanTokens], in[kPlanTokens];
+        int32_t* fresh[kPlanTokens];                // where a page newly taken is noted, by its first token
         int s = i0 < n_tok ? last_at_most(tok, n, static_cast<int32_t>(i0)) : 0;
 #pragma unroll
         for (int k = 0; k < kPlanTokens; k++) {     // the pages' loads first, together
             const int64_t i = i0 + k;
-            page[k] = -1;
-            pos[k] = slot[k] = 0;
+            page[k] = slot[k] = -1;
+            pos[k] = in[k] = 0;
+            fresh[k] = nullptr;
             if (i >= n_tok || i >= a.n_slots) continue;
             while (s + 1 < n && tok[s + 1] <= i) s++;
             pos[k] = had[s] + static_cast<int32_t>(i - tok[s]);
             if (have[s] < 0) continue;
-            slot[k] = 1;
-            const int32_t pi = static_cast<int32_t>(static_cast<uint32_t>(pos[k]) / static_cast<uint32_t>(a.page));
-            page[k] = pi < have[s] ? table_row(a.tables, a.tables_nb1, s)[pi] : a.free_pages[free_n - 1 - off[s] - (pi - have[s])];
+            slot[k] = 0;
+            const int32_t pi = page_of(pos[k]);
+            in[k] = pos[k] - pi * a.page;
+            int32_t* entry = table_row(a.tables, a.tables_nb1, s) + pi;
+            const bool taken = pi >= have[s];
+            page[k] = taken ? a.free_pages[free_n - 1 - off[s] - (pi - have[s])] : *entry;
+            if (taken && in[k] == 0) fresh[k] = entry;
         }
 #pragma unroll
         for (int k = 0; k < kPlanTokens; k++) {
-            if (i0 + k >= a.n_slots) break;
-            const int64_t p = static_cast<int64_t>(page[k]) * a.page + static_cast<uint32_t>(pos[k]) % static_cast<uint32_t>(a.page);
+            const int64_t p = static_cast<int64_t>(page[k]) * a.page + in[k];
             const bool good = page[k] >= 0 && p < kMostCount;
-            wrong |= slot[k] && !good;
-            a.slots[i0 + k] = slot[k] && good ? static_cast<int32_t>(p) : -1;
-            a.positions[i0 + k] = pos[k];
+            wrong |= slot[k] == 0 && !good;
+            slot[k] = slot[k] == 0 && good ? static_cast<int32_t>(p) : -1;
+            if (fresh[k]) *fresh[k] = page[k];
         }
-    }
-    // the pages newly taken: took of them, in the order of the requests
-    for (int64_t i = first; i < took; i += step) {
-        const int s = last_at_most(off, n, static_cast<int32_t>(i));
-        table_row(a.tables, a.tables_nb1, s)[have[s] + (i - off[s])] = a.free_pages[free_n - 1 - i];
+        if (i0 + kPlanTokens <= a.n_slots) {
+            *reinterpret_cast<i4u*>(a.slots + i0) = i4u{slot[0], slot[1], slot[2], slot[3]};
+            *reinterpret_cast<i4u*>(a.positions + i0) = i4u{pos[0], pos[1], pos[2], pos[3]};
+        } else {
+            for (int k = 0; k < static_cast<int>(a.n_slots - i0); k++) {
+                a.slots[i0 + k] = slot[k];
+                a.positions[i0 + k] = pos[k];
+            }
+        }
     }
     if (wrong) atomicOr(err, DEV_ERR_PAGE);
 }
@@ -227,7 +256,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_
 
 }  // namespace
 
-int launch_paged_append(const AppendArgs& a, DeviceState* st, hipStream_t s) {
+int launch_paged_append(const AppendArgs& args, DeviceState* st, hipStream_t s) {
+    AppendArgs a = args;
+    page_division(a.page, &a.page_mul, &a.page_shift);
     const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(cdiv(a.n_slots, kPlanThreads * kPlanTokens), 4 * st->n_cu));
     hipLaunchKernelGGL(k_append, dim3(static_cast<unsigned>(grid)), dim3(kPlanThreads), 16 * static_cast<size_t>(a.n_seq), s,
                        a, st->err_word);
