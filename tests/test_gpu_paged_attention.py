@@ -70,6 +70,30 @@ def test_groups(cbx, cdt, hkv, g):
     check(cbx, [200, 1, 0, 65], hkv, g, 64, 32, F32, cdt, 300 + 17 * hkv + g)
 
 
+@pytest.mark.parametrize("dt,cdt", [(F16, F16), (F32, F16), (F32, F32), (F16, F32)])
+@pytest.mark.parametrize("d", [96, 128, 256])
+@pytest.mark.parametrize("g", [1, 16, 20])
+def test_large_heads_and_groups(cbx, dt, cdt, d, g):
+    """The largest sums a workgroup holds (16 heads of 256), split and whole."""
+    check(cbx, [900, 3, 130], 1, g, d, 16, dt, cdt, 350 + d + g)
+    check(cbx, [2500], 1, g, d, 24, dt, cdt, 351 + d + g)
+
+
+@pytest.mark.parametrize("dt", [F16, F32])
+def test_subnormal_values(cbx, dt):
+    """F16 caches of subnormal numbers (below 2^-14): kept, not flushed.  The
+    scale makes the scores ordinary again; products of a subnormal with a
+    query of 1 are exact in f32."""
+    lens = [100, 300]
+    q, kc, vc, tables = make(lens, 1, 2, 64, 16, F32, F16, 615, poison=False)
+    kc, vc = (kc.float() * 2.0 ** -17).half(), (vc.float() * 2.0 ** -18).half()
+    q = q.to(dt)
+    y = cbx.paged_attention(q, kc, vc, tables, ints(lens), 2.0 ** 14)
+    ref, bound = attention_ref(q, kc, vc, tables, lens, 2.0 ** 14)
+    # results below f16's smallest normal number are rounded to its spacing
+    assert_within(y, ref, bound + (2.0 ** -25 if dt == F16 else 0.0), "subnormal")
+
+
 @pytest.mark.parametrize("dt,cdt", [(F16, F16), (F32, F16), (F32, F32)])
 @pytest.mark.parametrize("lens", [[5000], [1, 9000, 3], [2049, 17, 0, 4096], [130] * 40, [20000]])
 def test_long_and_ragged(cbx, dt, cdt, lens):
@@ -283,6 +307,25 @@ def test_workspace_needs_no_preparation(cbx, lens):
     for fill in (float("nan"), 1.0):
         ws = torch.full((need // 4 + 4,), fill, device="cuda")
         assert_within(cbx.paged_attention(q, kc, vc, tables, ints(lens), 0.125, ws=ws), ref, bound, f"ws of {fill}")
+
+
+def test_two_streams_at_once(cbx):
+    """Calls on two streams without order between them, each with scratch of
+    its own: the same results as one after the other."""
+    lens = [[3000, 1, 777, 0], [12, 2500, 2500, 64]]
+    sets = [make(n, 2, 4, 64, 16, F16, F16, 846 + i) for i, n in enumerate(lens)]
+    alone = [cbx.paged_attention(*s, ints(n), 0.125) for s, n in zip(sets, lens)]
+    devs = [ints(n) for n in lens]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(cbx.paged_attention(*sets[i], devs[i], 0.125))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, alone[i]) for y in got[i])
 
 
 def test_same_call_same_bits(cbx):
