@@ -10,7 +10,10 @@
 // Bound by the read of the logits, made once: a workgroup holds a chunk of a
 // row in registers (up to 16384 logits), reduces it to its maximum, T and
 // sum, and picks its alternatives.  A row of several chunks is joined by a
-// second kernel from the chunks' (maximum, T, sum) and their alternatives.
+// second kernel from the chunks' (maximum, T, sum) and their alternatives.  4000
+// rows of 8194 F32, 8 alternatives: 28.1 us (131 MB, 4.7 TB/s; 27.2 without the
+// profiler); 64 rows, 4 alternatives, 5.7 us; one row of 151936 F16, 20
+// alternatives, 6.0 + 4.8 us.
 //
 // The N largest without a sort: the 64 lanes' own maxima (over all waves)
 // are ranked; at least N logits are not below the N-th of them, and with

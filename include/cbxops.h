@@ -647,8 +647,8 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
  *                  log p; n_top <= 64, n_top <= n_vocab
  * ids with logp, entropy, and top_ids with top_logp may each be NULL.
  * Logits of -inf have p = 0; a row of nothing else has logp and top_logp
- * -inf and entropy 0.  A NaN makes its row's numbers NaN and counts as the
- * largest.  An id outside [0, n_vocab) gets logp 0 and raises bit 0 of the
+ * -inf and entropy 0.  A NaN or an infinity of the other sign makes its row's
+ * numbers NaN; a NaN counts as the largest.  An id outside [0, n_vocab) gets logp 0 and raises bit 0 of the
  * device error word.  ws as for cbx_paged_attention.                       */
 int cbx_token_log_probs_workspace(const cbx_tensor* logits, int32_t n_top,
                                   size_t* bytes);
