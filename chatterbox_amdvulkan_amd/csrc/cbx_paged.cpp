@@ -147,6 +147,27 @@ int check_apart(const char* what, const cbx_tensor* const* outs, const char* con
     return CBX_OK;
 }
 
+// Scratch of at least `need` bytes, apart from the call's n tensors.
+int check_scratch(const char* what, const void* ws, size_t ws_bytes, size_t need, const cbx_tensor* const* ts, int n) {
+    if (ws_bytes < need || (need && !ws)) {
+        return set_error(CBX_ERR_INVALID_ARG, std::string(what) + ": ws needs " + std::to_string(need) + " bytes");
+    }
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return bad(what, "ws must be 16-byte aligned");
+    if (need == 0) return CBX_OK;
+    cbx_tensor w{};
+    w.data = const_cast<void*>(ws);
+    w.type = CBX_TYPE_F32;
+    const int64_t words = cdiv(static_cast<int64_t>(need), 4);
+    for (int i = 0; i < 4; i++) {
+        w.ne[i] = i == 0 ? words : 1;
+        w.nb[i] = i == 0 ? 4 : 4 * static_cast<size_t>(words);
+    }
+    for (int i = 0; i < n; i++) {
+        if (ts[i] && nelements(ts[i]) > 0 && bytes_overlap(&w, ts[i])) return overlap_error(what, "ws", "a tensor of the call");
+    }
+    return CBX_OK;
+}
+
 const int32_t* ints_of(const cbx_tensor* t) { return static_cast<const int32_t*>(t->data); }
 int32_t* ints_of(cbx_tensor* t) { return static_cast<int32_t*>(t->data); }
 
@@ -438,10 +459,8 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache, const cb
     if (!st) return rc;
     if (nelements(q) == 0) return CBX_OK;
     const size_t need = paged_attention_workspace(q, k_cache, block_tables, st);
-    if (ws_bytes < need || (need && !ws)) {
-        return set_error(CBX_ERR_INVALID_ARG, std::string(what) + ": ws needs " + std::to_string(need) + " bytes");
-    }
-    if (reinterpret_cast<uintptr_t>(ws) % 16) return bad(what, "ws must be 16-byte aligned");
+    const cbx_tensor* all[] = {q, k_cache, v_cache, block_tables, seq_lens, y};
+    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 6))) return rc;
     PagedAttnCall c{q, k_cache, v_cache, block_tables, seq_lens, y, scale, softcap, window, ws};
     return launch_paged_attention(c, st, reinterpret_cast<hipStream_t>(stream));
 }
@@ -509,10 +528,8 @@ int cbx_token_log_probs(const cbx_tensor* logits, const cbx_tensor* ids, float s
     if (!st) return rc;
     if (rows == 0) return CBX_OK;
     const size_t need = token_log_probs_workspace(logits, static_cast<int>(n_top), st);
-    if (ws_bytes < need || (need && !ws)) {
-        return set_error(CBX_ERR_INVALID_ARG, std::string(what) + ": ws needs " + std::to_string(need) + " bytes");
-    }
-    if (reinterpret_cast<uintptr_t>(ws) % 16) return bad(what, "ws must be 16-byte aligned");
+    const cbx_tensor* all[] = {logits, ids, logp, entropy, top_ids, top_logp};
+    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 6))) return rc;
     LogProbCall c{logits, ids, logp, entropy, n_top ? top_ids : nullptr, n_top ? top_logp : nullptr, scale,
                   static_cast<int>(n_top), ws};
     return launch_token_log_probs(c, st, reinterpret_cast<hipStream_t>(stream));

@@ -624,7 +624,7 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
  * ws: 16-byte aligned scratch of at least the bytes that
  * cbx_paged_attention_workspace gives for these shapes (it may be 0), used by
  * this call only: nothing in it needs to be set or kept, and calls that may
- * run at the same time need one each.                                      */
+ * run at the same time need one each; it overlaps none of the tensors.     */
 int cbx_paged_attention_workspace(const cbx_tensor* q,
                                   const cbx_tensor* k_cache,
                                   const cbx_tensor* block_tables,
