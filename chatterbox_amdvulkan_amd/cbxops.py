@@ -919,6 +919,8 @@ def paged_append(n_past, n_new, free_pages, n_free, block_tables, page_size, n_s
     the last token).  A request that does not fit keeps its length and gets
     slots of -1.  out: the five tensors to write to."""
     a, b, c, d, e = out or (None,) * 5
+    if out and any(t is None for t in out):
+        raise CbxError(ERR_INVALID_ARG, "paged_append: out holds all five tensors")
     return _call("paged_append", n_past, n_new, free_pages, n_free, block_tables, page_size, n_slots, a, b, c, d, e)
 
 

@@ -12,6 +12,8 @@ namespace cbx {
 namespace {
 
 constexpr int64_t k2G = int64_t{1} << 31;
+// Workgroups of 256 threads stay below this many: a launch has fewer than 2^32 threads.
+constexpr int64_t kMostGroups = int64_t{1} << 24;
 
 int fail(int code, const char* what, const char* msg) { return set_error(code, std::string(what) + ": " + msg); }
 int bad(const char* what, const char* msg) { return fail(CBX_ERR_INVALID_ARG, what, msg); }
@@ -274,8 +276,8 @@ static int check_kv_rows(const cbx_tensor* k, const cbx_tensor* v, const cbx_ten
 }
 
 static int check_row_count(const char* what, int64_t tok, int64_t heads, int64_t d) {
-    if (tok >= k2G || heads >= k2G || tok * heads >= k2G || d > 512) {
-        return fail(CBX_ERR_UNSUPPORTED, what, "head_dim up to 512 and fewer than 2^31 rows");
+    if (tok >= kMostGroups || heads >= k2G || tok * heads >= k2G || d > 512) {
+        return fail(CBX_ERR_UNSUPPORTED, what, "head_dim up to 512, fewer than 2^24 tokens and 2^31 rows");
     }
     return CBX_OK;
 }
@@ -417,9 +419,9 @@ static int check_attention(const char* what, const cbx_tensor* q, const cbx_tens
     const int64_t hkv = k_cache->ne[2];
     if (hkv == 0 ? q->ne[1] != 0 : q->ne[1] % hkv != 0) return bad(what, "n_head must be a multiple of n_head_kv");
     const int64_t keys = tables->ne[0] * k_cache->ne[1];
-    if (q->ne[0] > 512 || q->ne[1] >= k2G || q->ne[2] >= k2G || q->ne[1] * q->ne[2] >= k2G / 64 ||
+    if (q->ne[0] > 512 || q->ne[1] >= k2G || q->ne[2] >= k2G || q->ne[1] * q->ne[2] >= kMostGroups ||
         (keys / 32 + 1) * q->ne[1] * q->ne[2] >= (int64_t{1} << 40)) {
-        return fail(CBX_ERR_UNSUPPORTED, what, "head_dim up to 512, n_head * n_seq below 2^25");
+        return fail(CBX_ERR_UNSUPPORTED, what, "head_dim up to 512, n_head * n_seq below 2^24");
     }
     return CBX_OK;
 }
@@ -471,7 +473,7 @@ static int check_logits(const char* what, const cbx_tensor* x, int64_t n_top) {
     if (x->ne[2] != 1 || x->ne[3] != 1) return bad(what, "logits must be (n_vocab, n_tok, 1, 1)");
     if (n_top < 0 || n_top > kLogProbTop) return fail(CBX_ERR_UNSUPPORTED, what, "n_top must be 0 to 64");
     if (x->ne[1] > 0 && (x->ne[0] == 0 || n_top > x->ne[0])) return bad(what, "n_vocab must be at least 1 and n_top");
-    if (x->ne[0] >= k2G - 65536 || x->ne[1] >= k2G / 64) return fail(CBX_ERR_UNSUPPORTED, what, "n_vocab or n_tok too large");
+    if (x->ne[0] >= k2G - 65536 || x->ne[1] >= kMostGroups) return fail(CBX_ERR_UNSUPPORTED, what, "n_vocab or n_tok too large");
     return CBX_OK;
 }
 

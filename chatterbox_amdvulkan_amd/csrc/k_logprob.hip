@@ -484,7 +484,9 @@ int launch_token_log_probs(const LogProbCall& c, DeviceState* st, hipStream_t s)
     a.chunks = p.chunks;
     a.sums = static_cast<float4*>(c.ws);
     a.keys = reinterpret_cast<uint64_t*>(static_cast<char*>(c.ws) + p.sums_bytes);
-    if (static_cast<uint64_t>(a.rows) * a.chunks * (a.n_top + 1) >= (uint64_t{1} << 31)) {
+    // a launch's threads below 2^32
+    if (static_cast<uint64_t>(a.rows) * a.chunks >= (uint64_t{1} << 24) ||
+        static_cast<uint64_t>(a.rows) * a.chunks * (a.n_top + 1) >= (uint64_t{1} << 31)) {
         return set_error(CBX_ERR_UNSUPPORTED, "cbx_token_log_probs: too many logits");
     }
     if (c.x->type == CBX_TYPE_F16) launch_lp<uint16_t>(a, s);

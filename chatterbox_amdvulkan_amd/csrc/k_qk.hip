@@ -327,6 +327,9 @@ int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
         else launch_heads<float, float>(a, tok, s);
         return check_launch("cbx_qk_norm_rope");
     }
+    if (grid.x >= 1u << 24) {     // a launch's threads below 2^32
+        return set_error(CBX_ERR_UNSUPPORTED, "cbx_qk_norm_rope: 2^26 rows or more, at sizes or alignments that vectors do not take");
+    }
     if (t16 && c16) hipLaunchKernelGGL((k_qk<uint16_t, uint16_t>), grid, block, 0, s, a);
     else if (t16) hipLaunchKernelGGL((k_qk<uint16_t, float>), grid, block, 0, s, a);
     else if (c16) hipLaunchKernelGGL((k_qk<float, uint16_t>), grid, block, 0, s, a);

@@ -580,7 +580,8 @@ int cbx_paged_release(const cbx_tensor* seq_lens, const cbx_tensor* release,
  * cache view): row t of k and v, F32 or F16 (head_dim, n_head_kv, n_tok),
  * goes to slot slots[t], rounded to the cache's type; negative slots are
  * skipped.  The non-negative slots of a call are distinct; a slot given
- * twice gets each head's row from one of its tokens.                       */
+ * twice gets each head's row from one of its tokens.  n_tok < 2^24 (as of
+ * the two calls below).                                                    */
 int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v,
                     const cbx_tensor* slots, cbx_tensor* k_cache,
                     cbx_tensor* v_cache, cbx_stream stream);
@@ -618,7 +619,8 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
  * q, y: F32 or F16 (head_dim, n_head, n_seq), one type; n_head a multiple of
  * n_head_kv, query head h reads key head h / (n_head / n_head_kv).  A request
  * without keys gets zeros; keys past its length are never looked at, whatever
- * the page holds there.  head_dim <= 512.  Scores, sums and products are
+ * the page holds there; an infinity among those looked at may give NaN.
+ * head_dim <= 512, n_head * n_seq < 2^24.  Scores, sums and products are
  * held in f32, also between the parts that a long request is split into;
  * where the parts begin depends on all of the call's lengths.
  * ws: 16-byte aligned scratch of at least the bytes that
@@ -644,7 +646,7 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
  *   top_ids, top_logp
  *                  I32 and F32 (n_top, n_tok): the n_top largest logits'
  *                  tokens, largest first, equal ones by number, and their
- *                  log p; n_top <= 64, n_top <= n_vocab
+ *                  log p; n_top <= 64, n_top <= n_vocab, n_tok < 2^24
  * ids with logp, entropy, and top_ids with top_logp may each be NULL.
  * Logits of -inf have p = 0; a row of nothing else has logp and top_logp
  * -inf and entropy 0.  A NaN or an infinity of the other sign makes its row's
