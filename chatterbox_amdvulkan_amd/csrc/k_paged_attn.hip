@@ -384,7 +384,7 @@ template <int DP> struct Core<uint16_t, DP> {
             for (int r = 0; r < 4; r++) s[4 * h + r] = t[r];
         }
     }
-    static constexpr float kBias = 14.0f;   // probabilities times 2^14
+    static constexpr float kUp = 16384.0f;   // what probabilities are multiplied by
     __device__ __forceinline__ void add_values(const float (&p)[NE]) {
         h8v ph, pl;
 #pragma unroll
@@ -458,7 +458,7 @@ template <int DP> struct Core<float, DP> {
 #pragma unroll
         for (int r = 0; r < 4; r++) s[r] = t[r];
     }
-    static constexpr float kBias = 0.0f;
+    static constexpr float kUp = 1.0f;
     __device__ __forceinline__ void add_values(const float (&p)[NE]) {
 #pragma unroll
         for (int r = 0; r < NE; r++) {
@@ -688,7 +688,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 float p[NE];
 #pragma unroll
                 for (int e = 0; e < NE; e++) {
-                    p[e] = __builtin_amdgcn_exp2f(sc[e] - (m - C::kBias));
+                    p[e] = __builtin_amdgcn_exp2f(sc[e] - m) * C::kUp;   // the difference alone: exact at the maximum, 0 there
                     l += p[e];
                 }
                 core.add_values(p);

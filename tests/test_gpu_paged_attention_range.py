@@ -1,0 +1,58 @@
+"""paged_attention at scores of millions."""
+import numpy as np
+import pytest
+import torch
+
+from tests._paged import U32, assert_within, gen, half_step, page_tables
+
+pytestmark = pytest.mark.gpu
+
+F32, F16 = torch.float32, torch.float16
+TYPES = [(F16, F16), (F32, F16), (F32, F32)]
+
+
+def ints(a):
+    return torch.tensor(np.asarray(a, dtype=np.int32), device="cuda")
+
+
+def caches(length, page, d, dt, seed, hkv=1):
+    pages = -(-length // page) + 2
+    tables = page_tables([length], page, -(-length // page), pages, seed).cuda()
+    r = gen(seed)
+    kc, vc = (torch.randn(pages, hkv, page, d, device="cuda", generator=r).to(dt) for _ in range(2))
+    return kc, vc, tables
+
+
+def rows_of(cache, tables, length):
+    """[length, d] of the one request and its one key head."""
+    return cache[tables[0].long(), 0].reshape(-1, cache.shape[-1])[:length]
+
+
+@pytest.mark.parametrize("dt,cdt", TYPES)
+@pytest.mark.parametrize("length,page", [(1, 16), (40, 16), (40, 24), (3000, 64), (3000, 24)])
+@pytest.mark.parametrize("top", [2.0 ** 25, 1.37 * 2 ** 25, 1.9 * 2 ** 25, 1.01 * 2 ** 26, 1.71 * 2 ** 26, 1.3 * 2 ** 27, 1.99 * 2 ** 28])
+def test_scores_of_millions(cbx, dt, cdt, length, page, top):
+    """Scores of `top` powers of two, of both signs, in a whole and in a split
+    key head.  One key ahead of all others by a thousandth (some 2^15 powers
+    of two): y is its value, to the rounding of v times 1 / 1.  All keys
+    alike: every score is rounded the same way, y is the mean of the values,
+    off by n sums and 8 more roundings."""
+    d = 64
+    kc, vc, tables = caches(length, page, d, cdt, 30 + length + page)
+    q = torch.zeros(1, 2, d, dtype=dt, device="cuda")
+    q[..., 3] = 1024.0
+    lens, v = ints([length]), rows_of(vc, tables, length).double()
+    for sign in (1.0, -1.0):
+        scale = sign * top / (1024.0 * 1000.0) * float(np.log(2.0))
+        kc.zero_()
+        kc[..., 3] = 1000.0
+        y = cbx.paged_attention(q, kc, vc, tables, lens, scale).double()
+        ref = v.mean(0).expand(2, d)[None]
+        bound = (length + 8) * U32 * v.abs().mean(0) + half_step(dt) * ref.abs()
+        assert_within(y, ref, bound, f"equal scores, sign {sign}")
+        best = length // 2
+        kc[..., 3] = 999.0 if sign > 0 else 1000.0
+        kc[tables[0, best // page], 0, best % page, 3] = 1000.0 if sign > 0 else 999.0
+        y = cbx.paged_attention(q, kc, vc, tables, lens, scale).double()
+        ref = v[best].expand(2, d)[None]
+        assert_within(y, ref, (2 * U32 + half_step(dt)) * ref.abs(), f"one score ahead, sign {sign}")
