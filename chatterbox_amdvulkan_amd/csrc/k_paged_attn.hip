@@ -748,7 +748,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
         }
     }
     if (a.W != 0 && tid == 0) a.split[blockIdx.x] = split;
-    if (wrong && n == 0) atomicOr(a.err, DEV_ERR_PAGE);
+    if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);   // of any lane: each may have looked up another key's page
 }
 
 // Adds up the parts of the key heads that several runs hold, in the order of

@@ -1,9 +1,9 @@
-"""paged_attention at scores of millions."""
+"""paged_attention at scores of millions, and with one bad page at a time."""
 import numpy as np
 import pytest
 import torch
 
-from tests._paged import U32, assert_within, gen, half_step, page_tables
+from tests._paged import U32, assert_within, attention_ref, gen, half_step, page_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,30 @@ def test_scores_of_millions(cbx, dt, cdt, length, page, top):
         y = cbx.paged_attention(q, kc, vc, tables, lens, scale).double()
         ref = v[best].expand(2, d)[None]
         assert_within(y, ref, (2 * U32 + half_step(dt)) * ref.abs(), f"one score ahead, sign {sign}")
+
+
+@pytest.mark.parametrize("cdt", [F16, F32])
+@pytest.mark.parametrize("d", [64, 60])
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 24, 64])
+def test_one_bad_page_alone(cbx, cdt, d, page):
+    """Every entry of a table in its turn no page of the cache, below 0 or
+    past the last: its keys are left out and bit 2 is raised, whichever keys
+    of a step the page holds."""
+    length = 100
+    kc, vc, tables = caches(length, page, d, cdt, 90 + page, hkv=2)
+    q = torch.randn(1, 4, d, device="cuda", generator=gen(91))
+    cbx.device_errors(clear=True)
+    for entry in range(tables.shape[1]):
+        for value in (-1, kc.shape[0], 2 ** 31 - 1):
+            bad = tables.clone()
+            bad[0, entry] = value
+            y = cbx.paged_attention(q, kc, vc, bad, ints([length]), 0.125)
+            assert cbx.device_errors(clear=True) == 4, f"entry {entry} of {value}"
+            ref, bound = attention_ref(q, kc, vc, bad, [length], 0.125)
+            assert_within(y, ref, bound, f"entry {entry} of {value}")
+            # the same entry behind the request's keys, or before its window: not looked at
+            if entry > 0:
+                cbx.paged_attention(q, kc, vc, bad, ints([entry * page]), 0.125)
+            if (entry + 1) * page < length:
+                cbx.paged_attention(q, kc, vc, bad, ints([length]), 0.125, window=length - (entry + 1) * page)
+            assert cbx.device_errors(clear=True) == 0, f"entry {entry} of {value} is not used"
