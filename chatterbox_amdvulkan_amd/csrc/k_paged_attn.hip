@@ -298,9 +298,12 @@ template <int PER> __device__ __forceinline__ uint32_t value_dim(uint32_t m, uin
 template <typename TC, int DP> struct Core;
 
 // f16 pages: 16x16x32 products, f32 sums.  An f32 query is scaled by a power
-// of two to below 2^15 and split into two f16 (22 bits); so is every
-// probability, times 2^14 (the smallest that keep their bits are then 2^-28
-// of the largest).
+// of two to below 2^15 and split into two f16, the lower times 2^12 and summed
+// apart: every element is held to 2^-23 of itself, or to 2^-51 of the largest
+// where that is more (f16 ends at 2^-24, so both halves in one sum ended at 2^-39).
+// A probability is two f16 as well, times 2^14: held to 2^-23 of itself, those
+// below 2^-28 of the largest to 2^-39 of it.  (Lower halves of these summed
+// apart would take as many registers again as the sums over the values.)
 template <int DP> struct Core<uint16_t, DP> {
     static constexpr int NK = 32, NH = 2, NE = 8;   // keys a step, halves of 16, keys whose values a lane holds
     static constexpr int CD = DP / 32, PER = DP / 16;
@@ -329,7 +332,7 @@ template <int DP> struct Core<uint16_t, DP> {
                 const float t = x[i] * up;
                 const _Float16 h = static_cast<_Float16>(t);
                 qh[i / 8][i % 8] = h;
-                ql[i / 8][i % 8] = static_cast<_Float16>(t - static_cast<float>(h));
+                ql[i / 8][i % 8] = static_cast<_Float16>((t - static_cast<float>(h)) * 4096.0f);   // below 2^15
             }
         } else {
 #pragma unroll
@@ -373,15 +376,15 @@ template <int DP> struct Core<uint16_t, DP> {
     __device__ __forceinline__ void scores(float (&s)[NE]) {
 #pragma unroll
         for (int h = 0; h < NH; h++) {
-            f4v t = {};
-            if (two) {
-#pragma unroll
-                for (int c = 0; c < CD; c++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][c], ql[c], t, 0, 0, 0);
-            }
+            f4v t = {}, low = {};
 #pragma unroll
             for (int c = 0; c < CD; c++) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][c], qh[c], t, 0, 0, 0);
+            if (two) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[4 * h + r] = t[r];
+                for (int c = 0; c < CD; c++) low = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[h][c], ql[c], low, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * h + r] = two ? fmaf(low[r], 0x1p-12f, t[r]) : t[r];
         }
     }
     static constexpr float kUp = 16384.0f;   // what probabilities are multiplied by

@@ -620,9 +620,12 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
  * n_head_kv, query head h reads key head h / (n_head / n_head_kv).  A request
  * without keys gets zeros; keys past its length are never looked at, whatever
  * the page holds there; an infinity among those looked at may give NaN.
- * head_dim <= 512, n_head * n_seq < 2^24.  Scores, sums and products are
- * held in f32, also between the parts that a long request is split into;
- * where the parts begin depends on all of the call's lengths.
+ * head_dim <= 512, n_head * n_seq < 2^24.  Scores and sums are held in f32,
+ * also between the parts that a long request is split into; where the parts
+ * begin depends on all of the call's lengths.  Over F16 caches the elements
+ * of an F32 query and the probabilities go into their products with 2^-23 of
+ * themselves (small ones with 2^-51 of their head's largest element, and
+ * 2^-39 of its largest probability).
  * ws: 16-byte aligned scratch of at least the bytes that
  * cbx_paged_attention_workspace gives for these shapes (it may be 0), used by
  * this call only: nothing in it needs to be set or kept, and calls that may

@@ -1,4 +1,5 @@
-"""paged_attention at scores of millions, and with one bad page at a time."""
+"""paged_attention at scores of millions, at queries of a wide range, and with
+one bad page at a time."""
 import numpy as np
 import pytest
 import torch
@@ -56,6 +57,30 @@ def test_scores_of_millions(cbx, dt, cdt, length, page, top):
         y = cbx.paged_attention(q, kc, vc, tables, lens, scale).double()
         ref = v[best].expand(2, d)[None]
         assert_within(y, ref, (2 * U32 + half_step(dt)) * ref.abs(), f"one score ahead, sign {sign}")
+
+
+@pytest.mark.parametrize("cdt", [F16, F32])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 24), (60, 16)])
+@pytest.mark.parametrize("large", [1.0, 1e4, 1e6, 1e8, 1e10])
+def test_queries_of_a_wide_range(cbx, cdt, d, page, large):
+    """An F32 query with one element `large` times the others, where the keys
+    are 0 in that dim: the scores come from the small ones.  Three dims of the
+    query are not 0, so a score is three products (all others are exact
+    zeros): an element is held to 2^-23 of itself or 2^-51 of the largest, 3
+    roundings of the products and sums, one of the scale."""
+    length = 300
+    kc, vc, tables = caches(length, page, d, cdt, 70 + d)
+    q = torch.zeros(1, 1, d, device="cuda")
+    q[..., 1], q[..., d - 2], q[..., 5] = 1.7, -2.3, 3.3 * large
+    kc[..., 5] = 0
+    k, v = rows_of(kc, tables, length).double(), rows_of(vc, tables, length).double()
+    y = cbx.paged_attention(q, kc, vc, tables, ints([length]), 1.0)
+    s = k @ q[0, 0].double()
+    p = torch.softmax(s, -1)
+    size = k.abs() @ q[0, 0].double().abs()
+    err = (6 * U32 * size + 2.0 ** -51 * float(q.abs().max()) * k.abs().sum(-1) + 4 * U32 * s.abs().amax() + 4 * U32).amax()
+    bound = (2 * err + (length + 8) * U32) * (p @ v.abs())
+    assert_within(y[0, 0], p @ v, bound, f"{large}")
 
 
 @pytest.mark.parametrize("cdt", [F16, F32])
