@@ -209,24 +209,68 @@ __global__ __launch_bounds__(kPlanThreads) void k_append(AppendArgs a, uint32_t*
     if (wrong) atomicOr(err, DEV_ERR_PAGE);
 }
 
+// Release.  An entry below 0 is no page (a row given back before, or never
+// filled) and is left out, so the pages of a request are known only from its
+// row, and a row is cleared as it is given back: k_release_count notes how
+// many each released request has (in seq_lens_out, which k_release sets to 0
+// once every workgroup has read them), k_release scans those and gives back.
+// A wave a request, eight entries a lane in flight, packed by ballots: 64
+// requests of 32 pages 5.6 us in a graph, 4096 of 128 23.6, 4 of 8192 23.2 (a
+// workgroup a request 6.4, 59 and 14.1).
+
+// The entries that a request's length covers, when it is released; a length
+// outside the table covers none.
+__device__ __forceinline__ uint32_t released_entries(const ReleaseArgs& a, int s, bool* wrong) {
+    if (a.release[s] == 0) return 0;
+    const int32_t len = a.seq_lens[s];
+    if (len < 0 || len > a.max_pages * a.page) {
+        *wrong = true;
+        return 0;
+    }
+    return (static_cast<uint32_t>(len) + a.page - 1) / a.page;
+}
+
+constexpr int kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanLoads = 8;     // entries of a lane
+
+// Entries i0 + 64 u + lane of a row, -1 past its end.
+__device__ __forceinline__ void load_entries(const int32_t* row, uint32_t i0, uint32_t entries, int32_t (&page)[kPlanLoads]) {
+    const uint32_t i = i0 + (threadIdx.x & 63);
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; u++) page[u] = row[min(i + 64 * u, entries - 1)];
+#pragma unroll
+    for (int u = 0; u < kPlanLoads; u++) if (i + 64 * u >= entries) page[u] = -1;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void k_release_count(ReleaseArgs a, uint32_t* err) {
+    const int s = blockIdx.x * kPlanWaves + (threadIdx.x >> 6);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.n_free_out = 0;      // k_release's workgroups that have read the counts
+    if (s >= a.n_seq) return;
+    bool wrong = false;
+    const uint32_t entries = released_entries(a, s, &wrong);
+    const int32_t* row = table_row(a.tables, a.tables_nb1, s);
+    uint32_t pages = 0;
+    for (uint32_t i0 = 0; i0 < entries; i0 += 64 * kPlanLoads) {
+        int32_t page[kPlanLoads];
+        load_entries(row, i0, entries, page);
+#pragma unroll
+        for (int u = 0; u < kPlanLoads; u++) pages += __popcll(__ballot(page[u] >= 0));
+    }
+    if ((threadIdx.x & 63) != 0) return;
+    a.seq_lens_out[s] = a.release[s] ? static_cast<int32_t>(pages) : a.seq_lens[s];
+    if (wrong || pages != entries) atomicOr(err, DEV_ERR_PAGE);
+}
+
 // LDS: off[n], the place above the stack of each released request's first page.
 __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_t* err) {
     extern __shared__ int32_t off[];
-    __shared__ uint32_t part[kPlanThreads / 64];
-    const int tid = threadIdx.x, n = a.n_seq;
-    const int32_t cap = a.max_pages * a.page;
+    __shared__ uint32_t part[kPlanWaves];
+    __shared__ bool last;
+    const int tid = threadIdx.x, lane = tid & 63, n = a.n_seq;
     int32_t free_n = *a.n_free;
     bool wrong = free_n < 0 || free_n > a.pool;
     free_n = free_n < 0 ? 0 : min(free_n, a.pool);
-    auto pages_of = [&](int s) -> uint32_t {
-        const int32_t len = a.seq_lens[s];
-        if (a.release[s] == 0) return 0;
-        if (len < 0 || len > cap) {
-            wrong = true;
-            return 0;
-        }
-        return (static_cast<uint32_t>(len) + a.page - 1) / a.page;
-    };
+    auto pages_of = [&](int s) -> uint32_t { return a.release[s] ? static_cast<uint32_t>(a.seq_lens_out[s]) : 0; };
     const int c = (n + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(tid * c, n), s1 = min(s0 + c, n);
     uint32_t sum = 0;
@@ -240,18 +284,31 @@ __global__ __launch_bounds__(kPlanThreads) void k_release(ReleaseArgs a, uint32_
     __syncthreads();
     const int64_t room = a.pool - free_n;
     wrong |= total > room;
-    if (blockIdx.x == 0) {
-        for (int s = tid; s < n; s += kPlanThreads) a.seq_lens_out[s] = a.release[s] ? 0 : a.seq_lens[s];
+    // the counts are read: whoever is last to say so may overwrite them
+    if (tid == 0) last = __hip_atomic_fetch_add(a.n_free_out, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int32_t>(gridDim.x) - 1;
+    __syncthreads();
+    if (last) {
+        for (int s = tid; s < n; s += kPlanThreads) if (a.release[s]) a.seq_lens_out[s] = 0;
         if (tid == 0) *a.n_free_out = static_cast<int32_t>(free_n + (total < room ? total : room));
     }
-    if (wrong) atomicOr(err, DEV_ERR_PAGE);
-    for (int s = blockIdx.x; s < n; s += gridDim.x) {
-        const uint32_t pages = pages_of(s);
+    if (wrong && tid == 0) atomicOr(err, DEV_ERR_PAGE);
+    bool told = false;     // by k_release_count
+    for (int s = blockIdx.x * kPlanWaves + (tid >> 6); s < n; s += gridDim.x * kPlanWaves) {
+        const uint32_t entries = released_entries(a, s, &told);
         int32_t* row = table_row(a.tables, a.tables_nb1, s);
-        for (uint32_t i = tid; i < pages; i += kPlanThreads) {
-            const int32_t page = row[i];
-            row[i] = -1;
-            if (static_cast<int64_t>(off[s]) + i < room) a.free_pages[free_n + off[s] + i] = page;
+        int64_t to = off[s];
+        for (uint32_t i0 = 0; i0 < entries; i0 += 64 * kPlanLoads) {
+            int32_t page[kPlanLoads];
+            load_entries(row, i0, entries, page);
+#pragma unroll
+            for (int u = 0; u < kPlanLoads; u++) {
+                const uint32_t i = i0 + 64 * u + lane;
+                if (i < entries) row[i] = -1;
+                const uint64_t given = __ballot(page[u] >= 0);
+                const int64_t at_page = to + __popcll(given & ((uint64_t{1} << lane) - 1));
+                if (page[u] >= 0 && at_page < room) a.free_pages[free_n + at_page] = page[u];
+                to += __popcll(given);
+            }
         }
     }
 }
@@ -268,7 +325,8 @@ int launch_paged_append(const AppendArgs& args, DeviceState* st, hipStream_t s) 
 }
 
 int launch_paged_release(const ReleaseArgs& a, DeviceState* st, hipStream_t s) {
-    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(a.n_seq, st->n_cu));
+    const int64_t all = std::max<int64_t>(1, cdiv(a.n_seq, kPlanWaves)), grid = std::min<int64_t>(all, st->n_cu);
+    hipLaunchKernelGGL(k_release_count, dim3(static_cast<unsigned>(all)), dim3(kPlanThreads), 0, s, a, st->err_word);
     hipLaunchKernelGGL(k_release, dim3(static_cast<unsigned>(grid)), dim3(kPlanThreads), 4 * static_cast<size_t>(a.n_seq), s,
                        a, st->err_word);
     return check_launch("cbx_paged_release");

@@ -568,8 +568,10 @@ int cbx_paged_append(const cbx_tensor* n_past, const cbx_tensor* n_new,
 /* Gives back the pages of every request s with release[s] != 0: pushed on
  * the stack in the order of the requests and of their tables, their table
  * entries set to -1, seq_lens_out[s] = 0; the other requests' lengths are
- * copied.  Pages past the stack's end (more given back than were taken) are
- * dropped and raise the error bit.                                         */
+ * copied.  Entries below 0 (a request released twice, a row never filled)
+ * are left out, so that the stack has no holes, and raise the error bit, as
+ * do pages past the stack's end (more given back than were taken), which are
+ * dropped.                                                                 */
 int cbx_paged_release(const cbx_tensor* seq_lens, const cbx_tensor* release,
                       cbx_tensor* block_tables, int32_t page_size,
                       cbx_tensor* free_pages, const cbx_tensor* n_free,
