@@ -555,8 +555,9 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  * A request is refused as a whole when its table row cannot hold
  * n_past + n_new keys, when its tokens do not all lie below n_slots, or when
  * the stack runs out (then also every later one that needs a page): it takes
- * no page, its slots are -1 and its seq_lens entry is n_past[s].  Nothing is
- * kept: the same arguments give the same results, and outputs overlap no
+ * no page, its slots are -1 and its seq_lens entry is n_past[s].  An entry of
+ * the stack that is no page is popped in its turn and noted in the table; the
+ * tokens of it get slots of -1, and bit 2 is raised.  Nothing is kept: the same arguments give the same results, and outputs overlap no
  * input.  n_seq <= 4096; max_pages * page_size < 2^31.                      */
 int cbx_paged_append(const cbx_tensor* n_past, const cbx_tensor* n_new,
                      const cbx_tensor* free_pages, const cbx_tensor* n_free,

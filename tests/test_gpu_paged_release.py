@@ -1,5 +1,5 @@
-"""paged_release where tables hold entries that are no page: whole numbers, so
-everything is equal."""
+"""paged_release where tables hold entries that are no page, and what append
+makes of malformed values: whole numbers, so everything is equal."""
 import numpy as np
 import pytest
 import torch
@@ -105,3 +105,25 @@ def test_captured_release(cbx):
         assert [out.tolist(), left.tolist(), tables.tolist(), stack.tolist()] == [exp[0], [exp[1]], exp[2], exp[3]], f"step {step}"
         check(cbx, *a, page, free, 3)
         cbx.device_errors(clear=True)
+
+
+def test_append_beside_malformed_requests(cbx):
+    """A request that needs no page is granted beside others that are
+    malformed and a stack count that is none."""
+    cbx.device_errors(clear=True)
+    t = ints([[-1, -1], [0, -1], [1, -1], [-1, -1]])
+    got = cbx.paged_append(ints([-3, 5, 100, 2]), ints([1, -1, 1, 1]), ints([9, 8]), ints([5]), t, 4, 4)
+    assert cbx.device_errors(clear=True) == 4
+    assert [g.tolist() for g in got] == [[-3, 5, 100, 3], [2], [0, 1, 1, 2, 3], [-1, -1, -1, -1], [-3, 100, 2, 0]]
+    assert t.tolist() == [[-1, -1], [0, -1], [1, -1], [-1, -1]]
+
+
+def test_append_from_a_stack_with_entries_that_are_no_page(cbx):
+    """They are handed out in their turn: noted in the table, their tokens'
+    slots -1, bit 2; the other pages' tokens have theirs."""
+    cbx.device_errors(clear=True)
+    t = ints([[-1, -1], [-1, -1]])
+    got = cbx.paged_append(ints([0, 0]), ints([5, 2]), ints([6, -4, 2]), ints([3]), t, 4, 7)
+    assert cbx.device_errors(clear=True) == 4
+    assert [g.tolist() for g in got] == [[5, 2], [0], [0, 5, 7], [8, 9, 10, 11, -1, 24, 25], [0, 1, 2, 3, 4, 0, 1]]
+    assert t.tolist() == [[2, -4], [6, -1]]
