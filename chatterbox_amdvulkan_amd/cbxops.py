@@ -936,7 +936,7 @@ def paged_store(k, v, slots, k_cache, v_cache):
     """Rows of k and v [n_tok, n_head_kv, head_dim] into their slots of the
     caches [n_pages, n_head_kv, page_size, head_dim] (any strides, so a
     permuted [n_pages, page_size, n_head_kv, head_dim] too), rounded to the
-    caches' type; negative slots are skipped."""
+    caches' type; negative slots are skipped, the others are distinct."""
     _call("paged_store", k, v, slots, k_cache, v_cache)
 
 

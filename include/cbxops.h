@@ -557,8 +557,9 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  * the stack runs out (then also every later one that needs a page): it takes
  * no page, its slots are -1 and its seq_lens entry is n_past[s].  An entry of
  * the stack that is no page is popped in its turn and noted in the table; the
- * tokens of it get slots of -1, and bit 2 is raised.  Nothing is kept: the same arguments give the same results, and outputs overlap no
- * input.  n_seq <= 4096; max_pages * page_size < 2^31.                      */
+ * tokens of it get slots of -1, and bit 2 is raised.  Nothing is kept: the
+ * same arguments give the same results, and outputs overlap no input.
+ * n_seq <= 4096; max_pages * page_size < 2^31.                             */
 int cbx_paged_append(const cbx_tensor* n_past, const cbx_tensor* n_new,
                      const cbx_tensor* free_pages, const cbx_tensor* n_free,
                      cbx_tensor* block_tables, int32_t page_size,
@@ -582,9 +583,9 @@ int cbx_paged_release(const cbx_tensor* seq_lens, const cbx_tensor* release,
 /* Writes key and value rows into their pages (t3.cpp:488-489's cpy into the
  * cache view): row t of k and v, F32 or F16 (head_dim, n_head_kv, n_tok),
  * goes to slot slots[t], rounded to the cache's type; negative slots are
- * skipped.  The non-negative slots of a call are distinct; a slot given
- * twice gets each head's row from one of its tokens.  n_tok < 2^24 (as of
- * the two calls below).                                                    */
+ * skipped.  The non-negative slots of a call are distinct: the rows of a slot
+ * given to several tokens hold elements of all of them in no fixed mixture.
+ * n_tok < 2^24 (as of the two calls below).                                */
 int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v,
                     const cbx_tensor* slots, cbx_tensor* k_cache,
                     cbx_tensor* v_cache, cbx_stream stream);
