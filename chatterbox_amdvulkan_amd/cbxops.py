@@ -917,7 +917,9 @@ def paged_append(n_past, n_new, free_pages, n_free, block_tables, page_size, n_s
     what is left on the stack, the number of each request's first token
     [n_seq + 1], and each token's slot and position [n_slots] (-1 and 0 past
     the last token).  A request that does not fit keeps its length and gets
-    slots of -1.  out: the five tensors to write to."""
+    slots of -1.  The five are views of one allocation: any of them keeps it,
+    and saving one saves all (clone what outlives the step).  out: the five
+    tensors to write to."""
     a, b, c, d, e = out or (None,) * 5
     if out and any(t is None for t in out):
         raise CbxError(ERR_INVALID_ARG, "paged_append: out holds all five tensors")
@@ -987,7 +989,8 @@ def token_log_probs(logits, ids=None, top_n=0, scale=1.0, entropy=True, ws=None)
     """(logp, entropy, top_ids, top_logp) of logits [n_tok, n_vocab] under
     softmax(scale * logits): the log probability of ids[t] (None without
     ids), the entropy (None when not asked for), and the top_n largest logits'
-    tokens and log probabilities [n_tok, top_n], equal logits by number.  ws as
+    tokens and log probabilities [n_tok, top_n], equal logits by number.  logp,
+    entropy and top_logp are views of one allocation, as paged_append's.  ws as
     for paged_attention."""
     return _call("token_log_probs", logits, ids, top_n, scale, entropy, ws)
 
