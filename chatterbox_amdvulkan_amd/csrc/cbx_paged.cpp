@@ -516,6 +516,8 @@ int cbx_token_log_probs(const cbx_tensor* logits, const cbx_tensor* ids, float s
     if (top_ids && ((rc = row_out(top_ids, "top_ids", CBX_TYPE_I32, n_top, rows)) ||
                     (rc = row_out(top_logp, "top_logp", CBX_TYPE_F32, n_top, rows)))) return rc;
     if (!(scale > 0.0f) || std::isinf(scale)) return bad(what, "scale must be finite and > 0");
+    // twice the scale times log2(e) is a factor of the kernels
+    if (scale >= 0x1p126f) return fail(CBX_ERR_UNSUPPORTED, what, "scale must be below 2^126");
     const cbx_tensor* outs[4];
     const char* names[4];
     int n = 0;

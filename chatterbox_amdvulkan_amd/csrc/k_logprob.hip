@@ -3,7 +3,9 @@
 //
 // With z_i = scale (x_i - max x), T = sum exp(z_i):
 //   log p_i = z_i - log T,  H = log T - (sum exp(z_i) z_i) / T
-// (both terms of H are >= 0: nothing cancels).  Order: 64-bit keys of the
+// (both terms of H are >= 0: nothing cancels).  The difference is taken of the
+// halves, exact as it is but for numbers below 2^-125, where it is 2^-150 off:
+// logits of both signs may lie further apart than the largest f32.  Order: 64-bit keys of the
 // logit's bits made monotone and the complement of its index, all distinct,
 // so that the alternatives do not depend on who finds them.
 //
@@ -201,6 +203,9 @@ __device__ __forceinline__ void keep(LpShared& sh, int which, uint64_t k) {
     if (i < kLpMost) sh.kept[i] = k;
 }
 
+// (x - m) / 2, which twice the scale then multiplies.
+__device__ __forceinline__ float half_below(float x, float m) { return fmaf(x, 0.5f, -0.5f * m); }
+
 // A row's results from its maximum, T and sum (in powers of 2).
 struct RowSums {
     float m, T, u;
@@ -209,7 +214,7 @@ struct RowSums {
     __device__ __forceinline__ float log_p(float x, float scale) const {
         if (nan || m == INFINITY) return __builtin_nanf("");
         if (x == -INFINITY) return x;
-        return (x - m) * scale - logf(T);
+        return half_below(x, m) * (2.0f * scale) - logf(T);
     }
     __device__ __forceinline__ float entropy() const {
         if (nan || m == INFINITY) return __builtin_nanf("");
@@ -302,13 +307,13 @@ __global__ __launch_bounds__(kLpThreads, NV <= 4 ? 8 : NV <= 9 ? 6 : 4) void k_l
     RowSums rs;
     rs.m = wave_f32(MaxOf(), lm);
     if (a.n_top) sh.above[wid][lane] = larger_of_16(lm);
-    const float sl = a.scale * kLog2e, off = rs.m == -INFINITY ? 0.0f : rs.m;
+    const float sl = 2.0f * a.scale * kLog2e, off = rs.m == -INFINITY ? 0.0f : rs.m;
     rs.T = rs.u = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float z = (v[j][e] - off) * sl, p = __builtin_amdgcn_exp2f(z);
+            const float z = half_below(v[j][e], off) * sl, p = __builtin_amdgcn_exp2f(z);
             rs.T += p;
             rs.u = fmaf(p, fmaxf(z, -200.0f), rs.u);   // exp2(-200) is 0: 0, not 0 * -inf
         }
@@ -396,13 +401,13 @@ __global__ __launch_bounds__(kLpThreads) void k_logprob_join(LpArgs a) {
     if (a.n_top) sh.above[wid][lane] = larger_of_16(best);
     RowSums rs;
     rs.m = fmaxf(fmaxf(sh.f[0][0], sh.f[0][1]), fmaxf(sh.f[0][2], sh.f[0][3]));
-    const float sl = a.scale * kLog2e;
+    const float sl = 2.0f * a.scale * kLog2e;
     rs.T = rs.u = 0.0f;
     for (uint32_t c = tid; c < a.chunks; c += kLpThreads) {
         const float4 s = sums[c];
         if (s.w != 0.0f) rs.T = __builtin_nanf("");
         if (s.x == -INFINITY) continue;
-        const float z = (s.x - rs.m) * sl, p = __builtin_amdgcn_exp2f(z);
+        const float z = half_below(s.x, rs.m) * sl, p = __builtin_amdgcn_exp2f(z);
         rs.T = fmaf(s.y, p, rs.T);
         if (p > 0.0f) rs.u = fmaf(p, fmaf(s.y, z, s.z), rs.u);
     }

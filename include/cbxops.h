@@ -646,8 +646,8 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
                         void* ws, size_t ws_bytes, cbx_stream stream);
 
 /* What a step answers with: of each row of logits x, F32 or F16
- * (n_vocab, n_tok), with p = softmax(scale * x) (scale > 0: one over the
- * temperature),
+ * (n_vocab, n_tok), with p = softmax(scale * x) (0 < scale < 2^126: one over
+ * the temperature),
  *   logp[t]        F32 (n_tok): log p of token ids[t]
  *   entropy[t]     F32 (n_tok): -sum p log p
  *   top_ids, top_logp
