@@ -534,6 +534,8 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  *   free_pages, n_free
  *             I32: a stack of free page numbers, n_free[0] of them, the top
  *             last
+ * A page has one owner, the stack or one entry of one table: nothing counts
+ * its users, so a page that two tables name is given back twice.
  * All of it lives on the device: no call reads a length on the host, so a
  * captured step replays as its requests grow.  Page numbers, slots and
  * lengths that lie outside their tensors are left out by the kernels that
@@ -624,12 +626,13 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
  * n_head_kv, query head h reads key head h / (n_head / n_head_kv).  A request
  * without keys gets zeros; keys past its length are never looked at, whatever
  * the page holds there; an infinity among those looked at may give NaN.
- * head_dim <= 512, n_head * n_seq < 2^24.  Scores and sums are held in f32,
- * also between the parts that a long request is split into; where the parts
- * begin depends on all of the call's lengths.  Over F16 caches the elements
- * of an F32 query and the probabilities go into their products with 2^-23 of
- * themselves (small ones with 2^-51 of their head's largest element, and
- * 2^-39 of its largest probability).
+ * q . k_i, s_i and the elements of scale * q lie below 2^126 in size (past it
+ * they may count as infinite).  head_dim <= 512, n_head * n_seq < 2^24.
+ * Scores and sums are held in f32, also between the parts that a long request
+ * is split into; where the parts begin depends on all of the call's lengths.
+ * Over F16 caches the elements of an F32 query and the probabilities are
+ * rounded for their products by up to 2^-23 of themselves (small ones by
+ * 2^-51 of their head's largest element, 2^-39 of its largest probability).
  * ws: 16-byte aligned scratch of at least the bytes that
  * cbx_paged_attention_workspace gives for these shapes (it may be 0), used by
  * this call only: nothing in it needs to be set or kept, and calls that may
@@ -657,8 +660,9 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
  * ids with logp, entropy, and top_ids with top_logp may each be NULL.
  * Logits of -inf have p = 0; a row of nothing else has logp and top_logp
  * -inf and entropy 0.  A NaN or an infinity of the other sign makes its row's
- * numbers NaN; a NaN counts as the largest.  An id outside [0, n_vocab) gets logp 0 and raises bit 0 of the
- * device error word.  ws as for cbx_paged_attention.                       */
+ * numbers NaN; a NaN counts as the largest.  An id outside [0, n_vocab) gets
+ * logp 0 and raises bit 0 of the device error word.  ws as for
+ * cbx_paged_attention.                                                     */
 int cbx_token_log_probs_workspace(const cbx_tensor* logits, int32_t n_top,
                                   size_t* bytes);
 int cbx_token_log_probs(const cbx_tensor* logits, const cbx_tensor* ids,
