@@ -2,7 +2,7 @@
 // for the calls of a decode step: descriptors filled and outputs allocated in
 // C++ (a step's call takes 4 to 11 tensors; in Python each descriptor costs
 // more than 1 us, these calls 12 to 14 us of host time together with their
-// outputs, and 5.5 to 6.2 here, the launch included).
+// outputs, and 5.4 to 6.5 here, the launch included).
 //
 // Every function takes its tensors and numbers by position, then the current
 // device's index and the current stream's handle.  It returns the outputs; an

@@ -13,9 +13,9 @@
 // row in registers (up to 16384 logits), reduces it to its maximum, T and
 // sum, and picks its alternatives.  A row of several chunks is joined by a
 // second kernel from the chunks' (maximum, T, sum) and their alternatives.  4000
-// rows of 8194 F32, 8 alternatives: 28.1 us (131 MB, 4.7 TB/s; 27.2 without the
-// profiler); 64 rows, 4 alternatives, 5.7 us; one row of 151936 F16, 20
-// alternatives, 6.0 + 4.8 us.
+// rows of 8194 F32, 8 alternatives: 28.3 us (131 MB, 4.6 TB/s; 27.4 without the
+// profiler); 64 rows, 4 alternatives, 5.6 us; one row of 151936 F16, 20
+// alternatives, 6.2 + 4.8 us.
 //
 // The N largest without a sort: the 64 lanes' own maxima (over all waves)
 // are ranked; at least N logits are not below the N-th of them, and with
@@ -455,6 +455,10 @@ LpPlan lp_plan(const cbx_tensor* x, int n_top, const DeviceState* st) {
 template <typename T>
 void launch_lp(const LpArgs& a, hipStream_t s) {
     const dim3 grid(a.rows * a.chunks), block(kLpThreads);
+    // vectors a thread: the fewest of these that hold the chunk, as those beyond it
+    // are work all the same (4000 rows of 8194 in 16 of them 33.8 us against 25.6 in
+    // 9, of 4096 29.9 / 15.9 in 4, 8000 rows of 1000 51.9 / 17.2 in 1; of 8192 in 9
+    // 25.2 / 24.1 in 8, which no other length would need)
     const uint32_t nv = (a.chunk + 4 * kLpThreads - 1) / (4 * kLpThreads);
     if (nv <= 1) hipLaunchKernelGGL((k_logprob<T, 1>), grid, block, 0, s, a);
     else if (nv <= 2) hipLaunchKernelGGL((k_logprob<T, 2>), grid, block, 0, s, a);

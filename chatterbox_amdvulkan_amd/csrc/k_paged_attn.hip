@@ -17,13 +17,15 @@
 // workgroup finds its run from a scan over them.  A key head whose tiles fall
 // into one run is written to y; the parts of one that spans runs go to the
 // workspace as (m, l, o) and k_attn_join adds them up in order.  8 requests of
-// 1500 to 65000 keys, 32 heads over 8 of 128, F16: 192.1 + 4.8 us (1.09 GB, 5.5
-// TB/s over both); 64 requests of 1 to 2048 keys, 16 heads of 64: 61.0 us (269 MB,
-// 4.4 TB/s; 57.8 without the profiler); 16 heads over 300 keys 7.4 us, dependent
+// 1500 to 65000 keys, 32 heads over 8 of 128, F16: 191.9 + 4.8 us (1.09 GB, 5.5
+// TB/s over both); 64 requests of 1 to 2048 keys, 16 heads of 64: 61.6 us (269 MB,
+// 4.4 TB/s; 58.7 without the profiler); 16 heads over 300 keys 7.0 us, dependent
 // reads (lengths, pages, keys and values).
 //
 // k_attn_rows: head sizes, strides and alignments that the tiles do not take,
-// a workgroup a request and query head, a key's elements over the lanes.
+// a workgroup a request and query head, a key's elements over the lanes: 64
+// requests of 1 to 2048 keys, 16 heads of 60 703 us (of 64, by tiles, 50; of 64 off
+// their alignment 784).
 #include "cbx_device.h"
 
 namespace cbx {
@@ -858,7 +860,10 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     // 9.3, 8 tiles 10.4 against 9.3; S 64, 8 tiles 11.2 / 11.5, 16 tiles 19.7 /
     // 14.0; S 256, 16 tiles 20.7 / 21.4 (head_dim 128: 35 / 41), 32 tiles 43 / 35;
     // S 512, 16 tiles 64 / 73, 32 tiles 123 / 117; S 1024, 32 tiles 114 / 114, 64
-    // tiles 221 / 204: they cross near the square root of S.
+    // tiles 221 / 204: they cross near the square root of S.  Lengths that the
+    // tables' width says little about are worse off by the rule: 300 keys in
+    // tables of 2048 are split for nothing (S 16: 9.6 us against 7.1), one
+    // request of 4096 keys beside 63 of 64 is not (S 1024: 34.7 / 14.0).
     const int64_t S = std::min<int64_t>(q->ne[2] * p.H, 1024);
     p.join = cap_tiles > 7 && cap_tiles * cap_tiles > S;
     if (p.join) {

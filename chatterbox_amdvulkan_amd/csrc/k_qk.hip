@@ -12,9 +12,9 @@
 // only the norm's sum crosses lanes (8 of them a head of 64).  The token's
 // cos and sin of those pairs are read once and serve all its heads: in F16
 // they are twice the bytes of a row.  9001 tokens of 24 + 8 heads of 128, F32 into
-// F16 pages, 62.8 us (328 MB, 5.2 TB/s; k_qk, with q off the alignment, 229), 64
-// tokens of 16 + 16 heads of 64 in F16 4.1 us.  k_qk: a wave a head row, for sizes and alignments that the
-// vectors do not take.
+// F16 pages, 64.2 us (328 MB, 5.1 TB/s; 62.0 without the profiler; k_qk, with q
+// off the alignment, 229), 64 tokens of 16 + 16 heads of 64 in F16 4.1 us.  k_qk:
+// a wave a head row, for sizes and alignments that the vectors do not take.
 #include "cbx_rowops.h"
 
 namespace cbx {
