@@ -84,6 +84,49 @@ def test_released_twice(cbx):
     assert t[:, :2].tolist() == [[7, 8], [5, 9], [6, -1]]
 
 
+def test_no_requests_empty_tables_and_strided_ones(cbx):
+    cbx.device_errors(clear=True)
+    out, left = cbx.paged_release(ints([]), ints([]), ints(np.zeros((0, 3))), 16, ints([4, 2]), ints([2]))
+    assert out.tolist() == [] and left.tolist() == [2]
+    out, left = cbx.paged_release(ints([0, 0]), ints([1, 0]), ints(np.zeros((2, 0))), 16, ints([4, 2]), ints([1]))
+    assert out.tolist() == [0, 0] and left.tolist() == [1]
+    wide = torch.full((3, 9), 77, dtype=torch.int32, device="cuda")
+    view = wide[:, 2:6]
+    view.copy_(ints([[3, -1, 5, 6], [7, 8, 9, -1], [1, 2, 0, 4]]))
+    stack = ints([-9] * 12)
+    _, left = cbx.paged_release(ints([9, 5, 16]), ints([1, 0, 1]), view, 4, stack, ints([0]))
+    assert cbx.device_errors(clear=True) == 4
+    assert left.tolist() == [6] and stack.tolist() == [3, 5, 1, 2, 0, 4] + [-9] * 6
+    assert view.tolist() == [[-1, -1, -1, 6], [7, 8, 9, -1], [-1] * 4]
+    assert bool((wide[:, :2] == 77).all()) and bool((wide[:, 6:] == 77).all())
+
+
+def test_two_streams_at_once(cbx):
+    """Releases of two pools without order between them: each as if alone."""
+    rng = np.random.RandomState(9)
+    n, page, width = 300, 4, 70
+    sets = []
+    for _ in range(2):
+        a = [rng.randint(0, page * width + 1, n).tolist(), rng.randint(0, 2, n).tolist(),
+             np.where(rng.rand(n, width) < 0.1, -1, rng.permutation(n * width).reshape(n, width)).tolist()]
+        sets.append((a, release_ref(*a, page, [-1] * n * width, 0)))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    runs = [[[ints(x) for x in a] + [ints([-1] * n * width), ints([0])] for _ in range(10)] for a, _ in sets]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for j in range(10):
+        for i in range(2):
+            lens, rel, tables, stack, count = runs[i][j]
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(cbx.paged_release(lens, rel, tables, page, stack, count))
+    torch.cuda.synchronize()
+    for i in range(2):
+        lens, n_free, tables, free, _ = sets[i][1]
+        for (out, left), run in zip(outs[i], runs[i]):
+            assert [out.tolist(), left.tolist(), run[2].tolist(), run[3].tolist()] == [lens, [n_free], tables, free]
+    cbx.device_errors(clear=True)
+
+
 def test_captured_release(cbx):
     """Replayed as lengths and tables change, with eager calls between."""
     n, page, width = 9, 4, 12
