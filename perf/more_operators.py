@@ -17,7 +17,7 @@ import torch
 
 own = False
 
-LOWEST_SCALE = 2.0 ** -126                                      # of a row in 8 bits: the smallest normal f32
+LOWEST = 127 * 2.0 ** -126                                      # a row's largest element counts as this at least: normal scales
 TYPES = {"f32": torch.float32, "f16": torch.float16, "i8": torch.int8}
 SIZE = {"f32": 4, "f16": 2, "i8": 1}
 
@@ -142,9 +142,9 @@ def prepare(case, seed):
         """Keys or values of so many pages, and the scale of every row of an 8-bit one."""
         if case["cdt"] != "i8":
             return randn(pages, hkv, page, d, dt=case["cdt"]), None
-        x = randn(pages, hkv, page, d, dt="f16")
-        s = (x.abs().amax(-1).float() / 127).clamp(min=LOWEST_SCALE)
-        return torch.round(x.float() / s[..., None]).to(torch.int8), s
+        x = randn(pages, hkv, page, d, dt="f16").float()
+        top = x.abs().amax(-1).clamp(min=LOWEST)
+        return torch.round(x * 127 / top[..., None]).to(torch.int8), top / 127
 
     if kind == "cache8":
         tok = case["tok"]
@@ -219,9 +219,10 @@ def _cache8(st):
     slots, at = st["slots"][rows].long(), st["slots"].long().clamp(min=0)
     back = []
     for x, c, sc in ((st["k"], st["kc"], st["ks"]), (st["v"], st["vc"], st["vs"])):
-        step = (x.double().abs().amax(-1) / 127).clamp(min=LOWEST_SCALE)   # 64 bits: many values lie next to a border
-        c[slots // page, :, slots % page] = torch.round(x.double() / step[..., None])[rows].to(torch.int8)
-        sc[slots // page, :, slots % page] = step[rows].float()
+        x64 = x.double()                                        # 64 bits: half the largest element lies on a border
+        top = x64.abs().amax(-1).clamp(min=LOWEST)
+        c[slots // page, :, slots % page] = torch.round(x64 * 127 / top[..., None])[rows].to(torch.int8)
+        sc[slots // page, :, slots % page] = (top / 127)[rows].float()
         y = c[at // page, :, at % page].float() * sc[at // page, :, at % page][..., None]
         back.append(torch.where(live[:, None, None], y, torch.zeros_like(y)).to(x.dtype))
     return {"k": back[0], "v": back[1]}
@@ -367,10 +368,12 @@ def exact(case, seed):
     if kind == "cache8":
         def held(x):
             x = x.double()
-            step = x.abs().amax(-1, keepdim=True) / 127
-            x = torch.where(step > 0, torch.round(x / step) * step, x)
-            x[st["slots"] < 0] = 0
-            return x
+            top = x.abs().amax(-1, keepdim=True).clamp(min=LOWEST)
+            n = x * 127 / top
+            whole = torch.floor(n.abs())                        # the nearest whole number, of two the even one
+            rest = n.abs() - whole
+            n = torch.sign(n) * (whole + ((rest > 0.5) | ((rest == 0.5) & (whole % 2 == 1))).double())
+            return torch.where((st["slots"] >= 0)[:, None, None], n * top / 127, torch.zeros_like(x))
 
         return {"k": held(st["k"]), "v": held(st["v"])}
 
