@@ -184,7 +184,7 @@ def prepare(case, seed):
     if kind == "shared":                                        # a group's shared pages are its first request's
         for a, b, p in zip(st["groups"], st["groups"][1:], st["shared"]):
             if b > a:
-                st["tables"][a:b, :p // page] = st["tables"][a, :p // page]
+                st["tables"][a:b, :p // page] = st["tables"][a, :p // page].clone()
     st["lens"], st["host_lens"] = ints(lens), lens.tolist()
     (st["kc"], st["ks"]), (st["vc"], st["vs"]) = cache(pages), cache(pages)
     return st
