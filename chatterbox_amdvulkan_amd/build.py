@@ -47,9 +47,10 @@ SOURCES = [
     "k_paged_plan.hip",
     "k_qk.hip",
     "k_paged_attn.hip",
+    "k_prompt_attn.hip",
     "k_logprob.hip",
 ]
-HEADERS = ["cbx_internal.h", "cbx_device.h", "cbx_rowops.h", os.path.join("..", "..", "include", "cbxops.h")]
+HEADERS = ["cbx_internal.h", "cbx_device.h", "cbx_rowops.h", "cbx_attn.h", os.path.join("..", "..", "include", "cbxops.h")]
 
 ARCH = "gfx950"
 COMMON = [

@@ -24,7 +24,7 @@ LIB_PATH = os.path.join(_HERE, "libcbxops.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "cbxops.h")
 
 # ggml_type numbering
-F32, F16, Q8_0, I32 = 0, 1, 8, 26
+F32, F16, Q8_0, I8, I32 = 0, 1, 8, 24, 26
 QK8_0, Q8_0_BLOCK = 32, 34
 
 # cbx_unary_op
@@ -201,10 +201,18 @@ def load() -> ctypes.CDLL:
         "cbx_paged_append": (i, [P, P, P, P, P, ctypes.c_int32, P, P, P, P, P, vp]),
         "cbx_paged_release": (i, [P, P, P, ctypes.c_int32, P, P, P, P, vp]),
         "cbx_paged_store": (i, [P, P, P, P, P, vp]),
+        "cbx_paged_store_q8": (i, [P, P, P, P, P, P, P, vp]),
+        "cbx_paged_load": (i, [P, P, P, P, P, P, P, vp]),
         "cbx_qk_norm_rope": (i, [P, P, P, P, f, P, vp, P, P, vp]),
         "cbx_qk_norm_rope_store": (i, [P, P, P, P, P, f, P, vp, P, P, P, P, vp]),
+        "cbx_qk_norm_rope_store_q8": (i, [P, P, P, P, P, f, P, vp, P, P, P, P, P, P, vp]),
         "cbx_paged_attention_workspace": (i, [P, P, P, ctypes.POINTER(ctypes.c_size_t)]),
         "cbx_paged_attention": (i, [P, P, P, P, P, f, f, ctypes.c_int32, P, vp, ctypes.c_size_t, vp]),
+        "cbx_paged_attention_q8": (i, [P, P, P, P, P, P, P, f, f, ctypes.c_int32, P, vp, ctypes.c_size_t, vp]),
+        "cbx_paged_prompt_attention_workspace": (i, [P, P, P, ctypes.POINTER(ctypes.c_size_t)]),
+        "cbx_paged_prompt_attention": (i, [P, P, P, P, P, P, P, P, f, f, ctypes.c_int32, P, vp, ctypes.c_size_t, vp]),
+        "cbx_paged_shared_attention_workspace": (i, [P, P, P, P, ctypes.POINTER(ctypes.c_size_t)]),
+        "cbx_paged_shared_attention": (i, [P, P, P, P, P, P, P, P, P, f, f, ctypes.c_int32, P, vp, ctypes.c_size_t, vp]),
         "cbx_token_log_probs_workspace": (i, [P, ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
         "cbx_token_log_probs": (i, [P, P, f, P, P, P, P, vp, ctypes.c_size_t, vp]),
         "cbx_run_ops": (i, [ctypes.POINTER(OpStruct), i, vp]),
@@ -324,6 +332,10 @@ def _layout(t: torch.Tensor, ggml_type: Optional[int]) -> Tensor:
         shape[0] = shape[0] // Q8_0_BLOCK * QK8_0
         strides[0] = Q8_0_BLOCK
         d.type = Q8_0
+    elif ggml_type == I8:
+        if t.dtype != torch.int8:
+            raise CbxError(ERR_INVALID_ARG, "I8 pages are int8")
+        d.type = I8
     else:
         if t.dtype not in _DTYPES:
             raise CbxError(ERR_INVALID_ARG, f"unsupported dtype {t.dtype}")
@@ -934,12 +946,24 @@ def paged_release(seq_lens, release, block_tables, page_size, free_pages, n_free
     return _call("paged_release", seq_lens, release, block_tables, page_size, free_pages, n_free, a, b)
 
 
-def paged_store(k, v, slots, k_cache, v_cache):
+def paged_store(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     """Rows of k and v [n_tok, n_head_kv, head_dim] into their slots of the
     caches [n_pages, n_head_kv, page_size, head_dim] (any strides, so a
     permuted [n_pages, page_size, n_head_kv, head_dim] too), rounded to the
-    caches' type; negative slots are skipped, the others are distinct."""
-    _call("paged_store", k, v, slots, k_cache, v_cache)
+    caches' type; negative slots are skipped, the others are distinct.  int8
+    caches come with k_scale and v_scale, float32 [n_pages, n_head_kv,
+    page_size], which get each row's largest element / 127."""
+    _call("paged_store", k, v, slots, k_cache, v_cache, k_scale, v_scale)
+
+
+def paged_load(slots, k_cache, v_cache, k_scale=None, v_scale=None, dtype=torch.float32, out=None):
+    """(k, v) [n_tok, n_head_kv, head_dim] of these slots read back, float32
+    or float16; negative slots give zeros.  k_scale, v_scale: of int8 caches.
+    out: the two tensors to write to."""
+    a, b = out or (None, None)
+    if dtype not in (torch.float32, torch.float16):
+        raise CbxError(ERR_UNSUPPORTED, "paged_load: dtype must be float32 or float16")
+    return _call("paged_load", slots, k_cache, v_cache, k_scale, v_scale, dtype == torch.float16, a, b)
 
 
 def qk_norm_rope(q, k, gq, gk, eps, pos, cache: RopeCache, out_q=None, out_k=None):
@@ -949,31 +973,72 @@ def qk_norm_rope(q, k, gq, gk, eps, pos, cache: RopeCache, out_q=None, out_k=Non
     return _call("qk_norm_rope", q, k, gq, gk, eps, pos, cache.handle.value or 0, out_q, out_k)
 
 
-def qk_norm_rope_store(q, k, v, gq, gk, eps, pos, cache: RopeCache, slots, k_cache, v_cache, out_q=None):
+def qk_norm_rope_store(q, k, v, gq, gk, eps, pos, cache: RopeCache, slots, k_cache, v_cache, out_q=None, k_scale=None,
+                       v_scale=None):
     """qk_norm_rope with the keys, and v beside them, written into the caches
     as paged_store does.  Returns q."""
-    return _call("qk_norm_rope_store", q, k, v, gq, gk, eps, pos, cache.handle.value or 0, slots, k_cache, v_cache, out_q)
+    return _call("qk_norm_rope_store", q, k, v, gq, gk, eps, pos, cache.handle.value or 0, slots, k_cache, v_cache, out_q, k_scale,
+                 v_scale)
+
+
+def _workspace(name, q, k_cache, *more) -> int:
+    _ready(q)
+    n = ctypes.c_size_t(0)
+    pages = desc(k_cache, I8 if k_cache.dtype == torch.int8 else None)
+    with torch.cuda.device(q.device):
+        _check(getattr(load(), name)(_ref(desc(q)), _ref(pages), *[_ref(desc(t)) for t in more], ctypes.byref(n)))
+    return n.value
 
 
 def paged_attention_workspace(q, k_cache, block_tables) -> int:
     """Bytes of scratch that paged_attention needs for these shapes."""
-    _ready(q)
-    n = ctypes.c_size_t(0)
-    with torch.cuda.device(q.device):
-        _check(load().cbx_paged_attention_workspace(_ref(desc(q)), _ref(desc(k_cache)), _ref(desc(block_tables)),
-                                                    ctypes.byref(n)))
-    return n.value
+    return _workspace("cbx_paged_attention_workspace", q, k_cache, block_tables)
 
 
-def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap=0.0, window=0, out=None, ws=None):
+def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, scale, softcap=0.0, window=0, out=None, ws=None, k_scale=None,
+                    v_scale=None):
     """Attention of one new token a request: q [n_seq, n_head, head_dim] over
     the seq_lens[s] keys in the pages block_tables[s] of the caches [n_pages,
     n_head_kv, page_size, head_dim]; softcap > 0: scores softcap * tanh(s /
-    softcap); window > 0: the last `window` keys only.  ws: scratch of
-    paged_attention_workspace bytes that no other call uses meanwhile
-    (default: taken from torch for this call; under capture, of the graph's
-    own pool)."""
-    return _call("paged_attention", q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window, out, ws)
+    softcap); window > 0: the last `window` keys only.  k_scale, v_scale: of
+    int8 caches (paged_store).  ws: scratch of paged_attention_workspace bytes
+    that no other call uses meanwhile (default: taken from torch for this call;
+    under capture, of the graph's own pool)."""
+    return _call("paged_attention", q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window, out, ws, k_scale, v_scale)
+
+
+def paged_prompt_attention_workspace(q, k_cache, block_tables) -> int:
+    """Bytes of scratch that paged_prompt_attention needs for these shapes."""
+    return _workspace("cbx_paged_prompt_attention_workspace", q, k_cache, block_tables)
+
+
+def paged_prompt_attention(q, k_cache, v_cache, block_tables, seq_lens, tok_start, scale, softcap=0.0, window=0, out=None, ws=None,
+                           k_scale=None, v_scale=None):
+    """Causal attention of all new tokens of packed requests: row t of q
+    [n_tok, n_head, head_dim] is a token of the request s whose
+    [tok_start[s], tok_start[s + 1]) holds it (paged_append's tok_start) and
+    attends over its request's keys up to its own, which lie in the cache by
+    then; the last token's is key seq_lens[s] - 1.  Rows of no request stay
+    unwritten: give `out` where they have to hold something.  The rest as for
+    paged_attention; ws of paged_prompt_attention_workspace bytes."""
+    return _call("paged_prompt_attention", q, k_cache, v_cache, block_tables, seq_lens, tok_start, scale, softcap, window, out, ws,
+                 k_scale, v_scale)
+
+
+def paged_shared_attention_workspace(q, k_cache, block_tables, group_start) -> int:
+    """Bytes of scratch that paged_shared_attention needs for these shapes."""
+    return _workspace("cbx_paged_shared_attention_workspace", q, k_cache, block_tables, group_start)
+
+
+def paged_shared_attention(q, k_cache, v_cache, block_tables, seq_lens, group_start, shared_lens, scale, softcap=0.0, window=0,
+                           out=None, ws=None, k_scale=None, v_scale=None):
+    """paged_attention for requests that begin with the same keys, which are
+    read once a group: the requests [group_start[p], group_start[p + 1]) have
+    their first shared_lens[p] keys in the same pages (their tables begin
+    alike).  group_start int32 [n_groups + 1], shared_lens int32 [n_groups];
+    ws of paged_shared_attention_workspace bytes."""
+    return _call("paged_shared_attention", q, k_cache, v_cache, block_tables, seq_lens, group_start, shared_lens, scale, softcap,
+                 window, out, ws, k_scale, v_scale)
 
 
 def token_log_probs_workspace(logits, top_n) -> int:

@@ -59,6 +59,7 @@ size_t type_size(int type) {
         case CBX_TYPE_F32: return 4;
         case CBX_TYPE_F16: return 2;
         case CBX_TYPE_Q8_0: return 34;
+        case CBX_TYPE_I8: return 1;
         case CBX_TYPE_I32: return 4;
         default: return 0;
     }
@@ -86,10 +87,10 @@ bool same_shape(const cbx_tensor* a, const cbx_tensor* b) {
     return true;
 }
 
-int validate(const cbx_tensor* t, const char* what, const char* name) {
+int validate(const cbx_tensor* t, const char* what, const char* name, bool i8) {
     const std::string where = std::string(what) + ": " + name;
     if (!t) return set_error(CBX_ERR_INVALID_ARG, where + " is NULL");
-    if (type_size(t->type) == 0) return set_error(CBX_ERR_INVALID_ARG, where + " has an unknown type " + std::to_string(t->type));
+    if (type_size(t->type) == 0 || (t->type == CBX_TYPE_I8 && !i8)) return set_error(CBX_ERR_INVALID_ARG, where + " has an unknown type " + std::to_string(t->type));
     if (t->reserved != 0) return set_error(CBX_ERR_INVALID_ARG, where + ".reserved must be 0");
     for (int i = 0; i < 4; i++) {
         if (t->ne[i] < 0) return set_error(CBX_ERR_INVALID_ARG, where + " has a negative ne[" + std::to_string(i) + "]");

@@ -79,8 +79,9 @@ bool    rows_contiguous(const cbx_tensor* t);   // nb[0] == element size
 bool    same_shape(const cbx_tensor* a, const cbx_tensor* b);
 bool    bytes_overlap(const cbx_tensor* a, const cbx_tensor* b);   // the byte ranges of the two tensors meet
 // Validates pointer, type, non-negative sizes and nb[0] for a float/int
-// tensor.  Returns 0 or a negative status with the error recorded.
-int validate(const cbx_tensor* t, const char* what, const char* name);
+// tensor; i8: I8 too, which only 8-bit caches are.  Returns 0 or a negative
+// status with the error recorded.
+int validate(const cbx_tensor* t, const char* what, const char* name, bool i8 = false);
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -305,17 +306,26 @@ struct ReleaseArgs {
 };
 int launch_paged_release(const ReleaseArgs& a, DeviceState* st, hipStream_t s);
 // q (with gq, yq), k and v may each be null; k goes to yk or to k_cache, v to
-// v_cache; norm: the norm and the rotation, else rows are copied.
+// v_cache (with their scales: I8); norm: the norm and the rotation, else rows
+// are copied.
 struct QkCall {
     const cbx_tensor *q, *gq, *k, *gk, *v, *pos, *slots;
-    cbx_tensor *yq, *yk, *k_cache, *v_cache;
+    cbx_tensor *yq, *yk, *k_cache, *v_cache, *k_scale, *v_scale;
     float eps;
     RopeTable rope;
     bool norm;
 };
 int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s);
+struct LoadCall {
+    const cbx_tensor *slots, *k_cache, *k_scale, *v_cache, *v_scale;
+    cbx_tensor *k, *v;
+};
+int launch_paged_load(const LoadCall& c, DeviceState* st, hipStream_t s);
+// k_scale, v_scale: of I8 pages, else null.  start: the tokens of packed
+// requests (paged_prompt_attention) or, with shared, the requests of groups
+// (paged_shared_attention); null: one token a request (paged_attention).
 struct PagedAttnCall {
-    const cbx_tensor *q, *k, *v, *tables, *lens;
+    const cbx_tensor *q, *k, *k_scale, *v, *v_scale, *tables, *lens, *start, *shared;
     cbx_tensor* y;
     float scale, softcap;
     int32_t window;
@@ -323,6 +333,11 @@ struct PagedAttnCall {
 };
 size_t paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
 int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s);
+size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
+int launch_paged_prompt(const PagedAttnCall& c, DeviceState* st, hipStream_t s);
+size_t paged_shared_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor* start,
+                              const DeviceState* st);
+int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s);
 struct LogProbCall {
     const cbx_tensor *x, *ids;
     cbx_tensor *logp, *entropy, *top_ids, *top_logp;

@@ -109,10 +109,38 @@ int check_tables(const cbx_tensor* t, int64_t n_seq, int64_t page, const char* w
     return CBX_OK;
 }
 
-// K and V pages: one float type and one shape, (head_dim, page_size, n_head_kv, n_pages).
-int check_cache(const cbx_tensor* k, const cbx_tensor* v, const char* what) {
+int check_pages(const cbx_tensor* t, bool i8, const char* what, const char* name) {
+    if (!i8) return check_floats(t, what, name);
+    int rc = validate(t, what, name, true);
+    if (rc) return rc;
+    if (t->type != CBX_TYPE_I8) return set_error(CBX_ERR_UNSUPPORTED, std::string(what) + ": " + name + " must be I8");
+    return CBX_OK;
+}
+
+// The scales of I8 pages: F32 (page_size, n_head_kv, n_pages), any strides of
+// whole elements, the first one's too.
+int check_scale(const cbx_tensor* t, const cbx_tensor* c, const char* what, const char* name) {
+    const std::string where = std::string(what) + ": " + name;
+    if (!t) return set_error(CBX_ERR_INVALID_ARG, where + " is NULL");
+    cbx_tensor row = *t;
+    row.nb[0] = type_size(t->type);
+    int rc = validate(&row, what, name);
+    if (rc) return rc;
+    if (t->type != CBX_TYPE_F32 || t->ne[0] != c->ne[1] || t->ne[1] != c->ne[2] || t->ne[2] != c->ne[3] || t->ne[3] != 1) {
+        return set_error(CBX_ERR_INVALID_ARG, where + " must be F32 with ne = (page_size, n_head_kv, n_pages, 1)");
+    }
+    for (int i = 0; i < 3; i++) {
+        if (t->ne[i] > 1 && t->nb[i] % 4) return set_error(CBX_ERR_INVALID_ARG, where + " strides must be whole elements");
+    }
+    if (reinterpret_cast<uintptr_t>(t->data) % 4) return set_error(CBX_ERR_INVALID_ARG, where + " must be aligned to its elements");
+    return CBX_OK;
+}
+
+// K and V pages: one type and one shape, (head_dim, page_size, n_head_kv, n_pages);
+// with scales I8 pages, without them F32 or F16.
+int check_cache(const cbx_tensor* k, const cbx_tensor* v, const char* what, bool i8 = false) {
     int rc;
-    if ((rc = check_floats(k, what, "k_cache")) || (rc = check_floats(v, what, "v_cache"))) return rc;
+    if ((rc = check_pages(k, i8, what, "k_cache")) || (rc = check_pages(v, i8, what, "v_cache"))) return rc;
     if (k->type != v->type) return fail(CBX_ERR_UNSUPPORTED, what, "k_cache and v_cache types differ");
     if (!same_shape(k, v)) return bad(what, "k_cache and v_cache shapes differ");
     const size_t es = type_size(k->type);
@@ -126,6 +154,15 @@ int check_cache(const cbx_tensor* k, const cbx_tensor* v, const char* what) {
         return fail(CBX_ERR_UNSUPPORTED, what, "page_size * n_pages must be below 2^31");
     }
     return CBX_OK;
+}
+
+// A cache whose scales may be given: both or neither.
+int check_cache_scaled(const cbx_tensor* k, const cbx_tensor* ks, const cbx_tensor* v, const cbx_tensor* vs, const char* what) {
+    if ((ks == nullptr) != (vs == nullptr)) return bad(what, "k_scale and v_scale go together");
+    int rc = check_cache(k, v, what, ks != nullptr);
+    if (rc || !ks) return rc;
+    if ((rc = check_scale(ks, k, what, "k_scale"))) return rc;
+    return check_scale(vs, v, what, "v_scale");
 }
 
 int overlap_error(const char* what, const char* out, const char* other) {
@@ -263,12 +300,12 @@ int cbx_paged_release(const cbx_tensor* seq_lens, const cbx_tensor* release, cbx
 // Shared by the calls over q, k and v rows: shapes and types of the rows,
 // the cache and its slots.
 static int check_kv_rows(const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* slots, const cbx_tensor* k_cache,
-                         const cbx_tensor* v_cache, const char* what) {
+                         const cbx_tensor* ks, const cbx_tensor* v_cache, const cbx_tensor* vs, const char* what) {
     int rc;
     if ((rc = check_floats(k, what, "k")) || (rc = check_floats(v, what, "v"))) return rc;
     if (k->type != v->type) return fail(CBX_ERR_UNSUPPORTED, what, "k and v types differ");
     if (!same_shape(k, v) || k->ne[3] != 1) return bad(what, "k and v must both be (head_dim, n_head_kv, n_tok, 1)");
-    if ((rc = check_cache(k_cache, v_cache, what))) return rc;
+    if ((rc = check_cache_scaled(k_cache, ks, v_cache, vs, what))) return rc;
     if (k_cache->ne[0] != k->ne[0] || k_cache->ne[2] != k->ne[1]) {
         return bad(what, "the cache must be (head_dim, page_size, n_head_kv, n_pages) with k's head_dim and n_head_kv");
     }
@@ -282,17 +319,15 @@ static int check_row_count(const char* what, int64_t tok, int64_t heads, int64_t
     return CBX_OK;
 }
 
-int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* slots, cbx_tensor* k_cache,
-                    cbx_tensor* v_cache, cbx_stream stream) {
-    const char* what = "cbx_paged_store";
-    clear_error();
+static int paged_store(const char* what, const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* slots, cbx_tensor* k_cache,
+                       cbx_tensor* k_scale, cbx_tensor* v_cache, cbx_tensor* v_scale, cbx_stream stream) {
     int rc;
-    if ((rc = check_kv_rows(k, v, slots, k_cache, v_cache, what))) return rc;
+    if ((rc = check_kv_rows(k, v, slots, k_cache, k_scale, v_cache, v_scale, what))) return rc;
     if ((rc = check_row_count(what, k->ne[2], 2 * k->ne[1], k->ne[0]))) return rc;
-    const cbx_tensor* outs[] = {k_cache, v_cache};
-    const char* names[] = {"k_cache", "v_cache"};
+    const cbx_tensor* outs[] = {k_cache, v_cache, k_scale, v_scale};
+    const char* names[] = {"k_cache", "v_cache", "k_scale", "v_scale"};
     const cbx_tensor* ins[] = {k, v, slots};
-    if ((rc = check_apart(what, outs, names, 2, ins, 3))) return rc;
+    if ((rc = check_apart(what, outs, names, k_scale ? 4 : 2, ins, 3))) return rc;
     DeviceState* st = current_state(&rc);
     if (!st) return rc;
     if (nelements(k) == 0) return CBX_OK;
@@ -302,7 +337,41 @@ int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* 
     c.slots = slots;
     c.k_cache = k_cache;
     c.v_cache = v_cache;
+    c.k_scale = k_scale;
+    c.v_scale = v_scale;
     return launch_qk(c, st, reinterpret_cast<hipStream_t>(stream));
+}
+
+int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* slots, cbx_tensor* k_cache,
+                    cbx_tensor* v_cache, cbx_stream stream) {
+    clear_error();
+    return paged_store("cbx_paged_store", k, v, slots, k_cache, nullptr, v_cache, nullptr, stream);
+}
+
+int cbx_paged_store_q8(const cbx_tensor* k, const cbx_tensor* v, const cbx_tensor* slots, cbx_tensor* k_cache,
+                       cbx_tensor* k_scale, cbx_tensor* v_cache, cbx_tensor* v_scale, cbx_stream stream) {
+    const char* what = "cbx_paged_store_q8";
+    clear_error();
+    if (!k_scale || !v_scale) return bad(what, "k_scale or v_scale is NULL");
+    return paged_store(what, k, v, slots, k_cache, k_scale, v_cache, v_scale, stream);
+}
+
+int cbx_paged_load(const cbx_tensor* slots, const cbx_tensor* k_cache, const cbx_tensor* k_scale,
+                   const cbx_tensor* v_cache, const cbx_tensor* v_scale, cbx_tensor* k, cbx_tensor* v,
+                   cbx_stream stream) {
+    const char* what = "cbx_paged_load";
+    clear_error();
+    int rc;
+    if ((rc = check_kv_rows(k, v, slots, k_cache, k_scale, v_cache, v_scale, what)) ||
+        (rc = check_row_count(what, k->ne[2], 2 * k->ne[1], k->ne[0]))) return rc;
+    const cbx_tensor* outs[] = {k, v};
+    const char* names[] = {"k", "v"};
+    const cbx_tensor* ins[] = {slots, k_cache, v_cache, k_scale, v_scale};
+    if ((rc = check_apart(what, outs, names, 2, ins, 5))) return rc;
+    DeviceState* st = current_state(&rc);
+    if (!st) return rc;
+    if (nelements(k) == 0) return CBX_OK;
+    return launch_paged_load(LoadCall{slots, k_cache, k_scale, v_cache, v_scale, k, v}, st, reinterpret_cast<hipStream_t>(stream));
 }
 
 static int check_gain(const cbx_tensor* g, int64_t d, const char* what, const char* name) {
@@ -375,20 +444,20 @@ int cbx_qk_norm_rope(const cbx_tensor* q, const cbx_tensor* gq, const cbx_tensor
     return launch_qk(c, st, reinterpret_cast<hipStream_t>(stream));
 }
 
-int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq, const cbx_tensor* k, const cbx_tensor* gk,
-                           const cbx_tensor* v, float eps, const cbx_tensor* pos, const cbx_rope_cache* rope,
-                           const cbx_tensor* slots, cbx_tensor* yq, cbx_tensor* k_cache, cbx_tensor* v_cache,
-                           cbx_stream stream) {
-    const char* what = "cbx_qk_norm_rope_store";
-    clear_error();
+static int qk_norm_rope_store(const char* what, const cbx_tensor* q, const cbx_tensor* gq, const cbx_tensor* k,
+                              const cbx_tensor* gk, const cbx_tensor* v, float eps, const cbx_tensor* pos,
+                              const cbx_rope_cache* rope, const cbx_tensor* slots, cbx_tensor* yq, cbx_tensor* k_cache,
+                              cbx_tensor* k_scale, cbx_tensor* v_cache, cbx_tensor* v_scale, cbx_stream stream) {
     int rc;
     if ((rc = check_qk(what, q, gq, k, gk, eps, pos, rope, yq)) ||
-        (rc = check_kv_rows(k, v, slots, k_cache, v_cache, what)) ||
+        (rc = check_kv_rows(k, v, slots, k_cache, k_scale, v_cache, v_scale, what)) ||
         (rc = check_row_count(what, q->ne[2], q->ne[1] + 2 * k->ne[1], q->ne[0]))) return rc;
-    const cbx_tensor* outs[] = {k_cache, v_cache, yq};
-    const char* names[] = {"k_cache", "v_cache", "yq"};
+    const cbx_tensor* outs[] = {k_cache, v_cache, yq, k_scale, v_scale};
+    const char* names[] = {"k_cache", "v_cache", "yq", "k_scale", "v_scale"};
+    const int scales = k_scale ? 2 : 0;
     const cbx_tensor* ins[] = {k, v, gq, gk, pos, slots, q};
-    if ((rc = check_apart(what, outs, names, 3, ins, 6)) || (rc = check_apart(what, outs, names, 2, ins + 6, 1))) return rc;
+    if ((rc = check_apart(what, outs, names, 3 + scales, ins, 6)) || (rc = check_apart(what, outs, names, 2, ins + 6, 1)) ||
+        (rc = check_apart(what, outs + 3, names + 3, scales, ins + 6, 1))) return rc;
     if (!is_itself(yq, q) && meets(yq, q)) return overlap_error(what, "yq", "an input");
     DeviceState* st = current_state(&rc);
     if (!st || (rc = check_rope(what, rope, q->ne[0], st))) return rc;
@@ -404,26 +473,66 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq, const cbx_
     c.yq = yq;
     c.k_cache = k_cache;
     c.v_cache = v_cache;
+    c.k_scale = k_scale;
+    c.v_scale = v_scale;
     c.eps = eps;
     c.rope = rope_table(rope);
     c.norm = true;
     return launch_qk(c, st, reinterpret_cast<hipStream_t>(stream));
 }
 
-static int check_attention(const char* what, const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* tables) {
+int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq, const cbx_tensor* k, const cbx_tensor* gk,
+                           const cbx_tensor* v, float eps, const cbx_tensor* pos, const cbx_rope_cache* rope,
+                           const cbx_tensor* slots, cbx_tensor* yq, cbx_tensor* k_cache, cbx_tensor* v_cache,
+                           cbx_stream stream) {
+    clear_error();
+    return qk_norm_rope_store("cbx_qk_norm_rope_store", q, gq, k, gk, v, eps, pos, rope, slots, yq, k_cache, nullptr, v_cache,
+                              nullptr, stream);
+}
+
+int cbx_qk_norm_rope_store_q8(const cbx_tensor* q, const cbx_tensor* gq, const cbx_tensor* k, const cbx_tensor* gk,
+                              const cbx_tensor* v, float eps, const cbx_tensor* pos, const cbx_rope_cache* rope,
+                              const cbx_tensor* slots, cbx_tensor* yq, cbx_tensor* k_cache, cbx_tensor* k_scale,
+                              cbx_tensor* v_cache, cbx_tensor* v_scale, cbx_stream stream) {
+    const char* what = "cbx_qk_norm_rope_store_q8";
+    clear_error();
+    if (!k_scale || !v_scale) return bad(what, "k_scale or v_scale is NULL");
+    return qk_norm_rope_store(what, q, gq, k, gk, v, eps, pos, rope, slots, yq, k_cache, k_scale, v_cache, v_scale, stream);
+}
+
+// The queries (rows: tokens or requests) and the tables of n_seq requests.
+static int check_attention(const char* what, const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* tables,
+                           bool packed = false) {
     int rc;
-    if ((rc = check_floats(q, what, "q")) || (rc = check_floats(k_cache, what, "k_cache")) ||
-        (rc = check_tables(tables, q->ne[2], k_cache->ne[1], what))) return rc;
-    if (q->ne[3] != 1) return bad(what, "q must be (head_dim, n_head, n_seq, 1)");
+    const bool i8 = k_cache && k_cache->type == CBX_TYPE_I8;
+    if ((rc = check_floats(q, what, "q")) || (rc = check_pages(k_cache, i8, what, "k_cache")) ||
+        (rc = tables ? check_tables(tables, packed ? tables->ne[1] : q->ne[2], k_cache->ne[1], what)
+                     : bad(what, "block_tables is NULL"))) return rc;
+    if (q->ne[3] != 1) return bad(what, packed ? "q must be (head_dim, n_head, n_tok, 1)" : "q must be (head_dim, n_head, n_seq, 1)");
     if (k_cache->ne[0] != q->ne[0]) return bad(what, "q and the cache differ in head_dim");
     const int64_t hkv = k_cache->ne[2];
     if (hkv == 0 ? q->ne[1] != 0 : q->ne[1] % hkv != 0) return bad(what, "n_head must be a multiple of n_head_kv");
     const int64_t keys = tables->ne[0] * k_cache->ne[1];
     if (q->ne[0] > 512 || q->ne[1] >= k2G || q->ne[2] >= k2G || q->ne[1] * q->ne[2] >= kMostGroups ||
-        (keys / 32 + 1) * q->ne[1] * q->ne[2] >= (int64_t{1} << 40)) {
-        return fail(CBX_ERR_UNSUPPORTED, what, "head_dim up to 512, n_head * n_seq below 2^24");
+        (keys / 32 + 1) * q->ne[1] * q->ne[2] >= (int64_t{1} << 40) || tables->ne[1] >= kMostGroups) {
+        return fail(CBX_ERR_UNSUPPORTED, what, packed ? "head_dim up to 512, n_head * n_tok below 2^24"
+                                                      : "head_dim up to 512, n_head * n_seq below 2^24");
     }
     return CBX_OK;
+}
+
+// Scores' numbers, the result and what it may not touch: shared by the calls.
+static int check_scores(const char* what, const cbx_tensor* q, float scale, float softcap, int32_t window, const cbx_tensor* y,
+                        const cbx_tensor* const* ins, int n) {
+    int rc = check_floats(y, what, "y");
+    if (rc) return rc;
+    if (y->type != q->type) return fail(CBX_ERR_UNSUPPORTED, what, "q and y types differ");
+    if (!same_shape(q, y)) return bad(what, "q and y shapes differ");
+    if (!std::isfinite(scale)) return bad(what, "scale must be finite");
+    if (!(softcap >= 0.0f) || std::isinf(softcap)) return bad(what, "softcap must be finite and >= 0");
+    if (window < 0) return bad(what, "window must be >= 0");
+    const char* names[] = {"y"};
+    return check_apart(what, &y, names, 1, ins, n);
 }
 
 int cbx_paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* block_tables,
@@ -440,31 +549,124 @@ int cbx_paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k_cache
     return CBX_OK;
 }
 
-int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* v_cache,
-                        const cbx_tensor* block_tables, const cbx_tensor* seq_lens, float scale, float softcap,
-                        int32_t window, cbx_tensor* y, void* ws, size_t ws_bytes, cbx_stream stream) {
-    const char* what = "cbx_paged_attention";
-    clear_error();
+static int paged_attention(const char* what, const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* k_scale,
+                           const cbx_tensor* v_cache, const cbx_tensor* v_scale, const cbx_tensor* block_tables,
+                           const cbx_tensor* seq_lens, float scale, float softcap, int32_t window, cbx_tensor* y, void* ws,
+                           size_t ws_bytes, cbx_stream stream) {
     int rc;
-    if ((rc = check_cache(k_cache, v_cache, what)) || (rc = check_attention(what, q, k_cache, block_tables)) ||
-        (rc = check_ints(seq_lens, q->ne[2], what, "seq_lens")) || (rc = check_floats(y, what, "y"))) return rc;
-    if (y->type != q->type) return fail(CBX_ERR_UNSUPPORTED, what, "q and y types differ");
-    if (!same_shape(q, y)) return bad(what, "q and y shapes differ");
-    if (!std::isfinite(scale)) return bad(what, "scale must be finite");
-    if (!(softcap >= 0.0f) || std::isinf(softcap)) return bad(what, "softcap must be finite and >= 0");
-    if (window < 0) return bad(what, "window must be >= 0");
-    const cbx_tensor* outs[] = {y};
-    const char* names[] = {"y"};
-    const cbx_tensor* ins[] = {q, k_cache, v_cache, block_tables, seq_lens};
-    if ((rc = check_apart(what, outs, names, 1, ins, 5))) return rc;
+    const cbx_tensor* all[] = {q, k_cache, v_cache, block_tables, seq_lens, k_scale, v_scale, y};
+    if ((rc = check_cache_scaled(k_cache, k_scale, v_cache, v_scale, what)) ||
+        (rc = check_attention(what, q, k_cache, block_tables)) ||
+        (rc = check_ints(seq_lens, q->ne[2], what, "seq_lens")) ||
+        (rc = check_scores(what, q, scale, softcap, window, y, all, 7))) return rc;
     DeviceState* st = current_state(&rc);
     if (!st) return rc;
     if (nelements(q) == 0) return CBX_OK;
     const size_t need = paged_attention_workspace(q, k_cache, block_tables, st);
-    const cbx_tensor* all[] = {q, k_cache, v_cache, block_tables, seq_lens, y};
-    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 6))) return rc;
-    PagedAttnCall c{q, k_cache, v_cache, block_tables, seq_lens, y, scale, softcap, window, ws};
+    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 8))) return rc;
+    PagedAttnCall c{q, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, nullptr, nullptr, y, scale, softcap, window, ws};
     return launch_paged_attention(c, st, reinterpret_cast<hipStream_t>(stream));
+}
+
+int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* v_cache,
+                        const cbx_tensor* block_tables, const cbx_tensor* seq_lens, float scale, float softcap,
+                        int32_t window, cbx_tensor* y, void* ws, size_t ws_bytes, cbx_stream stream) {
+    clear_error();
+    return paged_attention("cbx_paged_attention", q, k_cache, nullptr, v_cache, nullptr, block_tables, seq_lens, scale, softcap,
+                           window, y, ws, ws_bytes, stream);
+}
+
+int cbx_paged_attention_q8(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* k_scale,
+                           const cbx_tensor* v_cache, const cbx_tensor* v_scale, const cbx_tensor* block_tables,
+                           const cbx_tensor* seq_lens, float scale, float softcap, int32_t window, cbx_tensor* y, void* ws,
+                           size_t ws_bytes, cbx_stream stream) {
+    const char* what = "cbx_paged_attention_q8";
+    clear_error();
+    if (!k_scale || !v_scale) return bad(what, "k_scale or v_scale is NULL");
+    return paged_attention(what, q, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, scale, softcap, window, y, ws,
+                           ws_bytes, stream);
+}
+
+int cbx_paged_prompt_attention_workspace(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* block_tables,
+                                         size_t* bytes) {
+    const char* what = "cbx_paged_prompt_attention_workspace";
+    clear_error();
+    int rc;
+    if (!bytes) return bad(what, "bytes is NULL");
+    *bytes = 0;
+    if ((rc = check_attention(what, q, k_cache, block_tables, true))) return rc;
+    DeviceState* st = current_state(&rc);
+    if (!st) return rc;
+    if (nelements(q) > 0 && block_tables->ne[1] > 0) *bytes = paged_prompt_workspace(q, k_cache, block_tables, st);
+    return CBX_OK;
+}
+
+int cbx_paged_prompt_attention(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* k_scale,
+                               const cbx_tensor* v_cache, const cbx_tensor* v_scale, const cbx_tensor* block_tables,
+                               const cbx_tensor* seq_lens, const cbx_tensor* tok_start, float scale, float softcap,
+                               int32_t window, cbx_tensor* y, void* ws, size_t ws_bytes, cbx_stream stream) {
+    const char* what = "cbx_paged_prompt_attention";
+    clear_error();
+    int rc;
+    const cbx_tensor* all[] = {q, k_cache, v_cache, block_tables, seq_lens, tok_start, k_scale, v_scale, y};
+    if ((rc = check_cache_scaled(k_cache, k_scale, v_cache, v_scale, what)) ||
+        (rc = check_attention(what, q, k_cache, block_tables, true)) ||
+        (rc = check_ints(seq_lens, block_tables->ne[1], what, "seq_lens")) ||
+        (rc = check_ints(tok_start, block_tables->ne[1] + 1, what, "tok_start")) ||
+        (rc = check_scores(what, q, scale, softcap, window, y, all, 8))) return rc;
+    DeviceState* st = current_state(&rc);
+    if (!st) return rc;
+    if (nelements(q) == 0 || block_tables->ne[1] == 0) return CBX_OK;
+    const size_t need = paged_prompt_workspace(q, k_cache, block_tables, st);
+    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 9))) return rc;
+    PagedAttnCall c{q, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, tok_start, nullptr, y, scale, softcap, window, ws};
+    return launch_paged_prompt(c, st, reinterpret_cast<hipStream_t>(stream));
+}
+
+static int check_groups(const char* what, const cbx_tensor* start) {
+    int rc = check_ints(start, -1, what, "group_start");
+    if (rc) return rc;
+    if (start->ne[0] < 1) return bad(what, "group_start must have n_groups + 1 elements");
+    if (start->ne[0] >= kMostGroups) return fail(CBX_ERR_UNSUPPORTED, what, "2^24 groups or more");
+    return CBX_OK;
+}
+
+int cbx_paged_shared_attention_workspace(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* block_tables,
+                                         const cbx_tensor* group_start, size_t* bytes) {
+    const char* what = "cbx_paged_shared_attention_workspace";
+    clear_error();
+    int rc;
+    if (!bytes) return bad(what, "bytes is NULL");
+    *bytes = 0;
+    if ((rc = check_attention(what, q, k_cache, block_tables)) || (rc = check_groups(what, group_start))) return rc;
+    DeviceState* st = current_state(&rc);
+    if (!st) return rc;
+    if (nelements(q) > 0) *bytes = paged_shared_workspace(q, k_cache, block_tables, group_start, st);
+    return CBX_OK;
+}
+
+int cbx_paged_shared_attention(const cbx_tensor* q, const cbx_tensor* k_cache, const cbx_tensor* k_scale,
+                               const cbx_tensor* v_cache, const cbx_tensor* v_scale, const cbx_tensor* block_tables,
+                               const cbx_tensor* seq_lens, const cbx_tensor* group_start, const cbx_tensor* shared_lens,
+                               float scale, float softcap, int32_t window, cbx_tensor* y, void* ws, size_t ws_bytes,
+                               cbx_stream stream) {
+    const char* what = "cbx_paged_shared_attention";
+    clear_error();
+    int rc;
+    const cbx_tensor* all[] = {q, k_cache, v_cache, block_tables, seq_lens, group_start, shared_lens, k_scale, v_scale, y};
+    if ((rc = check_cache_scaled(k_cache, k_scale, v_cache, v_scale, what)) ||
+        (rc = check_attention(what, q, k_cache, block_tables)) || (rc = check_groups(what, group_start)) ||
+        (rc = check_ints(seq_lens, q->ne[2], what, "seq_lens")) ||
+        (rc = check_ints(shared_lens, group_start->ne[0] - 1, what, "shared_lens")) ||
+        (rc = check_scores(what, q, scale, softcap, window, y, all, 9))) return rc;
+    DeviceState* st = current_state(&rc);
+    if (!st) return rc;
+    if (nelements(q) == 0) return CBX_OK;
+    const size_t need = paged_shared_workspace(q, k_cache, block_tables, group_start, st);
+    if ((rc = check_scratch(what, ws, ws_bytes, need, all, 10))) return rc;
+    PagedAttnCall c{q, k_cache, k_scale, v_cache, v_scale, block_tables, seq_lens, group_start, shared_lens, y, scale, softcap,
+                    window, ws};
+    return launch_paged_shared(c, st, reinterpret_cast<hipStream_t>(stream));
 }
 
 static int check_logits(const char* what, const cbx_tensor* x, int64_t n_top) {

@@ -99,6 +99,7 @@ struct Call {
             case at::kFloat: o->type = CBX_TYPE_F32; es = 4; break;
             case at::kHalf: o->type = CBX_TYPE_F16; es = 2; break;
             case at::kInt: o->type = CBX_TYPE_I32; es = 4; break;
+            case at::kChar: o->type = CBX_TYPE_I8; es = 1; break;
             default: raise(CBX_ERR_INVALID_ARG, std::string("unsupported dtype ") + c10::toString(t.scalar_type()));
         }
         o->data = t.data_ptr();
@@ -214,13 +215,32 @@ PyObject* paged_release(PyObject* const* a, Py_ssize_t n) {
     return tuple_of({lo, left});
 }
 
-// k, v, slots, k_cache, v_cache
+// k, v, slots, k_cache, v_cache, k_scale, v_scale
 PyObject* paged_store(PyObject* const* a, Py_ssize_t n) {
-    Call c(a, n, 5);
-    cbx_tensor *k = c.describe(0), *v = c.describe(1), *sl = c.describe(2), *kc = c.describe(3), *vc = c.describe(4);
+    Call c(a, n, 7);
+    cbx_tensor *k = c.describe(0), *v = c.describe(1), *sl = c.describe(2), *kc = c.describe(3), *vc = c.describe(4),
+               *ks = c.maybe(5), *vs = c.maybe(6);
     if (c.elsewhere()) return c.todo();
-    if (!c.done(unlocked([&] { return cbx_paged_store(k, v, sl, kc, vc, c.stream); }))) return c.todo();
+    if (!c.done(unlocked([&] {
+            return ks || vs ? cbx_paged_store_q8(k, v, sl, kc, ks, vc, vs, c.stream) : cbx_paged_store(k, v, sl, kc, vc, c.stream);
+        }))) {
+        return c.todo();
+    }
     Py_RETURN_NONE;
+}
+
+// slots, k_cache, v_cache, k_scale, v_scale, F16 (else F32), out_k, out_v
+PyObject* paged_load(PyObject* const* a, Py_ssize_t n) {
+    Call c(a, n, 8);
+    cbx_tensor *sl = c.describe(0), *kc = c.describe(1), *vc = c.describe(2), *ks = c.maybe(3), *vs = c.maybe(4);
+    const int half = PyObject_IsTrue(a[5]);
+    if (half < 0) throw Raised{};
+    if (c.elsewhere()) return c.todo();
+    const at::DimVector rows{sl->ne[0], kc->ne[2], kc->ne[0]};
+    const at::Tensor k = c.or_empty(6, rows, half ? at::kHalf : at::kFloat), v = c.or_empty(7, rows, half ? at::kHalf : at::kFloat);
+    cbx_tensor *dk = c.describe(k), *dv = c.describe(v);
+    if (!c.done(unlocked([&] { return cbx_paged_load(sl, kc, ks, vc, vs, dk, dv, c.stream); }))) return c.todo();
+    return tuple_of({k, v});
 }
 
 // q, k, gq, gk, eps, pos, rope, out_q, out_k
@@ -237,18 +257,21 @@ PyObject* qk_norm_rope(PyObject* const* a, Py_ssize_t n) {
     return tuple_of({yq, yk});
 }
 
-// q, k, v, gq, gk, eps, pos, rope, slots, k_cache, v_cache, out_q
+// q, k, v, gq, gk, eps, pos, rope, slots, k_cache, v_cache, out_q, k_scale, v_scale
 PyObject* qk_norm_rope_store(PyObject* const* a, Py_ssize_t n) {
-    Call c(a, n, 12);
+    Call c(a, n, 14);
     cbx_tensor *q = c.describe(0), *k = c.describe(1), *v = c.describe(2), *gq = c.maybe(3), *gk = c.maybe(4), *pos = c.describe(6),
-               *sl = c.describe(8), *kc = c.describe(9), *vc = c.describe(10);
+               *sl = c.describe(8), *kc = c.describe(9), *vc = c.describe(10), *ks = c.maybe(12), *vs = c.maybe(13);
     const float eps = c.number(5);
     const auto* rope = static_cast<const cbx_rope_cache*>(c.handle(7));
     if (c.elsewhere()) return c.todo();
     const at::Tensor& tq = c.tensor(0);
     const at::Tensor yq = c.or_empty(11, tq.sizes(), tq.scalar_type());
     cbx_tensor* dq = c.describe(yq);
-    if (!c.done(unlocked([&] { return cbx_qk_norm_rope_store(q, gq, k, gk, v, eps, pos, rope, sl, dq, kc, vc, c.stream); }))) {
+    if (!c.done(unlocked([&] {
+            return ks || vs ? cbx_qk_norm_rope_store_q8(q, gq, k, gk, v, eps, pos, rope, sl, dq, kc, ks, vc, vs, c.stream)
+                            : cbx_qk_norm_rope_store(q, gq, k, gk, v, eps, pos, rope, sl, dq, kc, vc, c.stream);
+        }))) {
         return c.todo();
     }
     return wrap(yq);
@@ -276,10 +299,11 @@ Scratch scratch(const Call& c, Py_ssize_t i, size_t bytes) {
     return s;
 }
 
-// q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window, out, ws
+// q, k_cache, v_cache, block_tables, seq_lens, scale, softcap, window, out, ws, k_scale, v_scale
 PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
-    Call c(a, n, 10);
-    cbx_tensor *q = c.describe(0), *k = c.describe(1), *v = c.describe(2), *tab = c.describe(3), *len = c.describe(4);
+    Call c(a, n, 12);
+    cbx_tensor *q = c.describe(0), *k = c.describe(1), *v = c.describe(2), *tab = c.describe(3), *len = c.describe(4),
+               *ks = c.maybe(10), *vs = c.maybe(11);
     const float scale = c.number(5), cap = c.number(6);
     const int32_t window = c.int32(7);
     if (c.elsewhere()) return c.todo();
@@ -289,7 +313,54 @@ PyObject* paged_attention(PyObject* const* a, Py_ssize_t n) {
     const at::Tensor y = c.or_empty(8, tq.sizes(), tq.scalar_type());
     cbx_tensor* dy = c.describe(y);
     const Scratch ws = scratch(c, 9, bytes);
-    if (!c.done(unlocked([&] { return cbx_paged_attention(q, k, v, tab, len, scale, cap, window, dy, ws.p, ws.bytes, c.stream); }))) {
+    if (!c.done(unlocked([&] {
+            return ks || vs ? cbx_paged_attention_q8(q, k, ks, v, vs, tab, len, scale, cap, window, dy, ws.p, ws.bytes, c.stream)
+                            : cbx_paged_attention(q, k, v, tab, len, scale, cap, window, dy, ws.p, ws.bytes, c.stream);
+        }))) {
+        return c.todo();
+    }
+    return wrap(y);
+}
+
+// q, k_cache, v_cache, block_tables, seq_lens, tok_start, scale, softcap, window, out, ws, k_scale, v_scale
+PyObject* paged_prompt_attention(PyObject* const* a, Py_ssize_t n) {
+    Call c(a, n, 13);
+    cbx_tensor *q = c.describe(0), *k = c.describe(1), *v = c.describe(2), *tab = c.describe(3), *len = c.describe(4),
+               *start = c.describe(5), *ks = c.maybe(11), *vs = c.maybe(12);
+    const float scale = c.number(6), cap = c.number(7);
+    const int32_t window = c.int32(8);
+    if (c.elsewhere()) return c.todo();
+    size_t bytes = 0;
+    if (c.none(10) && !c.done(cbx_paged_prompt_attention_workspace(q, k, tab, &bytes))) return c.todo();
+    const at::Tensor& tq = c.tensor(0);
+    const at::Tensor y = c.or_empty(9, tq.sizes(), tq.scalar_type());
+    cbx_tensor* dy = c.describe(y);
+    const Scratch ws = scratch(c, 10, bytes);
+    if (!c.done(unlocked([&] {
+            return cbx_paged_prompt_attention(q, k, ks, v, vs, tab, len, start, scale, cap, window, dy, ws.p, ws.bytes, c.stream);
+        }))) {
+        return c.todo();
+    }
+    return wrap(y);
+}
+
+// q, k_cache, v_cache, block_tables, seq_lens, group_start, shared_lens, scale, softcap, window, out, ws, k_scale, v_scale
+PyObject* paged_shared_attention(PyObject* const* a, Py_ssize_t n) {
+    Call c(a, n, 14);
+    cbx_tensor *q = c.describe(0), *k = c.describe(1), *v = c.describe(2), *tab = c.describe(3), *len = c.describe(4),
+               *start = c.describe(5), *pre = c.describe(6), *ks = c.maybe(12), *vs = c.maybe(13);
+    const float scale = c.number(7), cap = c.number(8);
+    const int32_t window = c.int32(9);
+    if (c.elsewhere()) return c.todo();
+    size_t bytes = 0;
+    if (c.none(11) && !c.done(cbx_paged_shared_attention_workspace(q, k, tab, start, &bytes))) return c.todo();
+    const at::Tensor& tq = c.tensor(0);
+    const at::Tensor y = c.or_empty(10, tq.sizes(), tq.scalar_type());
+    cbx_tensor* dy = c.describe(y);
+    const Scratch ws = scratch(c, 11, bytes);
+    if (!c.done(unlocked([&] {
+            return cbx_paged_shared_attention(q, k, ks, v, vs, tab, len, start, pre, scale, cap, window, dy, ws.p, ws.bytes, c.stream);
+        }))) {
         return c.todo();
     }
     return wrap(y);
@@ -345,9 +416,12 @@ PyMethodDef g_methods[] = {
     method<paged_append>("paged_append"),
     method<paged_release>("paged_release"),
     method<paged_store>("paged_store"),
+    method<paged_load>("paged_load"),
     method<qk_norm_rope>("qk_norm_rope"),
     method<qk_norm_rope_store>("qk_norm_rope_store"),
     method<paged_attention>("paged_attention"),
+    method<paged_prompt_attention>("paged_prompt_attention"),
+    method<paged_shared_attention>("paged_shared_attention"),
     method<token_log_probs>("token_log_probs"),
     {nullptr, nullptr, 0, nullptr},
 };

@@ -26,34 +26,10 @@
 // a workgroup a request and query head, a key's elements over the lanes: 64
 // requests of 1 to 2048 keys, 16 heads of 60 703 us (of 64, by tiles, 50; of 64 off
 // their alignment 784).
-#include "cbx_device.h"
+#include "cbx_attn.h"
 
 namespace cbx {
 namespace {
-
-constexpr int kAttnThreads = 256;
-constexpr int kAttnMaxD = 512;
-constexpr float kLowest = -3.0e38f;   // below every score that matters; finite, so that m - m is 0
-constexpr float kLog2e = 1.44269504088896340736f;
-
-struct AttnArgs {
-    const char *q, *k, *v, *tables;
-    const int32_t* lens;
-    char* y;
-    int64_t q_nb1, q_nb2, y_nb1, y_nb2, k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3, t_nb1;
-    uint32_t n_seq, hq, hkv, g, D, page, max_pages, n_pages;
-    int32_t window;
-    float scale, softcap;
-    uint32_t* err;
-    // k_attn_tiles and k_attn_join
-    uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
-    uint32_t gc, ngr, H;             // heads a run holds (<= 16), runs of heads a group, hkv * ngr
-    uint32_t W;                      // runs; 0: a run a request and key head, none of them split
-    float* part_o;                   // [W][2][gc][D]
-    float2* part_ml;                 // [W][2][gc]
-    uint4* split;                    // [W]: request, first query head, heads and parts of the key head that begins
-                                     // in the run and ends in a later one; no parts: none does
-};
 
 __device__ __forceinline__ float wave_sum_f32(float v) {
 #pragma unroll
@@ -61,20 +37,41 @@ __device__ __forceinline__ float wave_sum_f32(float v) {
     return v;
 }
 
-template <typename T, typename TC>
+// An element of a row of keys or values, an I8 one without its scale.
+template <typename TC> __device__ __forceinline__ float held(const char* row, uint32_t e) {
+    if constexpr (sizeof(TC) == 1) return static_cast<float>(reinterpret_cast<const int8_t*>(row)[e]);
+    else return Elt<TC>::load1(row + e * Elt<TC>::size);
+}
+
+// PACKED: a row of q is a token of its request and attends up to itself.
+template <typename T, typename TC, bool PACKED>
 __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
     constexpr int W = kAttnThreads / 64, N = kAttnMaxD / 64;
     __shared__ float lds_o[W][kAttnMaxD];
     __shared__ float lds_m[W], lds_l[W];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    const uint32_t s = blockIdx.x / a.hq, h = blockIdx.x - s * a.hq, hk = h / a.g;
+    const uint32_t t = blockIdx.x / a.hq, h = blockIdx.x - t * a.hq, hk = h / a.g;
+    uint32_t s = t;
+    int64_t behind = 0;                          // tokens of the request after this one
+    if constexpr (PACKED) {
+        uint32_t lo = 0, hi = a.n_seq;           // the first request that starts behind t
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (a.start[mid] > static_cast<int32_t>(t)) hi = mid;
+            else lo = mid + 1;
+        }
+        s = lo - 1;
+        if (lo == 0 || a.start[s] > static_cast<int32_t>(t) || a.start[s + 1] <= static_cast<int32_t>(t)) return;
+        behind = static_cast<int64_t>(a.start[s + 1]) - 1 - t;
+    }
     const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
     int64_t len = a.lens[s];
     bool wrong = len < 0 || len > cap;
     len = len < 0 ? 0 : (len > cap ? cap : len);
+    len = len > behind ? len - behind : 0;
     const int64_t first = a.window > 0 && len > a.window ? len - a.window : 0;
     const int32_t* row = reinterpret_cast<const int32_t*>(a.tables + s * a.t_nb1);
-    const char* qr = a.q + s * a.q_nb2 + h * a.q_nb1;
+    const char* qr = a.q + t * a.q_nb2 + h * a.q_nb1;
     float q[N], o[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
@@ -96,9 +93,13 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const uint32_t e = lane + 64 * i;
-            if (e < a.D) dot = fmaf(q[i], Elt<TC>::load1(kr + e * Elt<TC>::size), dot);
+            if (e < a.D) dot = fmaf(q[i], held<TC>(kr, e), dot);
         }
-        float sc = wave_sum_f32(dot) * a.scale;
+        float sc = wave_sum_f32(dot) * a.scale, vsc = 1.0f;
+        if constexpr (sizeof(TC) == 1) {
+            sc *= *reinterpret_cast<const float*>(a.ks + pg * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0);
+            vsc = *reinterpret_cast<const float*>(a.vs + pg * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0);
+        }
         if (a.softcap > 0.0f) sc = a.softcap * tanhf(sc / a.softcap);
         const float m2 = fmaxf(m, sc);
         const float keep = expf(m - m2), p = expf(sc - m2);
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const uint32_t e = lane + 64 * i;
-            if (e < a.D) o[i] = fmaf(p, Elt<TC>::load1(vr + e * Elt<TC>::size), o[i] * keep);
+            if (e < a.D) o[i] = fmaf(p * vsc, held<TC>(vr, e), o[i] * keep);
         }
         m = m2;
     }
@@ -129,12 +130,12 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_rows(AttnArgs a) {
         f[w] = expf(lds_m[w] - mm);
         ll = fmaf(lds_l[w], f[w], ll);
     }
-    char* yr = a.y + s * a.y_nb2 + h * a.y_nb1;
+    char* yr = a.y + t * a.y_nb2 + h * a.y_nb1;
     for (uint32_t e = threadIdx.x; e < a.D; e += kAttnThreads) {
-        float t = 0.0f;
+        float o1 = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; w++) t = fmaf(lds_o[w][e], f[w], t);
-        Elt<T>::store1(yr + e * Elt<T>::size, ll == 0.0f ? 0.0f : t / ll);
+        for (int w = 0; w < W; w++) o1 = fmaf(lds_o[w][e], f[w], o1);
+        Elt<T>::store1(yr + e * Elt<T>::size, ll == 0.0f ? 0.0f : o1 / ll);
     }
 }
 
@@ -192,10 +193,6 @@ struct LaneRow {
     }
     __device__ __forceinline__ u2v load8(uint32_t o) const { return *reinterpret_cast<const u2w*>(p + o); }
 };
-
-__device__ __forceinline__ uint32_t page_of(const AttnArgs& a, uint32_t key) {
-    return static_cast<uint32_t>((static_cast<uint64_t>(key) * a.page_mul) >> a.page_shift);
-}
 
 // A request's keys: [first, len), and the tiles of KT keys they lie in; a
 // request without keys has one tile all the same, which writes its zeros.
@@ -850,7 +847,7 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     p.H = static_cast<uint32_t>(hkv) * p.ngr;
     const int64_t cap_tiles = std::max<int64_t>(1, cdiv(cap, p.kt));
     const int64_t most = q->ne[2] * p.H * cap_tiles;
-    p.tiles = D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
+    p.tiles = k->type != CBX_TYPE_I8 && D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
     if (!p.tiles) return p;
     p.W = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(per_cu(p.dp, uniform_pages(k))) * st->n_cu, most));
     // A run a key head, without a join, while the longest a table can hold ends
@@ -872,12 +869,6 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
         p.bytes = p.o_bytes + p.ml_bytes + static_cast<size_t>(p.W) * sizeof(uint4);
     }
     return p;
-}
-
-bool vector_rows(const cbx_tensor* t) {
-    if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
-    for (int i = 1; i < 4; i++) if (t->ne[i] > 1 && t->nb[i] % 16) return false;
-    return t->nb[1] < (size_t{1} << 26);
 }
 
 template <typename TQ, typename TC, int DP>
@@ -908,20 +899,34 @@ size_t paged_attention_workspace(const cbx_tensor* q, const cbx_tensor* k, const
     return attn_plan(q, k, tables, st).bytes;
 }
 
-int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
+bool vector_rows(const cbx_tensor* t) {
+    if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
+    for (int i = 1; i < 4; i++) if (t->ne[i] > 1 && t->nb[i] % 16) return false;
+    return t->nb[1] < (size_t{1} << 26);
+}
+
+AttnArgs attn_args(const PagedAttnCall& c, const DeviceState* st) {
     AttnArgs a{};
-    a.q = static_cast<const char*>(c.q->data);
-    a.k = static_cast<const char*>(c.k->data);
-    a.v = static_cast<const char*>(c.v->data);
-    a.tables = static_cast<const char*>(c.tables->data);
-    a.lens = static_cast<const int32_t*>(c.lens->data);
+    auto at = [](const cbx_tensor* t) { return t ? static_cast<const char*>(t->data) : nullptr; };
+    auto nb = [](const cbx_tensor* t, int i) { return t ? static_cast<int64_t>(t->nb[i]) : 0; };
+    a.q = at(c.q);
+    a.k = at(c.k);
+    a.v = at(c.v);
+    a.ks = at(c.k_scale);
+    a.vs = at(c.v_scale);
+    a.tables = at(c.tables);
+    a.lens = reinterpret_cast<const int32_t*>(at(c.lens));
+    a.start = reinterpret_cast<const int32_t*>(at(c.start));
     a.y = static_cast<char*>(c.y->data);
-    a.q_nb1 = c.q->nb[1]; a.q_nb2 = c.q->nb[2];
-    a.y_nb1 = c.y->nb[1]; a.y_nb2 = c.y->nb[2];
-    a.k_nb1 = c.k->nb[1]; a.k_nb2 = c.k->nb[2]; a.k_nb3 = c.k->nb[3];
-    a.v_nb1 = c.v->nb[1]; a.v_nb2 = c.v->nb[2]; a.v_nb3 = c.v->nb[3];
-    a.t_nb1 = c.tables->nb[1];
-    a.n_seq = static_cast<uint32_t>(c.q->ne[2]);
+    a.q_nb1 = nb(c.q, 1); a.q_nb2 = nb(c.q, 2);
+    a.y_nb1 = nb(c.y, 1); a.y_nb2 = nb(c.y, 2);
+    a.k_nb1 = nb(c.k, 1); a.k_nb2 = nb(c.k, 2); a.k_nb3 = nb(c.k, 3);
+    a.v_nb1 = nb(c.v, 1); a.v_nb2 = nb(c.v, 2); a.v_nb3 = nb(c.v, 3);
+    a.ks_nb0 = nb(c.k_scale, 0); a.ks_nb1 = nb(c.k_scale, 1); a.ks_nb2 = nb(c.k_scale, 2);
+    a.vs_nb0 = nb(c.v_scale, 0); a.vs_nb1 = nb(c.v_scale, 1); a.vs_nb2 = nb(c.v_scale, 2);
+    a.t_nb1 = nb(c.tables, 1);
+    a.n_seq = static_cast<uint32_t>(c.tables->ne[1]);
+    a.n_rows = static_cast<uint32_t>(c.q->ne[2]);
     a.hq = static_cast<uint32_t>(c.q->ne[1]);
     a.hkv = static_cast<uint32_t>(c.k->ne[2]);
     a.g = a.hq / a.hkv;
@@ -933,9 +938,30 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
     a.scale = c.scale;
     a.softcap = c.softcap;
     a.err = st->err_word;
+    if (a.page > 0) page_division(a.page, &a.page_mul, &a.page_shift);
+    return a;
+}
+
+int launch_attention_rows(const AttnArgs& a, const PagedAttnCall& c, const char* what, hipStream_t s) {
+    const dim3 grid(a.n_rows * a.hq), block(kAttnThreads);
+    auto go = [&](auto t, auto tc) {
+        if (a.start) hipLaunchKernelGGL((k_attn_rows<decltype(t), decltype(tc), true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_attn_rows<decltype(t), decltype(tc), false>), grid, block, 0, s, a);
+    };
+    auto with = [&](auto t) {
+        if (c.k->type == CBX_TYPE_I8) go(t, int8_t());
+        else if (c.k->type == CBX_TYPE_F16) go(t, uint16_t());
+        else go(t, float());
+    };
+    if (c.q->type == CBX_TYPE_F16) with(uint16_t());
+    else with(float());
+    return check_launch(what);
+}
+
+int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
+    AttnArgs a = attn_args(c, st);
     const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
     if (p.tiles && vector_rows(c.k) && vector_rows(c.v)) {
-        page_division(a.page, &a.page_mul, &a.page_shift);
         a.gc = p.gc;
         a.ngr = p.ngr;
         a.H = p.H;
@@ -950,13 +976,7 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
         else launch_tiles<float, float>(p, uniform_pages(c.k), a, s);
         return check_launch("cbx_paged_attention");
     }
-    const dim3 grid(static_cast<unsigned>(c.q->ne[1] * c.q->ne[2])), block(kAttnThreads);
-    const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
-    if (t16 && c16) hipLaunchKernelGGL((k_attn_rows<uint16_t, uint16_t>), grid, block, 0, s, a);
-    else if (t16) hipLaunchKernelGGL((k_attn_rows<uint16_t, float>), grid, block, 0, s, a);
-    else if (c16) hipLaunchKernelGGL((k_attn_rows<float, uint16_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_attn_rows<float, float>), grid, block, 0, s, a);
-    return check_launch("cbx_paged_attention");
+    return launch_attention_rows(a, c, "cbx_paged_attention", s);
 }
 
 }  // namespace cbx

@@ -15,6 +15,12 @@
 // F16 pages, 64.2 us (328 MB, 5.1 TB/s; 62.0 without the profiler; k_qk, with q
 // off the alignment, 229), 64 tokens of 16 + 16 heads of 64 in F16 4.1 us.  k_qk:
 // a wave a head row, for sizes and alignments that the vectors do not take.
+//
+// Into I8 pages (Q8Row): the row's largest element over its lanes, then 8
+// elements a lane rounded to whole numbers of steps.
+//
+// k_load reads slots back: a workgroup a token, 8 elements of a key or value a
+// thread; bound by the bytes.
 #include "cbx_rowops.h"
 
 namespace cbx {
@@ -32,6 +38,8 @@ struct QkArgs {
     const float* ff;
     int64_t q_nb1, q_nb2, k_nb1, k_nb2, v_nb1, v_nb2, yq_nb1, yq_nb2, yk_nb1, yk_nb2;
     int64_t kc_nb1, kc_nb2, kc_nb3, vc_nb1, vc_nb2, vc_nb3;
+    char *ks, *vs;                      // I8 pages: their rows' scales
+    int64_t ks_nb0, ks_nb1, ks_nb2, vs_nb0, vs_nb1, vs_nb2;
     uint32_t hq, hkv, heads, rows, D;   // heads: hq + hkv (+ hkv value rows)
     uint32_t page, n_slot;              // page size, slots of the cache
     int32_t n_pos;
@@ -41,6 +49,46 @@ struct QkArgs {
     RopeParams rp;
     uint32_t* err;
 };
+
+// |x| as a number that compares as |x| does, infinities and NaN above all.
+__device__ __forceinline__ uint32_t size_of(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+// A row in 8 bits: scale = top / 127, n = 127 x / top to the nearest whole
+// number, ties to the even one, top its largest |x| (127 * 2^-126 at least, so
+// that the scale is a normal number).  In f32, 127 / top and the product are
+// 2^-22 of |n| <= 127 off, less than 2^-15: a result further than that from the
+// middle of two whole numbers is right, the others (and the rows whose 127 / top
+// leaves f32's range) are decided in f64, where 127 x is exact and the quotient
+// is a tie only where the true one is.
+struct Q8Row {
+    double top;
+    float mul, scale;
+    bool rough, bad;      // f32 decides nothing; an infinity or NaN among them
+    __device__ __forceinline__ explicit Q8Row(uint32_t largest) {
+        bad = largest >= 0x7f800000u;
+        const float t = fmaxf(bad ? 0.0f : __builtin_bit_cast(float, largest), 127 * 0x1p-126f);
+        top = static_cast<double>(t);
+        rough = t < 0x1p-100f;
+        mul = 127.0f / t;
+        scale = bad ? NAN : static_cast<float>(top / 127.0);
+    }
+    __device__ __forceinline__ int32_t of(float x) const {
+        if (bad) return 0;
+        const float t = x * mul, n = rintf(t);
+        if (rough || fabsf(t - n) > 0.5f - 0x1p-14f) return static_cast<int32_t>(rint(127.0 * static_cast<double>(x) / top));
+        return static_cast<int32_t>(n);
+    }
+    __device__ __forceinline__ uint32_t of4(const float4& v) const {
+        return (static_cast<uint32_t>(of(v.x)) & 0xffu) | (static_cast<uint32_t>(of(v.y)) & 0xffu) << 8 |
+               (static_cast<uint32_t>(of(v.z)) & 0xffu) << 16 | static_cast<uint32_t>(of(v.w)) << 24;
+    }
+};
+
+// The scale of a key (kind 1) or value.
+__device__ __forceinline__ void store_scale(const QkArgs& a, int kind, uint32_t pg, uint32_t h, uint32_t at, float scale) {
+    char* p = kind == 1 ? a.ks + pg * a.ks_nb2 + h * a.ks_nb1 + at * a.ks_nb0 : a.vs + pg * a.vs_nb2 + h * a.vs_nb1 + at * a.vs_nb0;
+    *reinterpret_cast<float*>(p) = scale;
+}
 
 template <typename T, typename TC>
 __global__ __launch_bounds__(kQkThreads) void k_qk(QkArgs a) {
@@ -115,10 +163,25 @@ __global__ __launch_bounds__(kQkThreads) void k_qk(QkArgs a) {
     const uint32_t pg = static_cast<uint32_t>(slot) / a.page, at = static_cast<uint32_t>(slot) - pg * a.page;
     char* y = kind == 1 ? a.kc + pg * a.kc_nb3 + hh * a.kc_nb2 + at * a.kc_nb1
                         : a.vc + pg * a.vc_nb3 + hh * a.vc_nb2 + at * a.vc_nb1;
+    if constexpr (sizeof(TC) == 1) {
+        uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const uint32_t e = lane + 64 * i;
-        if (e < D) Elt<TC>::store1(y + e * Elt<TC>::size, v[i]);
+        for (int i = 0; i < N; i++) top = max(top, static_cast<uint32_t>(lane + 64 * i) < D ? size_of(v[i]) : 0u);
+        for (int d = 32; d > 0; d >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+        const Q8Row row(top);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t e = lane + 64 * i;
+            if (e < D) y[e] = static_cast<char>(row.of(v[i]));
+        }
+        if (lane == 0) store_scale(a, kind, pg, hh, at, row.scale);
+        return;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t e = lane + 64 * i;
+            if (e < D) Elt<TC>::store1(y + e * Elt<TC>::size, v[i]);
+        }
     }
 }
 
@@ -131,6 +194,14 @@ template <int LPR> __device__ __forceinline__ double head_sum(double v) {
     if constexpr (LPR >= 16) v += dpp_f64<0x140>(v);
     if constexpr (LPR >= 32) v += __shfl_xor(v, 16);
     if constexpr (LPR >= 64) v += __shfl_xor(v, 32);
+    return v;
+}
+
+// Largest over them.
+template <int LPR> __device__ __forceinline__ uint32_t head_max(uint32_t v) {
+    auto step = [&](int d) { v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d))); };
+#pragma unroll
+    for (int d = 1; d < LPR; d *= 2) step(d);
     return v;
 }
 
@@ -235,6 +306,12 @@ __global__ __launch_bounds__(kQkThreads) void k_qk_heads(QkArgs a) {
                     }
                 }
             }
+            uint32_t top = 0;
+            if constexpr (sizeof(TC) == 1) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = max(top, max(size_of(get(xa[u], e)), size_of(get(xb[u], e))));
+                top = head_max<LPR>(in ? top : 0);
+            }
             if (!in) continue;
             if (kind == 0 || !a.slots) {
                 char* y = kind == 0 ? a.yq + tok * a.yq_nb2 + h * a.yq_nb1 : a.yk + tok * a.yk_nb2 + (h - a.hq) * a.yk_nb1;
@@ -244,8 +321,15 @@ __global__ __launch_bounds__(kQkThreads) void k_qk_heads(QkArgs a) {
                 const uint32_t hh = h - a.hq - (kind == 2 ? a.hkv : 0);
                 char* y = kind == 1 ? a.kc + pg * a.kc_nb3 + hh * a.kc_nb2 + at * a.kc_nb1
                                     : a.vc + pg * a.vc_nb3 + hh * a.vc_nb2 + at * a.vc_nb1;
-                Elt<TC>::store4(y + ia * Elt<TC>::size, xa[u]);
-                Elt<TC>::store4(y + ib * Elt<TC>::size, xb[u]);
+                if constexpr (sizeof(TC) == 1) {
+                    const Q8Row row(top);
+                    *reinterpret_cast<uint32_t*>(y + ia) = row.of4(xa[u]);
+                    *reinterpret_cast<uint32_t*>(y + ib) = row.of4(xb[u]);
+                    if (li == 0) store_scale(a, kind, pg, hh, at, row.scale);
+                } else {
+                    Elt<TC>::store4(y + ia * Elt<TC>::size, xa[u]);
+                    Elt<TC>::store4(y + ib * Elt<TC>::size, xb[u]);
+                }
             }
         }
     }
@@ -274,7 +358,124 @@ void launch_heads(QkArgs& a, uint32_t tok, hipStream_t s) {
     else hipLaunchKernelGGL((k_qk_heads<T, TC, 64>), grid, block, 0, s, a);
 }
 
+struct LoadArgs {
+    const char *kc, *vc, *ks, *vs;
+    const int32_t* slots;
+    char *k, *v;
+    int64_t k_nb1, k_nb2, v_nb1, v_nb2, kc_nb1, kc_nb2, kc_nb3, vc_nb1, vc_nb2, vc_nb3;
+    int64_t ks_nb0, ks_nb1, ks_nb2, vs_nb0, vs_nb1, vs_nb2;
+    uint32_t hkv, D, cpr, page, n_slot;   // cpr: runs of VEC elements a row
+    uint32_t* err;
+};
+
+template <typename TC, int VEC> __device__ __forceinline__ void load_row(const char* p, float (&x)[VEC]) {
+    if constexpr (VEC == 1) {
+        if constexpr (sizeof(TC) == 1) x[0] = static_cast<float>(*reinterpret_cast<const int8_t*>(p));
+        else x[0] = Elt<TC>::load1(p);
+    } else if constexpr (sizeof(TC) == 1) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? t.x : t.y) >> 8 * (i & 3)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 t = Elt<TC>::load4(p + i * Elt<TC>::size);
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[i + j] = get(t, j);
+        }
+    }
+}
+
+template <typename T, typename TC, int VEC>
+__global__ __launch_bounds__(kQkThreads) void k_load(LoadArgs a) {
+    const uint32_t tok = blockIdx.x;
+    int32_t slot = a.slots[tok];
+    if (slot >= 0 && static_cast<uint32_t>(slot) >= a.n_slot) {
+        if (threadIdx.x == 0) atomicOr(a.err, DEV_ERR_PAGE);
+        slot = -1;
+    }
+    const uint32_t pg = slot < 0 ? 0 : static_cast<uint32_t>(slot) / a.page, at = slot < 0 ? 0 : static_cast<uint32_t>(slot) - pg * a.page;
+    const uint32_t runs = a.hkv * a.cpr;
+    for (uint32_t i = threadIdx.x; i < 2 * runs; i += blockDim.x) {
+        const bool val = i >= runs;
+        const uint32_t j = val ? i - runs : i, h = j / a.cpr, e = (j - h * a.cpr) * VEC;
+        float x[VEC] = {};
+        if (slot >= 0) {
+            const char* p = val ? a.vc + pg * a.vc_nb3 + h * a.vc_nb2 + at * a.vc_nb1 : a.kc + pg * a.kc_nb3 + h * a.kc_nb2 + at * a.kc_nb1;
+            load_row<TC, VEC>(p + e * sizeof(TC), x);
+            if constexpr (sizeof(TC) == 1) {
+                const char* sp = val ? a.vs + pg * a.vs_nb2 + h * a.vs_nb1 + at * a.vs_nb0
+                                     : a.ks + pg * a.ks_nb2 + h * a.ks_nb1 + at * a.ks_nb0;
+                const float sc = *reinterpret_cast<const float*>(sp);
+#pragma unroll
+                for (int u = 0; u < VEC; u++) x[u] *= sc;
+            }
+        }
+        char* y = val ? a.v + tok * a.v_nb2 + h * a.v_nb1 : a.k + tok * a.k_nb2 + h * a.k_nb1;
+        if constexpr (VEC == 1) {
+            Elt<T>::store1(y + e * Elt<T>::size, x[0]);
+        } else {
+            Elt<T>::store4(y + e * Elt<T>::size, make_float4(x[0], x[1], x[2], x[3]));
+            Elt<T>::store4(y + (e + 4) * Elt<T>::size, make_float4(x[4], x[5], x[6], x[7]));
+        }
+    }
+}
+
+// Rows of a cache at steps that k_load's reads of 8 elements take.
+bool eights(const cbx_tensor* t) {
+    const size_t al = t->type == CBX_TYPE_F32 ? 16 : 8;
+    if (reinterpret_cast<uintptr_t>(t->data) % al) return false;
+    for (int i = 1; i < 4; i++) if (t->ne[i] > 1 && t->nb[i] % al) return false;
+    return true;
+}
+
+template <typename T, typename TC>
+void launch_load(const LoadArgs& a, bool vec, uint32_t tok, hipStream_t s) {
+    const int64_t runs = 2 * static_cast<int64_t>(a.hkv) * a.cpr;
+    const dim3 block(static_cast<unsigned>(std::min<int64_t>(kQkThreads, cdiv(runs, 64) * 64)));
+    if (vec) hipLaunchKernelGGL((k_load<T, TC, 8>), dim3(tok), block, 0, s, a);
+    else hipLaunchKernelGGL((k_load<T, TC, 1>), dim3(tok), block, 0, s, a);
+}
+
 }  // namespace
+
+int launch_paged_load(const LoadCall& c, DeviceState* st, hipStream_t s) {
+    LoadArgs a{};
+    auto in = [](const cbx_tensor* t) { return t ? static_cast<const char*>(t->data) : nullptr; };
+    a.kc = in(c.k_cache);
+    a.vc = in(c.v_cache);
+    a.ks = in(c.k_scale);
+    a.vs = in(c.v_scale);
+    a.slots = reinterpret_cast<const int32_t*>(in(c.slots));
+    a.k = static_cast<char*>(c.k->data);
+    a.v = static_cast<char*>(c.v->data);
+    a.k_nb1 = nb(c.k, 1); a.k_nb2 = nb(c.k, 2);
+    a.v_nb1 = nb(c.v, 1); a.v_nb2 = nb(c.v, 2);
+    a.kc_nb1 = nb(c.k_cache, 1); a.kc_nb2 = nb(c.k_cache, 2); a.kc_nb3 = nb(c.k_cache, 3);
+    a.vc_nb1 = nb(c.v_cache, 1); a.vc_nb2 = nb(c.v_cache, 2); a.vc_nb3 = nb(c.v_cache, 3);
+    a.ks_nb0 = nb(c.k_scale, 0); a.ks_nb1 = nb(c.k_scale, 1); a.ks_nb2 = nb(c.k_scale, 2);
+    a.vs_nb0 = nb(c.v_scale, 0); a.vs_nb1 = nb(c.v_scale, 1); a.vs_nb2 = nb(c.v_scale, 2);
+    a.hkv = static_cast<uint32_t>(c.k->ne[1]);
+    a.D = static_cast<uint32_t>(c.k->ne[0]);
+    a.page = static_cast<uint32_t>(c.k_cache->ne[1]);
+    a.n_slot = static_cast<uint32_t>(c.k_cache->ne[1] * c.k_cache->ne[3]);
+    a.err = st->err_word;
+    const bool vec = a.D % 8 == 0 && quads(c.k) && quads(c.v) && eights(c.k_cache) && eights(c.v_cache);
+    a.cpr = vec ? a.D / 8 : a.D;
+    const uint32_t tok = static_cast<uint32_t>(c.k->ne[2]);
+    const bool t16 = c.k->type == CBX_TYPE_F16;
+    if (c.k_cache->type == CBX_TYPE_I8) {
+        if (t16) launch_load<uint16_t, int8_t>(a, vec, tok, s);
+        else launch_load<float, int8_t>(a, vec, tok, s);
+    } else if (c.k_cache->type == CBX_TYPE_F16) {
+        if (t16) launch_load<uint16_t, uint16_t>(a, vec, tok, s);
+        else launch_load<float, uint16_t>(a, vec, tok, s);
+    } else {
+        if (t16) launch_load<uint16_t, float>(a, vec, tok, s);
+        else launch_load<float, float>(a, vec, tok, s);
+    }
+    return check_launch("cbx_paged_load");
+}
 
 int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
     const cbx_tensor* k = c.k;
@@ -303,6 +504,10 @@ int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
     a.yk_nb1 = nb(c.yk, 1); a.yk_nb2 = nb(c.yk, 2);
     a.kc_nb1 = nb(c.k_cache, 1); a.kc_nb2 = nb(c.k_cache, 2); a.kc_nb3 = nb(c.k_cache, 3);
     a.vc_nb1 = nb(c.v_cache, 1); a.vc_nb2 = nb(c.v_cache, 2); a.vc_nb3 = nb(c.v_cache, 3);
+    a.ks = out(c.k_scale);
+    a.vs = out(c.v_scale);
+    a.ks_nb0 = nb(c.k_scale, 0); a.ks_nb1 = nb(c.k_scale, 1); a.ks_nb2 = nb(c.k_scale, 2);
+    a.vs_nb0 = nb(c.v_scale, 0); a.vs_nb1 = nb(c.v_scale, 1); a.vs_nb2 = nb(c.v_scale, 2);
     a.hq = c.q ? static_cast<uint32_t>(c.q->ne[1]) : 0;
     a.hkv = static_cast<uint32_t>(k->ne[1]);
     a.heads = a.hq + a.hkv * (c.v ? 2 : 1);
@@ -318,10 +523,13 @@ int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
     const bool vec = a.D % 8 == 0 && quads(c.q) && quads(k) && quads(c.v) && quads(c.yq) && quads(c.yk) && quads(c.k_cache) &&
                      quads(c.v_cache) && quads(c.gq) && quads(c.gk) && reinterpret_cast<uintptr_t>(a.table) % 16 == 0;
     const dim3 grid(static_cast<unsigned>(cdiv(rows, kQkThreads / 64))), block(kQkThreads);
+    const bool i8 = c.k_scale != nullptr;
     const bool t16 = k->type == CBX_TYPE_F16, c16 = c.k_cache ? c.k_cache->type == CBX_TYPE_F16 : t16;
     if (vec) {
         const uint32_t tok = static_cast<uint32_t>(k->ne[2]);
-        if (t16 && c16) launch_heads<uint16_t, uint16_t>(a, tok, s);
+        if (i8 && t16) launch_heads<uint16_t, int8_t>(a, tok, s);
+        else if (i8) launch_heads<float, int8_t>(a, tok, s);
+        else if (t16 && c16) launch_heads<uint16_t, uint16_t>(a, tok, s);
         else if (t16) launch_heads<uint16_t, float>(a, tok, s);
         else if (c16) launch_heads<float, uint16_t>(a, tok, s);
         else launch_heads<float, float>(a, tok, s);
@@ -330,7 +538,9 @@ int launch_qk(const QkCall& c, DeviceState* st, hipStream_t s) {
     if (grid.x >= 1u << 24) {     // a launch's threads below 2^32
         return set_error(CBX_ERR_UNSUPPORTED, "cbx_qk_norm_rope: 2^26 rows or more, at sizes or alignments that vectors do not take");
     }
-    if (t16 && c16) hipLaunchKernelGGL((k_qk<uint16_t, uint16_t>), grid, block, 0, s, a);
+    if (i8 && t16) hipLaunchKernelGGL((k_qk<uint16_t, int8_t>), grid, block, 0, s, a);
+    else if (i8) hipLaunchKernelGGL((k_qk<float, int8_t>), grid, block, 0, s, a);
+    else if (t16 && c16) hipLaunchKernelGGL((k_qk<uint16_t, uint16_t>), grid, block, 0, s, a);
     else if (t16) hipLaunchKernelGGL((k_qk<uint16_t, float>), grid, block, 0, s, a);
     else if (c16) hipLaunchKernelGGL((k_qk<float, uint16_t>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((k_qk<float, float>), grid, block, 0, s, a);

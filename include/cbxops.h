@@ -35,6 +35,7 @@ typedef enum cbx_type {
     CBX_TYPE_F32  = 0,
     CBX_TYPE_F16  = 1,
     CBX_TYPE_Q8_0 = 8,   /* blocks of 32: f16 scale d + int8 qs[32], 34 bytes */
+    CBX_TYPE_I8   = 24,  /* only the pages of an 8-bit key-value cache */
     CBX_TYPE_I32  = 26,
 } cbx_type;
 
@@ -529,13 +530,19 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  *   block_tables
  *             I32 (max_pages, n_seq): entry i of request s is the page that
  *             holds its keys [i * page_size, (i + 1) * page_size)
+ *             or I8 with k_scale, v_scale (the _q8 calls): F32, ne =
+ *             (page_size, n_head_kv, n_pages), any strides, one scale for the
+ *             head_dim elements of a key (value) of one head, which stand for
+ *             scale * element: a cache of half the F16 one's bytes
  *   slot      page * page_size + place in the page; a negative slot belongs
  *             to no request (the padding of a batch)
  *   free_pages, n_free
  *             I32: a stack of free page numbers, n_free[0] of them, the top
  *             last
  * A page has one owner, the stack or one entry of one table: nothing counts
- * its users, so a page that two tables name is given back twice.
+ * its users, so a page that two tables name is given back twice.  Requests
+ * that share the P whole pages they begin with are released by the view of
+ * their tables behind those P columns, their lengths less P * page_size.
  * All of it lives on the device: no call reads a length on the host, so a
  * captured step replays as its requests grow.  Page numbers, slots and
  * lengths that lie outside their tensors are left out by the kernels that
@@ -592,6 +599,27 @@ int cbx_paged_store(const cbx_tensor* k, const cbx_tensor* v,
                     const cbx_tensor* slots, cbx_tensor* k_cache,
                     cbx_tensor* v_cache, cbx_stream stream);
 
+/* The same into an 8-bit cache (I8 with its scales).  With top the largest
+ * |x| of a row's head_dim elements, but 127 * 2^-126 at least:
+ *   scale = top / 127, element = 127 x / top to the nearest whole number, of
+ *   two the even one
+ * decided exactly, and the scale rounded to F32; what the row stands for is
+ * within scale / 2 of x (half a step of F32 aside).  A row with an infinity
+ * or a NaN gets the scale NaN.                                             */
+int cbx_paged_store_q8(const cbx_tensor* k, const cbx_tensor* v,
+                       const cbx_tensor* slots, cbx_tensor* k_cache,
+                       cbx_tensor* k_scale, cbx_tensor* v_cache,
+                       cbx_tensor* v_scale, cbx_stream stream);
+
+/* Reads the keys and values of slots back: row t of k and v, F32 or F16
+ * (head_dim, n_head_kv, n_tok), is what slot slots[t] of the caches stands
+ * for, rounded to the rows' type; negative slots give zeros.  k_scale and
+ * v_scale: of an I8 cache, NULL for F32 and F16.  n_tok < 2^24.            */
+int cbx_paged_load(const cbx_tensor* slots, const cbx_tensor* k_cache,
+                   const cbx_tensor* k_scale, const cbx_tensor* v_cache,
+                   const cbx_tensor* v_scale, cbx_tensor* k, cbx_tensor* v,
+                   cbx_stream stream);
+
 /* RMS norm of every query and key head, then the rotation, in one pass:
  *   yq = ggml_rope_ext(ggml_mul(ggml_rms_norm(q, eps), gq), pos, ...)
  *   yk = ggml_rope_ext(ggml_mul(ggml_rms_norm(k, eps), gk), pos, ...)
@@ -616,6 +644,16 @@ int cbx_qk_norm_rope_store(const cbx_tensor* q, const cbx_tensor* gq,
                            const cbx_tensor* slots, cbx_tensor* yq,
                            cbx_tensor* k_cache, cbx_tensor* v_cache,
                            cbx_stream stream);
+/* ... into an 8-bit cache, as cbx_paged_store_q8.                          */
+int cbx_qk_norm_rope_store_q8(const cbx_tensor* q, const cbx_tensor* gq,
+                              const cbx_tensor* k, const cbx_tensor* gk,
+                              const cbx_tensor* v, float eps,
+                              const cbx_tensor* pos,
+                              const cbx_rope_cache* rope,
+                              const cbx_tensor* slots, cbx_tensor* yq,
+                              cbx_tensor* k_cache, cbx_tensor* k_scale,
+                              cbx_tensor* v_cache, cbx_tensor* v_scale,
+                              cbx_stream stream);
 
 /* Attention of one new token a request over its cached keys
  * (t3.cpp:494-522 with N_new = 1, for every request at once):
@@ -647,6 +685,79 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
                         const cbx_tensor* seq_lens, float scale,
                         float softcap, int32_t window, cbx_tensor* y,
                         void* ws, size_t ws_bytes, cbx_stream stream);
+/* ... over an 8-bit cache: k_i and v_i are scale * element.  The scales
+ * multiply the products' sums and the probabilities in f32.  Workspace as
+ * above, of the I8 k_cache.                                                */
+int cbx_paged_attention_q8(const cbx_tensor* q, const cbx_tensor* k_cache,
+                           const cbx_tensor* k_scale,
+                           const cbx_tensor* v_cache,
+                           const cbx_tensor* v_scale,
+                           const cbx_tensor* block_tables,
+                           const cbx_tensor* seq_lens, float scale,
+                           float softcap, int32_t window, cbx_tensor* y,
+                           void* ws, size_t ws_bytes, cbx_stream stream);
+
+/* Causal attention of all new tokens of packed requests (t3.cpp:494-522 with
+ * N_new tokens and its causal mask, for every request at once): prompts,
+ * pieces of them behind what is cached already, drafted tokens.  The new
+ * keys are in the cache by then (cbx_paged_append, then a store).
+ *   q, y       F32 or F16 (head_dim, n_head, n_tok), one type
+ *   tok_start  I32 (n_seq + 1), as cbx_paged_append gives it: request s has
+ *              the tokens [tok_start[s], tok_start[s + 1]), never falling
+ *   seq_lens   I32 (n_seq): keys, the new tokens' own among them: token j of
+ *              n_new sits at position p = seq_lens[s] - n_new + j and attends
+ *              over the keys i <= p, window > 0: p - window < i <= p
+ * Rows of q before tok_start[0] and from tok_start[n_seq] on belong to no
+ * request: their rows of y stay as they are.  A token with nothing to attend
+ * over (p < 0: more tokens than keys, as of a request that append refused)
+ * gets zeros.  What lies at keys that a token does not attend over never
+ * reaches its row, infinities and NaN included.  k_scale, v_scale: of an I8
+ * cache, NULL for F32 and F16.  The rest as for cbx_paged_attention, with
+ * n_head * n_tok < 2^24 and one choice more: where the matrix cores are the
+ * bound (an F16 query in a call of many rows), probabilities are rounded to F16
+ * for their products, by up to 2^-11 of themselves, and the sums they are
+ * divided by are sums of the rounded ones.                                 */
+int cbx_paged_prompt_attention_workspace(const cbx_tensor* q,
+                                         const cbx_tensor* k_cache,
+                                         const cbx_tensor* block_tables,
+                                         size_t* bytes);
+int cbx_paged_prompt_attention(const cbx_tensor* q,
+                               const cbx_tensor* k_cache,
+                               const cbx_tensor* k_scale,
+                               const cbx_tensor* v_cache,
+                               const cbx_tensor* v_scale,
+                               const cbx_tensor* block_tables,
+                               const cbx_tensor* seq_lens,
+                               const cbx_tensor* tok_start, float scale,
+                               float softcap, int32_t window, cbx_tensor* y,
+                               void* ws, size_t ws_bytes, cbx_stream stream);
+
+/* cbx_paged_attention (one new token a request) for requests that begin with
+ * the same keys: takes of one text, questions to one document.  Those keys are
+ * read once for all of a group.
+ *   group_start  I32 (n_groups + 1): group p is the requests
+ *                [group_start[p], group_start[p + 1]), never falling; requests
+ *                outside share nothing
+ *   shared_lens  I32 (n_groups): so many keys at the beginning of the group's
+ *                requests lie in the same pages, by each one's table
+ * block_tables and seq_lens are as cbx_paged_attention's, the shared keys
+ * among them (a request may be shorter than its group's shared keys), and so
+ * are the results, up to the rounding of sums that are split elsewhere.    */
+int cbx_paged_shared_attention_workspace(const cbx_tensor* q,
+                                         const cbx_tensor* k_cache,
+                                         const cbx_tensor* block_tables,
+                                         const cbx_tensor* group_start,
+                                         size_t* bytes);
+int cbx_paged_shared_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
+                               const cbx_tensor* k_scale,
+                               const cbx_tensor* v_cache,
+                               const cbx_tensor* v_scale,
+                               const cbx_tensor* block_tables,
+                               const cbx_tensor* seq_lens,
+                               const cbx_tensor* group_start,
+                               const cbx_tensor* shared_lens, float scale,
+                               float softcap, int32_t window, cbx_tensor* y,
+                               void* ws, size_t ws_bytes, cbx_stream stream);
 
 /* What a step answers with: of each row of logits x, F32 or F16
  * (n_vocab, n_tok), with p = softmax(scale * x) (0 < scale < 2^126: one over
