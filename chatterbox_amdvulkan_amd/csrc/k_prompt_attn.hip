@@ -1,14 +1,689 @@
 // k_prompt_attn.hip -- causal attention of all new tokens of packed requests
 // over a paged cache, and of one new token a request where groups of requests
 // begin with the same pages.
+//
+// Row i attends over its keys [first_i, limit_i): y_i = sum_j softmax(s_i)_j v_j
+// with s_ij = scale q_i . k_j, in one pass over the keys: with a running maximum
+// m, l = sum exp(s - m) and o = sum exp(s - m) v, both rescaled when the maximum
+// rises, and y = o / l at the end.
 #include "cbx_attn.h"
 
 namespace cbx {
+namespace {
 
-size_t paged_prompt_workspace(const cbx_tensor*, const cbx_tensor*, const cbx_tensor*, const DeviceState*) { return 0; }
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h4v __attribute__((ext_vector_type(4)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+
+constexpr int kRows = 128;     // rows of q a workgroup: 4 waves of 32
+
+struct PromptArgs {
+    AttnArgs a;
+    const int32_t* shared;     // shared keys a group; null: packed tokens
+    uint32_t n_start;          // requests or groups: start has one more
+    uint32_t n_split, n_part;  // runs that a row tile's keys are dealt to; parts a row has in part_o
+    uint32_t tiles;            // row tiles at most
+    uint32_t g_mul, g_shift;   // i / g
+    float* part_o;             // [row * hq + head][n_part][D], null: y
+    float2* part_ml;
+    int32_t* own_first;        // [n_seq]: first key behind the group's shared ones
+};
+
+// Four neighbouring elements at any element alignment.
+__device__ __forceinline__ void load4u(const char* p, float* v, float) {
+    const f4u t = *reinterpret_cast<const f4u*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = t[j];
+}
+__device__ __forceinline__ void load4u(const char* p, float* v, uint16_t) {
+    const h4u t = *reinterpret_cast<const h4u*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = static_cast<float>(t[j]);
+}
+__device__ __forceinline__ void store4u(char* p, const float* v, float) {
+    *reinterpret_cast<f4u*>(p) = f4u{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ void store4u(char* p, const float* v, uint16_t) {
+    *reinterpret_cast<h4u*>(p) = h4u{static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
+                                     static_cast<_Float16>(v[3])};
+}
+
+__device__ __forceinline__ h4v read_turned(const char* lds) {
+    typedef __attribute__((address_space(3))) s4v lds_s4;
+    return __builtin_bit_cast(h4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(lds)));
+}
+
+// tanh without branches: an odd series below 1/2 (its next term is 2^-26 of the
+// sum), 1 - 2 / (1 + exp 2x) above; 3 units in the last place.
+__device__ __forceinline__ float tanh_of(float x) {
+    const float y = fabsf(x), z = y * y;
+    float p = fmaf(z, -929569.0f / 638512875.0f, 21844.0f / 6081075.0f);
+    p = fmaf(z, p, -1382.0f / 155925.0f);
+    p = fmaf(z, p, 62.0f / 2835.0f);
+    p = fmaf(z, p, -17.0f / 315.0f);
+    p = fmaf(z, p, 2.0f / 15.0f);
+    p = fmaf(z, p, -1.0f / 3.0f);
+    const float small = fmaf(y * z, p, y);
+    const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+    const float large = 1.0f - 2.0f / (1.0f + e);
+    return copysignf(y < 0.5f ? small : large, x);
+}
+
+// A tile of KT keys and values in LDS, and the products over it.  A wave holds
+// 32 rows of q: S^T = K Q^T by 32 x 32 products, whose result has the lane's row
+// lane % 32 and keys 8 (r / 4) + 4 (lane / 32) + r % 4; O^T = V^T P^T takes these
+// as its B operand as they are (the sum over keys in any order, as long as V's
+// come in the same one), V^T's columns by turning 4 x 16 blocks on the way out of
+// LDS.  So a row's maximum and sum are its lane's, and nothing else crosses lanes.
+//
+// LDS holds rows of DP elements as 16-byte chunks, chunk c of key r at place
+// c ^ f(r): the 16 lanes that read together meet 16 different places of 256
+// bytes.
+template <typename TC, int DP> struct Tile;
+
+// F16 pages, and I8 ones as whole numbers: keys in f16; values in f16, of I8 pages
+// in bf16, whose range holds a probability times any scale.
+template <typename TC, int DP> struct Tile {
+    static constexpr bool I8 = sizeof(TC) == 1;
+    static constexpr int KT = DP <= 128 ? 64 : 32, PITCH = DP * 2, CH = DP / 8;      // bytes a row, chunks
+    static constexpr int BYTES = KT * PITCH;
+    static constexpr int QC = DP / 16;
+    // which elements a lane reads of a row: 16 bytes
+    static constexpr int PER = I8 ? 16 : 8, LANES = DP / PER <= 4 ? 4 : DP / PER <= 8 ? 8 : DP / PER <= 16 ? 16 : 32;
+    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) {
+        if constexpr (DP == 64) return c ^ (r >> 1 & 7);
+        else if constexpr (DP == 96) return c ^ (r >> 2 & 3);
+        else return c ^ (r & 15);
+    }
+    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) {
+        if constexpr (DP == 64) return c ^ (r >> 1 & 1) << 2;
+        else if constexpr (DP == 96) return c;
+        else return c ^ (r & 3) << 2;
+    }
+};
+
+template <typename TQ, typename TC, int DP, int PP>
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_prompt(PromptArgs pa) {
+    using T = Tile<TC, DP>;
+    constexpr bool I8 = T::I8, Q2 = sizeof(TQ) == 4;
+    constexpr int KT = T::KT, PITCH = T::PITCH, CH = T::CH, QC = T::QC, LANES = T::LANES;
+    constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave reads at a time, times
+    constexpr float kUp = PP == 1 ? 9.0f : 14.0f, kRise = PP == 1 ? 6.0f : 1.0f;
+    const AttnArgs& a = pa.a;
+    __shared__ __attribute__((aligned(16))) char lds_k[2][T::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds_v[2][T::BYTES];
+    __shared__ __attribute__((aligned(16))) float lds_s[2][2][I8 ? KT : 4];
+    __shared__ int32_t lds_ext[4][4];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+    const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    // this workgroup's key head, run of keys and row tile (the last rows, which have the most keys, first)
+    const uint32_t hk = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, run = rest % pa.n_split;
+    const uint32_t x = pa.tiles - 1 - rest / pa.n_split;
+    // the request (group) p whose tiles x lies among: tiles of p start at start[p] * g / 128 + p, which leaves one more than it has
+    auto start_of = [&](uint32_t p) {
+        const int32_t t = a.start[p];
+        return t < 0 ? 0u : min(static_cast<uint32_t>(t), a.n_rows);
+    };
+    uint32_t p = 0;
+    for (uint32_t width = pa.n_start;;) {                    // p among [p, p + width)
+        const uint32_t step = (width + 63) / 64, q = p + lane * step;
+        const bool in = lane * step < width && start_of(q) * a.g / kRows + q <= x;
+        const uint32_t at = 64 - __builtin_clzll(__ballot(in) | 1) - 1;
+        p = __builtin_amdgcn_readfirstlane(p + at * step);
+        width = min(step, width - min(width, at * step));
+        if (step == 1) break;
+    }
+    const uint32_t t0 = start_of(p), t1 = start_of(p + 1);
+    const uint32_t base = t0 * a.g / kRows + p;
+    if (x < base || t1 <= t0 || static_cast<uint64_t>(x - base) * kRows >= static_cast<uint64_t>(t1 - t0) * a.g) return;
+    const uint32_t row0 = (x - base) * kRows, rows = min(static_cast<uint32_t>(kRows), (t1 - t0) * a.g - row0);
+
+    // the lane's row: token or request t, head, keys [first, limit)
+    const uint32_t r = wid * 32 + n;
+    const bool live_row = r < rows;
+    const uint32_t ri = row0 + (live_row ? r : 0);
+    const uint32_t j = static_cast<uint32_t>((static_cast<uint64_t>(ri) * pa.g_mul) >> pa.g_shift);
+    const uint32_t t = t0 + j, hq = hk * a.g + (ri - j * a.g);
+    const int32_t cap = static_cast<int32_t>(a.max_pages * a.page);
+    bool wrong = false;
+    int32_t limit, first;
+    uint32_t seq;                                            // whose table
+    {
+        seq = pa.shared ? t0 : p;
+        const int32_t given = a.lens[pa.shared ? t : p];
+        wrong = given < 0 || given > cap;
+        const int32_t len = min(max(given, 0), cap);
+        if (pa.shared) {
+            const int32_t pre = min(max(pa.shared[p], 0), cap);
+            first = a.window > 0 && len > a.window ? len - a.window : 0;
+            limit = min(len, pre);
+            if (hk == 0 && run == 0 && half == 0 && live_row) pa.own_first[t] = limit;
+        } else {
+            limit = max(0, len - static_cast<int32_t>(t1 - 1 - t));
+            first = a.window > 0 && limit > a.window ? limit - a.window : 0;
+        }
+        if (!live_row) limit = first = 0;
+    }
+    // the wave's rows: keys that any of them has, that all of them have
+    int32_t w_end = limit, w_begin = limit > first ? first : 0x7fffffff, all_end = live_row ? limit : 0x7fffffff, all_begin = first;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        w_end = max(w_end, __shfl_xor(w_end, d));
+        w_begin = min(w_begin, __shfl_xor(w_begin, d));
+        all_end = min(all_end, __shfl_xor(all_end, d));
+        all_begin = max(all_begin, __shfl_xor(all_begin, d));
+    }
+    w_end = __builtin_amdgcn_readfirstlane(w_end);
+    w_begin = __builtin_amdgcn_readfirstlane(w_begin);
+    all_end = __builtin_amdgcn_readfirstlane(all_end);
+    all_begin = __builtin_amdgcn_readfirstlane(all_begin);
+    if (lane == 0) {
+        lds_ext[0][wid] = w_end;
+        lds_ext[1][wid] = w_begin;
+        lds_ext[2][wid] = all_end;
+        lds_ext[3][wid] = all_begin;
+    }
+    __syncthreads();
+    const int32_t end = max(max(lds_ext[0][0], lds_ext[0][1]), max(lds_ext[0][2], lds_ext[0][3]));
+    const int32_t begin = min(min(min(lds_ext[1][0], lds_ext[1][1]), min(lds_ext[1][2], lds_ext[1][3])), end);
+    const int32_t every_end = min(min(lds_ext[2][0], lds_ext[2][1]), min(lds_ext[2][2], lds_ext[2][3]));
+    const int32_t every_begin = max(max(lds_ext[3][0], lds_ext[3][1]), max(lds_ext[3][2], lds_ext[3][3]));
+    const uint32_t tile0 = static_cast<uint32_t>(begin) / KT, n_tiles = (static_cast<uint32_t>(end) + KT - 1) / KT - tile0;
+    const uint32_t ta = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * run / pa.n_split));
+    const uint32_t tb = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * (run + 1) / pa.n_split));
+
+    // the lane's query: dims 16 c + 8 half + [0, 8).  An F32 one is scaled by a power of two to below 2^15 and split into two f16, the
+    // lower times 2^12 and summed apart
+    h8v qh[QC], ql[Q2 ? QC : 1];
+    float mul = fabsf(a.scale) * kLog2e;
+    {
+        float v[QC * 8];
+        const char* qr = a.q + t * a.q_nb2 + hq * a.q_nb1;
+#pragma unroll
+        for (int i = 0; i < QC * 8; i += 4) {
+            const uint32_t d = 16 * (i / 8) + 8 * half + i % 8;
+            const bool in = live_row && d < a.D;
+            float tmp[4];
+            load4u(qr + (in ? d : 0) * Elt<TQ>::size, tmp, TQ());
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[i + u] = in ? (a.scale < 0.0f ? -tmp[u] : tmp[u]) : 0.0f;
+        }
+        if constexpr (Q2) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QC * 8; i++) m = fmaxf(m, fabsf(v[i]));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            int e = m > 0.0f && m < INFINITY ? static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23) - 127 : 14;
+            e = e < -100 ? -100 : e;
+            mul *= ldexpf(1.0f, e - 14);
+            const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+            for (int i = 0; i < QC * 8; i++) {
+                const float y = v[i] * up;
+                const _Float16 h = static_cast<_Float16>(y);
+                qh[i / 8][i % 8] = h;
+                ql[i / 8][i % 8] = static_cast<_Float16>((y - static_cast<float>(h)) * 4096.0f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < QC * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(v[i]);
+        }
+    }
+    const float cap_in = a.softcap > 0.0f ? mul / kLog2e / a.softcap : 0.0f;
+    if (a.softcap > 0.0f) mul = 1.0f;
+
+    // a tile's pages: of key lane % KT of it; what the wave stages of it
+    const int32_t* table = reinterpret_cast<const int32_t*>(a.tables + seq * a.t_nb1);
+    auto look_up = [&](uint32_t tile) { return table[min(page_of(a, tile * KT + (lane & (KT - 1))), a.max_pages - 1)]; };
+    u4v rk[NI], rv[NI];
+    float rs = 0.0f;
+    uint64_t have = 0, have_next = 0;                        // keys of the tile that are there
+    const uint32_t sub_row = lane / LANES, sub_c = lane % LANES;
+    const bool sub_in = sub_c * T::PER < a.D;
+    auto fetch = [&](uint32_t tile, int32_t pg) {
+        const uint32_t key = tile * KT + (lane & (KT - 1));
+        const bool in = key < static_cast<uint32_t>(end) && key >= static_cast<uint32_t>(begin);
+        const bool good = static_cast<uint32_t>(pg) < a.n_pages;
+        wrong |= in && !good;
+        have_next = __ballot(in && good);
+        if constexpr (KT == 32) have_next &= 0xffffffffull;
+        const int64_t pl = in && good ? pg : 0, at = in && good ? key - page_of(a, key) * a.page : 0;
+        const uint64_t ko = static_cast<uint64_t>(pl * a.k_nb3 + at * a.k_nb1), vo = static_cast<uint64_t>(pl * a.v_nb3 + at * a.v_nb1);
+        const char* kb = a.k + hk * a.k_nb2 + (sub_in ? sub_c : 0) * 16;
+        const char* vb = a.v + hk * a.v_nb2 + (sub_in ? sub_c : 0) * 16;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int src = wid * (KT / 4) + i * RPI + sub_row;
+            auto of = [&](uint64_t o) {
+                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), src), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), src);
+                return static_cast<uint64_t>(hi) << 32 | lo;
+            };
+            rk[i] = *reinterpret_cast<const u4v*>(kb + of(ko));
+            rv[i] = *reinterpret_cast<const u4v*>(vb + of(vo));
+        }
+        if constexpr (I8) {
+            if (wid < 2 && in && good) {
+                const char* sp = wid == 0 ? a.ks + pl * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0
+                                          : a.vs + pl * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0;
+                rs = *reinterpret_cast<const float*>(sp);
+            } else {
+                rs = 0.0f;
+            }
+        }
+    };
+    // into LDS: keys that are not there and dims past D as zeros
+    bool clean = false, bad = false;
+    auto put = [&](int buf, bool edge) {
+        const bool whole = have_next == (KT == 64 ? ~0ull : 0xffffffffull);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
+            if (!sub_in || (!whole && !(have_next >> row & 1))) rk[i] = rv[i] = u4v{};
+            if constexpr (I8) {
+                u4v k0, k1, v0, v1;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    float fk[4], fv[4];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        fk[b] = static_cast<float>(static_cast<int8_t>(rk[i][w] >> 8 * b));
+                        fv[b] = static_cast<float>(static_cast<int8_t>(rv[i][w] >> 8 * b));
+                    }
+                    u4v& kk = w < 2 ? k0 : k1;
+                    u4v& vv = w < 2 ? v0 : v1;
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        kk[2 * (w & 1) + b] = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(fk[2 * b]), static_cast<_Float16>(fk[2 * b + 1])});
+                        vv[2 * (w & 1) + b] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fv[2 * b + 1]),
+                                                                    __builtin_bit_cast(uint32_t, fv[2 * b]), 0x07060302u);
+                    }
+                }
+                if (2 * sub_c < CH) {
+                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, 2 * sub_c) * 16) = k0;
+                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
+                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, 2 * sub_c) * 16) = v0;
+                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
+                }
+            } else {
+                if (edge) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t y = rv[i][w];
+                        const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
+                        bad |= lo || hi;
+                        if (clean) rv[i][w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
+                    }
+                }
+                if (sub_c < CH) {
+                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, sub_c) * 16) = rk[i];
+                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, sub_c) * 16) = rv[i];
+                }
+            }
+        }
+        if constexpr (I8) {
+            if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
+        }
+    };
+
+    f16v o[DP / 32];
+    float m, mc, l;
+    bool far;                                                // a maximum so large that its rounding would be a factor
+
+    // LDS addresses that a lane reads keys and values at
+    const uint32_t k_row = n * PITCH;
+    const uint32_t l16 = lane & 15, v_key = 4 * half + l16 / 4, v_c = 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
+    const uint32_t v_at = v_key * PITCH + (l16 & 1) * 8;
+
+    auto add_values = [&](int buf, int sub, const f16v& s) { // O^T += V^T P^T over 32 keys
+        const char* lv = lds_v[buf] + sub * 32 * PITCH;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {                        // 16 keys
+            h8v ph, pl;
+            b8v b0, b1, b2;
+            if constexpr (I8) {
+                u4v w0, w1, w2;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t part[3][2];
+#pragma unroll
+                    for (int z = 0; z < 2; z++) {
+                        float y = s[8 * u + 2 * i + z];
+#pragma unroll
+                        for (int k = 0; k < PP; k++) {
+                            part[k][z] = __builtin_bit_cast(uint32_t, y);
+                            y -= __builtin_bit_cast(float, part[k][z] & 0xffff0000u);
+                        }
+                    }
+                    w0[i] = __builtin_amdgcn_perm(part[0][1], part[0][0], 0x07060302u);
+                    w1[i] = __builtin_amdgcn_perm(part[1][1], part[1][0], 0x07060302u);
+                    if constexpr (PP == 3) w2[i] = __builtin_amdgcn_perm(part[2][1], part[2][0], 0x07060302u);
+                }
+                b0 = __builtin_bit_cast(b8v, w0);
+                b1 = __builtin_bit_cast(b8v, w1);
+                if constexpr (PP == 3) b2 = __builtin_bit_cast(b8v, w2);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    ph[i] = static_cast<_Float16>(s[8 * u + i]);
+                    if constexpr (PP == 2) pl[i] = static_cast<_Float16>(s[8 * u + i] - static_cast<float>(ph[i]));
+                }
+                if constexpr (PP == 1) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(h2v{ph[i], ph[i + 1]}, h2v{1, 1}, l, false);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) {
+                // place of chunk 4 d + v_c in the lane's rows: these are alike modulo 4
+                const char* at = lv + v_at + T::v_place(v_key, 4 * d + v_c) * 16 + 16 * u * PITCH;
+                const h4v x0 = read_turned(at), x1 = read_turned(at + 8 * PITCH);
+                const h8v vf = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+                if constexpr (I8) {
+                    const b8v vb = __builtin_bit_cast(b8v, vf);
+                    if constexpr (PP == 3) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b2, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b1, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b0, o[d], 0, 0, 0);
+                } else {
+                    if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[d], 0, 0, 0);
+                }
+            }
+        }
+    };
+
+    auto products = [&](int buf, uint32_t kb, int sub) {     // 32 keys
+        const char* lk = lds_k[buf] + sub * 32 * PITCH;
+        f16v s = {};
+        {
+            f16v low = {};
+#pragma unroll
+            for (int c = 0; c < QC; c++) {
+                const h8v kf = *reinterpret_cast<const h8v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[c], s, 0, 0, 0);
+                if constexpr (Q2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[c], low, 0, 0, 0);
+            }
+            if constexpr (Q2) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[e] = fmaf(low[e], 0x1p-12f, s[e]);
+            }
+        }
+        if constexpr (I8) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][0][32 * sub + 2 * e + 4 * half]);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[e + u] *= sc[u];
+            }
+        }
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = tanh_of(s[e] * cap_in) * (a.softcap * kLog2e);
+        }
+        const uint32_t there = static_cast<uint32_t>(have >> 32 * sub);
+        const bool whole = static_cast<int32_t>(kb) >= all_begin && static_cast<int32_t>(kb) + 32 <= all_end && there == ~0u;
+        uint32_t live = ~0u;                                 // bit e: the row has key e of the lane's
+        if (!whole) {
+            live = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const uint32_t i = 8 * (e / 4) + 4 * half + e % 4;
+                const int32_t key = static_cast<int32_t>(kb + i);
+                if (key < limit && key >= first && (there >> i & 1)) live |= 1u << e;
+                else s[e] = kLowest;
+            }
+        }
+        float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int e = 2; e < 16; e++) mx = fmaxf(mx, s[e]);
+        auto rises = [&] { return mx > m && (m == kLowest || (mx - m) * mul > kRise); };
+        if (__any(rises())) {                                // rare after the first keys: the row's sums are rescaled
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (rises()) {                                   // of this row alone: its neighbours' keys say nothing about it
+                const float mc2 = fmaf(mx, mul, -kUp);
+                const bool big = fabsf(mc2) >= 0x1p22f;
+                const float keep = far || big ? __builtin_amdgcn_exp2f((m - mx) * mul) : __builtin_amdgcn_exp2f(mc - mc2);
+                far |= big;
+                m = mx;
+                mc = mc2;
+                l *= keep;
+#pragma unroll
+                for (int d = 0; d < DP / 32; d++) o[d] *= keep;
+            }
+        }
+        if (__any(far)) {
+            const float off = far ? m : 0.0f, add = far ? kUp : -mc;
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e] - off, mul, add));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -mc));
+        }
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[e] = live >> e & 1 ? s[e] : 0.0f;
+        }
+        if constexpr (I8 || PP == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) l += s[e];
+        }
+        if constexpr (I8) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][1][32 * sub + 2 * e + 4 * half]);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[e + u] = live >> (e + u) & 1 ? s[e + u] * sc[u] : 0.0f;
+            }
+        }
+        add_values(buf, sub, s);
+    };
+
+    // A value that is no number, at a key that some of the rows do not have, would reach these as 0 times it: met at such a tile, the
+    // keys are gone through once more without them, and the rows that have them get them at the end.
+    for (;;) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++) o[d] = f16v{};
+        m = mc = kLowest;
+        l = 0.0f;
+        far = false;
+        if (ta < tb) {
+            auto edge = [&](uint32_t tile) {
+                return static_cast<int32_t>(tile * KT) < every_begin || static_cast<int32_t>(tile * KT + KT) > every_end;
+            };
+            int32_t pg = look_up(ta);
+            fetch(ta, pg);
+            pg = look_up(ta + 1);
+            put(0, edge(ta));
+            have = have_next;
+            for (uint32_t tile = ta; tile < tb; tile++) {
+                const int buf = (tile - ta) & 1;
+                const bool more = tile + 1 < tb;
+                __syncthreads();
+                if (more) {
+                    fetch(tile + 1, pg);
+                    pg = look_up(tile + 2);
+                }
+#pragma unroll 1
+                for (int sub = 0; sub < KT / 32; sub++) {
+                    const uint32_t kb = tile * KT + 32 * sub;
+                    if (static_cast<int32_t>(kb) < w_end && static_cast<int32_t>(kb) + 32 > w_begin) products(buf, kb, sub);
+                }
+                if (more) put(buf ^ 1, edge(tile + 1));
+                have = have_next;
+            }
+        }
+        if constexpr (I8) break;
+        if (clean || !__syncthreads_or(bad)) break;
+        clean = true;
+    }
+    l += __shfl_xor(l, 32);
+    if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
+    const uint64_t part = (static_cast<uint64_t>(t) * a.hq + hq) * pa.n_part + run;
+    char* yr = a.y + t * a.y_nb2 + hq * a.y_nb1;
+    if (pa.part_o && half == 0 && live_row) pa.part_ml[part] = make_float2(mc, l);
+#pragma unroll
+    for (int d = 0; d < DP / 32; d++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t dim = 32 * d + 8 * c + 4 * half;
+            if (dim >= a.D || !live_row) continue;
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = o[d][4 * c + u];
+            if (pa.part_o) {
+                store4u(reinterpret_cast<char*>(pa.part_o + part * a.D + dim), v, float());
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) v[u] = l == 0.0f ? 0.0f : v[u] / l;
+                store4u(yr + dim * Elt<TQ>::size, v, TQ());
+            }
+        }
+    }
+    if constexpr (!I8) {
+        if (!clean) return;
+        __syncthreads();                                     // what is written above is corrected
+#pragma unroll 1
+        for (int i = 0; i < 32; i++) {                       // a row at a time, its dims over the lanes
+            if (wid * 32 + i >= rows) break;
+            const int32_t lim = min(__shfl(limit, i), static_cast<int32_t>(tb * KT)), from = max(__shfl(first, i), static_cast<int32_t>(ta * KT));
+            const uint32_t ti = __shfl(static_cast<int>(t), i), hi = __shfl(static_cast<int>(hq), i);
+            uint32_t found[DP / 64 + 1] = {};                // 1, 2, 4: infinity, -infinity, NaN
+            for (int32_t key = from; key < lim; key++) {
+                const uint32_t pi = page_of(a, key);
+                const int32_t pg = table[pi];
+                if (static_cast<uint32_t>(pg) >= a.n_pages) continue;
+                const char* vr = a.v + pg * a.v_nb3 + hk * a.v_nb2 + (key - pi * a.page) * a.v_nb1;
+#pragma unroll
+                for (int k = 0; k < DP / 64 + 1; k++) {
+                    const uint32_t d = lane + 64 * k;
+                    if (d >= a.D) continue;
+                    const float y = Elt<TC>::load1(vr + d * Elt<TC>::size);
+                    if (!(fabsf(y) < INFINITY)) found[k] |= y > 0.0f ? 1 : y < 0.0f ? 2 : 4;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < DP / 64 + 1; k++) {
+                const uint32_t d = lane + 64 * k;
+                if (d >= a.D || !found[k]) continue;
+                const float y = found[k] == 1 ? INFINITY : found[k] == 2 ? -INFINITY : NAN;
+                if (pa.part_o) pa.part_o[((static_cast<uint64_t>(ti) * a.hq + hi) * pa.n_part + run) * a.D + d] = y;
+                else Elt<TQ>::store1(a.y + ti * a.y_nb2 + hi * a.y_nb1 + d * Elt<TQ>::size, y);
+            }
+        }
+    }
+}
+
+// Adds up a row's parts: a wave a row of y, its dims over the lanes.
+template <typename TQ>
+__global__ __launch_bounds__(256) void k_prompt_join(PromptArgs pa) {
+    const AttnArgs& a = pa.a;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const uint32_t t = static_cast<uint32_t>(row / a.hq), h = static_cast<uint32_t>(row - static_cast<uint64_t>(t) * a.hq);
+    if (t >= a.n_rows) return;
+    if (!pa.shared && (static_cast<int32_t>(t) < a.start[0] || static_cast<int32_t>(t) >= a.start[pa.n_start])) return;
+    const float2* ml = pa.part_ml + row * pa.n_part;
+    float m = kLowest;
+    for (uint32_t i = 0; i < pa.n_part; i++) m = fmaxf(m, ml[i].x);
+    float l = 0.0f, o[4] = {};
+    for (uint32_t i = 0; i < pa.n_part; i++) {
+        const float2 x = ml[i];
+        if (x.y == 0.0f) continue;
+        const float f = __builtin_amdgcn_exp2f(x.x - m);
+        l = fmaf(x.y, f, l);
+        const float* p = pa.part_o + (row * pa.n_part + i) * a.D;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t d = lane + 64 * k;
+            if (d < a.D) o[k] = fmaf(p[d], f, o[k]);
+        }
+    }
+    char* yr = a.y + t * a.y_nb2 + h * a.y_nb1;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t d = lane + 64 * k;
+        if (d < a.D) Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : o[k] / l);
+    }
+}
+
+struct PromptPlan {
+    bool tiles;
+    int dp;
+    uint32_t row_tiles, n_split;
+    size_t o_bytes, bytes;
+};
+
+PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, int64_t n_start, const DeviceState* st) {
+    PromptPlan p{};
+    const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0, cap = tables->ne[0] * k->ne[1];
+    p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+    const int64_t most = q->ne[2] * g / kRows + n_start;
+    p.tiles = k->type != CBX_TYPE_F32 && D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0;
+    if (!p.tiles) return p;
+    p.row_tiles = static_cast<uint32_t>(most);
+    const int64_t groups = std::max<int64_t>(1, most * hkv);
+    p.n_split = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(2 * st->n_cu / groups, cap / 256)));
+    p.tiles = most * hkv * p.n_split < (int64_t{1} << 24);
+    if (p.n_split > 1) {
+        const int64_t parts = q->ne[1] * q->ne[2] * p.n_split;
+        p.o_bytes = static_cast<size_t>(parts) * D * 4;
+        p.bytes = p.o_bytes + static_cast<size_t>(parts) * 8;
+    }
+    return p;
+}
+
+template <typename TQ, typename TC, int PP> void launch_dp(int dp, dim3 grid, hipStream_t s, const PromptArgs& a) {
+    if (dp == 64) hipLaunchKernelGGL((k_prompt<TQ, TC, 64, PP>), grid, dim3(256), 0, s, a);
+    else if (dp == 96) hipLaunchKernelGGL((k_prompt<TQ, TC, 96, PP>), grid, dim3(256), 0, s, a);
+    else if (dp == 128) hipLaunchKernelGGL((k_prompt<TQ, TC, 128, PP>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_prompt<TQ, TC, 256, PP>), grid, dim3(256), 0, s, a);
+}
+
+void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs& a, hipStream_t s) {
+    const dim3 grid(p.row_tiles * p.n_split * a.a.hkv);
+    const bool t16 = c.q->type == CBX_TYPE_F16, i8 = c.k->type == CBX_TYPE_I8;
+    if (t16 && i8) launch_dp<uint16_t, int8_t, 2>(p.dp, grid, s, a);
+    else if (i8) launch_dp<float, int8_t, 3>(p.dp, grid, s, a);
+    else if (!t16) launch_dp<float, uint16_t, 2>(p.dp, grid, s, a);
+    else if (c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p.dp, grid, s, a);
+    else launch_dp<uint16_t, uint16_t, 1>(p.dp, grid, s, a);
+}
+
+}  // namespace
+
+size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
+    return prompt_plan(q, k, tables, tables->ne[1], st).bytes;
+}
 
 int launch_paged_prompt(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
-    return launch_attention_rows(attn_args(c, st), c, "cbx_paged_prompt_attention", s);
+    const char* what = "cbx_paged_prompt_attention";
+    const PromptPlan p = prompt_plan(c.q, c.k, c.tables, c.tables->ne[1], st);
+    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_attention_rows(attn_args(c, st), c, what, s);
+    PromptArgs a{};
+    a.a = attn_args(c, st);
+    a.n_start = a.a.n_seq;
+    a.n_split = a.n_part = p.n_split;
+    a.tiles = p.row_tiles;
+    page_division(a.a.g, &a.g_mul, &a.g_shift);
+    if (p.n_split > 1) {
+        a.part_o = static_cast<float*>(c.ws);
+        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
+    }
+    launch_tiles(c, p, a, s);
+    if (p.n_split > 1) {
+        const dim3 grid(static_cast<unsigned>(cdiv(c.q->ne[1] * c.q->ne[2], 4)));
+        if (c.q->type == CBX_TYPE_F16) hipLaunchKernelGGL((k_prompt_join<uint16_t>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_prompt_join<float>), grid, dim3(256), 0, s, a);
+    }
+    return check_launch(what);
 }
 
 size_t paged_shared_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor*,
