@@ -28,6 +28,7 @@ struct AttnArgs {
     // k_attn_tiles and k_attn_join
     uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
     uint32_t gc, ngr, H;             // heads a run holds (<= 16), runs of heads a group, hkv * ngr
+    bool s_quads;                    // scales can be read four at a time
     uint32_t W;                      // runs; 0: a run a request and key head, none of them split
     float* part_o;                   // [W][2][gc][D]
     float2* part_ml;                 // [W][2][gc]

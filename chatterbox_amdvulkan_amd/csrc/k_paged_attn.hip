@@ -146,6 +146,7 @@ typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f4v __attribute__((ext_vector_type(4)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef const int32_t __attribute__((address_space(4))) const_i32;
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
@@ -183,6 +184,9 @@ struct WaveRows {
     __device__ __forceinline__ u2v load8(uint32_t o) const {
         return __builtin_amdgcn_raw_buffer_load_b64(base, static_cast<int>(off + o), static_cast<int>(step), 0);
     }
+    __device__ __forceinline__ uint32_t load4(uint32_t o) const {
+        return __builtin_amdgcn_raw_buffer_load_b32(base, static_cast<int>(off + o), static_cast<int>(step), 0);
+    }
 };
 struct LaneRow {
     const char* p;
@@ -192,6 +196,7 @@ struct LaneRow {
         return u3v{t.x, t.y, *reinterpret_cast<const uint32_t*>(p + o + 8)};
     }
     __device__ __forceinline__ u2v load8(uint32_t o) const { return *reinterpret_cast<const u2w*>(p + o); }
+    __device__ __forceinline__ uint32_t load4(uint32_t o) const { return *reinterpret_cast<const uint32_t*>(p + o); }
 };
 
 // A request's keys: [first, len), and the tiles of KT keys they lie in; a
@@ -285,6 +290,34 @@ template <int N, typename Row> __device__ __forceinline__ void load_dwords(const
 // end stand for its last dims again, and make the same sums of them.
 template <int PER> __device__ __forceinline__ uint32_t value_dim(uint32_t m, uint32_t D) { return min(m * PER, D - PER); }
 
+// A query's elements as f16: an F32 one's in two parts, see Core<uint16_t>.
+template <int CD>
+__device__ __forceinline__ void split_query(const float (&x)[CD * 8], bool f32, h8v (&qh)[CD], h8v (&ql)[CD], float* qmul) {
+    *qmul = 1.0f;
+    float m = 0.0f;
+    if (f32) {
+#pragma unroll
+        for (int i = 0; i < CD * 8; i++) m = fmaxf(m, fabsf(x[i]));
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        // 2^e <= m < 2^(e + 1) goes to [2^14, 2^15)
+        int e = m > 0.0f && m < INFINITY ? static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23) - 127 : 14;
+        e = e < -100 ? -100 : e;
+        *qmul = ldexpf(1.0f, e - 14);
+        const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+        for (int i = 0; i < CD * 8; i++) {
+            const float t = x[i] * up;
+            const _Float16 h = static_cast<_Float16>(t);
+            qh[i / 8][i % 8] = h;
+            ql[i / 8][i % 8] = static_cast<_Float16>((t - static_cast<float>(h)) * 4096.0f);   // below 2^15
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < CD * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(x[i]);
+    }
+}
+
 // A matrix core's view of NK keys and 16 heads.  S^T = K Q^T: the A operand's
 // row is the key (lane % 16), the B operand's column the head (lane % 16),
 // both hold for the lane group lane / 16 the same dims; the result's lane has
@@ -304,6 +337,7 @@ template <typename TC, int DP> struct Core;
 // below 2^-28 of the largest to 2^-39 of it.  (Lower halves of these summed
 // apart would take as many registers again as the sums over the values.)
 template <int DP> struct Core<uint16_t, DP> {
+    static constexpr bool SCALED = false;
     static constexpr int NK = 32, NH = 2, NE = 8;   // keys a step, halves of 16, keys whose values a lane holds
     static constexpr int CD = DP / 32, PER = DP / 16;
     h8v qh[CD], ql[CD], kf[NH][CD];
@@ -314,29 +348,7 @@ template <int DP> struct Core<uint16_t, DP> {
 
     __device__ __forceinline__ void load_q(const float (&x)[CD * 8], bool f32) {
         two = f32;
-        qmul = 1.0f;
-        float m = 0.0f;
-        if (f32) {
-#pragma unroll
-            for (int i = 0; i < CD * 8; i++) m = fmaxf(m, fabsf(x[i]));
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            // 2^e <= m < 2^(e + 1) goes to [2^14, 2^15)
-            int e = m > 0.0f && m < INFINITY ? static_cast<int>(__builtin_bit_cast(uint32_t, m) >> 23) - 127 : 14;
-            e = e < -100 ? -100 : e;
-            qmul = ldexpf(1.0f, e - 14);
-            const float up = ldexpf(1.0f, 14 - e);
-#pragma unroll
-            for (int i = 0; i < CD * 8; i++) {
-                const float t = x[i] * up;
-                const _Float16 h = static_cast<_Float16>(t);
-                qh[i / 8][i % 8] = h;
-                ql[i / 8][i % 8] = static_cast<_Float16>((t - static_cast<float>(h)) * 4096.0f);   // below 2^15
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < CD * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(x[i]);
-        }
+        split_query<CD>(x, f32, qh, ql, &qmul);
     }
     // dims the lane holds of its query and keys: 8 at 32 c + 8 grp
     static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 32 * c + 8 * grp; }
@@ -412,8 +424,134 @@ template <int DP> struct Core<uint16_t, DP> {
     }
 };
 
+// I8 pages: the elements as whole numbers, exact in f16 and bf16.  Scores from
+// f16 products as above, times the keys' scales in f32.  A probability times its
+// value's scale may lie anywhere in f32's range, so it is split into bf16 parts
+// for products of bf16: three under an F32 query (all 24 bits), two under an F16
+// one (held to 2^-16).  A lane reads 16 dims of a key at once: MFMA c takes dims
+// 64 (c / 2) + 16 (lane / 16) + 8 (c % 2) + [0, 8).
+template <int DP> struct Core<int8_t, DP> {
+    static constexpr bool SCALED = true;
+    static constexpr int NK = 32, NH = 2, NE = 8;
+    static constexpr int CD = DP / 32, PER = DP / 16;
+    h8v qh[CD], ql[CD];
+    u4v kf[NH][CD / 2];
+    uint32_t vr[NE][PER / 4];
+    float ks[NE], vs[NE];
+    f4v acc[DP / 16];
+    float qmul;
+    bool two;
+    __device__ __forceinline__ void load_q(const float (&x)[CD * 8], bool f32) {
+        two = f32;
+        split_query<CD>(x, f32, qh, ql, &qmul);
+    }
+    static __device__ __forceinline__ uint32_t dim_of(int c, uint32_t grp) { return 64 * (c / 2) + 16 * grp + 8 * (c & 1); }
+    static constexpr int QC = CD, QN = 8;
+    uint32_t ko[CD / 2], vo;
+    __device__ __forceinline__ void offsets(uint32_t n, uint32_t grp, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CD / 2; c++) ko[c] = 64 * c + 16 * grp < D ? 64 * c + 16 * grp : 0;
+        vo = value_dim<PER>(n, D);
+    }
+    template <typename Row> __device__ __forceinline__ void load_k(int h, const Row& r) {
+#pragma unroll
+        for (int c = 0; c < CD / 2; c++) kf[h][c] = r.load16(ko[c]);
+    }
+    __device__ __forceinline__ void trim_k(uint32_t grp, uint32_t D) {
+#pragma unroll
+        for (int c = 0; c < CD / 2; c++) {
+            if (64 * c + 16 * grp >= D) {
+#pragma unroll
+                for (int h = 0; h < NH; h++) kf[h][c] = u4v{};
+            }
+        }
+    }
+    template <typename Row> __device__ __forceinline__ void load_v(int e, const Row& r) {
+        if constexpr (PER == 4) vr[e][0] = r.load4(vo);
+        else if constexpr (PER == 8) {
+            const u2v t = r.load8(vo);
+            vr[e][0] = t.x;
+            vr[e][1] = t.y;
+        } else {
+            const u4v t = r.load16(vo);
+#pragma unroll
+            for (int i = 0; i < 4; i++) vr[e][i] = t[i];
+        }
+    }
+    __device__ __forceinline__ void drop_v(int e) {
+        vs[e] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < PER / 4; c++) vr[e][c] = 0;
+    }
+    static __device__ __forceinline__ uint32_t key_of(int e, uint32_t grp) { return 16 * (e >> 2) + 4 * grp + (e & 3); }
+    static constexpr int half_of(int e) { return e >> 2; }
+
+    // 8 whole numbers to f16: 1024 + 128 + x is a half with x + 128 in its low byte
+    static __device__ __forceinline__ h8v wide(uint32_t lo, uint32_t hi) {
+        h8v r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x = (i < 2 ? lo : hi) ^ 0x80808080u;
+            const h2v t = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, x, i & 1 ? 0x04030402u : 0x04010400u)) -
+                          h2v{static_cast<_Float16>(1152), static_cast<_Float16>(1152)};
+            r[2 * i] = t[0];
+            r[2 * i + 1] = t[1];
+        }
+        return r;
+    }
+    __device__ __forceinline__ void scores(float (&s)[NE]) {
+#pragma unroll
+        for (int h = 0; h < NH; h++) {
+            f4v t = {}, low = {};
+#pragma unroll
+            for (int c = 0; c < CD; c++) {
+                const u4v& w = kf[h][c / 2];
+                const h8v k = c & 1 ? wide(w[2], w[3]) : wide(w[0], w[1]);
+                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[c], t, 0, 0, 0);
+                if (two) low = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[c], low, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * h + r] = (two ? fmaf(low[r], 0x1p-12f, t[r]) : t[r]) * ks[4 * h + r];
+        }
+    }
+    static constexpr float kUp = 1.0f;
+    __device__ __forceinline__ void add_values(const float (&p)[NE]) {
+        u4v part[3];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t b[3][2];
+#pragma unroll
+            for (int z = 0; z < 2; z++) {
+                float y = p[2 * i + z] * vs[2 * i + z];
+#pragma unroll
+                for (int k = 0; k < 3; k++) {
+                    b[k][z] = __builtin_bit_cast(uint32_t, y);
+                    y -= __builtin_bit_cast(float, b[k][z] & 0xffff0000u);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 3; k++) part[k][i] = __builtin_amdgcn_perm(b[k][1], b[k][0], 0x07060302u);
+        }
+#pragma unroll
+        for (int d = 0; d < PER; d++) {
+            u4v w;   // dim d of the lane's eight keys
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x0 = static_cast<float>(static_cast<int8_t>(vr[2 * i][d / 4] >> 8 * (d & 3)));
+                const float x1 = static_cast<float>(static_cast<int8_t>(vr[2 * i + 1][d / 4] >> 8 * (d & 3)));
+                w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x1), __builtin_bit_cast(uint32_t, x0), 0x07060302u);
+            }
+            const b8v v = __builtin_bit_cast(b8v, w);
+            if (two) acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(b8v, part[2]), acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(b8v, part[1]), acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(b8v, part[0]), acc[d], 0, 0, 0);
+        }
+    }
+};
+
 // f32 pages: 16x16x4 products of f32.
 template <int DP> struct Core<float, DP> {
+    static constexpr bool SCALED = false;
     static constexpr int NK = 16, NH = 1, NE = 4;
     static constexpr int CD = DP / 16, PER = DP / 16;
     f4v qf[CD], kf[NH][CD];
@@ -600,8 +738,31 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 if (!in || !good) r.pg[0] = -1;
             }
         };
+        // the scales of the lane's keys: those of four neighbours at once where they lie together in 16 bytes of one page
+        auto fetch_s = [&](const Pages& r, uint32_t kb, const char* base, int64_t nb0, int64_t nb1, int64_t nb2, float (&to)[NE]) {
+            const char* sb = base + hk * nb1;
+            if (UNI && a.s_quads) {
+#pragma unroll
+                for (int i = 0; i < NH; i++) {
+                    const uint32_t key = kb + 16 * i, in = key - page_of(a, key) * a.page;
+                    const f4v t = *reinterpret_cast<const f4v*>(sb + (r.pg[i] * nb2 + in * 4) + 16 * grp);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) to[4 * i + e] = t[e];
+                }
+                return;
+            }
+#pragma unroll
+            for (int e = 0; e < NE; e++) {
+                const uint32_t key = kb + C::key_of(e, grp);
+                int32_t g;
+                if constexpr (UNI) g = r.pg[C::half_of(e)];
+                else g = __shfl(r.pg[0], C::key_of(e, grp));
+                to[e] = *reinterpret_cast<const float*>(sb + (g < 0 ? 0 : g * nb2 + (key - page_of(a, key) * a.page) * nb0));
+            }
+        };
         // UNI: the half's first row is the wave's, the key's place in it the lane's
         auto fetch_k = [&](const Pages& r, uint32_t kb) {
+            if constexpr (C::SCALED) fetch_s(r, kb, a.ks, a.ks_nb0, a.ks_nb1, a.ks_nb2, core.ks);
 #pragma unroll
             for (int i = 0; i < NH; i++) {
                 if constexpr (UNI) {
@@ -615,6 +776,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
             }
         };
         auto fetch_v = [&](const Pages& r, uint32_t kb) {
+            if constexpr (C::SCALED) fetch_s(r, kb, a.vs, a.vs_nb0, a.vs_nb1, a.vs_nb2, core.vs);
             if constexpr (UNI) {
 #pragma unroll
                 for (int i = 0; i < NH; i++) {
@@ -840,14 +1002,14 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     AttnPlan p{};
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0;
     const int64_t cap = tables->ne[0] * k->ne[1];
-    p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
-    p.kt = (k->type == CBX_TYPE_F16 ? 32 : 16) * (kAttnThreads / 64);
+    p.dp = D <= 64 ? 64 : D <= 96 && k->type != CBX_TYPE_I8 ? 96 : D <= 128 ? 128 : 256;
+    p.kt = (k->type == CBX_TYPE_F32 ? 16 : 32) * (kAttnThreads / 64);
     p.ngr = static_cast<uint32_t>(cdiv(g, 16));
     p.gc = static_cast<uint32_t>(cdiv(g, p.ngr));
     p.H = static_cast<uint32_t>(hkv) * p.ngr;
     const int64_t cap_tiles = std::max<int64_t>(1, cdiv(cap, p.kt));
     const int64_t most = q->ne[2] * p.H * cap_tiles;
-    p.tiles = k->type != CBX_TYPE_I8 && D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
+    p.tiles = D % (k->type == CBX_TYPE_I8 ? 16 : 8) == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most < (int64_t{1} << 31);
     if (!p.tiles) return p;
     p.W = static_cast<uint32_t>(std::min<int64_t>(static_cast<int64_t>(per_cu(p.dp, uniform_pages(k))) * st->n_cu, most));
     // A run a key head, without a join, while the longest a table can hold ends
@@ -883,7 +1045,9 @@ void launch_tiles(const AttnPlan& p, bool uni, AttnArgs& a, hipStream_t s) {
     const dim3 grid(p.join ? p.W : a.n_seq * a.H);
     const size_t lds = static_cast<size_t>(kAttnThreads / 64) * p.gc * (p.dp + 4) * sizeof(float);
     if (p.dp == 64) tiles_uni<TQ, TC, 64>(uni, grid, lds, s, a);
-    else if (p.dp == 96) tiles_uni<TQ, TC, 96>(uni, grid, lds, s, a);
+    else if (p.dp == 96) {
+        if constexpr (sizeof(TC) > 1) tiles_uni<TQ, TC, 96>(uni, grid, lds, s, a);
+    }
     else if (p.dp == 128) tiles_uni<TQ, TC, 128>(uni, grid, lds, s, a);
     else tiles_uni<TQ, TC, 256>(uni, grid, lds, s, a);
     if (!p.join) return;
@@ -903,6 +1067,14 @@ bool vector_rows(const cbx_tensor* t) {
     if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
     for (int i = 1; i < 4; i++) if (t->ne[i] > 1 && t->nb[i] % 16) return false;
     return t->nb[1] < (size_t{1} << 26);
+}
+
+// Scales that can be read four at a time.
+static bool quad_scales(const cbx_tensor* t) {
+    if (t->ne[0] > 1 && t->nb[0] != 4) return false;
+    if (reinterpret_cast<uintptr_t>(t->data) % 16) return false;
+    for (int i = 1; i < 3; i++) if (t->ne[i] > 1 && t->nb[i] % 16) return false;
+    return true;
 }
 
 AttnArgs attn_args(const PagedAttnCall& c, const DeviceState* st) {
@@ -970,7 +1142,11 @@ int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t 
         a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
         a.split = reinterpret_cast<uint4*>(static_cast<char*>(c.ws) + p.o_bytes + p.ml_bytes);
         const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
-        if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, uniform_pages(c.k), a, s);
+        if (c.k->type == CBX_TYPE_I8) {
+            a.s_quads = quad_scales(c.k_scale) && quad_scales(c.v_scale);
+            if (t16) launch_tiles<uint16_t, int8_t>(p, uniform_pages(c.k), a, s);
+            else launch_tiles<float, int8_t>(p, uniform_pages(c.k), a, s);
+        } else if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, uniform_pages(c.k), a, s);
         else if (t16) launch_tiles<uint16_t, float>(p, uniform_pages(c.k), a, s);
         else if (c16) launch_tiles<float, uint16_t>(p, uniform_pages(c.k), a, s);
         else launch_tiles<float, float>(p, uniform_pages(c.k), a, s);

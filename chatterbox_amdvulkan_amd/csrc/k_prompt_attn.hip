@@ -92,7 +92,7 @@ template <typename TC, int DP> struct Tile;
 // F16 pages, and I8 ones as whole numbers: keys in f16; values in f16, of I8 pages
 // in bf16, whose range holds a probability times any scale.
 template <typename TC, int DP> struct Tile {
-    static constexpr bool I8 = sizeof(TC) == 1;
+    static constexpr bool F32 = false, I8 = sizeof(TC) == 1;
     static constexpr int KT = DP <= 128 ? 64 : 32, PITCH = DP * 2, CH = DP / 8;      // bytes a row, chunks
     static constexpr int BYTES = KT * PITCH;
     static constexpr int QC = DP / 16;
@@ -110,13 +110,33 @@ template <typename TC, int DP> struct Tile {
     }
 };
 
+// F32 pages: products of f32, 32 x 32 x 2.
+template <int DP> struct Tile<float, DP> {
+    static constexpr bool F32 = true, I8 = false;
+    static constexpr int KT = 32, PITCH = DP * 4, CH = DP / 4;
+    static constexpr int BYTES = KT * PITCH;
+    static constexpr int QC = DP / 16;
+    static constexpr int PER = 4, LANES = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
+    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) {
+        if constexpr (DP == 96) return c ^ (r >> 1 & 7);
+        else return c ^ (r & 15);
+    }
+    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) {
+        if constexpr (DP == 96) return c;
+        else return c ^ (r >> 2 & 1) << 3;
+    }
+};
+
+// Workgroups of k_prompt that a CU holds, which their registers are limited to.
+constexpr int waves_per_simd(int dp, bool f32) { return dp <= 64 && !f32 ? 3 : dp <= 128 ? 2 : 1; }
+
 template <typename TQ, typename TC, int DP, int PP>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_prompt(PromptArgs pa) {
+__global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_prompt(PromptArgs pa) {
     using T = Tile<TC, DP>;
-    constexpr bool I8 = T::I8, Q2 = sizeof(TQ) == 4;
+    constexpr bool F32 = T::F32, I8 = T::I8, Q2 = sizeof(TQ) == 4 && !F32;
     constexpr int KT = T::KT, PITCH = T::PITCH, CH = T::CH, QC = T::QC, LANES = T::LANES;
     constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave reads at a time, times
-    constexpr float kUp = PP == 1 ? 9.0f : 14.0f, kRise = PP == 1 ? 6.0f : 1.0f;
+    constexpr float kUp = F32 ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = F32 ? 8.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
     __shared__ __attribute__((aligned(16))) char lds_k[2][T::BYTES];
     __shared__ __attribute__((aligned(16))) char lds_v[2][T::BYTES];
@@ -201,16 +221,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_promp
     const uint32_t ta = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * run / pa.n_split));
     const uint32_t tb = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * (run + 1) / pa.n_split));
 
-    // the lane's query: dims 16 c + 8 half + [0, 8).  An F32 one is scaled by a power of two to below 2^15 and split into two f16, the
+    // the lane's query: dims 16 c + 8 half + [0, 8), for F32 pages 8 c + 4 half + [0, 4).  Else an F32 one is scaled by a power of two to below 2^15 and split into two f16, the
     // lower times 2^12 and summed apart
-    h8v qh[QC], ql[Q2 ? QC : 1];
+    h8v qh[F32 ? 1 : QC], ql[Q2 ? QC : 1];
+    float qf[F32 ? QC * 8 : 1];
     float mul = fabsf(a.scale) * kLog2e;
     {
         float v[QC * 8];
         const char* qr = a.q + t * a.q_nb2 + hq * a.q_nb1;
 #pragma unroll
         for (int i = 0; i < QC * 8; i += 4) {
-            const uint32_t d = 16 * (i / 8) + 8 * half + i % 8;
+            const uint32_t d = F32 ? 2 * i + 4 * half : 16 * (i / 8) + 8 * half + i % 8;
             const bool in = live_row && d < a.D;
             float tmp[4];
             load4u(qr + (in ? d : 0) * Elt<TQ>::size, tmp, TQ());
@@ -233,6 +254,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_promp
                 qh[i / 8][i % 8] = h;
                 ql[i / 8][i % 8] = static_cast<_Float16>((y - static_cast<float>(h)) * 4096.0f);
             }
+        } else if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < QC * 8; i++) qf[i] = v[i];
         } else {
 #pragma unroll
             for (int i = 0; i < QC * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(v[i]);
@@ -318,6 +342,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_promp
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         const uint32_t y = rv[i][w];
+                        if constexpr (F32) {
+                            const bool no = (y & 0x7f800000u) == 0x7f800000u;
+                            bad |= no;
+                            if (clean) rv[i][w] = no ? 0u : y;
+                            continue;
+                        }
                         const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
                         bad |= lo || hi;
                         if (clean) rv[i][w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
@@ -345,8 +375,21 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_promp
 
     auto add_values = [&](int buf, int sub, const f16v& s) { // O^T += V^T P^T over 32 keys
         const char* lv = lds_v[buf] + sub * 32 * PITCH;
+        if constexpr (F32) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {                        // 16 keys
+            for (int e = 0; e < 16; e++) {
+                const uint32_t key = 8 * (e / 4) + 4 * half + e % 4;
+#pragma unroll
+                for (int d = 0; d < DP / 32; d++) {
+                    const float v = *reinterpret_cast<const float*>(lv + key * PITCH + T::v_place(4 * half, 8 * d + n / 4) * 16 + n % 4 * 4);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[d], 0, 0, 0);
+                }
+                if (e % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // else every value of the 16 keys is held at once
+            }
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < 2 && !F32; u++) {                // 16 keys
             h8v ph, pl;
             b8v b0, b1, b2;
             if constexpr (I8) {
@@ -403,7 +446,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void k_promp
     auto products = [&](int buf, uint32_t kb, int sub) {     // 32 keys
         const char* lk = lds_k[buf] + sub * 32 * PITCH;
         f16v s = {};
-        {
+        if constexpr (F32) {
+#pragma unroll
+            for (int c = 0; c < DP / 8; c++) {
+                const f4v kf = *reinterpret_cast<const f4v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u], qf[4 * c + u], s, 0, 0, 0);
+            }
+        } else {
             f16v low = {};
 #pragma unroll
             for (int c = 0; c < QC; c++) {
@@ -626,7 +676,7 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0, cap = tables->ne[0] * k->ne[1];
     p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
     const int64_t most = q->ne[2] * g / kRows + n_start;
-    p.tiles = k->type != CBX_TYPE_F32 && D % 8 == 0 && D <= 256 && cap > 0 && k->ne[3] > 0;
+    p.tiles = D % (k->type == CBX_TYPE_I8 ? 16 : 8) == 0 && D <= 256 && cap > 0 && k->ne[3] > 0;
     if (!p.tiles) return p;
     p.row_tiles = static_cast<uint32_t>(most);
     const int64_t groups = std::max<int64_t>(1, most * hkv);
@@ -652,6 +702,7 @@ void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs&
     const bool t16 = c.q->type == CBX_TYPE_F16, i8 = c.k->type == CBX_TYPE_I8;
     if (t16 && i8) launch_dp<uint16_t, int8_t, 2>(p.dp, grid, s, a);
     else if (i8) launch_dp<float, int8_t, 3>(p.dp, grid, s, a);
+    else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p.dp, grid, s, a) : launch_dp<float, float, 2>(p.dp, grid, s, a);
     else if (!t16) launch_dp<float, uint16_t, 2>(p.dp, grid, s, a);
     else if (c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p.dp, grid, s, a);
     else launch_dp<uint16_t, uint16_t, 1>(p.dp, grid, s, a);
