@@ -34,6 +34,14 @@ struct AttnArgs {
     float2* part_ml;                 // [W][2][gc]
     uint4* split;                    // [W]: request, first query head, heads and parts of the key head that begins
                                      // in the run and ends in a later one; no parts: none does
+    // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt): own_first, null: all
+    // keys, says where a request's begin, and (o, m, l) go to the last of its own_parts parts instead of y
+    const int32_t* own_first;
+    const int32_t* groups;           // own_first holds for the requests [groups[0], groups[n_groups])
+    uint32_t n_groups, own_parts;
+    float own_up;                    // log2 of what the probabilities in o and l are multiplied by
+    float* own_o;
+    float2* own_ml;
 };
 
 __device__ __forceinline__ uint32_t page_of(const AttnArgs& a, uint32_t key) {
@@ -45,6 +53,9 @@ AttnArgs attn_args(const PagedAttnCall& c, const DeviceState* st);
 // A workgroup a row of q and query head, for what no other kernel takes: any
 // sizes, strides and types.
 int launch_attention_rows(const AttnArgs& a, const PagedAttnCall& c, const char* what, hipStream_t s);
+// paged_attention's kernels by tiles over a's tensors: launches them if they take the call; the workspace they need.
+bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, DeviceState* st, hipStream_t s);
+size_t attention_tiles_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
 // Whether rows can be read 16 bytes at a time.
 bool vector_rows(const cbx_tensor* t);
 

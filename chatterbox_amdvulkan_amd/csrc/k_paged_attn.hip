@@ -213,6 +213,9 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     r.wrong = n < 0 || static_cast<uint32_t>(n) > cap;
     r.len = n < 0 ? 0 : min(static_cast<uint32_t>(n), cap);
     r.first = a.window > 0 && r.len > static_cast<uint32_t>(a.window) ? r.len - a.window : 0;
+    if (a.own_first && static_cast<int32_t>(s) >= a.groups[0] && static_cast<int32_t>(s) < a.groups[a.n_groups]) {
+        r.first = max(r.first, min(static_cast<uint32_t>(max(a.own_first[s], 0)), r.len));
+    }
     r.tile0 = r.first / KT;
     r.tiles = max(1u, (r.len + KT - 1) / KT - r.tile0);
     return r;
@@ -897,7 +900,11 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 ll = fmaf(lds_l[w][hh], f, ll);
                 oo = fmaf(lds_o[(w * a.gc + hh) * ld + d], f, oo);
             }
-            if (entire) {
+            if (entire && a.own_first) {
+                const uint64_t own = (static_cast<uint64_t>(s) * a.hq + hq0 + hh) * a.own_parts + a.own_parts - 1;
+                a.own_o[own * a.D + d] = oo;
+                if (d == 0) a.own_ml[own] = make_float2(mm - a.own_up, ll);
+            } else if (entire) {
                 Elt<TQ>::store1(a.y + s * a.y_nb2 + (hq0 + hh) * a.y_nb1 + d * Elt<TQ>::size, ll == 0.0f ? 0.0f : oo / ll);
             } else {
                 a.part_o[(slot + hh) * a.D + d] = oo;
@@ -978,10 +985,13 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     for (int j = 0; j < N; j++) lds_o[wid][lane + 64 * j] = o[j];
     __syncthreads();
     l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
+    const uint64_t own = (static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh) * a.own_parts + a.own_parts - 1;
+    if (a.own_first && tid == 0) a.own_ml[own] = make_float2(m - a.own_up, l);
     char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
     for (uint32_t d = tid; d < a.D; d += kAttnThreads) {
         const float t = ((lds_o[0][d] + lds_o[1][d]) + lds_o[2][d]) + lds_o[3][d];
-        Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
+        if (a.own_first) a.own_o[own * a.D + d] = t;
+        else Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
     }
 }
 
@@ -1130,28 +1140,36 @@ int launch_attention_rows(const AttnArgs& a, const PagedAttnCall& c, const char*
     return check_launch(what);
 }
 
-int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
-    AttnArgs a = attn_args(c, st);
+size_t attention_tiles_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
+    return attn_plan(q, k, tables, st).bytes;
+}
+
+bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, DeviceState* st, hipStream_t s) {
     const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
-    if (p.tiles && vector_rows(c.k) && vector_rows(c.v)) {
-        a.gc = p.gc;
-        a.ngr = p.ngr;
-        a.H = p.H;
-        a.W = p.W;
-        a.part_o = static_cast<float*>(c.ws);
-        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
-        a.split = reinterpret_cast<uint4*>(static_cast<char*>(c.ws) + p.o_bytes + p.ml_bytes);
-        const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16;
-        if (c.k->type == CBX_TYPE_I8) {
-            a.s_quads = quad_scales(c.k_scale) && quad_scales(c.v_scale);
-            if (t16) launch_tiles<uint16_t, int8_t>(p, uniform_pages(c.k), a, s);
-            else launch_tiles<float, int8_t>(p, uniform_pages(c.k), a, s);
-        } else if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, uniform_pages(c.k), a, s);
-        else if (t16) launch_tiles<uint16_t, float>(p, uniform_pages(c.k), a, s);
-        else if (c16) launch_tiles<float, uint16_t>(p, uniform_pages(c.k), a, s);
-        else launch_tiles<float, float>(p, uniform_pages(c.k), a, s);
-        return check_launch("cbx_paged_attention");
-    }
+    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return false;
+    a.gc = p.gc;
+    a.ngr = p.ngr;
+    a.H = p.H;
+    a.W = p.W;
+    a.part_o = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.o_bytes);
+    a.split = reinterpret_cast<uint4*>(static_cast<char*>(ws) + p.o_bytes + p.ml_bytes);
+    a.own_up = c.k->type == CBX_TYPE_F16 ? 14.0f : 0.0f;         // Core's kUp
+    const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16, uni = uniform_pages(c.k);
+    if (c.k->type == CBX_TYPE_I8) {
+        a.s_quads = quad_scales(c.k_scale) && quad_scales(c.v_scale);
+        if (t16) launch_tiles<uint16_t, int8_t>(p, uni, a, s);
+        else launch_tiles<float, int8_t>(p, uni, a, s);
+    } else if (t16 && c16) launch_tiles<uint16_t, uint16_t>(p, uni, a, s);
+    else if (t16) launch_tiles<uint16_t, float>(p, uni, a, s);
+    else if (c16) launch_tiles<float, uint16_t>(p, uni, a, s);
+    else launch_tiles<float, float>(p, uni, a, s);
+    return true;
+}
+
+int launch_paged_attention(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
+    const AttnArgs a = attn_args(c, st);
+    if (launch_attention_tiles(a, c, c.ws, st, s)) return check_launch("cbx_paged_attention");
     return launch_attention_rows(a, c, "cbx_paged_attention", s);
 }
 

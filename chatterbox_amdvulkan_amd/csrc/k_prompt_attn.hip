@@ -639,12 +639,15 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptArgs pa) {
     const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const uint32_t t = static_cast<uint32_t>(row / a.hq), h = static_cast<uint32_t>(row - static_cast<uint64_t>(t) * a.hq);
     if (t >= a.n_rows) return;
-    if (!pa.shared && (static_cast<int32_t>(t) < a.start[0] || static_cast<int32_t>(t) >= a.start[pa.n_start])) return;
+    // rows of no request stay as they are; a request of no group has its own keys' part alone, the last one
+    const bool outside = static_cast<int32_t>(t) < a.start[0] || static_cast<int32_t>(t) >= a.start[pa.n_start];
+    if (outside && !pa.shared) return;
+    const uint32_t i0 = outside ? pa.n_part - 1 : 0;
     const float2* ml = pa.part_ml + row * pa.n_part;
     float m = kLowest;
-    for (uint32_t i = 0; i < pa.n_part; i++) m = fmaxf(m, ml[i].x);
+    for (uint32_t i = i0; i < pa.n_part; i++) m = fmaxf(m, ml[i].x);
     float l = 0.0f, o[4] = {};
-    for (uint32_t i = 0; i < pa.n_part; i++) {
+    for (uint32_t i = i0; i < pa.n_part; i++) {
         const float2 x = ml[i];
         if (x.y == 0.0f) continue;
         const float f = __builtin_amdgcn_exp2f(x.x - m);
@@ -704,8 +707,14 @@ void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs&
     else if (i8) launch_dp<float, int8_t, 3>(p.dp, grid, s, a);
     else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p.dp, grid, s, a) : launch_dp<float, float, 2>(p.dp, grid, s, a);
     else if (!t16) launch_dp<float, uint16_t, 2>(p.dp, grid, s, a);
-    else if (c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p.dp, grid, s, a);
+    else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p.dp, grid, s, a);
     else launch_dp<uint16_t, uint16_t, 1>(p.dp, grid, s, a);
+}
+
+void launch_join(const PagedAttnCall& c, const PromptArgs& a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(cdiv(c.q->ne[1] * c.q->ne[2], 4)));
+    if (c.q->type == CBX_TYPE_F16) hipLaunchKernelGGL((k_prompt_join<uint16_t>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_prompt_join<float>), grid, dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -729,23 +738,75 @@ int launch_paged_prompt(const PagedAttnCall& c, DeviceState* st, hipStream_t s) 
         a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
     }
     launch_tiles(c, p, a, s);
-    if (p.n_split > 1) {
-        const dim3 grid(static_cast<unsigned>(cdiv(c.q->ne[1] * c.q->ne[2], 4)));
-        if (c.q->type == CBX_TYPE_F16) hipLaunchKernelGGL((k_prompt_join<uint16_t>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_prompt_join<float>), grid, dim3(256), 0, s, a);
-    }
+    if (p.n_split > 1) launch_join(c, a, s);
     return check_launch(what);
 }
 
-size_t paged_shared_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor*,
+// ---- groups ---------------------------------------------------------------------
+
+namespace {
+
+// k_prompt over the shared keys, k_attn_tiles over each request's own, the
+// parts of both added up.
+struct SharedPlan {
+    PromptPlan pre;
+    bool tiles;
+    size_t rows, o_bytes, ml_bytes, first_bytes, bytes;
+};
+
+SharedPlan shared_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor* start,
+                       const DeviceState* st) {
+    SharedPlan p{};
+    const int64_t n_groups = start->ne[0] - 1;
+    p.pre = prompt_plan(q, k, tables, n_groups, st);
+    p.tiles = p.pre.tiles && n_groups > 0 && n_groups < q->ne[2];
+    p.bytes = attention_tiles_workspace(q, k, tables, st);
+    if (!p.tiles) return p;
+    const auto up = [](int64_t n) { return static_cast<size_t>(cdiv(n, 16) * 16); };
+    const int64_t parts = q->ne[1] * q->ne[2] * (p.pre.n_split + 1);
+    p.o_bytes = up(parts * q->ne[0] * 4);
+    p.ml_bytes = up(parts * 8);
+    p.first_bytes = up(q->ne[2] * 4);
+    p.bytes = up(static_cast<int64_t>(p.bytes)) + p.o_bytes + p.ml_bytes + p.first_bytes;
+    return p;
+}
+
+}  // namespace
+
+size_t paged_shared_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor* start,
                               const DeviceState* st) {
-    return paged_attention_workspace(q, k, tables, st);
+    return shared_plan(q, k, tables, start, st).bytes;
 }
 
 int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
+    const char* what = "cbx_paged_shared_attention";
+    const SharedPlan p = shared_plan(c.q, c.k, c.tables, c.start, st);
     PagedAttnCall own = c;
     own.start = own.shared = nullptr;
-    return launch_paged_attention(own, st, s);
+    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_paged_attention(own, st, s);
+    char* ws = static_cast<char*>(c.ws);
+    PromptArgs a{};
+    a.a = attn_args(c, st);
+    a.shared = static_cast<const int32_t*>(c.shared->data);
+    a.n_start = static_cast<uint32_t>(c.start->ne[0] - 1);
+    a.n_split = p.pre.n_split;
+    a.n_part = p.pre.n_split + 1;
+    a.tiles = p.pre.row_tiles;
+    page_division(a.a.g, &a.g_mul, &a.g_shift);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
+    a.own_first = reinterpret_cast<int32_t*>(ws + p.o_bytes + p.ml_bytes);
+    launch_tiles(c, p.pre, a, s);
+    AttnArgs b = attn_args(own, st);
+    b.own_first = a.own_first;
+    b.groups = a.a.start;
+    b.n_groups = a.n_start;
+    b.own_parts = a.n_part;
+    b.own_o = a.part_o;
+    b.own_ml = a.part_ml;
+    launch_attention_tiles(b, own, ws + p.o_bytes + p.ml_bytes + p.first_bytes, st, s);
+    launch_join(c, a, s);
+    return check_launch(what);
 }
 
 }  // namespace cbx
