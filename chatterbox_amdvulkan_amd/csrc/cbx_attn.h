@@ -35,10 +35,10 @@ struct AttnArgs {
     uint4* split;                    // [W]: request, first query head, heads and parts of the key head that begins
                                      // in the run and ends in a later one; no parts: none does
     // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt): own_first, null: all
-    // keys, says where a request's begin, and (o, m, l) go to the last of its own_parts parts instead of y
+    // keys, says where a request's begin, and (o, m, l) go to own_o and own_ml at request * hq + head instead of y
     const int32_t* own_first;
     const int32_t* groups;           // own_first holds for the requests [groups[0], groups[n_groups])
-    uint32_t n_groups, own_parts;
+    uint32_t n_groups;
     float own_up;                    // log2 of what the probabilities in o and l are multiplied by
     float* own_o;
     float2* own_ml;

@@ -901,7 +901,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 oo = fmaf(lds_o[(w * a.gc + hh) * ld + d], f, oo);
             }
             if (entire && a.own_first) {
-                const uint64_t own = (static_cast<uint64_t>(s) * a.hq + hq0 + hh) * a.own_parts + a.own_parts - 1;
+                const uint64_t own = static_cast<uint64_t>(s) * a.hq + hq0 + hh;
                 a.own_o[own * a.D + d] = oo;
                 if (d == 0) a.own_ml[own] = make_float2(mm - a.own_up, ll);
             } else if (entire) {
@@ -985,7 +985,7 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     for (int j = 0; j < N; j++) lds_o[wid][lane + 64 * j] = o[j];
     __syncthreads();
     l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
-    const uint64_t own = (static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh) * a.own_parts + a.own_parts - 1;
+    const uint64_t own = static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh;
     if (a.own_first && tid == 0) a.own_ml[own] = make_float2(m - a.own_up, l);
     char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
     for (uint32_t d = tid; d < a.D; d += kAttnThreads) {

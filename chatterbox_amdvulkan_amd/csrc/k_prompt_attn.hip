@@ -29,12 +29,16 @@ struct PromptArgs {
     AttnArgs a;
     const int32_t* shared;     // shared keys a group; null: packed tokens
     uint32_t n_start;          // requests or groups: start has one more
-    uint32_t n_split, n_part;  // runs that a row tile's keys are dealt to; parts a row has in part_o
     uint32_t tiles;            // row tiles at most
     uint32_t g_mul, g_shift;   // i / g
-    float* part_o;             // [row * hq + head][n_part][D], null: y
-    float2* part_ml;
+    // row tiles' keys dealt to workgroups in pieces (see Piece); deal: how many are aimed at, 0: a row tile is one workgroup's
+    uint32_t deal, slots, row_cap;   // pieces there is room for, rows of each
+    float* part_o;             // [piece][row_cap][D]
+    float2* part_ml;           // [piece][row_cap]
+    uint2* row_parts;          // [row * hq + head]: its first piece, pieces | row of theirs << 16; the next piece is hkv on
     int32_t* own_first;        // [n_seq]: first key behind the group's shared ones
+    const float* own_o;        // [row * hq + head][D], own_ml: the part of a request's own keys
+    const float2* own_ml;
 };
 
 // Four neighbouring elements at any element alignment.
@@ -76,6 +80,108 @@ __device__ __forceinline__ float tanh_of(float x) {
     const float large = 1.0f - 2.0f / (1.0f + e);
     return copysignf(y < 0.5f ? small : large, x);
 }
+
+// Tiles of kRows rows: those of request (group) p, whose rows are start[p] * g on, are numbered from start[p] * g / kRows + p on,
+// which is one more than it needs at most, so that a tile is found without a sum over the requests before it.
+__device__ __forceinline__ uint32_t start_of(const AttnArgs& a, uint32_t p) {
+    const int32_t t = a.start[p];
+    return t < 0 ? 0u : min(static_cast<uint32_t>(t), a.n_rows);
+}
+__device__ __forceinline__ uint32_t first_tile(const AttnArgs& a, uint32_t start, uint32_t p) { return start * a.g / kRows + p; }
+
+// Few row tiles: their keys are cut into pieces of one size, so that about `deal` workgroups have one each whatever the lengths, which
+// only the device knows.  Every workgroup counts the key tiles of all row tiles for itself.
+constexpr uint32_t kDealTiles = 1024;   // row tiles, requests at most
+struct Piece {
+    uint32_t first = 0, count = 1, at = 0;      // the row tile's first piece, how many it has, which of them
+    uint32_t tile0 = 0, tiles = 0;              // key tiles
+
+    template <int KT> __device__ __forceinline__ bool find(const PromptArgs& pa, uint32_t q, uint32_t* lds, uint32_t* x, uint32_t* p) {
+        const AttnArgs& a = pa.a;
+        constexpr int N = kDealTiles / 256;
+        __shared__ uint32_t sums[4], found[6];
+        const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+        for (uint32_t i = tid; i <= pa.n_start; i += 256) lds[i] = start_of(a, i);
+        if (tid == 0) found[0] = ~0u;
+        __syncthreads();
+        uint32_t keys[N], begin[N], whose[N], sum = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t xi = tid * N + i;
+            keys[i] = begin[i] = whose[i] = 0;
+            if (xi >= pa.tiles) continue;
+            uint32_t lo = 0, hi = pa.n_start;                // the last one whose tiles start at or before xi
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (first_tile(a, lds[mid], mid) <= xi) lo = mid;
+                else hi = mid;
+            }
+            const uint32_t t0 = lds[lo], t1 = lds[lo + 1], base = first_tile(a, t0, lo);
+            if (xi < base || t1 <= t0 || (xi - base) * kRows >= (t1 - t0) * a.g) continue;
+            const uint32_t row0 = (xi - base) * kRows, row1 = min(row0 + kRows, (t1 - t0) * a.g) - 1;
+            const int32_t cap = static_cast<int32_t>(a.max_pages * a.page);
+            int32_t first = 0, end;
+            if (pa.shared) {
+                end = min(max(pa.shared[lo], 0), cap);
+            } else {
+                const int32_t len = min(max(a.lens[lo], 0), cap), n = static_cast<int32_t>(t1 - t0);
+                auto limit = [&](uint32_t row) {
+                    return max(0, len - (n - 1 - static_cast<int32_t>((static_cast<uint64_t>(row) * pa.g_mul) >> pa.g_shift)));
+                };
+                end = limit(row1);
+                if (a.window > 0) first = max(0, limit(row0) - a.window);
+            }
+            begin[i] = first / KT;
+            keys[i] = max(1u, (static_cast<uint32_t>(end) + KT - 1) / KT - min(begin[i], (static_cast<uint32_t>(end) + KT - 1) / KT));
+            whose[i] = lo;
+            sum += keys[i];
+        }
+        uint32_t all = sum;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d);
+        if (lane == 0) sums[wid] = all;
+        __syncthreads();
+        all = sums[0] + sums[1] + sums[2] + sums[3];
+        __syncthreads();
+        // key tiles a piece: a piece's row tile is written and read again, so not too few
+        const uint32_t size = max(4u, static_cast<uint32_t>((static_cast<uint64_t>(all) * a.hkv + pa.deal - 1) / pa.deal));
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) sum += (keys[i] + size - 1) / size;
+        uint32_t before = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t y = __shfl_up(before, d);
+            if (lane >= static_cast<uint32_t>(d)) before += y;
+        }
+        if (lane == 63) sums[wid] = before;
+        __syncthreads();
+        before -= sum;
+        for (uint32_t w = 0; w < wid; w++) before += sums[w];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t n = (keys[i] + size - 1) / size;
+            if (q >= before && q - before < n) {
+                found[0] = before;
+                found[1] = n;
+                found[2] = begin[i] + (q - before) * size;
+                found[3] = tid * N + i;
+                found[4] = whose[i];
+            }
+            before += n;
+        }
+        __syncthreads();
+        first = __builtin_amdgcn_readfirstlane(found[0]);
+        if (first == ~0u) return false;
+        count = __builtin_amdgcn_readfirstlane(found[1]);
+        at = q - first;
+        tile0 = __builtin_amdgcn_readfirstlane(found[2]);
+        tiles = size;
+        *x = __builtin_amdgcn_readfirstlane(found[3]);
+        *p = __builtin_amdgcn_readfirstlane(found[4]);
+        return true;
+    }
+};
 
 // A tile of KT keys and values in LDS, and the products over it.  A wave holds
 // 32 rows of q: S^T = K Q^T by 32 x 32 products, whose result has the lane's row
@@ -138,37 +244,41 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave reads at a time, times
     constexpr float kUp = F32 ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = F32 ? 8.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
-    __shared__ __attribute__((aligned(16))) char lds_k[2][T::BYTES];
-    __shared__ __attribute__((aligned(16))) char lds_v[2][T::BYTES];
+    __shared__ __attribute__((aligned(16))) char lds[4][T::BYTES];   // keys, values of two tiles
+    char (*const lds_k)[T::BYTES] = lds, (*const lds_v)[T::BYTES] = lds + 2;
     __shared__ __attribute__((aligned(16))) float lds_s[2][2][I8 ? KT : 4];
     __shared__ int32_t lds_ext[4][4];
+    __shared__ float lds_pair[2 * 64 * 2];
     const uint32_t tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
     const uint32_t wid = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-    // this workgroup's key head, run of keys and row tile (the last rows, which have the most keys, first)
-    const uint32_t hk = blockIdx.x % a.hkv, rest = blockIdx.x / a.hkv, run = rest % pa.n_split;
-    const uint32_t x = pa.tiles - 1 - rest / pa.n_split;
-    // the request (group) p whose tiles x lies among: tiles of p start at start[p] * g / 128 + p, which leaves one more than it has
-    auto start_of = [&](uint32_t p) {
-        const int32_t t = a.start[p];
-        return t < 0 ? 0u : min(static_cast<uint32_t>(t), a.n_rows);
-    };
-    uint32_t p = 0;
-    for (uint32_t width = pa.n_start;;) {                    // p among [p, p + width)
-        const uint32_t step = (width + 63) / 64, q = p + lane * step;
-        const bool in = lane * step < width && start_of(q) * a.g / kRows + q <= x;
-        const uint32_t at = 64 - __builtin_clzll(__ballot(in) | 1) - 1;
-        p = __builtin_amdgcn_readfirstlane(p + at * step);
-        width = min(step, width - min(width, at * step));
-        if (step == 1) break;
+    // this workgroup's key head, row tile (undealt: the last rows, which have the most keys, first) and piece of its keys
+    const uint32_t hk = blockIdx.x % a.hkv;
+    uint32_t x = pa.tiles - 1 - blockIdx.x / a.hkv, p = 0;
+    Piece piece;
+    if (pa.deal) {
+        if (!piece.find<KT>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds), &x, &p)) return;
+    } else {
+        // the request (group) p whose tiles x lies among
+        for (uint32_t width = pa.n_start;;) {                // p among [p, p + width)
+            const uint32_t step = (width + 63) / 64, q = p + lane * step;
+            const bool in = lane * step < width && first_tile(a, start_of(a, q), q) <= x;
+            const uint32_t at = 64 - __builtin_clzll(__ballot(in) | 1) - 1;
+            p = __builtin_amdgcn_readfirstlane(p + at * step);
+            width = min(step, width - min(width, at * step));
+            if (step == 1) break;
+        }
     }
-    const uint32_t t0 = start_of(p), t1 = start_of(p + 1);
-    const uint32_t base = t0 * a.g / kRows + p;
+    const uint32_t t0 = start_of(a, p), t1 = start_of(a, p + 1);
+    const uint32_t base = first_tile(a, t0, p);
     if (x < base || t1 <= t0 || static_cast<uint64_t>(x - base) * kRows >= static_cast<uint64_t>(t1 - t0) * a.g) return;
     const uint32_t row0 = (x - base) * kRows, rows = min(static_cast<uint32_t>(kRows), (t1 - t0) * a.g - row0);
+    // 64 rows or fewer: two waves a row, for every other run of 32 keys
+    const bool paired = rows <= 64;
+    const uint32_t row_wave = paired ? wid & 1 : wid, turn = wid >> 1;
 
     // the lane's row: token or request t, head, keys [first, limit)
-    const uint32_t r = wid * 32 + n;
+    const uint32_t r = row_wave * 32 + n;
     const bool live_row = r < rows;
     const uint32_t ri = row0 + (live_row ? r : 0);
     const uint32_t j = static_cast<uint32_t>((static_cast<uint64_t>(ri) * pa.g_mul) >> pa.g_shift);
@@ -186,7 +296,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             const int32_t pre = min(max(pa.shared[p], 0), cap);
             first = a.window > 0 && len > a.window ? len - a.window : 0;
             limit = min(len, pre);
-            if (hk == 0 && run == 0 && half == 0 && live_row) pa.own_first[t] = limit;
+            if (hk == 0 && piece.at == 0 && half == 0 && live_row && wid == row_wave) pa.own_first[t] = limit;
         } else {
             limit = max(0, len - static_cast<int32_t>(t1 - 1 - t));
             first = a.window > 0 && limit > a.window ? limit - a.window : 0;
@@ -218,8 +328,13 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     const int32_t every_end = min(min(lds_ext[2][0], lds_ext[2][1]), min(lds_ext[2][2], lds_ext[2][3]));
     const int32_t every_begin = max(max(lds_ext[3][0], lds_ext[3][1]), max(lds_ext[3][2], lds_ext[3][3]));
     const uint32_t tile0 = static_cast<uint32_t>(begin) / KT, n_tiles = (static_cast<uint32_t>(end) + KT - 1) / KT - tile0;
-    const uint32_t ta = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * run / pa.n_split));
-    const uint32_t tb = __builtin_amdgcn_readfirstlane(tile0 + static_cast<uint32_t>(static_cast<uint64_t>(n_tiles) * (run + 1) / pa.n_split));
+    uint32_t ta = tile0, tb = tile0 + n_tiles;
+    if (pa.deal) {
+        ta = max(ta, piece.tile0);
+        tb = min(tb, piece.tile0 + piece.tiles);
+    }
+    ta = __builtin_amdgcn_readfirstlane(ta);
+    tb = __builtin_amdgcn_readfirstlane(tb);
 
     // the lane's query: dims 16 c + 8 half + [0, 8), for F32 pages 8 c + 4 half + [0, 4).  Else an F32 one is scaled by a power of two to below 2^15 and split into two f16, the
     // lower times 2^12 and summed apart
@@ -564,6 +679,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll 1
                 for (int sub = 0; sub < KT / 32; sub++) {
                     const uint32_t kb = tile * KT + 32 * sub;
+                    if (paired && (kb >> 5 & 1) != turn) continue;
                     if (static_cast<int32_t>(kb) < w_end && static_cast<int32_t>(kb) + 32 > w_begin) products(buf, kb, sub);
                 }
                 if (more) put(buf ^ 1, edge(tile + 1));
@@ -576,19 +692,50 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     }
     l += __shfl_xor(l, 32);
     if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
-    const uint64_t part = (static_cast<uint64_t>(t) * a.hq + hq) * pa.n_part + run;
+    if (paired) {                                            // the two waves' parts added up
+        float* part = reinterpret_cast<float*>(lds) + row_wave * (DP / 2 * 64) + lane;
+        float2* ml = reinterpret_cast<float2*>(lds_pair) + row_wave * 64 + lane;
+        __syncthreads();
+        if (turn == 1) {
+            *ml = make_float2(mc, l);
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) part[(16 * d + e) * 64] = o[d][e];
+            }
+        }
+        __syncthreads();
+        if (turn == 0) {
+            const float2 other = *ml;
+            const float m2 = fmaxf(mc, other.x), f0 = __builtin_amdgcn_exp2f(mc - m2), f1 = __builtin_amdgcn_exp2f(other.x - m2);
+            mc = m2;
+            l = fmaf(l, f0, other.y * f1);
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] = fmaf(o[d][e], f0, part[(16 * d + e) * 64] * f1);
+            }
+        }
+    }
+    const bool mine = live_row && wid == row_wave;
+    const bool to_parts = pa.shared || piece.count > 1;
+    const uint32_t slot = piece.first * a.hkv + hk;          // of the row tile's first piece
+    const uint64_t part = static_cast<uint64_t>(slot + piece.at * a.hkv) * pa.row_cap + r;
     char* yr = a.y + t * a.y_nb2 + hq * a.y_nb1;
-    if (pa.part_o && half == 0 && live_row) pa.part_ml[part] = make_float2(mc, l);
+    if (pa.deal && half == 0 && mine) {
+        if (piece.at == 0) pa.row_parts[static_cast<uint64_t>(t) * a.hq + hq] = make_uint2(slot, piece.count | r << 16);
+        if (to_parts) pa.part_ml[part] = make_float2(mc, l);
+    }
 #pragma unroll
     for (int d = 0; d < DP / 32; d++) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             const uint32_t dim = 32 * d + 8 * c + 4 * half;
-            if (dim >= a.D || !live_row) continue;
+            if (dim >= a.D || !mine) continue;
             float v[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) v[u] = o[d][4 * c + u];
-            if (pa.part_o) {
+            if (to_parts) {
                 store4u(reinterpret_cast<char*>(pa.part_o + part * a.D + dim), v, float());
             } else {
 #pragma unroll
@@ -602,7 +749,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         __syncthreads();                                     // what is written above is corrected
 #pragma unroll 1
         for (int i = 0; i < 32; i++) {                       // a row at a time, its dims over the lanes
-            if (wid * 32 + i >= rows) break;
+            if (wid != row_wave || wid * 32 + i >= rows) break;
             const int32_t lim = min(__shfl(limit, i), static_cast<int32_t>(tb * KT)), from = max(__shfl(first, i), static_cast<int32_t>(ta * KT));
             const uint32_t ti = __shfl(static_cast<int>(t), i), hi = __shfl(static_cast<int>(hq), i);
             uint32_t found[DP / 64 + 1] = {};                // 1, 2, 4: infinity, -infinity, NaN
@@ -624,73 +771,120 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 const uint32_t d = lane + 64 * k;
                 if (d >= a.D || !found[k]) continue;
                 const float y = found[k] == 1 ? INFINITY : found[k] == 2 ? -INFINITY : NAN;
-                if (pa.part_o) pa.part_o[((static_cast<uint64_t>(ti) * a.hq + hi) * pa.n_part + run) * a.D + d] = y;
+                if (to_parts) pa.part_o[(static_cast<uint64_t>(slot + piece.at * a.hkv) * pa.row_cap + wid * 32 + i) * a.D + d] = y;
                 else Elt<TQ>::store1(a.y + ti * a.y_nb2 + hi * a.y_nb1 + d * Elt<TQ>::size, y);
             }
         }
     }
 }
 
-// Adds up a row's parts: a wave a row of y, its dims over the lanes.
+// Adds up a row's parts (those of its pieces, then the one of a request's own keys): a wave a row of y, its dims over the lanes, U
+// parts in flight.
 template <typename TQ>
 __global__ __launch_bounds__(256) void k_prompt_join(PromptArgs pa) {
+    constexpr int U = 8, N = 4;
     const AttnArgs& a = pa.a;
     const uint32_t lane = threadIdx.x & 63;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const uint32_t t = static_cast<uint32_t>(row / a.hq), h = static_cast<uint32_t>(row - static_cast<uint64_t>(t) * a.hq);
+    const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), t = row / a.hq, h = row - t * a.hq;
     if (t >= a.n_rows) return;
-    // rows of no request stay as they are; a request of no group has its own keys' part alone, the last one
+    // rows of no request stay as they are; a request of no group has its own keys' part alone
     const bool outside = static_cast<int32_t>(t) < a.start[0] || static_cast<int32_t>(t) >= a.start[pa.n_start];
     if (outside && !pa.shared) return;
-    const uint32_t i0 = outside ? pa.n_part - 1 : 0;
-    const float2* ml = pa.part_ml + row * pa.n_part;
-    float m = kLowest;
-    for (uint32_t i = i0; i < pa.n_part; i++) m = fmaxf(m, ml[i].x);
-    float l = 0.0f, o[4] = {};
-    for (uint32_t i = i0; i < pa.n_part; i++) {
-        const float2 x = ml[i];
-        if (x.y == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f(x.x - m);
-        l = fmaf(x.y, f, l);
-        const float* p = pa.part_o + (row * pa.n_part + i) * a.D;
+    uint2 parts = outside ? make_uint2(0, 0) : pa.row_parts[row];
+    uint32_t n = parts.y & 0xffff;
+    const uint32_t r = parts.y >> 16;
+    // a row that no request has after all (`start` falls somewhere): what the scratch holds for it is anything
+    if (n > 0 && (parts.x >= pa.slots || (n - 1) * a.hkv >= pa.slots - parts.x || r >= pa.row_cap)) n = 0;
+    if (n <= 1 && !pa.shared) return;                        // written by its only piece
+    auto at = [&](uint32_t i) { return static_cast<uint64_t>(parts.x + i * a.hkv) * pa.row_cap + r; };
+    float m = pa.shared ? pa.own_ml[row].x : kLowest;
+    for (uint32_t i = lane; i < n; i += 64) m = fmaxf(m, pa.part_ml[at(i)].x);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t d = lane + 64 * k;
-            if (d < a.D) o[k] = fmaf(p[d], f, o[k]);
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    float l = 0.0f, o[N] = {};
+    auto add = [&](float2 ml, const float (&v)[N]) {
+        const float f = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int k = 0; k < N; k++) o[k] = fmaf(v[k], f, o[k]);
+    };
+    auto fetch = [&](const float* p, float (&v)[N]) {
+#pragma unroll
+        for (int k = 0; k < N; k++) v[k] = lane + 64 * k < a.D ? p[lane + 64 * k] : 0.0f;
+    };
+    for (uint32_t i = 0; i < n; i += U) {
+        float v[U][N];
+        float2 ml[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint64_t part = at(min(i + u, n - 1));
+            ml[u] = pa.part_ml[part];
+            fetch(pa.part_o + part * a.D, v[u]);
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u < n) add(ml[u], v[u]);
+        }
+    }
+    if (pa.shared) {
+        float v[N];
+        fetch(pa.own_o + static_cast<uint64_t>(row) * a.D, v);
+        add(pa.own_ml[row], v);
     }
     char* yr = a.y + t * a.y_nb2 + h * a.y_nb1;
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
+    for (int k = 0; k < N; k++) {
         const uint32_t d = lane + 64 * k;
         if (d < a.D) Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : o[k] / l);
     }
 }
 
 struct PromptPlan {
-    bool tiles;
+    bool tiles;                // k_prompt, else k_attn_rows
     int dp;
-    uint32_t row_tiles, n_split;
-    size_t o_bytes, bytes;
+    uint32_t row_tiles, deal, row_cap, grid;
+    size_t o_bytes, ml_bytes, bytes;
 };
 
-PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, int64_t n_start, const DeviceState* st) {
+size_t up16(int64_t n) { return static_cast<size_t>(cdiv(n, 16) * 16); }
+
+// n_start: requests, or groups of them (shared).
+PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, int64_t n_start, bool shared,
+                       const DeviceState* st) {
     PromptPlan p{};
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0, cap = tables->ne[0] * k->ne[1];
     p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
-    const int64_t most = q->ne[2] * g / kRows + n_start;
-    p.tiles = D % (k->type == CBX_TYPE_I8 ? 16 : 8) == 0 && D <= 256 && cap > 0 && k->ne[3] > 0;
+    const int64_t most = q->ne[2] * g / kRows + n_start, wide = 2 * st->n_cu;
+    p.tiles = D % (k->type == CBX_TYPE_I8 ? 16 : 8) == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most * hkv < (int64_t{1} << 24) &&
+              k->ne[2] <= wide;
     if (!p.tiles) return p;
     p.row_tiles = static_cast<uint32_t>(most);
-    const int64_t groups = std::max<int64_t>(1, most * hkv);
-    p.n_split = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(2 * st->n_cu / groups, cap / 256)));
-    p.tiles = most * hkv * p.n_split < (int64_t{1} << 24);
-    if (p.n_split > 1) {
-        const int64_t parts = q->ne[1] * q->ne[2] * p.n_split;
-        p.o_bytes = static_cast<size_t>(parts) * D * 4;
-        p.bytes = p.o_bytes + static_cast<size_t>(parts) * 8;
-    }
+    p.grid = static_cast<uint32_t>(most * hkv);
+    if (most > kDealTiles || n_start > kDealTiles || (!shared && (most * hkv > wide || cap < 512))) return p;
+    p.deal = static_cast<uint32_t>(wide);
+    p.grid = static_cast<uint32_t>((wide / hkv + most) * hkv);
+    p.row_cap = static_cast<uint32_t>(std::min<int64_t>(kRows, q->ne[2] * g));
+    const int64_t parts = static_cast<int64_t>(p.grid) * p.row_cap;
+    p.o_bytes = up16(parts * D * 4);
+    p.ml_bytes = up16(parts * 8);
+    p.bytes = p.o_bytes + p.ml_bytes + up16(q->ne[1] * q->ne[2] * 8);
     return p;
+}
+
+PromptArgs prompt_args(const PagedAttnCall& c, const PromptPlan& p, uint32_t n_start, DeviceState* st) {
+    PromptArgs a{};
+    a.a = attn_args(c, st);
+    a.n_start = n_start;
+    a.tiles = p.row_tiles;
+    a.deal = p.deal;
+    a.slots = p.grid;
+    a.row_cap = p.row_cap;
+    page_division(a.a.g, &a.g_mul, &a.g_shift);
+    char* ws = static_cast<char*>(c.ws);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
+    a.row_parts = reinterpret_cast<uint2*>(ws + p.o_bytes + p.ml_bytes);
+    return a;
 }
 
 template <typename TQ, typename TC, int PP> void launch_dp(int dp, dim3 grid, hipStream_t s, const PromptArgs& a) {
@@ -701,7 +895,7 @@ template <typename TQ, typename TC, int PP> void launch_dp(int dp, dim3 grid, hi
 }
 
 void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs& a, hipStream_t s) {
-    const dim3 grid(p.row_tiles * p.n_split * a.a.hkv);
+    const dim3 grid(p.grid);
     const bool t16 = c.q->type == CBX_TYPE_F16, i8 = c.k->type == CBX_TYPE_I8;
     if (t16 && i8) launch_dp<uint16_t, int8_t, 2>(p.dp, grid, s, a);
     else if (i8) launch_dp<float, int8_t, 3>(p.dp, grid, s, a);
@@ -720,25 +914,16 @@ void launch_join(const PagedAttnCall& c, const PromptArgs& a, hipStream_t s) {
 }  // namespace
 
 size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
-    return prompt_plan(q, k, tables, tables->ne[1], st).bytes;
+    return prompt_plan(q, k, tables, tables->ne[1], false, st).bytes;
 }
 
 int launch_paged_prompt(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
     const char* what = "cbx_paged_prompt_attention";
-    const PromptPlan p = prompt_plan(c.q, c.k, c.tables, c.tables->ne[1], st);
+    const PromptPlan p = prompt_plan(c.q, c.k, c.tables, c.tables->ne[1], false, st);
     if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_attention_rows(attn_args(c, st), c, what, s);
-    PromptArgs a{};
-    a.a = attn_args(c, st);
-    a.n_start = a.a.n_seq;
-    a.n_split = a.n_part = p.n_split;
-    a.tiles = p.row_tiles;
-    page_division(a.a.g, &a.g_mul, &a.g_shift);
-    if (p.n_split > 1) {
-        a.part_o = static_cast<float*>(c.ws);
-        a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(c.ws) + p.o_bytes);
-    }
+    const PromptArgs a = prompt_args(c, p, static_cast<uint32_t>(c.tables->ne[1]), st);
     launch_tiles(c, p, a, s);
-    if (p.n_split > 1) launch_join(c, a, s);
+    if (p.deal) launch_join(c, a, s);
     return check_launch(what);
 }
 
@@ -751,23 +936,21 @@ namespace {
 struct SharedPlan {
     PromptPlan pre;
     bool tiles;
-    size_t rows, o_bytes, ml_bytes, first_bytes, bytes;
+    size_t o_bytes, ml_bytes, first_bytes, bytes;   // behind pre's: the own keys' parts, where these begin, k_attn_tiles' scratch
 };
 
 SharedPlan shared_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const cbx_tensor* start,
                        const DeviceState* st) {
     SharedPlan p{};
-    const int64_t n_groups = start->ne[0] - 1;
-    p.pre = prompt_plan(q, k, tables, n_groups, st);
-    p.tiles = p.pre.tiles && n_groups > 0 && n_groups < q->ne[2];
+    const int64_t n_groups = start->ne[0] - 1, rows = q->ne[1] * q->ne[2];
+    p.pre = prompt_plan(q, k, tables, n_groups, true, st);
+    p.tiles = p.pre.tiles && p.pre.deal && n_groups > 0 && n_groups < q->ne[2];
     p.bytes = attention_tiles_workspace(q, k, tables, st);
     if (!p.tiles) return p;
-    const auto up = [](int64_t n) { return static_cast<size_t>(cdiv(n, 16) * 16); };
-    const int64_t parts = q->ne[1] * q->ne[2] * (p.pre.n_split + 1);
-    p.o_bytes = up(parts * q->ne[0] * 4);
-    p.ml_bytes = up(parts * 8);
-    p.first_bytes = up(q->ne[2] * 4);
-    p.bytes = up(static_cast<int64_t>(p.bytes)) + p.o_bytes + p.ml_bytes + p.first_bytes;
+    p.o_bytes = up16(rows * q->ne[0] * 4);
+    p.ml_bytes = up16(rows * 8);
+    p.first_bytes = up16(q->ne[2] * 4);
+    p.bytes += p.pre.bytes + p.o_bytes + p.ml_bytes + p.first_bytes;
     return p;
 }
 
@@ -784,26 +967,21 @@ int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s) 
     PagedAttnCall own = c;
     own.start = own.shared = nullptr;
     if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_paged_attention(own, st, s);
-    char* ws = static_cast<char*>(c.ws);
-    PromptArgs a{};
-    a.a = attn_args(c, st);
+    PromptArgs a = prompt_args(c, p.pre, static_cast<uint32_t>(c.start->ne[0] - 1), st);
+    char* ws = static_cast<char*>(c.ws) + p.pre.bytes;
+    float* own_o = reinterpret_cast<float*>(ws);
+    float2* own_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
     a.shared = static_cast<const int32_t*>(c.shared->data);
-    a.n_start = static_cast<uint32_t>(c.start->ne[0] - 1);
-    a.n_split = p.pre.n_split;
-    a.n_part = p.pre.n_split + 1;
-    a.tiles = p.pre.row_tiles;
-    page_division(a.a.g, &a.g_mul, &a.g_shift);
-    a.part_o = reinterpret_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(ws + p.o_bytes);
+    a.own_o = own_o;
+    a.own_ml = own_ml;
     a.own_first = reinterpret_cast<int32_t*>(ws + p.o_bytes + p.ml_bytes);
     launch_tiles(c, p.pre, a, s);
     AttnArgs b = attn_args(own, st);
     b.own_first = a.own_first;
     b.groups = a.a.start;
     b.n_groups = a.n_start;
-    b.own_parts = a.n_part;
-    b.own_o = a.part_o;
-    b.own_ml = a.part_ml;
+    b.own_o = own_o;
+    b.own_ml = own_ml;
     launch_attention_tiles(b, own, ws + p.o_bytes + p.ml_bytes + p.first_bytes, st, s);
     launch_join(c, a, s);
     return check_launch(what);
