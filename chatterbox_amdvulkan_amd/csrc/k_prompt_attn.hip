@@ -236,7 +236,7 @@ template <int DP> struct Tile<float, DP> {
 // Workgroups of k_prompt that a CU holds, which their registers are limited to.
 constexpr int waves_per_simd(int dp, bool f32) { return dp <= 64 && !f32 ? 3 : dp <= 128 ? 2 : 1; }
 
-template <typename TQ, typename TC, int DP, int PP>
+template <typename TQ, typename TC, int DP, int PP, bool CAP>
 __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_prompt(PromptArgs pa) {
     using T = Tile<TC, DP>;
     constexpr bool F32 = T::F32, I8 = T::I8, Q2 = sizeof(TQ) == 4 && !F32;
@@ -377,8 +377,11 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             for (int i = 0; i < QC * 8; i++) qh[i / 8][i % 8] = static_cast<_Float16>(v[i]);
         }
     }
-    const float cap_in = a.softcap > 0.0f ? mul / kLog2e / a.softcap : 0.0f;
-    if (a.softcap > 0.0f) mul = 1.0f;
+    float cap_in = 0.0f;
+    if constexpr (CAP) {
+        cap_in = mul / kLog2e / a.softcap;
+        mul = 1.0f;
+    }
 
     // a tile's pages: of key lane % KT of it; what the wave stages of it
     const int32_t* table = reinterpret_cast<const int32_t*>(a.tables + seq * a.t_nb1);
@@ -422,11 +425,11 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     // into LDS: keys that are not there and dims past D as zeros
     bool clean = false, bad = false;
     auto put = [&](int buf, bool edge) {
-        const bool whole = have_next == (KT == 64 ? ~0ull : 0xffffffffull);
+        const bool some = have_next != (KT == 64 ? ~0ull : 0xffffffffull) || a.D != DP;   // not all of it is brought
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
-            if (!sub_in || (!whole && !(have_next >> row & 1))) rk[i] = rv[i] = u4v{};
+            if (some && (!sub_in || !(have_next >> row & 1))) rk[i] = rv[i] = u4v{};
             if constexpr (I8) {
                 u4v k0, k1, v0, v1;
 #pragma unroll
@@ -539,22 +542,34 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                     for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(h2v{ph[i], ph[i + 1]}, h2v{1, 1}, l, false);
                 }
             }
+            h8v vf[DP / 32];
 #pragma unroll
             for (int d = 0; d < DP / 32; d++) {
                 // place of chunk 4 d + v_c in the lane's rows: these are alike modulo 4
                 const char* at = lv + v_at + T::v_place(v_key, 4 * d + v_c) * 16 + 16 * u * PITCH;
                 const h4v x0 = read_turned(at), x1 = read_turned(at + 8 * PITCH);
-                const h8v vf = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+                vf[d] = h8v{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 32; d++) {
                 if constexpr (I8) {
-                    const b8v vb = __builtin_bit_cast(b8v, vf);
+                    const b8v vb = __builtin_bit_cast(b8v, vf[d]);
                     if constexpr (PP == 3) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b2, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b1, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b0, o[d], 0, 0, 0);
                 } else {
-                    if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph, o[d], 0, 0, 0);
+                    if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, o[d], 0, 0, 0);
                 }
             }
+        }
+        // the first reads, then a product for every read
+        constexpr int ND = DP / 32 < 4 ? DP / 32 : 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * ND, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * (DP / 32); i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PP, 0);
+            if (i + ND < 2 * (DP / 32)) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
     };
 
@@ -570,11 +585,20 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             }
         } else {
             f16v low = {};
+            constexpr int A = 4;                             // reads ahead of their products
+            h8v kf[QC];
+#pragma unroll
+            for (int c = 0; c < QC; c++) kf[c] = *reinterpret_cast<const h8v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
 #pragma unroll
             for (int c = 0; c < QC; c++) {
-                const h8v kf = *reinterpret_cast<const h8v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[c], s, 0, 0, 0);
-                if constexpr (Q2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[c], low, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qh[c], s, 0, 0, 0);
+                if constexpr (Q2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], ql[c], low, 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+            for (int c = 0; c < QC; c++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, Q2 ? 2 : 1, 0);
+                if (c + A < QC) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
             if constexpr (Q2) {
 #pragma unroll
@@ -589,7 +613,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 for (int u = 0; u < 4; u++) s[e + u] *= sc[u];
             }
         }
-        if (a.softcap > 0.0f) {
+        if constexpr (CAP) {
 #pragma unroll
             for (int e = 0; e < 16; e++) s[e] = tanh_of(s[e] * cap_in) * (a.softcap * kLog2e);
         }
@@ -722,6 +746,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     const uint32_t slot = piece.first * a.hkv + hk;          // of the row tile's first piece
     const uint64_t part = static_cast<uint64_t>(slot + piece.at * a.hkv) * pa.row_cap + r;
     char* yr = a.y + t * a.y_nb2 + hq * a.y_nb1;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (pa.deal && half == 0 && mine) {
         if (piece.at == 0) pa.row_parts[static_cast<uint64_t>(t) * a.hq + hq] = make_uint2(slot, piece.count | r << 16);
         if (to_parts) pa.part_ml[part] = make_float2(mc, l);
@@ -739,7 +764,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 store4u(reinterpret_cast<char*>(pa.part_o + part * a.D + dim), v, float());
             } else {
 #pragma unroll
-                for (int u = 0; u < 4; u++) v[u] = l == 0.0f ? 0.0f : v[u] / l;
+                for (int u = 0; u < 4; u++) v[u] *= inv;
                 store4u(yr + dim * Elt<TQ>::size, v, TQ());
             }
         }
@@ -888,10 +913,15 @@ PromptArgs prompt_args(const PagedAttnCall& c, const PromptPlan& p, uint32_t n_s
 }
 
 template <typename TQ, typename TC, int PP> void launch_dp(int dp, dim3 grid, hipStream_t s, const PromptArgs& a) {
-    if (dp == 64) hipLaunchKernelGGL((k_prompt<TQ, TC, 64, PP>), grid, dim3(256), 0, s, a);
-    else if (dp == 96) hipLaunchKernelGGL((k_prompt<TQ, TC, 96, PP>), grid, dim3(256), 0, s, a);
-    else if (dp == 128) hipLaunchKernelGGL((k_prompt<TQ, TC, 128, PP>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_prompt<TQ, TC, 256, PP>), grid, dim3(256), 0, s, a);
+    auto go = [&](auto d) {
+        constexpr int DP = decltype(d)::value;
+        if (a.a.softcap > 0.0f) hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, false>), grid, dim3(256), 0, s, a);
+    };
+    if (dp == 64) go(std::integral_constant<int, 64>());
+    else if (dp == 96) go(std::integral_constant<int, 96>());
+    else if (dp == 128) go(std::integral_constant<int, 128>());
+    else go(std::integral_constant<int, 256>());
 }
 
 void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs& a, hipStream_t s) {
