@@ -190,62 +190,49 @@ struct Piece {
 // come in the same one), V^T's columns by turning 4 x 16 blocks on the way out of
 // LDS.  So a row's maximum and sum are its lane's, and nothing else crosses lanes.
 //
-// LDS holds rows of DP elements as 16-byte chunks, chunk c of key r at place
+// LDS holds rows of PITCH bytes as 16-byte chunks, chunk c of key r at place
 // c ^ f(r): the 16 lanes that read together meet 16 different places of 256
-// bytes.
-template <typename TC, int DP> struct Tile;
-
+// bytes.  F16 and F32 pages come there straight from memory (1 KiB a wave and
+// instruction, lane l to byte 16 l: the lane asks for the chunk whose place
+// that is), I8 ones through registers, where they are widened.
+//
 // F16 pages, and I8 ones as whole numbers: keys in f16; values in f16, of I8 pages
 // in bf16, whose range holds a probability times any scale.
 template <typename TC, int DP> struct Tile {
     static constexpr bool F32 = false, I8 = sizeof(TC) == 1;
-    static constexpr int KT = DP <= 128 ? 64 : 32, PITCH = DP * 2, CH = DP / 8;      // bytes a row, chunks
-    static constexpr int BYTES = KT * PITCH;
-    static constexpr int QC = DP / 16;
-    // which elements a lane reads of a row: 16 bytes
-    static constexpr int PER = I8 ? 16 : 8, LANES = DP / PER <= 4 ? 4 : DP / PER <= 8 ? 8 : DP / PER <= 16 ? 16 : 32;
-    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) {
-        if constexpr (DP == 64) return c ^ (r >> 1 & 7);
-        else if constexpr (DP == 96) return c ^ (r >> 2 & 3);
-        else return c ^ (r & 15);
-    }
-    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) {
-        if constexpr (DP == 64) return c ^ (r >> 1 & 1) << 2;
-        else if constexpr (DP == 96) return c;
-        else return c ^ (r & 3) << 2;
-    }
+    static constexpr int KT = DP <= 128 ? 64 : 32, PITCH = DP == 64 ? 128 : DP <= 128 ? 256 : 512;
+    static constexpr int PER = I8 ? 16 : 8, LANES = PITCH / 2 / PER;     // elements in 16 bytes of a page, lanes that bring a row
+    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) { return DP == 64 ? c ^ (r >> 1 & 7) : c ^ (r & 15); }
+    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) { return DP == 64 ? c ^ (r >> 1 & 1) << 2 : c ^ (r & 3) << 2; }
 };
 
 // F32 pages: products of f32, 32 x 32 x 2.
 template <int DP> struct Tile<float, DP> {
     static constexpr bool F32 = true, I8 = false;
-    static constexpr int KT = 32, PITCH = DP * 4, CH = DP / 4;
-    static constexpr int BYTES = KT * PITCH;
-    static constexpr int QC = DP / 16;
-    static constexpr int PER = 4, LANES = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
-    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) {
-        if constexpr (DP == 96) return c ^ (r >> 1 & 7);
-        else return c ^ (r & 15);
-    }
-    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) {
-        if constexpr (DP == 96) return c;
-        else return c ^ (r >> 2 & 1) << 3;
-    }
+    static constexpr int KT = 32, PITCH = DP == 64 ? 256 : DP <= 128 ? 512 : 1024;
+    static constexpr int PER = 4, LANES = PITCH / 16;
+    static __device__ __forceinline__ uint32_t k_place(uint32_t r, uint32_t c) { return c ^ (r & 15); }
+    static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) { return c ^ (r >> 2 & 1) << 3; }
 };
+
+// What keys that are not there are read as.
+static __device__ const uint4 g_zeros[64] = {};
 
 // Workgroups of k_prompt that a CU holds, which their registers are limited to.
 constexpr int waves_per_simd(int dp, bool f32) { return dp <= 64 && !f32 ? 3 : dp <= 128 ? 2 : 1; }
 
+// PP: f16 (I8 pages: bf16) parts that a probability is split into.  CAP: capped scores.
 template <typename TQ, typename TC, int DP, int PP, bool CAP>
 __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_prompt(PromptArgs pa) {
     using T = Tile<TC, DP>;
     constexpr bool F32 = T::F32, I8 = T::I8, Q2 = sizeof(TQ) == 4 && !F32;
-    constexpr int KT = T::KT, PITCH = T::PITCH, CH = T::CH, QC = T::QC, LANES = T::LANES;
-    constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave reads at a time, times
+    constexpr int KT = T::KT, PITCH = T::PITCH, LANES = T::LANES, BYTES = KT * PITCH, QC = DP / 16;
+    constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave brings at a time, times
     constexpr float kUp = F32 ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = F32 ? 8.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
-    __shared__ __attribute__((aligned(16))) char lds[4][T::BYTES];   // keys, values of two tiles
-    char (*const lds_k)[T::BYTES] = lds, (*const lds_v)[T::BYTES] = lds + 2;
+    // keys and values of one tile each; two arrays, so that reads of one are known to be apart from what is on its way into the other
+    __shared__ __attribute__((aligned(16))) char lds0[2 * BYTES];
+    __shared__ __attribute__((aligned(16))) char lds1[2 * BYTES];
     __shared__ __attribute__((aligned(16))) float lds_s[2][2][I8 ? KT : 4];
     __shared__ int32_t lds_ext[4][4];
     __shared__ float lds_pair[2 * 64 * 2];
@@ -257,7 +244,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     uint32_t x = pa.tiles - 1 - blockIdx.x / a.hkv, p = 0;
     Piece piece;
     if (pa.deal) {
-        if (!piece.find<KT>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds), &x, &p)) return;
+        if (!piece.find<KT>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds0), &x, &p)) return;
     } else {
         // the request (group) p whose tiles x lies among
         for (uint32_t width = pa.n_start;;) {                // p among [p, p + width)
@@ -383,54 +370,93 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         mul = 1.0f;
     }
 
-    // a tile's pages: of key lane % KT of it; what the wave stages of it
+    // places that nothing is brought to hold zeros
+    if (a.D * sizeof(TC) != LANES * 16) {
+        for (uint32_t i = tid; i < 2 * BYTES / 16; i += 256) reinterpret_cast<u4v*>(lds0)[i] = reinterpret_cast<u4v*>(lds1)[i] = u4v{};
+        __syncthreads();
+    }
+
+    // A tile on its way to LDS.  Each lane looks its key lane % KT up and works out where it lies, the lanes that bring it ask for that:
+    // where the rows that they bring together lie in one page, at an offset of the wave's and one of their own that stays.  Keys that
+    // are not there are brought from a row of zeros.
     const int32_t* table = reinterpret_cast<const int32_t*>(a.tables + seq * a.t_nb1);
     auto look_up = [&](uint32_t tile) { return table[min(page_of(a, tile * KT + (lane & (KT - 1))), a.max_pages - 1)]; };
-    u4v rk[NI], rv[NI];
+    u4v rk[I8 ? NI : 1], rv[I8 ? NI : 1];
     float rs = 0.0f;
     uint64_t have = 0, have_next = 0;                        // keys of the tile that are there
+    constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
     const uint32_t sub_row = lane / LANES, sub_c = lane % LANES;
-    const bool sub_in = sub_c * T::PER < a.D;
-    auto fetch = [&](uint32_t tile, int32_t pg) {
+    const char *kb = a.k + hk * a.k_nb2, *vb = a.v + hk * a.v_nb2;
+    const bool together = a.page % RPI == 0;
+    auto fetch = [&](uint32_t tile, int32_t pg, char* to) __attribute__((always_inline)) {
         const uint32_t key = tile * KT + (lane & (KT - 1));
         const bool in = key < static_cast<uint32_t>(end) && key >= static_cast<uint32_t>(begin);
         const bool good = static_cast<uint32_t>(pg) < a.n_pages;
         wrong |= in && !good;
-        have_next = __ballot(in && good);
-        if constexpr (KT == 32) have_next &= 0xffffffffull;
-        const int64_t pl = in && good ? pg : 0, at = in && good ? key - page_of(a, key) * a.page : 0;
-        const uint64_t ko = static_cast<uint64_t>(pl * a.k_nb3 + at * a.k_nb1), vo = static_cast<uint64_t>(pl * a.v_nb3 + at * a.v_nb1);
-        const char* kb = a.k + hk * a.k_nb2 + (sub_in ? sub_c : 0) * 16;
-        const char* vb = a.v + hk * a.v_nb2 + (sub_in ? sub_c : 0) * 16;
+        have_next = __ballot(in && good) & ALL;
+        const uint32_t at = key - page_of(a, key) * a.page;
+        uint64_t ko = static_cast<uint64_t>(pg * a.k_nb3 + at * a.k_nb1), vo = static_cast<uint64_t>(pg * a.v_nb3 + at * a.v_nb1);
+        typedef __attribute__((address_space(3))) void lds_void;
+        typedef const __attribute__((address_space(1))) void global_void;
+        char* l = to + wid * NI * 1024;
+        if (!I8 && together && have_next == ALL) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int src = wid * (KT / 4) + i * RPI;
+                const uint32_t row = src + sub_row;
+                auto of = [&](uint64_t o) {
+                    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o)), src);
+                    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o >> 32)), src);
+                    return static_cast<uint64_t>(hi) << 32 | lo;
+                };
+                const uint32_t kc = T::k_place(row, sub_c), vc = T::v_place(row, sub_c);
+                const char *kw = kb + of(ko), *vw = vb + of(vo);
+                const uint32_t kl = sub_row * static_cast<uint32_t>(a.k_nb1) + kc * 16, vl = sub_row * static_cast<uint32_t>(a.v_nb1) + vc * 16;
+                if (kc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(kw + kl), (lds_void*)(l + i * 1024), 16, 0, 0);
+                if (vc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(vw + vl), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
+            }
+            return;
+        }
+        if (!in || !good) {
+            ko = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(kb);
+            vo = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(vb);
+        }
 #pragma unroll
         for (int i = 0; i < NI; i++) {
-            const int src = wid * (KT / 4) + i * RPI + sub_row;
+            const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
             auto of = [&](uint64_t o) {
-                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), src), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), src);
+                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), row), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), row);
                 return static_cast<uint64_t>(hi) << 32 | lo;
             };
-            rk[i] = *reinterpret_cast<const u4v*>(kb + of(ko));
-            rv[i] = *reinterpret_cast<const u4v*>(vb + of(vo));
+            const char *kw = kb + of(ko), *vw = vb + of(vo);
+            if constexpr (I8) {
+                const uint32_t c = sub_c * T::PER < a.D ? sub_c * 16 : 0;
+                rk[i] = *reinterpret_cast<const u4v*>(kw + c);
+                rv[i] = *reinterpret_cast<const u4v*>(vw + c);
+            } else {
+                const uint32_t kc = T::k_place(row, sub_c), vc = T::v_place(row, sub_c);
+                if (kc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(kw + kc * 16), (lds_void*)(l + i * 1024), 16, 0, 0);
+                if (vc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(vw + vc * 16), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
+            }
         }
         if constexpr (I8) {
             if (wid < 2 && in && good) {
-                const char* sp = wid == 0 ? a.ks + pl * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0
-                                          : a.vs + pl * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0;
+                const char* sp = wid == 0 ? a.ks + pg * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0
+                                          : a.vs + pg * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0;
                 rs = *reinterpret_cast<const float*>(sp);
             } else {
                 rs = 0.0f;
             }
         }
     };
-    // into LDS: keys that are not there and dims past D as zeros
+    // The tile in LDS, as far as this wave brings it.  Edge tiles, some of whose keys some rows do not have: values that are no numbers
+    // are found there, and cleared once `clean`.
     bool clean = false, bad = false;
-    auto put = [&](int buf, bool edge) {
-        const bool some = have_next != (KT == 64 ? ~0ull : 0xffffffffull) || a.D != DP;   // not all of it is brought
+    auto arrive = [&](char* to, int buf, bool edge) __attribute__((always_inline)) {
+        if constexpr (I8) {
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
-            if (some && (!sub_in || !(have_next >> row & 1))) rk[i] = rv[i] = u4v{};
-            if constexpr (I8) {
+            for (int i = 0; i < NI; i++) {
+                const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
                 u4v k0, k1, v0, v1;
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
@@ -449,36 +475,40 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                                                                     __builtin_bit_cast(uint32_t, fv[2 * b]), 0x07060302u);
                     }
                 }
-                if (2 * sub_c < CH) {
-                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, 2 * sub_c) * 16) = k0;
-                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
-                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, 2 * sub_c) * 16) = v0;
-                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
-                }
-            } else {
-                if (edge) {
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t y = rv[i][w];
-                        if constexpr (F32) {
-                            const bool no = (y & 0x7f800000u) == 0x7f800000u;
-                            bad |= no;
-                            if (clean) rv[i][w] = no ? 0u : y;
-                            continue;
-                        }
-                        const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
-                        bad |= lo || hi;
-                        if (clean) rv[i][w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
-                    }
-                }
-                if (sub_c < CH) {
-                    *reinterpret_cast<u4v*>(lds_k[buf] + row * PITCH + T::k_place(row, sub_c) * 16) = rk[i];
-                    *reinterpret_cast<u4v*>(lds_v[buf] + row * PITCH + T::v_place(row, sub_c) * 16) = rv[i];
+                if (sub_c * T::PER < a.D) {
+                    char *lk = to + row * PITCH, *lv = lk + BYTES;
+                    *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c) * 16) = k0;
+                    *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
+                    *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c) * 16) = v0;
+                    *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
                 }
             }
-        }
-        if constexpr (I8) {
             if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
+        } else {
+            wait_vector_memory();                            // what this wave brings to LDS
+            if (edge) {
+#pragma unroll 1
+                for (int i = 0; i < NI; i++) {
+                    u4v* at = reinterpret_cast<u4v*>(to + BYTES + (wid * NI + i) * 1024 + lane * 16);
+                    u4v v = *at;
+                    bool any = false;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t y = v[w];
+                        if constexpr (F32) {
+                            const bool no = (y & 0x7f800000u) == 0x7f800000u;
+                            any |= no;
+                            v[w] = no ? 0u : y;
+                        } else {
+                            const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
+                            any |= lo || hi;
+                            v[w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
+                        }
+                    }
+                    bad |= any;
+                    if (clean && any) *at = v;
+                }
+            }
         }
     };
 
@@ -491,8 +521,9 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     const uint32_t l16 = lane & 15, v_key = 4 * half + l16 / 4, v_c = 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
     const uint32_t v_at = v_key * PITCH + (l16 & 1) * 8;
 
-    auto add_values = [&](int buf, int sub, const f16v& s) { // O^T += V^T P^T over 32 keys
-        const char* lv = lds_v[buf] + sub * 32 * PITCH;
+    // O^T += V^T P^T over 32 keys
+    auto add_values = [&](const char* tile_lds, int sub, const f16v& s) __attribute__((always_inline)) {
+        const char* lv = tile_lds + BYTES + sub * 32 * PITCH;
         if constexpr (F32) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -573,8 +604,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         }
     };
 
-    auto products = [&](int buf, uint32_t kb, int sub) {     // 32 keys
-        const char* lk = lds_k[buf] + sub * 32 * PITCH;
+    auto products = [&](const char* tile_lds, int buf, uint32_t kb, int sub) __attribute__((always_inline)) {   // 32 keys
+        const char* lk = tile_lds + sub * 32 * PITCH;
         f16v s = {};
         if constexpr (F32) {
 #pragma unroll
@@ -672,7 +703,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 for (int u = 0; u < 4; u++) s[e + u] = live >> (e + u) & 1 ? s[e + u] * sc[u] : 0.0f;
             }
         }
-        add_values(buf, sub, s);
+        add_values(tile_lds, sub, s);
     };
 
     // A value that is no number, at a key that some of the rows do not have, would reach these as 0 times it: met at such a tile, the
@@ -688,26 +719,29 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 return static_cast<int32_t>(tile * KT) < every_begin || static_cast<int32_t>(tile * KT + KT) > every_end;
             };
             int32_t pg = look_up(ta);
-            fetch(ta, pg);
+            fetch(ta, pg, lds0);
             pg = look_up(ta + 1);
-            put(0, edge(ta));
+            arrive(lds0, 0, edge(ta));
             have = have_next;
-            for (uint32_t tile = ta; tile < tb; tile++) {
-                const int buf = (tile - ta) & 1;
+            auto step = [&](uint32_t tile, char* cur, char* next, int buf) __attribute__((always_inline)) {
                 const bool more = tile + 1 < tb;
-                __syncthreads();
+                __syncthreads();                             // cur is there, and next is done with
                 if (more) {
-                    fetch(tile + 1, pg);
+                    fetch(tile + 1, pg, next);
                     pg = look_up(tile + 2);
                 }
-#pragma unroll 1
+#pragma unroll
                 for (int sub = 0; sub < KT / 32; sub++) {
-                    const uint32_t kb = tile * KT + 32 * sub;
-                    if (paired && (kb >> 5 & 1) != turn) continue;
-                    if (static_cast<int32_t>(kb) < w_end && static_cast<int32_t>(kb) + 32 > w_begin) products(buf, kb, sub);
+                    const uint32_t k0 = tile * KT + 32 * sub;
+                    if (paired && (k0 >> 5 & 1) != turn) continue;
+                    if (static_cast<int32_t>(k0) < w_end && static_cast<int32_t>(k0) + 32 > w_begin) products(cur, buf, k0, sub);
                 }
-                if (more) put(buf ^ 1, edge(tile + 1));
+                if (more) arrive(next, buf ^ 1, edge(tile + 1));
                 have = have_next;
+            };
+            for (uint32_t tile = ta; tile < tb; tile += 2) {
+                step(tile, lds0, lds1, 0);
+                if (tile + 1 < tb) step(tile + 1, lds1, lds0, 1);
             }
         }
         if constexpr (I8) break;
@@ -716,28 +750,37 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     }
     l += __shfl_xor(l, 32);
     if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
-    if (paired) {                                            // the two waves' parts added up
-        float* part = reinterpret_cast<float*>(lds) + row_wave * (DP / 2 * 64) + lane;
+    if (paired) {                                            // the two waves' parts added up, ND runs of 32 dims at a time
+        constexpr int ND = 2 * BYTES / 8192 < DP / 32 ? 2 * BYTES / 8192 : DP / 32;
+        float* part = reinterpret_cast<float*>(lds0) + row_wave * (ND * 16 * 64) + lane;
         float2* ml = reinterpret_cast<float2*>(lds_pair) + row_wave * 64 + lane;
-        __syncthreads();
-        if (turn == 1) {
-            *ml = make_float2(mc, l);
+        float f0 = 0.0f, f1 = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) {
+        for (int d0 = 0; d0 < DP / 32; d0 += ND) {
+            __syncthreads();
+            if (turn == 1) {
+                *ml = make_float2(mc, l);
 #pragma unroll
-                for (int e = 0; e < 16; e++) part[(16 * d + e) * 64] = o[d][e];
+                for (int d = 0; d < ND && d0 + d < DP / 32; d++) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) part[(16 * d + e) * 64] = o[d0 + d][e];
+                }
             }
-        }
-        __syncthreads();
-        if (turn == 0) {
-            const float2 other = *ml;
-            const float m2 = fmaxf(mc, other.x), f0 = __builtin_amdgcn_exp2f(mc - m2), f1 = __builtin_amdgcn_exp2f(other.x - m2);
-            mc = m2;
-            l = fmaf(l, f0, other.y * f1);
+            __syncthreads();
+            if (turn == 0) {
+                if (d0 == 0) {
+                    const float2 other = *ml;
+                    const float m2 = fmaxf(mc, other.x);
+                    f0 = __builtin_amdgcn_exp2f(mc - m2);
+                    f1 = __builtin_amdgcn_exp2f(other.x - m2);
+                    mc = m2;
+                    l = fmaf(l, f0, other.y * f1);
+                }
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++) {
+                for (int d = 0; d < ND && d0 + d < DP / 32; d++) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[d][e] = fmaf(o[d][e], f0, part[(16 * d + e) * 64] * f1);
+                    for (int e = 0; e < 16; e++) o[d0 + d][e] = fmaf(o[d0 + d][e], f0, part[(16 * d + e) * 64] * f1);
+                }
             }
         }
     }
