@@ -23,7 +23,6 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 128;     // rows of q a workgroup: 4 waves of 32
 
 struct PromptArgs {
     AttnArgs a;
@@ -81,13 +80,13 @@ __device__ __forceinline__ float tanh_of(float x) {
     return copysignf(y < 0.5f ? small : large, x);
 }
 
-// Tiles of kRows rows: those of request (group) p, whose rows are start[p] * g on, are numbered from start[p] * g / kRows + p on,
+// Row tiles: those of request (group) p, whose rows are start[p] * g on, are numbered from start[p] * g / ROWS + p on,
 // which is one more than it needs at most, so that a tile is found without a sum over the requests before it.
 __device__ __forceinline__ uint32_t start_of(const AttnArgs& a, uint32_t p) {
     const int32_t t = a.start[p];
     return t < 0 ? 0u : min(static_cast<uint32_t>(t), a.n_rows);
 }
-__device__ __forceinline__ uint32_t first_tile(const AttnArgs& a, uint32_t start, uint32_t p) { return start * a.g / kRows + p; }
+template <int ROWS> __device__ __forceinline__ uint32_t first_tile(const AttnArgs& a, uint32_t start, uint32_t p) { return start * a.g / ROWS + p; }
 
 // Few row tiles: their keys are cut into pieces of one size, so that about `deal` workgroups have one each whatever the lengths, which
 // only the device knows.  Every workgroup counts the key tiles of all row tiles for itself.
@@ -96,7 +95,7 @@ struct Piece {
     uint32_t first = 0, count = 1, at = 0;      // the row tile's first piece, how many it has, which of them
     uint32_t tile0 = 0, tiles = 0;              // key tiles
 
-    template <int KT> __device__ __forceinline__ bool find(const PromptArgs& pa, uint32_t q, uint32_t* lds, uint32_t* x, uint32_t* p) {
+    template <int KT, int ROWS> __device__ __forceinline__ bool find(const PromptArgs& pa, uint32_t q, uint32_t* lds, uint32_t* x, uint32_t* p) {
         const AttnArgs& a = pa.a;
         constexpr int N = kDealTiles / 256;
         __shared__ uint32_t sums[4], found[6];
@@ -113,12 +112,12 @@ struct Piece {
             uint32_t lo = 0, hi = pa.n_start;                // the last one whose tiles start at or before xi
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) / 2;
-                if (first_tile(a, lds[mid], mid) <= xi) lo = mid;
+                if (first_tile<ROWS>(a, lds[mid], mid) <= xi) lo = mid;
                 else hi = mid;
             }
-            const uint32_t t0 = lds[lo], t1 = lds[lo + 1], base = first_tile(a, t0, lo);
-            if (xi < base || t1 <= t0 || (xi - base) * kRows >= (t1 - t0) * a.g) continue;
-            const uint32_t row0 = (xi - base) * kRows, row1 = min(row0 + kRows, (t1 - t0) * a.g) - 1;
+            const uint32_t t0 = lds[lo], t1 = lds[lo + 1], base = first_tile<ROWS>(a, t0, lo);
+            if (xi < base || t1 <= t0 || static_cast<uint64_t>(xi - base) * ROWS >= static_cast<uint64_t>(t1 - t0) * a.g) continue;
+            const uint32_t row0 = (xi - base) * ROWS, row1 = min(row0 + ROWS, (t1 - t0) * a.g) - 1;
             const int32_t cap = static_cast<int32_t>(a.max_pages * a.page);
             int32_t first = 0, end;
             if (pa.shared) {
@@ -215,19 +214,35 @@ template <int DP> struct Tile<float, DP> {
     static __device__ __forceinline__ uint32_t v_place(uint32_t r, uint32_t c) { return c ^ (r >> 2 & 1) << 3; }
 };
 
+// A value made anew where it is asked for: what rare paths and the end work out again would else be kept, in registers, through the
+// loop over the keys.
+template <typename V> __device__ __forceinline__ V anew(V v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// The kernel's arguments read again, likewise.
+typedef const __attribute__((address_space(4))) PromptArgs const_args;
+__device__ __forceinline__ const_args* args_anew() {
+    const_args* p = (const_args*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // What keys that are not there are read as.
 static __device__ const uint4 g_zeros[64] = {};
 
 // Workgroups of k_prompt that a CU holds, which their registers are limited to.
 constexpr int waves_per_simd(int dp, bool f32) { return dp <= 64 && !f32 ? 3 : dp <= 128 ? 2 : 1; }
 
-// PP: f16 (I8 pages: bf16) parts that a probability is split into.  CAP: capped scores.
-template <typename TQ, typename TC, int DP, int PP, bool CAP>
+// PP: f16 (I8 pages: bf16) parts that a probability is split into.  CAP: capped scores.  PAIR: two waves share 32 rows, each with every
+// other run of 32 keys (64 rows a workgroup); else each wave has 32 rows and all keys (128).
+template <typename TQ, typename TC, int DP, int PP, bool CAP, bool PAIR>
 __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_prompt(PromptArgs pa) {
     using T = Tile<TC, DP>;
     constexpr bool F32 = T::F32, I8 = T::I8, Q2 = sizeof(TQ) == 4 && !F32;
-    constexpr int KT = T::KT, PITCH = T::PITCH, LANES = T::LANES, BYTES = KT * PITCH, QC = DP / 16;
+    constexpr int ROWS = PAIR ? 64 : 128, KT = T::KT, PITCH = T::PITCH, LANES = T::LANES, BYTES = KT * PITCH, QC = DP / 16;
     constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave brings at a time, times
+    constexpr int NS = PAIR || KT == 32 || Q2 || DP == 64 ? 1 : 2;   // runs of 32 keys taken together
     constexpr float kUp = F32 ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = F32 ? 8.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
     // keys and values of one tile each; two arrays, so that reads of one are known to be apart from what is on its way into the other
@@ -241,79 +256,111 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 
     // this workgroup's key head, row tile (undealt: the last rows, which have the most keys, first) and piece of its keys
     const uint32_t hk = blockIdx.x % a.hkv;
-    uint32_t x = pa.tiles - 1 - blockIdx.x / a.hkv, p = 0;
+    uint32_t x = pa.tiles - 1 - blockIdx.x / a.hkv, p = 0, t0, t1;
+    int32_t given = 0;                                       // the request's length
     Piece piece;
     if (pa.deal) {
-        if (!piece.find<KT>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds0), &x, &p)) return;
+        if (!piece.find<KT, ROWS>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds0), &x, &p)) return;
+        t0 = start_of(a, p);
+        t1 = start_of(a, p + 1);
+        if (!pa.shared) given = a.lens[p];
     } else {
-        // the request (group) p whose tiles x lies among
+        // the request p whose tiles x lies among; what is read with it in one go: where it and the next one start, and its length
         for (uint32_t width = pa.n_start;;) {                // p among [p, p + width)
-            const uint32_t step = (width + 63) / 64, q = p + lane * step;
-            const bool in = lane * step < width && first_tile(a, start_of(a, q), q) <= x;
+            const uint32_t step = (width + 63) / 64, q = min(p + lane * step, pa.n_start - 1);
+            const uint32_t from = start_of(a, q), to = start_of(a, q + 1);
+            const int32_t len = a.lens[q];
+            const bool in = lane * step < width && first_tile<ROWS>(a, from, q) <= x;
             const uint32_t at = 64 - __builtin_clzll(__ballot(in) | 1) - 1;
             p = __builtin_amdgcn_readfirstlane(p + at * step);
             width = min(step, width - min(width, at * step));
+            t0 = __builtin_amdgcn_readlane(static_cast<int>(from), at);
+            t1 = __builtin_amdgcn_readlane(static_cast<int>(to), at);
+            given = __builtin_amdgcn_readlane(len, at);
             if (step == 1) break;
         }
     }
-    const uint32_t t0 = start_of(a, p), t1 = start_of(a, p + 1);
-    const uint32_t base = first_tile(a, t0, p);
-    if (x < base || t1 <= t0 || static_cast<uint64_t>(x - base) * kRows >= static_cast<uint64_t>(t1 - t0) * a.g) return;
-    const uint32_t row0 = (x - base) * kRows, rows = min(static_cast<uint32_t>(kRows), (t1 - t0) * a.g - row0);
-    // 64 rows or fewer: two waves a row, for every other run of 32 keys
-    const bool paired = rows <= 64;
-    const uint32_t row_wave = paired ? wid & 1 : wid, turn = wid >> 1;
+    const uint32_t base = first_tile<ROWS>(a, t0, p);
+    if (x < base || t1 <= t0 || static_cast<uint64_t>(x - base) * ROWS >= static_cast<uint64_t>(t1 - t0) * a.g) return;
+    const uint32_t row0 = (x - base) * ROWS, rows = min(static_cast<uint32_t>(ROWS), (t1 - t0) * a.g - row0);
+    const uint32_t row_wave = PAIR ? wid & 1 : wid, turn = wid >> 1;
 
-    // the lane's row: token or request t, head, keys [first, limit)
-    const uint32_t r = row_wave * 32 + n;
-    const bool live_row = r < rows;
-    const uint32_t ri = row0 + (live_row ? r : 0);
-    const uint32_t j = static_cast<uint32_t>((static_cast<uint64_t>(ri) * pa.g_mul) >> pa.g_shift);
-    const uint32_t t = t0 + j, hq = hk * a.g + (ri - j * a.g);
+    // the lane's row: row r of the tile, of token or request t and query head hq, keys [first, limit)
     const int32_t cap = static_cast<int32_t>(a.max_pages * a.page);
-    bool wrong = false;
+    auto row_of = [&](uint32_t r, uint32_t* t, uint32_t* hq) {
+        const uint32_t ri = row0 + (r < rows ? r : 0), j = static_cast<uint32_t>((static_cast<uint64_t>(ri) * pa.g_mul) >> pa.g_shift);
+        *t = t0 + j;
+        *hq = hk * a.g + (ri - j * a.g);
+    };
+    const bool live_row = row_wave * 32 + n < rows;
+    bool wrong;
     int32_t limit, first;
-    uint32_t seq;                                            // whose table
-    {
-        seq = pa.shared ? t0 : p;
-        const int32_t given = a.lens[pa.shared ? t : p];
+    // keys that any row of the workgroup has, that all of them have; those of the wave's rows
+    int32_t begin, end, every_begin, every_end, w_begin, w_end, all_begin, all_end;
+    const uint32_t seq = pa.shared ? t0 : p;                 // whose table
+    const uint32_t lane_row = live_row ? row_wave * 32 + n : rows - 1;
+    auto first_of = [&](int32_t lim) { return a.window > 0 && lim > a.window ? lim - a.window : 0; };
+    if (pa.shared) {
+        uint32_t t, hq;
+        row_of(lane_row, &t, &hq);
+        given = a.lens[t];
         wrong = given < 0 || given > cap;
-        const int32_t len = min(max(given, 0), cap);
-        if (pa.shared) {
-            const int32_t pre = min(max(pa.shared[p], 0), cap);
-            first = a.window > 0 && len > a.window ? len - a.window : 0;
-            limit = min(len, pre);
-            if (hk == 0 && piece.at == 0 && half == 0 && live_row && wid == row_wave) pa.own_first[t] = limit;
-        } else {
-            limit = max(0, len - static_cast<int32_t>(t1 - 1 - t));
-            first = a.window > 0 && limit > a.window ? limit - a.window : 0;
-        }
+        const int32_t len = min(max(given, 0), cap), pre = min(max(pa.shared[p], 0), cap);
+        first = first_of(len);
+        limit = min(len, pre);
+        if (hk == 0 && piece.at == 0 && half == 0 && live_row && wid == row_wave) pa.own_first[t] = limit;
         if (!live_row) limit = first = 0;
-    }
-    // the wave's rows: keys that any of them has, that all of them have
-    int32_t w_end = limit, w_begin = limit > first ? first : 0x7fffffff, all_end = live_row ? limit : 0x7fffffff, all_begin = first;
+        w_end = limit;
+        w_begin = limit > first ? first : 0x7fffffff;
+        all_end = live_row ? limit : 0x7fffffff;
+        all_begin = first;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        w_end = max(w_end, __shfl_xor(w_end, d));
-        w_begin = min(w_begin, __shfl_xor(w_begin, d));
-        all_end = min(all_end, __shfl_xor(all_end, d));
-        all_begin = max(all_begin, __shfl_xor(all_begin, d));
+        for (int d = 1; d < 32; d *= 2) {
+            w_end = max(w_end, __shfl_xor(w_end, d));
+            w_begin = min(w_begin, __shfl_xor(w_begin, d));
+            all_end = min(all_end, __shfl_xor(all_end, d));
+            all_begin = max(all_begin, __shfl_xor(all_begin, d));
+        }
+        w_end = __builtin_amdgcn_readfirstlane(w_end);
+        w_begin = __builtin_amdgcn_readfirstlane(w_begin);
+        all_end = __builtin_amdgcn_readfirstlane(all_end);
+        all_begin = __builtin_amdgcn_readfirstlane(all_begin);
+        if (lane == 0) {
+            lds_ext[0][wid] = w_end;
+            lds_ext[1][wid] = w_begin;
+            lds_ext[2][wid] = all_end;
+            lds_ext[3][wid] = all_begin;
+        }
+        __syncthreads();
+        end = max(max(lds_ext[0][0], lds_ext[0][1]), max(lds_ext[0][2], lds_ext[0][3]));
+        begin = min(min(lds_ext[1][0], lds_ext[1][1]), min(lds_ext[1][2], lds_ext[1][3]));
+        every_end = min(min(lds_ext[2][0], lds_ext[2][1]), min(lds_ext[2][2], lds_ext[2][3]));
+        every_begin = max(max(lds_ext[3][0], lds_ext[3][1]), max(lds_ext[3][2], lds_ext[3][3]));
+    } else {
+        // limits rise with the rows
+        wrong = given < 0 || given > cap;
+        const int32_t len = min(max(given, 0), cap), behind = static_cast<int32_t>(t1 - t0) - 1;
+        auto limit_of = [&](uint32_t r) {
+            return max(0, len - (behind - static_cast<int32_t>((static_cast<uint64_t>(row0 + r) * pa.g_mul) >> pa.g_shift)));
+        };
+        limit = live_row ? limit_of(lane_row) : 0;
+        first = first_of(limit);
+        const uint32_t ra = row_wave * 32, rb = min(ra + 31, rows - 1);
+        every_end = limit_of(0);
+        end = limit_of(rows - 1);
+        begin = first_of(every_end);
+        every_begin = first_of(end);
+        all_end = w_end = 0;
+        all_begin = w_begin = 0;
+        if (ra < rows) {
+            all_end = limit_of(ra);
+            w_end = limit_of(rb);
+            w_begin = first_of(all_end);
+            all_begin = first_of(w_end);
+        }
     }
-    w_end = __builtin_amdgcn_readfirstlane(w_end);
-    w_begin = __builtin_amdgcn_readfirstlane(w_begin);
-    all_end = __builtin_amdgcn_readfirstlane(all_end);
-    all_begin = __builtin_amdgcn_readfirstlane(all_begin);
-    if (lane == 0) {
-        lds_ext[0][wid] = w_end;
-        lds_ext[1][wid] = w_begin;
-        lds_ext[2][wid] = all_end;
-        lds_ext[3][wid] = all_begin;
-    }
-    __syncthreads();
-    const int32_t end = max(max(lds_ext[0][0], lds_ext[0][1]), max(lds_ext[0][2], lds_ext[0][3]));
-    const int32_t begin = min(min(min(lds_ext[1][0], lds_ext[1][1]), min(lds_ext[1][2], lds_ext[1][3])), end);
-    const int32_t every_end = min(min(lds_ext[2][0], lds_ext[2][1]), min(lds_ext[2][2], lds_ext[2][3]));
-    const int32_t every_begin = max(max(lds_ext[3][0], lds_ext[3][1]), max(lds_ext[3][2], lds_ext[3][3]));
+    begin = __builtin_amdgcn_readfirstlane(min(begin, end));
+    end = __builtin_amdgcn_readfirstlane(end);
     const uint32_t tile0 = static_cast<uint32_t>(begin) / KT, n_tiles = (static_cast<uint32_t>(end) + KT - 1) / KT - tile0;
     uint32_t ta = tile0, tb = tile0 + n_tiles;
     if (pa.deal) {
@@ -323,6 +370,150 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     ta = __builtin_amdgcn_readfirstlane(ta);
     tb = __builtin_amdgcn_readfirstlane(tb);
 
+    // A tile on its way to LDS.  Each lane looks its key lane % KT up and works out where it lies, the lanes that bring it ask for that:
+    // where the rows that they bring together lie in one page, at an offset of the wave's and one of their own that stays.  Keys that
+    // are not there are brought from a row of zeros; the places of dims past D get the row's first ones again, which the query meets with
+    // zeros and whose sums of values nobody asks for.
+    const int32_t* table = reinterpret_cast<const int32_t*>(a.tables + seq * a.t_nb1);
+    auto look_up = [&](uint32_t tile) { return table[min(page_of(a, tile * KT + (lane & (KT - 1))), a.max_pages - 1)]; };
+    u4v rk[I8 ? NI : 1], rv[I8 ? NI : 1];
+    float rs = 0.0f;
+    uint64_t have = 0, have_next = 0;                        // keys of the tile that are there
+    constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
+    const uint32_t sub_row = lane / LANES, sub_c = lane % LANES;
+    const char *kb = a.k + hk * a.k_nb2, *vb = a.v + hk * a.v_nb2;
+    const bool together = a.page % RPI == 0;
+    auto chunk = [&](uint32_t c) { return c * T::PER < a.D ? c * 16 : 0; };
+    auto fetch = [&](uint32_t tile, int32_t pg, char* to) __attribute__((always_inline)) {
+        const uint32_t key = tile * KT + (lane & (KT - 1));
+        const bool in = key < static_cast<uint32_t>(end) && key >= static_cast<uint32_t>(begin);
+        const bool good = static_cast<uint32_t>(pg) < a.n_pages;
+        wrong |= in && !good;
+        have_next = __ballot(in && good) & ALL;
+        const uint32_t at = key - page_of(a, key) * a.page;
+        uint64_t ko = static_cast<uint64_t>(pg * a.k_nb3 + at * a.k_nb1), vo = static_cast<uint64_t>(pg * a.v_nb3 + at * a.v_nb1);
+        typedef __attribute__((address_space(3))) void lds_void;
+        typedef const __attribute__((address_space(1))) void global_void;
+        char* l = to + wid * NI * 1024;
+        if (!I8 && together && have_next == ALL) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int src = wid * (KT / 4) + i * RPI;
+                const uint32_t row = src + sub_row;
+                auto of = [&](uint64_t o) {
+                    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o)), src);
+                    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o >> 32)), src);
+                    return static_cast<uint64_t>(hi) << 32 | lo;
+                };
+                const char *kw = kb + of(ko), *vw = vb + of(vo);
+                asm volatile("" : "+s"(kw), "+s"(vw));       // bases of the wave's, the lane's offset beside them
+                const uint32_t kl = sub_row * static_cast<uint32_t>(a.k_nb1) + chunk(T::k_place(row, sub_c));
+                const uint32_t vl = sub_row * static_cast<uint32_t>(a.v_nb1) + chunk(T::v_place(row, sub_c));
+                __builtin_amdgcn_global_load_lds((global_void*)(kw + kl), (lds_void*)(l + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(vw + vl), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
+            }
+            return;
+        }
+        if (!in || !good) {
+            ko = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(kb);
+            vo = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(vb);
+        }
+        const uint32_t lane1 = I8 ? lane : anew(lane), sub_row = lane1 / LANES, sub_c = lane1 % LANES;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
+            auto of = [&](uint64_t o) {
+                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), row), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), row);
+                return static_cast<uint64_t>(hi) << 32 | lo;
+            };
+            const char *kw = kb + of(ko), *vw = vb + of(vo);
+            if constexpr (I8) {
+                rk[i] = *reinterpret_cast<const u4v*>(kw + chunk(sub_c));
+                rv[i] = *reinterpret_cast<const u4v*>(vw + chunk(sub_c));
+            } else {
+                __builtin_amdgcn_global_load_lds((global_void*)(kw + chunk(T::k_place(row, sub_c))), (lds_void*)(l + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((global_void*)(vw + chunk(T::v_place(row, sub_c))), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
+            }
+        }
+        if constexpr (I8) {
+            if (wid < 2 && in && good) {
+                const char* sp = wid == 0 ? a.ks + pg * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0
+                                          : a.vs + pg * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0;
+                rs = *reinterpret_cast<const float*>(sp);
+            } else {
+                rs = 0.0f;
+            }
+        }
+    };
+    // The tile in LDS, as far as this wave brings it.  Edge tiles, some of whose keys some rows do not have: values that are no numbers
+    // are found there, and cleared once `clean`.
+    bool clean = false, bad = false;
+    auto arrive = [&](char* to, int buf, bool edge) __attribute__((always_inline)) {
+        if constexpr (I8) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
+                u4v k0, k1, v0, v1;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    float fk[4], fv[4];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        fk[b] = static_cast<float>(static_cast<int8_t>(rk[i][w] >> 8 * b));
+                        fv[b] = static_cast<float>(static_cast<int8_t>(rv[i][w] >> 8 * b));
+                    }
+                    u4v& kk = w < 2 ? k0 : k1;
+                    u4v& vv = w < 2 ? v0 : v1;
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        kk[2 * (w & 1) + b] = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(fk[2 * b]), static_cast<_Float16>(fk[2 * b + 1])});
+                        vv[2 * (w & 1) + b] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fv[2 * b + 1]),
+                                                                    __builtin_bit_cast(uint32_t, fv[2 * b]), 0x07060302u);
+                    }
+                }
+                char *lk = to + row * PITCH, *lv = lk + BYTES;
+                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c) * 16) = k0;
+                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
+                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c) * 16) = v0;
+                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
+            }
+            if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
+        } else {
+            wait_vector_memory();                            // what this wave brings to LDS
+            if (edge) {
+#pragma unroll 1
+                for (int i = 0; i < NI; i++) {
+                    u4v* at = reinterpret_cast<u4v*>(to + BYTES + (wid * NI + i) * 1024 + anew(lane) * 16);
+                    u4v v = *at;
+                    bool any = false;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t y = v[w];
+                        if constexpr (F32) {
+                            const bool no = (y & 0x7f800000u) == 0x7f800000u;
+                            any |= no;
+                            v[w] = no ? 0u : y;
+                        } else {
+                            const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
+                            any |= lo || hi;
+                            v[w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
+                        }
+                    }
+                    bad |= any;
+                    if (clean && any) *at = v;
+                }
+            }
+        }
+    };
+
+    // the first tile is on its way while the query is read
+    int32_t pg = 0, pg1 = 0;
+    if (ta < tb) {
+        pg = look_up(ta);
+        pg1 = look_up(ta + 1);
+        fetch(ta, pg, lds0);
+    }
+
     // the lane's query: dims 16 c + 8 half + [0, 8), for F32 pages 8 c + 4 half + [0, 4).  Else an F32 one is scaled by a power of two to below 2^15 and split into two f16, the
     // lower times 2^12 and summed apart
     h8v qh[F32 ? 1 : QC], ql[Q2 ? QC : 1];
@@ -330,6 +521,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     float mul = fabsf(a.scale) * kLog2e;
     {
         float v[QC * 8];
+        uint32_t t, hq;
+        row_of(row_wave * 32 + n, &t, &hq);
         const char* qr = a.q + t * a.q_nb2 + hq * a.q_nb1;
 #pragma unroll
         for (int i = 0; i < QC * 8; i += 4) {
@@ -369,148 +562,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         cap_in = mul / kLog2e / a.softcap;
         mul = 1.0f;
     }
-
-    // places that nothing is brought to hold zeros
-    if (a.D * sizeof(TC) != LANES * 16) {
-        for (uint32_t i = tid; i < 2 * BYTES / 16; i += 256) reinterpret_cast<u4v*>(lds0)[i] = reinterpret_cast<u4v*>(lds1)[i] = u4v{};
-        __syncthreads();
-    }
-
-    // A tile on its way to LDS.  Each lane looks its key lane % KT up and works out where it lies, the lanes that bring it ask for that:
-    // where the rows that they bring together lie in one page, at an offset of the wave's and one of their own that stays.  Keys that
-    // are not there are brought from a row of zeros.
-    const int32_t* table = reinterpret_cast<const int32_t*>(a.tables + seq * a.t_nb1);
-    auto look_up = [&](uint32_t tile) { return table[min(page_of(a, tile * KT + (lane & (KT - 1))), a.max_pages - 1)]; };
-    u4v rk[I8 ? NI : 1], rv[I8 ? NI : 1];
-    float rs = 0.0f;
-    uint64_t have = 0, have_next = 0;                        // keys of the tile that are there
-    constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
-    const uint32_t sub_row = lane / LANES, sub_c = lane % LANES;
-    const char *kb = a.k + hk * a.k_nb2, *vb = a.v + hk * a.v_nb2;
-    const bool together = a.page % RPI == 0;
-    auto fetch = [&](uint32_t tile, int32_t pg, char* to) __attribute__((always_inline)) {
-        const uint32_t key = tile * KT + (lane & (KT - 1));
-        const bool in = key < static_cast<uint32_t>(end) && key >= static_cast<uint32_t>(begin);
-        const bool good = static_cast<uint32_t>(pg) < a.n_pages;
-        wrong |= in && !good;
-        have_next = __ballot(in && good) & ALL;
-        const uint32_t at = key - page_of(a, key) * a.page;
-        uint64_t ko = static_cast<uint64_t>(pg * a.k_nb3 + at * a.k_nb1), vo = static_cast<uint64_t>(pg * a.v_nb3 + at * a.v_nb1);
-        typedef __attribute__((address_space(3))) void lds_void;
-        typedef const __attribute__((address_space(1))) void global_void;
-        char* l = to + wid * NI * 1024;
-        if (!I8 && together && have_next == ALL) {
-#pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const int src = wid * (KT / 4) + i * RPI;
-                const uint32_t row = src + sub_row;
-                auto of = [&](uint64_t o) {
-                    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o)), src);
-                    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(static_cast<uint32_t>(o >> 32)), src);
-                    return static_cast<uint64_t>(hi) << 32 | lo;
-                };
-                const uint32_t kc = T::k_place(row, sub_c), vc = T::v_place(row, sub_c);
-                const char *kw = kb + of(ko), *vw = vb + of(vo);
-                const uint32_t kl = sub_row * static_cast<uint32_t>(a.k_nb1) + kc * 16, vl = sub_row * static_cast<uint32_t>(a.v_nb1) + vc * 16;
-                if (kc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(kw + kl), (lds_void*)(l + i * 1024), 16, 0, 0);
-                if (vc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(vw + vl), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
-            }
-            return;
-        }
-        if (!in || !good) {
-            ko = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(kb);
-            vo = reinterpret_cast<uintptr_t>(g_zeros) - reinterpret_cast<uintptr_t>(vb);
-        }
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
-            auto of = [&](uint64_t o) {
-                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), row), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), row);
-                return static_cast<uint64_t>(hi) << 32 | lo;
-            };
-            const char *kw = kb + of(ko), *vw = vb + of(vo);
-            if constexpr (I8) {
-                const uint32_t c = sub_c * T::PER < a.D ? sub_c * 16 : 0;
-                rk[i] = *reinterpret_cast<const u4v*>(kw + c);
-                rv[i] = *reinterpret_cast<const u4v*>(vw + c);
-            } else {
-                const uint32_t kc = T::k_place(row, sub_c), vc = T::v_place(row, sub_c);
-                if (kc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(kw + kc * 16), (lds_void*)(l + i * 1024), 16, 0, 0);
-                if (vc * T::PER < a.D) __builtin_amdgcn_global_load_lds((global_void*)(vw + vc * 16), (lds_void*)(l + BYTES + i * 1024), 16, 0, 0);
-            }
-        }
-        if constexpr (I8) {
-            if (wid < 2 && in && good) {
-                const char* sp = wid == 0 ? a.ks + pg * a.ks_nb2 + hk * a.ks_nb1 + at * a.ks_nb0
-                                          : a.vs + pg * a.vs_nb2 + hk * a.vs_nb1 + at * a.vs_nb0;
-                rs = *reinterpret_cast<const float*>(sp);
-            } else {
-                rs = 0.0f;
-            }
-        }
-    };
-    // The tile in LDS, as far as this wave brings it.  Edge tiles, some of whose keys some rows do not have: values that are no numbers
-    // are found there, and cleared once `clean`.
-    bool clean = false, bad = false;
-    auto arrive = [&](char* to, int buf, bool edge) __attribute__((always_inline)) {
-        if constexpr (I8) {
-#pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
-                u4v k0, k1, v0, v1;
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    float fk[4], fv[4];
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        fk[b] = static_cast<float>(static_cast<int8_t>(rk[i][w] >> 8 * b));
-                        fv[b] = static_cast<float>(static_cast<int8_t>(rv[i][w] >> 8 * b));
-                    }
-                    u4v& kk = w < 2 ? k0 : k1;
-                    u4v& vv = w < 2 ? v0 : v1;
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        kk[2 * (w & 1) + b] = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(fk[2 * b]), static_cast<_Float16>(fk[2 * b + 1])});
-                        vv[2 * (w & 1) + b] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fv[2 * b + 1]),
-                                                                    __builtin_bit_cast(uint32_t, fv[2 * b]), 0x07060302u);
-                    }
-                }
-                if (sub_c * T::PER < a.D) {
-                    char *lk = to + row * PITCH, *lv = lk + BYTES;
-                    *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c) * 16) = k0;
-                    *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
-                    *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c) * 16) = v0;
-                    *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
-                }
-            }
-            if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
-        } else {
-            wait_vector_memory();                            // what this wave brings to LDS
-            if (edge) {
-#pragma unroll 1
-                for (int i = 0; i < NI; i++) {
-                    u4v* at = reinterpret_cast<u4v*>(to + BYTES + (wid * NI + i) * 1024 + lane * 16);
-                    u4v v = *at;
-                    bool any = false;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t y = v[w];
-                        if constexpr (F32) {
-                            const bool no = (y & 0x7f800000u) == 0x7f800000u;
-                            any |= no;
-                            v[w] = no ? 0u : y;
-                        } else {
-                            const bool lo = (y & 0x7c00u) == 0x7c00u, hi = (y & 0x7c000000u) == 0x7c000000u;
-                            any |= lo || hi;
-                            v[w] = (lo ? 0u : y & 0xffffu) | (hi ? 0u : y & 0xffff0000u);
-                        }
-                    }
-                    bad |= any;
-                    if (clean && any) *at = v;
-                }
-            }
-        }
-    };
+    mul = fmaxf(mul, 0x1p-126f);                             // -inf, the score of a key that a row does not have, stays that
 
     f16v o[DP / 32];
     float m, mc, l;
@@ -521,9 +573,134 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     const uint32_t l16 = lane & 15, v_key = 4 * half + l16 / 4, v_c = 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
     const uint32_t v_at = v_key * PITCH + (l16 & 1) * 8;
 
-    // O^T += V^T P^T over 32 keys
-    auto add_values = [&](const char* tile_lds, int sub, const f16v& s) __attribute__((always_inline)) {
-        const char* lv = tile_lds + BYTES + sub * 32 * PITCH;
+    // NS runs of 32 keys, from the tile's run `sub` on
+    auto products = [&](const char* tile_lds, int buf, uint32_t key0, int sub) __attribute__((always_inline)) {
+        const char* lk = tile_lds + sub * 32 * PITCH;
+        const char* lv = lk + BYTES;
+        f16v s[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) s[i] = f16v{};
+        if constexpr (F32) {
+#pragma unroll
+            for (int c = 0; c < DP / 8; c++) {
+                const f4v kf = *reinterpret_cast<const f4v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
+#pragma unroll
+                for (int u = 0; u < 4; u++) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u], qf[4 * c + u], s[0], 0, 0, 0);
+            }
+        } else {
+            f16v low = {};
+            constexpr int A = 4;                             // reads ahead of their products
+            h8v kf[NS][QC];
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+#pragma unroll
+                for (int c = 0; c < QC; c++) kf[i][c] = *reinterpret_cast<const h8v*>(lk + i * 32 * PITCH + k_row + T::k_place(n, 2 * c + half) * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+#pragma unroll
+                for (int c = 0; c < QC; c++) {
+                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i][c], qh[c], s[i], 0, 0, 0);
+                    if constexpr (Q2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i][c], ql[c], low, 0, 0, 0);
+                }
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+            for (int c = 0; c < NS * QC; c++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, Q2 ? 2 : 1, 0);
+                if (c + A < NS * QC) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            if constexpr (Q2) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[0][e] = fmaf(low[e], 0x1p-12f, s[0][e]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            if constexpr (I8) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][0][32 * (sub + i) + 2 * e + 4 * half]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) s[i][e + u] *= sc[u];
+                }
+            }
+            if constexpr (CAP) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[i][e] = tanh_of(s[i][e] * cap_in) * (a.softcap * kLog2e);
+            }
+        }
+        constexpr uint64_t EACH = NS == 2 ? ~0ull : 0xffffffffull;
+        const uint64_t there = have >> 32 * sub & EACH;
+        const bool whole = static_cast<int32_t>(key0) >= all_begin && static_cast<int32_t>(key0) + 32 * NS <= all_end && there == EACH;
+        // bit 8 (e / 4) + e % 4: the lane's row has the key of its score e in run i
+        auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+        auto has = [&](int i) {
+            const int32_t at = static_cast<int32_t>(key0) + 32 * i + 4 * static_cast<int32_t>(half);
+            return static_cast<uint32_t>(there >> 32 * i) >> 4 * half & below(limit - at) & ~below(first - at);
+        };
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const uint32_t live = has(i);
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[i][e] = live & 1u << (8 * (e / 4) + e % 4) ? s[i][e] : -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int e = i == 0 ? 1 : 0; e < 16; e++) mx = fmaxf(mx, s[i][e]);
+        }
+        auto rises = [&] { return mx > m && (m == kLowest || (mx - m) * mul > kRise); };
+        if (__any(rises())) {                                // rare after the first keys: the row's sums are rescaled
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (rises()) {                                   // of this row alone: its neighbours' keys say nothing about it
+                const float mc2 = fmaf(mx, mul, -kUp);
+                const bool big = fabsf(mc2) >= 0x1p22f;
+                const float keep = far || big ? __builtin_amdgcn_exp2f((m - mx) * mul) : __builtin_amdgcn_exp2f(mc - mc2);
+                far |= big;
+                m = mx;
+                mc = mc2;
+                l *= keep;
+#pragma unroll
+                for (int d = 0; d < DP / 32; d++) o[d] *= keep;
+            }
+        }
+        float add = -mc;
+        if (__any(far)) {                                    // the maximum off first
+            const float off = far ? m : 0.0f;
+            add = far ? kUp : add;
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[i][e] -= off;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[i][e] = __builtin_amdgcn_exp2f(fmaf(s[i][e], mul, add));
+            if constexpr (I8 || F32 || PP == 2) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) l += s[i][e];
+            }
+            if constexpr (I8) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][1][32 * (sub + i) + 2 * e + 4 * half]);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) s[i][e + u] *= sc[u];
+                }
+                if (!whole) {                                // the scale of a key that the row does not have may be no number
+                    const uint32_t live = has(i);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[i][e] = live & 1u << (8 * (e / 4) + e % 4) ? s[i][e] : 0.0f;
+                }
+            }
+        }
+        // O^T += V^T P^T
         if constexpr (F32) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -531,42 +708,37 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
                 for (int d = 0; d < DP / 32; d++) {
                     const float v = *reinterpret_cast<const float*>(lv + key * PITCH + T::v_place(4 * half, 8 * d + n / 4) * 16 + n % 4 * 4);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[e], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][e], o[d], 0, 0, 0);
                 }
                 if (e % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // else every value of the 16 keys is held at once
             }
             return;
         }
 #pragma unroll
-        for (int u = 0; u < 2 && !F32; u++) {                // 16 keys
+        for (int u = 0; u < 2 * NS && !F32; u++) {           // 16 keys
+            f16v& su = s[u / 2];
             h8v ph, pl;
-            b8v b0, b1, b2;
+            b8v pb[3];
             if constexpr (I8) {
-                u4v w0, w1, w2;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t part[3][2];
+                for (int k = 0; k < PP; k++) {
+                    u4v w;
 #pragma unroll
-                    for (int z = 0; z < 2; z++) {
-                        float y = s[8 * u + 2 * i + z];
-#pragma unroll
-                        for (int k = 0; k < PP; k++) {
-                            part[k][z] = __builtin_bit_cast(uint32_t, y);
-                            y -= __builtin_bit_cast(float, part[k][z] & 0xffff0000u);
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        const int e = 8 * (u % 2) + 2 * i;
+                        const uint32_t z0 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e])), z1 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e + 1]));
+                        w[i] = __builtin_amdgcn_perm(z1, z0, 0x07060302u);
+                        su[e] -= __builtin_bit_cast(float, z0 & 0xffff0000u);
+                        su[e + 1] -= __builtin_bit_cast(float, z1 & 0xffff0000u);
                     }
-                    w0[i] = __builtin_amdgcn_perm(part[0][1], part[0][0], 0x07060302u);
-                    w1[i] = __builtin_amdgcn_perm(part[1][1], part[1][0], 0x07060302u);
-                    if constexpr (PP == 3) w2[i] = __builtin_amdgcn_perm(part[2][1], part[2][0], 0x07060302u);
+                    pb[k] = __builtin_bit_cast(b8v, w);
                 }
-                b0 = __builtin_bit_cast(b8v, w0);
-                b1 = __builtin_bit_cast(b8v, w1);
-                if constexpr (PP == 3) b2 = __builtin_bit_cast(b8v, w2);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    ph[i] = static_cast<_Float16>(s[8 * u + i]);
-                    if constexpr (PP == 2) pl[i] = static_cast<_Float16>(s[8 * u + i] - static_cast<float>(ph[i]));
+                    const float y = su[8 * (u % 2) + i];
+                    ph[i] = static_cast<_Float16>(y);
+                    if constexpr (PP == 2) pl[i] = static_cast<_Float16>(y - static_cast<float>(ph[i]));
                 }
                 if constexpr (PP == 1) {
 #pragma unroll
@@ -584,126 +756,24 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
             for (int d = 0; d < DP / 32; d++) {
                 if constexpr (I8) {
-                    const b8v vb = __builtin_bit_cast(b8v, vf[d]);
-                    if constexpr (PP == 3) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b2, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b1, o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, b0, o[d], 0, 0, 0);
+#pragma unroll
+                    for (int k = PP - 1; k >= 0; k--) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, vf[d]), pb[k], o[d], 0, 0, 0);
                 } else {
                     if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, o[d], 0, 0, 0);
                 }
             }
         }
-        // the first reads, then a product for every read
-        constexpr int ND = DP / 32 < 4 ? DP / 32 : 4;
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * ND, 0);
+        if constexpr (NS == 1) {
+            // the first reads, then products for every read
+            constexpr int ND = DP / 32 < 4 ? DP / 32 : 4;
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * ND, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * (DP / 32); i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, PP, 0);
-            if (i + ND < 2 * (DP / 32)) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        }
-    };
-
-    auto products = [&](const char* tile_lds, int buf, uint32_t kb, int sub) __attribute__((always_inline)) {   // 32 keys
-        const char* lk = tile_lds + sub * 32 * PITCH;
-        f16v s = {};
-        if constexpr (F32) {
-#pragma unroll
-            for (int c = 0; c < DP / 8; c++) {
-                const f4v kf = *reinterpret_cast<const f4v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
-#pragma unroll
-                for (int u = 0; u < 4; u++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u], qf[4 * c + u], s, 0, 0, 0);
-            }
-        } else {
-            f16v low = {};
-            constexpr int A = 4;                             // reads ahead of their products
-            h8v kf[QC];
-#pragma unroll
-            for (int c = 0; c < QC; c++) kf[c] = *reinterpret_cast<const h8v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
-#pragma unroll
-            for (int c = 0; c < QC; c++) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], qh[c], s, 0, 0, 0);
-                if constexpr (Q2) low = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[c], ql[c], low, 0, 0, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
-#pragma unroll
-            for (int c = 0; c < QC; c++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, Q2 ? 2 : 1, 0);
-                if (c + A < QC) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            if constexpr (Q2) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = fmaf(low[e], 0x1p-12f, s[e]);
+            for (int i = 0; i < 2 * (DP / 32); i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, PP, 0);
+                if (i + ND < 2 * (DP / 32)) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
             }
         }
-        if constexpr (I8) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][0][32 * sub + 2 * e + 4 * half]);
-#pragma unroll
-                for (int u = 0; u < 4; u++) s[e + u] *= sc[u];
-            }
-        }
-        if constexpr (CAP) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = tanh_of(s[e] * cap_in) * (a.softcap * kLog2e);
-        }
-        const uint32_t there = static_cast<uint32_t>(have >> 32 * sub);
-        const bool whole = static_cast<int32_t>(kb) >= all_begin && static_cast<int32_t>(kb) + 32 <= all_end && there == ~0u;
-        uint32_t live = ~0u;                                 // bit e: the row has key e of the lane's
-        if (!whole) {
-            live = 0;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const uint32_t i = 8 * (e / 4) + 4 * half + e % 4;
-                const int32_t key = static_cast<int32_t>(kb + i);
-                if (key < limit && key >= first && (there >> i & 1)) live |= 1u << e;
-                else s[e] = kLowest;
-            }
-        }
-        float mx = fmaxf(s[0], s[1]);
-#pragma unroll
-        for (int e = 2; e < 16; e++) mx = fmaxf(mx, s[e]);
-        auto rises = [&] { return mx > m && (m == kLowest || (mx - m) * mul > kRise); };
-        if (__any(rises())) {                                // rare after the first keys: the row's sums are rescaled
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            if (rises()) {                                   // of this row alone: its neighbours' keys say nothing about it
-                const float mc2 = fmaf(mx, mul, -kUp);
-                const bool big = fabsf(mc2) >= 0x1p22f;
-                const float keep = far || big ? __builtin_amdgcn_exp2f((m - mx) * mul) : __builtin_amdgcn_exp2f(mc - mc2);
-                far |= big;
-                m = mx;
-                mc = mc2;
-                l *= keep;
-#pragma unroll
-                for (int d = 0; d < DP / 32; d++) o[d] *= keep;
-            }
-        }
-        if (__any(far)) {
-            const float off = far ? m : 0.0f, add = far ? kUp : -mc;
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e] - off, mul, add));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -mc));
-        }
-        if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[e] = live >> e & 1 ? s[e] : 0.0f;
-        }
-        if constexpr (I8 || PP == 2) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) l += s[e];
-        }
-        if constexpr (I8) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const f4v sc = *reinterpret_cast<const f4v*>(&lds_s[buf][1][32 * sub + 2 * e + 4 * half]);
-#pragma unroll
-                for (int u = 0; u < 4; u++) s[e + u] = live >> (e + u) & 1 ? s[e + u] * sc[u] : 0.0f;
-            }
-        }
-        add_values(tile_lds, sub, s);
     };
 
     // A value that is no number, at a key that some of the rows do not have, would reach these as 0 times it: met at such a tile, the
@@ -718,10 +788,9 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             auto edge = [&](uint32_t tile) {
                 return static_cast<int32_t>(tile * KT) < every_begin || static_cast<int32_t>(tile * KT + KT) > every_end;
             };
-            int32_t pg = look_up(ta);
-            fetch(ta, pg, lds0);
-            pg = look_up(ta + 1);
+            if (clean) fetch(ta, look_up(ta), lds0);
             arrive(lds0, 0, edge(ta));
+            pg = pg1;
             have = have_next;
             auto step = [&](uint32_t tile, char* cur, char* next, int buf) __attribute__((always_inline)) {
                 const bool more = tile + 1 < tb;
@@ -731,10 +800,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                     pg = look_up(tile + 2);
                 }
 #pragma unroll
-                for (int sub = 0; sub < KT / 32; sub++) {
+                for (int sub = 0; sub < KT / 32; sub += NS) {
                     const uint32_t k0 = tile * KT + 32 * sub;
-                    if (paired && (k0 >> 5 & 1) != turn) continue;
-                    if (static_cast<int32_t>(k0) < w_end && static_cast<int32_t>(k0) + 32 > w_begin) products(cur, buf, k0, sub);
+                    if (PAIR && (k0 >> 5 & 1) != turn) continue;
+                    if (static_cast<int32_t>(k0) < w_end && static_cast<int32_t>(k0) + 32 * NS > w_begin) products(cur, buf, k0, sub);
                 }
                 if (more) arrive(next, buf ^ 1, edge(tile + 1));
                 have = have_next;
@@ -750,7 +819,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     }
     l += __shfl_xor(l, 32);
     if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
-    if (paired) {                                            // the two waves' parts added up, ND runs of 32 dims at a time
+    if constexpr (PAIR) {                                    // the two waves' parts added up, ND runs of 32 dims at a time
         constexpr int ND = 2 * BYTES / 8192 < DP / 32 ? 2 * BYTES / 8192 : DP / 32;
         float* part = reinterpret_cast<float*>(lds0) + row_wave * (ND * 16 * 64) + lane;
         float2* ml = reinterpret_cast<float2*>(lds_pair) + row_wave * 64 + lane;
@@ -784,42 +853,45 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             }
         }
     }
-    const bool mine = live_row && wid == row_wave;
-    const bool to_parts = pa.shared || piece.count > 1;
-    const uint32_t slot = piece.first * a.hkv + hk;          // of the row tile's first piece
-    const uint64_t part = static_cast<uint64_t>(slot + piece.at * a.hkv) * pa.row_cap + r;
-    char* yr = a.y + t * a.y_nb2 + hq * a.y_nb1;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (pa.deal && half == 0 && mine) {
-        if (piece.at == 0) pa.row_parts[static_cast<uint64_t>(t) * a.hq + hq] = make_uint2(slot, piece.count | r << 16);
-        if (to_parts) pa.part_ml[part] = make_float2(mc, l);
-    }
+    if (wid != row_wave) return;
+    const_args& late = *args_anew();
+    const uint32_t lane1 = anew(lane), n1 = lane1 & 31, half1 = lane1 >> 5, r = row_wave * 32 + n1, D = late.a.D;
+    const bool to_parts = late.shared || piece.count > 1;
+    const uint32_t slot = piece.first * late.a.hkv + hk;     // of the row tile's first piece
+    const uint64_t part0 = static_cast<uint64_t>(slot + piece.at * late.a.hkv) * late.row_cap;
+    if (r < rows) {
+        uint32_t t, hq;
+        row_of(r, &t, &hq);
+        if (late.deal && half1 == 0) {
+            if (piece.at == 0) late.row_parts[static_cast<uint64_t>(t) * late.a.hq + hq] = make_uint2(slot, piece.count | r << 16);
+            if (to_parts) late.part_ml[part0 + r] = make_float2(mc, l);
+        }
+        char* yr = to_parts ? reinterpret_cast<char*>(late.part_o + (part0 + r) * D) : late.a.y + t * late.a.y_nb2 + hq * late.a.y_nb1;
+        const float f = to_parts ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++) {
+        for (int d = 0; d < DP / 32; d++) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const uint32_t dim = 32 * d + 8 * c + 4 * half;
-            if (dim >= a.D || !mine) continue;
-            float v[4];
+            for (int c = 0; c < 4; c++) {
+                const uint32_t dim = 32 * d + 8 * c + 4 * half1;
+                if (dim >= D) continue;
+                float v[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = o[d][4 * c + u];
-            if (to_parts) {
-                store4u(reinterpret_cast<char*>(pa.part_o + part * a.D + dim), v, float());
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; u++) v[u] *= inv;
-                store4u(yr + dim * Elt<TQ>::size, v, TQ());
+                for (int u = 0; u < 4; u++) v[u] = o[d][4 * c + u] * f;
+                if (to_parts) store4u(yr + dim * 4, v, float());
+                else store4u(yr + dim * Elt<TQ>::size, v, TQ());
             }
         }
     }
     if constexpr (!I8) {
         if (!clean) return;
-        __syncthreads();                                     // what is written above is corrected
+        wait_vector_memory();                                // what this wave wrote above is corrected
 #pragma unroll 1
         for (int i = 0; i < 32; i++) {                       // a row at a time, its dims over the lanes
-            if (wid != row_wave || wid * 32 + i >= rows) break;
+            const uint32_t ri = row_wave * 32 + i;
+            if (ri >= rows) break;
             const int32_t lim = min(__shfl(limit, i), static_cast<int32_t>(tb * KT)), from = max(__shfl(first, i), static_cast<int32_t>(ta * KT));
-            const uint32_t ti = __shfl(static_cast<int>(t), i), hi = __shfl(static_cast<int>(hq), i);
+            uint32_t t, hq;
+            row_of(ri, &t, &hq);
             uint32_t found[DP / 64 + 1] = {};                // 1, 2, 4: infinity, -infinity, NaN
             for (int32_t key = from; key < lim; key++) {
                 const uint32_t pi = page_of(a, key);
@@ -828,19 +900,19 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 const char* vr = a.v + pg * a.v_nb3 + hk * a.v_nb2 + (key - pi * a.page) * a.v_nb1;
 #pragma unroll
                 for (int k = 0; k < DP / 64 + 1; k++) {
-                    const uint32_t d = lane + 64 * k;
-                    if (d >= a.D) continue;
+                    const uint32_t d = lane1 + 64 * k;
+                    if (d >= D) continue;
                     const float y = Elt<TC>::load1(vr + d * Elt<TC>::size);
                     if (!(fabsf(y) < INFINITY)) found[k] |= y > 0.0f ? 1 : y < 0.0f ? 2 : 4;
                 }
             }
 #pragma unroll
             for (int k = 0; k < DP / 64 + 1; k++) {
-                const uint32_t d = lane + 64 * k;
-                if (d >= a.D || !found[k]) continue;
+                const uint32_t d = lane1 + 64 * k;
+                if (d >= D || !found[k]) continue;
                 const float y = found[k] == 1 ? INFINITY : found[k] == 2 ? -INFINITY : NAN;
-                if (to_parts) pa.part_o[(static_cast<uint64_t>(slot + piece.at * a.hkv) * pa.row_cap + wid * 32 + i) * a.D + d] = y;
-                else Elt<TQ>::store1(a.y + ti * a.y_nb2 + hi * a.y_nb1 + d * Elt<TQ>::size, y);
+                if (to_parts) late.part_o[(part0 + ri) * D + d] = y;
+                else Elt<TQ>::store1(late.a.y + t * late.a.y_nb2 + hq * late.a.y_nb1 + d * Elt<TQ>::size, y);
             }
         }
     }
@@ -908,7 +980,7 @@ __global__ __launch_bounds__(256) void k_prompt_join(PromptArgs pa) {
 }
 
 struct PromptPlan {
-    bool tiles;                // k_prompt, else k_attn_rows
+    bool tiles, pair;          // k_prompt, else k_attn_rows; its PAIR
     int dp;
     uint32_t row_tiles, deal, row_cap, grid;
     size_t o_bytes, ml_bytes, bytes;
@@ -922,7 +994,9 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     PromptPlan p{};
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0, cap = tables->ne[0] * k->ne[1];
     p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
-    const int64_t most = q->ne[2] * g / kRows + n_start, wide = 2 * st->n_cu;
+    p.pair = q->ne[2] * g < 96 * n_start;
+    const int64_t rows = p.pair ? 64 : 128;
+    const int64_t most = q->ne[2] * g / rows + n_start, wide = 2 * st->n_cu;
     p.tiles = D % (k->type == CBX_TYPE_I8 ? 16 : 8) == 0 && D <= 256 && cap > 0 && k->ne[3] > 0 && most * hkv < (int64_t{1} << 24) &&
               k->ne[2] <= wide;
     if (!p.tiles) return p;
@@ -931,7 +1005,7 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     if (most > kDealTiles || n_start > kDealTiles || (!shared && (most * hkv > wide || cap < 512))) return p;
     p.deal = static_cast<uint32_t>(wide);
     p.grid = static_cast<uint32_t>((wide / hkv + most) * hkv);
-    p.row_cap = static_cast<uint32_t>(std::min<int64_t>(kRows, q->ne[2] * g));
+    p.row_cap = static_cast<uint32_t>(std::min<int64_t>(rows, q->ne[2] * g));
     const int64_t parts = static_cast<int64_t>(p.grid) * p.row_cap;
     p.o_bytes = up16(parts * D * 4);
     p.ml_bytes = up16(parts * 8);
@@ -955,27 +1029,31 @@ PromptArgs prompt_args(const PagedAttnCall& c, const PromptPlan& p, uint32_t n_s
     return a;
 }
 
-template <typename TQ, typename TC, int PP> void launch_dp(int dp, dim3 grid, hipStream_t s, const PromptArgs& a) {
-    auto go = [&](auto d) {
+template <typename TQ, typename TC, int PP> void launch_dp(const PromptPlan& p, hipStream_t s, const PromptArgs& a) {
+    auto go = [&](auto d, auto pair) {
         constexpr int DP = decltype(d)::value;
-        if (a.a.softcap > 0.0f) hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, false>), grid, dim3(256), 0, s, a);
+        constexpr bool PAIR = decltype(pair)::value;
+        if (a.a.softcap > 0.0f) hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, true, PAIR>), dim3(p.grid), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_prompt<TQ, TC, DP, PP, false, PAIR>), dim3(p.grid), dim3(256), 0, s, a);
     };
-    if (dp == 64) go(std::integral_constant<int, 64>());
-    else if (dp == 96) go(std::integral_constant<int, 96>());
-    else if (dp == 128) go(std::integral_constant<int, 128>());
-    else go(std::integral_constant<int, 256>());
+    auto both = [&](auto d) {
+        if (p.pair) go(d, std::true_type());
+        else go(d, std::false_type());
+    };
+    if (p.dp == 64) both(std::integral_constant<int, 64>());
+    else if (p.dp == 96) both(std::integral_constant<int, 96>());
+    else if (p.dp == 128) both(std::integral_constant<int, 128>());
+    else both(std::integral_constant<int, 256>());
 }
 
 void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs& a, hipStream_t s) {
-    const dim3 grid(p.grid);
     const bool t16 = c.q->type == CBX_TYPE_F16, i8 = c.k->type == CBX_TYPE_I8;
-    if (t16 && i8) launch_dp<uint16_t, int8_t, 2>(p.dp, grid, s, a);
-    else if (i8) launch_dp<float, int8_t, 3>(p.dp, grid, s, a);
-    else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p.dp, grid, s, a) : launch_dp<float, float, 2>(p.dp, grid, s, a);
-    else if (!t16) launch_dp<float, uint16_t, 2>(p.dp, grid, s, a);
-    else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p.dp, grid, s, a);
-    else launch_dp<uint16_t, uint16_t, 1>(p.dp, grid, s, a);
+    if (t16 && i8) launch_dp<uint16_t, int8_t, 2>(p, s, a);
+    else if (i8) launch_dp<float, int8_t, 3>(p, s, a);
+    else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p, s, a) : launch_dp<float, float, 2>(p, s, a);
+    else if (!t16) launch_dp<float, uint16_t, 2>(p, s, a);
+    else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p, s, a);
+    else launch_dp<uint16_t, uint16_t, 1>(p, s, a);
 }
 
 void launch_join(const PagedAttnCall& c, const PromptArgs& a, hipStream_t s) {
