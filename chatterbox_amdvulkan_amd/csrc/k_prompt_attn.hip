@@ -23,7 +23,6 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 
-
 struct PromptArgs {
     AttnArgs a;
     const int32_t* shared;     // shared keys a group; null: packed tokens
@@ -91,6 +90,7 @@ template <int ROWS> __device__ __forceinline__ uint32_t first_tile(const AttnArg
 // Few row tiles: their keys are cut into pieces of one size, so that about `deal` workgroups have one each whatever the lengths, which
 // only the device knows.  Every workgroup counts the key tiles of all row tiles for itself.
 constexpr uint32_t kDealTiles = 1024;   // row tiles, requests at most
+constexpr int64_t kLeast = 4;           // key tiles a piece at least: its rows' sums are written and read again
 struct Piece {
     uint32_t first = 0, count = 1, at = 0;      // the row tile's first piece, how many it has, which of them
     uint32_t tile0 = 0, tiles = 0;              // key tiles
@@ -142,8 +142,8 @@ struct Piece {
         __syncthreads();
         all = sums[0] + sums[1] + sums[2] + sums[3];
         __syncthreads();
-        // key tiles a piece: a piece's row tile is written and read again, so not too few
-        const uint32_t size = max(4u, static_cast<uint32_t>((static_cast<uint64_t>(all) * a.hkv + pa.deal - 1) / pa.deal));
+        // key tiles a piece
+        const uint32_t size = max(static_cast<uint32_t>(kLeast), static_cast<uint32_t>((static_cast<uint64_t>(all) * a.hkv + pa.deal - 1) / pa.deal));
         sum = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) sum += (keys[i] + size - 1) / size;
@@ -994,6 +994,8 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     PromptPlan p{};
     const int64_t D = q->ne[0], hkv = k->ne[2], g = hkv ? q->ne[1] / hkv : 0, cap = tables->ne[0] * k->ne[1];
     p.dp = D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+    // Fewer rows a request than fill three of a tile's four waves: pairs (4 texts of 20 to 150 rows: 9.8 us for 11.0; 8 drafts of up to
+    // 36 rows: 128 for 145; 4 groups of 96 rows: 252 for 193).
     p.pair = q->ne[2] * g < 96 * n_start;
     const int64_t rows = p.pair ? 64 : 128;
     const int64_t most = q->ne[2] * g / rows + n_start, wide = 2 * st->n_cu;
@@ -1002,9 +1004,15 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     if (!p.tiles) return p;
     p.row_tiles = static_cast<uint32_t>(most);
     p.grid = static_cast<uint32_t>(most * hkv);
+    // Row tiles that fit at once leave CUs idle at the end, or from the start; where there are more, dealing them gains nothing (660 on 512
+    // places, F32: 393 to 405 us for 355 to 403).  Below 512 keys the join costs what the pieces save.
     if (most > kDealTiles || n_start > kDealTiles || (!shared && (most * hkv > wide || cap < 512))) return p;
-    p.deal = static_cast<uint32_t>(wide);
-    p.grid = static_cast<uint32_t>((wide / hkv + most) * hkv);
+    // A piece for every workgroup that fits at once (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5 times as many 217, half
+    // 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows: 105 us for 120).
+    const int64_t aim = p.pair ? 2 * wide : wide;
+    p.deal = static_cast<uint32_t>(aim);
+    const int64_t key_tiles = cdiv(cap, k->type == CBX_TYPE_F32 || p.dp > 128 ? 32 : 64);
+    p.grid = static_cast<uint32_t>(std::min(aim / hkv + most, most * cdiv(key_tiles, kLeast)) * hkv);
     p.row_cap = static_cast<uint32_t>(std::min<int64_t>(rows, q->ne[2] * g));
     const int64_t parts = static_cast<int64_t>(p.grid) * p.row_cap;
     p.o_bytes = up16(parts * D * 4);
@@ -1052,6 +1060,9 @@ void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs&
     else if (i8) launch_dp<float, int8_t, 3>(p, s, a);
     else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p, s, a) : launch_dp<float, float, 2>(p, s, a);
     else if (!t16) launch_dp<float, uint16_t, 2>(p, s, a);
+    // F16 throughout: a probability rounded to one f16 (2^-11 of itself at most) makes the result's error 1.4 times that of its own rounding,
+    // in two parts nothing; two cost a third more products and more conversions.  Where there are many rows, that is time (16000 tokens:
+    // 3.15 ms for 2.27; 48 requests, 25 thousand tokens: 515 us for 391); where there are few, the pages' bytes are, and both take the same.
     else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p, s, a);
     else launch_dp<uint16_t, uint16_t, 1>(p, s, a);
 }
