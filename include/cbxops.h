@@ -526,14 +526,14 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  *   page      page_size consecutive keys (values) of one request, all heads
  *   k_cache, v_cache
  *             F32 or F16 (both one type), ne = (head_dim, page_size,
- *             n_head_kv, n_pages), any strides past nb[0]
- *   block_tables
- *             I32 (max_pages, n_seq): entry i of request s is the page that
- *             holds its keys [i * page_size, (i + 1) * page_size)
+ *             n_head_kv, n_pages), any strides past nb[0];
  *             or I8 with k_scale, v_scale (the _q8 calls): F32, ne =
  *             (page_size, n_head_kv, n_pages), any strides, one scale for the
  *             head_dim elements of a key (value) of one head, which stand for
  *             scale * element: a cache of half the F16 one's bytes
+ *   block_tables
+ *             I32 (max_pages, n_seq): entry i of request s is the page that
+ *             holds its keys [i * page_size, (i + 1) * page_size)
  *   slot      page * page_size + place in the page; a negative slot belongs
  *             to no request (the padding of a batch)
  *   free_pages, n_free
@@ -543,6 +543,9 @@ int cbx_causal_conv1d(const cbx_tensor* x, const cbx_conv1d_weights* w,
  * its users, so a page that two tables name is given back twice.  Requests
  * that share the P whole pages they begin with are released by the view of
  * their tables behind those P columns, their lengths less P * page_size.
+ * Append takes a new page wherever a request's tokens enter one: tokens are
+ * taken back (drafts that were refused) by a smaller length, after the pages
+ * that it leaves empty have been released likewise, by their columns.
  * All of it lives on the device: no call reads a length on the host, so a
  * captured step replays as its requests grow.  Page numbers, slots and
  * lengths that lie outside their tensors are left out by the kernels that
