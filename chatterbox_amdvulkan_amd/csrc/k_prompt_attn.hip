@@ -559,7 +559,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     }
     float cap_in = 0.0f;
     if constexpr (CAP) {
-        cap_in = mul / kLog2e / a.softcap;
+        cap_in = fminf(mul / kLog2e / a.softcap, 0x1p127f);  // finite: 0 stays 0
         mul = 1.0f;
     }
     mul = fmaxf(mul, 0x1p-126f);                             // -inf, the score of a key that a row does not have, stays that
@@ -632,12 +632,13 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         }
         constexpr uint64_t EACH = NS == 2 ? ~0ull : 0xffffffffull;
         const uint64_t there = have >> 32 * sub & EACH;
-        const bool whole = static_cast<int32_t>(key0) >= all_begin && static_cast<int32_t>(key0) + 32 * NS <= all_end && there == EACH;
+        const bool whole = key0 >= static_cast<uint32_t>(all_begin) && key0 + 32 * NS <= static_cast<uint32_t>(all_end) && there == EACH;
         // bit 8 (e / 4) + e % 4: the lane's row has the key of its score e in run i
         auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
         auto has = [&](int i) {
-            const int32_t at = static_cast<int32_t>(key0) + 32 * i + 4 * static_cast<int32_t>(half);
-            return static_cast<uint32_t>(there >> 32 * i) >> 4 * half & below(limit - at) & ~below(first - at);
+            const uint32_t at = key0 + 32 * i + 4 * half;
+            return static_cast<uint32_t>(there >> 32 * i) >> 4 * half & below(static_cast<int32_t>(limit - at)) &
+                   ~below(static_cast<int32_t>(first - at));
         };
         if (!whole) {
 #pragma unroll
@@ -786,7 +787,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         far = false;
         if (ta < tb) {
             auto edge = [&](uint32_t tile) {
-                return static_cast<int32_t>(tile * KT) < every_begin || static_cast<int32_t>(tile * KT + KT) > every_end;
+                return tile * KT < static_cast<uint32_t>(every_begin) || tile * KT + KT > static_cast<uint32_t>(every_end);
             };
             if (clean) fetch(ta, look_up(ta), lds0);
             arrive(lds0, 0, edge(ta));
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 for (int sub = 0; sub < KT / 32; sub += NS) {
                     const uint32_t k0 = tile * KT + 32 * sub;
                     if (PAIR && (k0 >> 5 & 1) != turn) continue;
-                    if (static_cast<int32_t>(k0) < w_end && static_cast<int32_t>(k0) + 32 * NS > w_begin) products(cur, buf, k0, sub);
+                    if (k0 < static_cast<uint32_t>(w_end) && k0 + 32 * NS > static_cast<uint32_t>(w_begin)) products(cur, buf, k0, sub);
                 }
                 if (more) arrive(next, buf ^ 1, edge(tile + 1));
                 have = have_next;
@@ -889,11 +890,11 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         for (int i = 0; i < 32; i++) {                       // a row at a time, its dims over the lanes
             const uint32_t ri = row_wave * 32 + i;
             if (ri >= rows) break;
-            const int32_t lim = min(__shfl(limit, i), static_cast<int32_t>(tb * KT)), from = max(__shfl(first, i), static_cast<int32_t>(ta * KT));
+            const uint32_t lim = min(static_cast<uint32_t>(__shfl(limit, i)), tb * KT), from = max(static_cast<uint32_t>(__shfl(first, i)), ta * KT);
             uint32_t t, hq;
             row_of(ri, &t, &hq);
             uint32_t found[DP / 64 + 1] = {};                // 1, 2, 4: infinity, -infinity, NaN
-            for (int32_t key = from; key < lim; key++) {
+            for (uint32_t key = from; key < lim; key++) {
                 const uint32_t pi = page_of(a, key);
                 const int32_t pg = table[pi];
                 if (static_cast<uint32_t>(pg) >= a.n_pages) continue;
@@ -1006,12 +1007,13 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     p.grid = static_cast<uint32_t>(most * hkv);
     // Row tiles that fit at once leave CUs idle at the end, or from the start; where there are more, dealing them gains nothing (660 on 512
     // places, F32: 393 to 405 us for 355 to 403).  Below 512 keys the join costs what the pieces save.
-    if (most > kDealTiles || n_start > kDealTiles || (!shared && (most * hkv > wide || cap < 512))) return p;
+    const int64_t key_tiles = cdiv(cap, k->type == CBX_TYPE_F32 || p.dp > 128 ? 32 : 64);
+    if (most > kDealTiles || n_start > kDealTiles || most * key_tiles >= (int64_t{1} << 32) ||
+        (!shared && (most * hkv > wide || cap < 512))) return p;
     // A piece for every workgroup that fits at once (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5 times as many 217, half
     // 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows: 105 us for 120).
     const int64_t aim = p.pair ? 2 * wide : wide;
     p.deal = static_cast<uint32_t>(aim);
-    const int64_t key_tiles = cdiv(cap, k->type == CBX_TYPE_F32 || p.dp > 128 ? 32 : 64);
     p.grid = static_cast<uint32_t>(std::min(aim / hkv + most, most * cdiv(key_tiles, kLeast)) * hkv);
     p.row_cap = static_cast<uint32_t>(std::min<int64_t>(rows, q->ne[2] * g));
     const int64_t parts = static_cast<int64_t>(p.grid) * p.row_cap;

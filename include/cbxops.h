@@ -718,8 +718,9 @@ int cbx_paged_attention_q8(const cbx_tensor* q, const cbx_tensor* k_cache,
  * cache, NULL for F32 and F16.  The rest as for cbx_paged_attention, with
  * n_head * n_tok < 2^24 and one choice more: where the matrix cores are the
  * bound (an F16 query in a call of many rows), probabilities are rounded to F16
- * for their products, by up to 2^-11 of themselves, and the sums they are
- * divided by are sums of the rounded ones.                                 */
+ * for their products, by up to 2^-11 of themselves (small ones by 2^-34 of
+ * their row's largest), and the sums they are divided by are sums of the
+ * rounded ones.                                                            */
 int cbx_paged_prompt_attention_workspace(const cbx_tensor* q,
                                          const cbx_tensor* k_cache,
                                          const cbx_tensor* block_tables,

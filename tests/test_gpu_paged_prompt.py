@@ -338,3 +338,37 @@ def test_pages_past_four_gigabytes(cbx, cdt, d):
     low = torch.arange(n, dtype=torch.int32, device="cuda")[None]
     call = lambda tab: cbx.paged_prompt_attention(q, kc, vc, tab, ints([190]), ints([0, 70]), 0.1, k_scale=ks, v_scale=vs)  # noqa: E731
     assert torch.equal(call(low), call(low + pages - n))
+
+
+@pytest.mark.parametrize("dt,cdt", [(F16, F16), (F32, F16), (F16, I8), (F32, F32)])
+def test_lengths_up_to_the_last(cbx, dt, cdt):
+    """2^31 - 2 keys, the most that a table can hold, all in one page that its
+    entries repeat: the window's keys are the page's last."""
+    page, width, d, n, window = 42966, 49981, 64, 5, 70
+    kc, vc, ks, vs = make_cache(1, 2, page, d, cdt, gen(4))
+    tables = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    q = torch.randn(n, 4, d, device="cuda", generator=gen(5)).to(dt)
+    last = slice(page - 200, page)
+    short = [c[:, :, last].contiguous() if c is not None else None for c in (kc, vc, ks, vs)]
+    one = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    y = cbx.paged_prompt_attention(q, kc, vc, tables, ints([page * width]), ints([0, n]), 0.125, window=window, k_scale=ks, v_scale=vs)
+    ref, bound = rows_ref(q, *short, one, [200], [0, n], 0.125, window=window, p_err=half_step(dt))
+    assert_within(y, ref, bound)
+    both = tables.expand(2, width)
+    y = cbx.paged_shared_attention(q[:2], kc, vc, both, ints([page * width, page * width - 3]), ints([0, 2]), ints([page * width]),
+                                   0.125, window=window, k_scale=ks, v_scale=vs)
+    ref, bound = rows_ref(q[:2], *short, one.expand(2, 1), [200, 197], None, 0.125, window=window, p_err=half_step(dt))
+    assert_within(y, ref, bound)
+    assert cbx.device_errors(clear=True) == 0
+
+
+@pytest.mark.parametrize("dt,cdt", TYPES)
+def test_a_cap_next_to_nothing(cbx, dt, cdt):
+    """softcap 2^-140: every score is 0 to f32's precision, also one that was 0 before."""
+    lens, start, tables, pages = packed([100, 0], [20, 30], 16, 3)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, 64, cdt, gen(4))
+    q = torch.randn(50, 4, 64, device="cuda", generator=gen(5)).to(dt)
+    q[3], q[40] = 0, 0
+    y = cbx.paged_prompt_attention(q, kc, vc, tables, ints(lens), ints(start), 0.125, softcap=2.0 ** -140, k_scale=ks, v_scale=vs)
+    ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, 0.125, 2.0 ** -140, p_err=half_step(dt))
+    assert_within(y, ref, bound)
