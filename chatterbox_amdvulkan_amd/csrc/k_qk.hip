@@ -17,10 +17,12 @@
 // a wave a head row, for sizes and alignments that the vectors do not take.
 //
 // Into I8 pages (Q8Row): the row's largest element over its lanes, then 8
-// elements a lane rounded to whole numbers of steps.
+// elements a lane rounded to whole numbers of steps.  Rows that are neither
+// normed nor turned go through k_store8.
 //
 // k_load reads slots back: a workgroup a token, 8 elements of a key or value a
-// thread; bound by the bytes.
+// thread; bound by the bytes (9001 tokens of 8 + 8 heads of 128, I8 to F16, 11.8
+// to 12.8 us: 56 MB, 4.4 to 4.7 TB/s; 64 tokens of 16 + 16 heads of 64 3.3 us).
 #include "cbx_rowops.h"
 
 namespace cbx {
@@ -55,32 +57,58 @@ __device__ __forceinline__ uint32_t size_of(float x) { return __builtin_bit_cast
 
 // A row in 8 bits: scale = top / 127, n = 127 x / top to the nearest whole
 // number, ties to the even one, top its largest |x| (127 * 2^-126 at least, so
-// that the scale is a normal number).  In f32, 127 / top and the product are
-// 2^-22 of |n| <= 127 off, less than 2^-15: a result further than that from the
-// middle of two whole numbers is right, the others (and the rows whose 127 / top
-// leaves f32's range) are decided in f64, where 127 x is exact and the quotient
-// is a tie only where the true one is.
+// that the scale is a normal number).  In f32, 127 times the reciprocal and the
+// product are 2^-22 of |n| <= 127 off, 2^-15 at most: a result t further than
+// that from the middle of two whole numbers is right.  The others, one in 8000,
+// lie above or below the middle as 254 x lies to (2 floor(t) + 1) top, both
+// exact in f64.  Rows near the ends of f32's range are moved by 2^60 first
+// (exact but for elements that are 0 all the same).
 struct Q8Row {
-    double top;
-    float mul, scale;
-    bool rough, bad;      // f32 decides nothing; an infinity or NaN among them
+    float top, mul, scale, lift;
+    bool bad;             // an infinity or NaN among them
     __device__ __forceinline__ explicit Q8Row(uint32_t largest) {
         bad = largest >= 0x7f800000u;
-        const float t = fmaxf(bad ? 0.0f : __builtin_bit_cast(float, largest), 127 * 0x1p-126f);
-        top = static_cast<double>(t);
-        rough = t < 0x1p-100f;
-        mul = 127.0f / t;
-        scale = bad ? NAN : static_cast<float>(top / 127.0);
+        top = fmaxf(bad ? 0.0f : __builtin_bit_cast(float, largest), 127 * 0x1p-126f);
+        scale = bad ? NAN : top / 127.0f;
+        lift = top < 0x1p-60f ? 0x1p60f : top > 0x1p60f ? 0x1p-60f : 1.0f;
+        top *= lift;
+        mul = 127.0f * __builtin_amdgcn_rcpf(top) * lift;
     }
-    __device__ __forceinline__ int32_t of(float x) const {
-        if (bad) return 0;
-        const float t = x * mul, n = rintf(t);
-        if (rough || fabsf(t - n) > 0.5f - 0x1p-14f) return static_cast<int32_t>(rint(127.0 * static_cast<double>(x) / top));
-        return static_cast<int32_t>(n);
+    // Four of the row's elements as bytes: a sum with 1.5 * 2^23 has the whole
+    // number in its last bits.  off: the furthest of all from a whole number.
+    __device__ __forceinline__ uint32_t quick(const float4& x, float* off) const {
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float t = get(x, i) * mul, s = t + 0x1.8p23f;
+            *off = fmaxf(*off, fabsf(t - (s - 0x1.8p23f)));
+            b[i] = __builtin_bit_cast(uint32_t, s);
+        }
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), 0x05040100u);
     }
-    __device__ __forceinline__ uint32_t of4(const float4& v) const {
-        return (static_cast<uint32_t>(of(v.x)) & 0xffu) | (static_cast<uint32_t>(of(v.y)) & 0xffu) << 8 |
-               (static_cast<uint32_t>(of(v.z)) & 0xffu) << 16 | static_cast<uint32_t>(of(v.w)) << 24;
+    static constexpr float kUnsure = 0.5f - 0x1p-14f;
+    __device__ __forceinline__ uint32_t sure(const float4& x) const {
+        uint32_t r = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float t = get(x, i) * mul, f = floorf(t);
+            const double d = 254.0 * static_cast<double>(get(x, i) * lift) - static_cast<double>(2.0f * f + 1.0f) * static_cast<double>(top);
+            const int32_t low = static_cast<int32_t>(f);
+            int32_t n = static_cast<int32_t>(rintf(t));
+            if (fabsf(t - rintf(t)) > kUnsure) n = d > 0.0 ? low + 1 : d < 0.0 ? low : low + (low & 1);
+            r |= (static_cast<uint32_t>(n) & 0xffu) << 8 * i;
+        }
+        return r;
+    }
+    // The lane's eight elements.
+    __device__ __forceinline__ uint2 of(const float4& xa, const float4& xb) const {
+        float off = 0.0f;
+        uint32_t a = quick(xa, &off), b = quick(xb, &off);
+        if (__builtin_expect(off > kUnsure, 0)) {
+            a = sure(xa);
+            b = sure(xb);
+        }
+        return bad ? make_uint2(0, 0) : make_uint2(a, b);
     }
 };
 
@@ -169,10 +197,12 @@ __global__ __launch_bounds__(kQkThreads) void k_qk(QkArgs a) {
         for (int i = 0; i < N; i++) top = max(top, static_cast<uint32_t>(lane + 64 * i) < D ? size_of(v[i]) : 0u);
         for (int d = 32; d > 0; d >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
         const Q8Row row(top);
+        static_assert(N == 8);
+        const uint2 w = row.of(make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]));
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const uint32_t e = lane + 64 * i;
-            if (e < D) y[e] = static_cast<char>(row.of(v[i]));
+            if (e < D) y[e] = static_cast<char>((i < 4 ? w.x : w.y) >> 8 * (i % 4));
         }
         if (lane == 0) store_scale(a, kind, pg, hh, at, row.scale);
         return;
@@ -198,10 +228,16 @@ template <int LPR> __device__ __forceinline__ double head_sum(double v) {
 }
 
 // Largest over them.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true)));
+}
 template <int LPR> __device__ __forceinline__ uint32_t head_max(uint32_t v) {
-    auto step = [&](int d) { v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d))); };
-#pragma unroll
-    for (int d = 1; d < LPR; d *= 2) step(d);
+    v = dpp_max<0xB1>(v);
+    v = dpp_max<0x4E>(v);
+    v = dpp_max<0x141>(v);
+    if constexpr (LPR >= 16) v = dpp_max<0x140>(v);
+    if constexpr (LPR >= 32) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+    if constexpr (LPR >= 64) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)));
     return v;
 }
 
@@ -323,8 +359,9 @@ __global__ __launch_bounds__(kQkThreads) void k_qk_heads(QkArgs a) {
                                     : a.vc + pg * a.vc_nb3 + hh * a.vc_nb2 + at * a.vc_nb1;
                 if constexpr (sizeof(TC) == 1) {
                     const Q8Row row(top);
-                    *reinterpret_cast<uint32_t*>(y + ia) = row.of4(xa[u]);
-                    *reinterpret_cast<uint32_t*>(y + ib) = row.of4(xb[u]);
+                    const uint2 w = row.of(xa[u], xb[u]);
+                    *reinterpret_cast<uint32_t*>(y + ia) = w.x;
+                    *reinterpret_cast<uint32_t*>(y + ib) = w.y;
                     if (li == 0) store_scale(a, kind, pg, hh, at, row.scale);
                 } else {
                     Elt<TC>::store4(y + ia * Elt<TC>::size, xa[u]);
@@ -332,6 +369,40 @@ __global__ __launch_bounds__(kQkThreads) void k_qk_heads(QkArgs a) {
                 }
             }
         }
+    }
+}
+
+// Rows as they are into I8 pages: a workgroup a token, LPR lanes a row of 8
+// elements each.  Half of what a row costs here is instructions, not bytes, and
+// k_qk_heads has twice as many: 9001 tokens of 8 + 8 heads of 128 in F16 14.0
+// us at the least (56 MB, 4.0 TB/s) for its 21.0.  F16 and F32 pages are at the copy's rate there.
+template <typename T, int LPR>
+__global__ __launch_bounds__(kQkThreads) void k_store8(QkArgs a) {
+    typedef uint32_t u2w __attribute__((ext_vector_type(2), aligned(4)));
+    const uint32_t tok = blockIdx.x, li = threadIdx.x % LPR;
+    const int32_t slot = a.slots[tok];
+    if (slot < 0) return;
+    if (static_cast<uint32_t>(slot) >= a.n_slot) {
+        if (threadIdx.x == 0) atomicOr(a.err, DEV_ERR_PAGE);
+        return;
+    }
+    const uint32_t pg = static_cast<uint32_t>(slot) / a.page, at = static_cast<uint32_t>(slot) - pg * a.page;
+    const char *k = a.k + tok * a.k_nb2, *v = a.v + tok * a.v_nb2;
+    char *kc = a.kc + pg * a.kc_nb3 + at * a.kc_nb1, *vc = a.vc + pg * a.vc_nb3 + at * a.vc_nb1;
+    char *ks = a.ks + pg * a.ks_nb2 + at * a.ks_nb0, *vs = a.vs + pg * a.vs_nb2 + at * a.vs_nb0;
+    const bool in = 8 * li < a.D;
+    for (uint32_t r = threadIdx.x / LPR; r < 2 * a.hkv; r += a.nth / LPR) {
+        const bool val = r >= a.hkv;
+        const uint32_t h = val ? r - a.hkv : r;
+        const char* x = (val ? v + h * a.v_nb1 : k + h * a.k_nb1) + (in ? 8 * li : 0) * Elt<T>::size;
+        const float4 xa = Elt<T>::load4(x), xb = Elt<T>::load4(x + 4 * Elt<T>::size);
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = max(top, max(size_of(get(xa, e)), size_of(get(xb, e))));
+        const Q8Row row(head_max<LPR>(in ? top : 0));
+        const uint2 w = row.of(xa, xb);
+        if (in) *reinterpret_cast<u2w*>((val ? vc + h * a.vc_nb2 : kc + h * a.kc_nb2) + 8 * li) = u2w{w.x, w.y};
+        if (li == 0) *reinterpret_cast<float*>(val ? vs + h * a.vs_nb1 : ks + h * a.ks_nb1) = row.scale;
     }
 }
 
@@ -352,6 +423,15 @@ void launch_heads(QkArgs& a, uint32_t tok, hipStream_t s) {
     // as many waves as the token's heads fill, 4 at most
     a.nth = static_cast<uint32_t>(std::min<int64_t>(kQkThreads, cdiv(static_cast<int64_t>(a.heads) * lpr, 64) * 64));
     const dim3 grid(tok), block(a.nth);
+    if constexpr (sizeof(TC) == 1) {
+        if (!a.norm) {
+            if (lpr == 8) hipLaunchKernelGGL((k_store8<T, 8>), grid, block, 0, s, a);
+            else if (lpr == 16) hipLaunchKernelGGL((k_store8<T, 16>), grid, block, 0, s, a);
+            else if (lpr == 32) hipLaunchKernelGGL((k_store8<T, 32>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_store8<T, 64>), grid, block, 0, s, a);
+            return;
+        }
+    }
     if (lpr == 8) hipLaunchKernelGGL((k_qk_heads<T, TC, 8>), grid, block, 0, s, a);
     else if (lpr == 16) hipLaunchKernelGGL((k_qk_heads<T, TC, 16>), grid, block, 0, s, a);
     else if (lpr == 32) hipLaunchKernelGGL((k_qk_heads<T, TC, 32>), grid, block, 0, s, a);
