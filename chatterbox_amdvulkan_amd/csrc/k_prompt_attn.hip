@@ -6,6 +6,20 @@
 // with s_ij = scale q_i . k_j, in one pass over the keys: with a running maximum
 // m, l = sum exp(s - m) and o = sum exp(s - m) v, both rescaled when the maximum
 // rises, and y = o / l at the end.
+//
+// 4 D products a row and key against 4 D bytes (F16) a key and row tile: bound by
+// the products from some hundred rows on, or rather by what a score takes beside
+// them, an exponential (four issue slots), two to four multiply-adds, a maximum
+// and a conversion for 2 D products of its row.  Measured: 16000 tokens, 32 heads
+// of 128 on 8, F16, 2.28 ms (920 TFLOP/s of the 1156 that a large product
+// reaches; without the softmax 1010, without the copies into LDS 1050); 48
+// requests of 1 to 2047 tokens, 16 heads of 64, 0.39 ms (593); 8 requests of 1 to
+// 9 tokens on 900 to 32000 keys in 8 bits, 103 us (2.7 TB/s, latency).
+//
+// 32 rows a wave, because a wave's 32 x 32 products then need each key and value
+// once out of LDS for 32 rows (64 rows a wave, one workgroup a CU: 616 TFLOP/s for
+// 736; 256 rows a workgroup: 570), and 128 rows a workgroup, so that two or three
+// fit a CU and one's products run beside another's softmax.
 #include "cbx_attn.h"
 
 namespace cbx {
@@ -90,7 +104,9 @@ template <int ROWS> __device__ __forceinline__ uint32_t first_tile(const AttnArg
 // Few row tiles: their keys are cut into pieces of one size, so that about `deal` workgroups have one each whatever the lengths, which
 // only the device knows.  Every workgroup counts the key tiles of all row tiles for itself.
 constexpr uint32_t kDealTiles = 1024;   // row tiles, requests at most
-constexpr int64_t kLeast = 4;           // key tiles a piece at least: its rows' sums are written and read again
+// Key tiles a piece at least: its rows' sums are written and read again (64 takes of 1150 shared keys: 44.8 us; 2: 43.9, 8: 49.5;
+// 7 groups of up to 3500 over 8 bits 49.4; 2: 50.3, 8: 60.2).
+constexpr int64_t kLeast = 4;
 struct Piece {
     uint32_t first = 0, count = 1, at = 0;      // the row tile's first piece, how many it has, which of them
     uint32_t tile0 = 0, tiles = 0;              // key tiles
@@ -423,7 +439,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         for (int i = 0; i < NI; i++) {
             const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
             auto of = [&](uint64_t o) {
-                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), row), hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), row);
+                const uint32_t lo = __shfl(static_cast<int>(static_cast<uint32_t>(o)), row);
+                const uint32_t hi = __shfl(static_cast<int>(static_cast<uint32_t>(o >> 32)), row);
                 return static_cast<uint64_t>(hi) << 32 | lo;
             };
             const char *kw = kb + of(ko), *vw = vb + of(vo);
@@ -453,29 +470,26 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
             for (int i = 0; i < NI; i++) {
                 const uint32_t row = wid * (KT / 4) + i * RPI + sub_row;
-                u4v k0, k1, v0, v1;
+                // keys: 1024 + 128 + x is a half with x + 128 in its low byte
+                u4v k[2], v[2];
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
-                    float fk[4], fv[4];
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        fk[b] = static_cast<float>(static_cast<int8_t>(rk[i][w] >> 8 * b));
-                        fv[b] = static_cast<float>(static_cast<int8_t>(rv[i][w] >> 8 * b));
-                    }
-                    u4v& kk = w < 2 ? k0 : k1;
-                    u4v& vv = w < 2 ? v0 : v1;
+                    const uint32_t y = rk[i][w] ^ 0x80808080u;
 #pragma unroll
                     for (int b = 0; b < 2; b++) {
-                        kk[2 * (w & 1) + b] = __builtin_bit_cast(uint32_t, h2v{static_cast<_Float16>(fk[2 * b]), static_cast<_Float16>(fk[2 * b + 1])});
-                        vv[2 * (w & 1) + b] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, fv[2 * b + 1]),
-                                                                    __builtin_bit_cast(uint32_t, fv[2 * b]), 0x07060302u);
+                        const h2v t = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, y, b ? 0x04030402u : 0x04010400u));
+                        const int at = 2 * (w & 1) + b;
+                        k[w / 2][at] = __builtin_bit_cast(uint32_t, t - h2v{static_cast<_Float16>(1152), static_cast<_Float16>(1152)});
+                        const float f0 = static_cast<float>(static_cast<int8_t>(rv[i][w] >> 16 * b));
+                        const float f1 = static_cast<float>(static_cast<int8_t>(rv[i][w] >> (16 * b + 8)));
+                        v[w / 2][at] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f1), __builtin_bit_cast(uint32_t, f0), 0x07060302u);
                     }
                 }
                 char *lk = to + row * PITCH, *lv = lk + BYTES;
-                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c) * 16) = k0;
-                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c + 1) * 16) = k1;
-                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c) * 16) = v0;
-                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c + 1) * 16) = v1;
+                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c) * 16) = k[0];
+                *reinterpret_cast<u4v*>(lk + T::k_place(row, 2 * sub_c + 1) * 16) = k[1];
+                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c) * 16) = v[0];
+                *reinterpret_cast<u4v*>(lv + T::v_place(row, 2 * sub_c + 1) * 16) = v[1];
             }
             if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
         } else {
@@ -514,8 +528,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         fetch(ta, pg, lds0);
     }
 
-    // the lane's query: dims 16 c + 8 half + [0, 8), for F32 pages 8 c + 4 half + [0, 4).  Else an F32 one is scaled by a power of two to below 2^15 and split into two f16, the
-    // lower times 2^12 and summed apart
+    // the lane's query: dims 16 c + 8 half + [0, 8), for F32 pages 8 c + 4 half + [0, 4).  Over other pages an F32 one is scaled by a
+    // power of two to below 2^15 and split into two f16, the lower times 2^12 and summed apart
     h8v qh[F32 ? 1 : QC], ql[Q2 ? QC : 1];
     float qf[F32 ? QC * 8 : 1];
     float mul = fabsf(a.scale) * kLog2e;
@@ -594,7 +608,9 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
             for (int i = 0; i < NS; i++) {
 #pragma unroll
-                for (int c = 0; c < QC; c++) kf[i][c] = *reinterpret_cast<const h8v*>(lk + i * 32 * PITCH + k_row + T::k_place(n, 2 * c + half) * 16);
+                for (int c = 0; c < QC; c++) {
+                    kf[i][c] = *reinterpret_cast<const h8v*>(lk + i * 32 * PITCH + k_row + T::k_place(n, 2 * c + half) * 16);
+                }
             }
 #pragma unroll
             for (int i = 0; i < NS; i++) {
@@ -708,7 +724,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 const uint32_t key = 8 * (e / 4) + 4 * half + e % 4;
 #pragma unroll
                 for (int d = 0; d < DP / 32; d++) {
-                    const float v = *reinterpret_cast<const float*>(lv + key * PITCH + T::v_place(4 * half, 8 * d + n / 4) * 16 + n % 4 * 4);
+                    const char* at = lv + key * PITCH + T::v_place(4 * half, 8 * d + n / 4) * 16 + n % 4 * 4;
+                    const float v = *reinterpret_cast<const float*>(at);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][e], o[d], 0, 0, 0);
                 }
                 if (e % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // else every value of the 16 keys is held at once
@@ -727,7 +744,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int e = 8 * (u % 2) + 2 * i;
-                        const uint32_t z0 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e])), z1 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e + 1]));
+                        const uint32_t z0 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e]));
+                        const uint32_t z1 = __builtin_bit_cast(uint32_t, static_cast<float>(su[e + 1]));
                         w[i] = __builtin_amdgcn_perm(z1, z0, 0x07060302u);
                         su[e] -= __builtin_bit_cast(float, z0 & 0xffff0000u);
                         su[e + 1] -= __builtin_bit_cast(float, z1 & 0xffff0000u);
@@ -758,7 +776,9 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             for (int d = 0; d < DP / 32; d++) {
                 if constexpr (I8) {
 #pragma unroll
-                    for (int k = PP - 1; k >= 0; k--) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, vf[d]), pb[k], o[d], 0, 0, 0);
+                    for (int k = PP - 1; k >= 0; k--) {
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, vf[d]), pb[k], o[d], 0, 0, 0);
+                    }
                 } else {
                     if constexpr (PP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, o[d], 0, 0, 0);
@@ -890,7 +910,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         for (int i = 0; i < 32; i++) {                       // a row at a time, its dims over the lanes
             const uint32_t ri = row_wave * 32 + i;
             if (ri >= rows) break;
-            const uint32_t lim = min(static_cast<uint32_t>(__shfl(limit, i)), tb * KT), from = max(static_cast<uint32_t>(__shfl(first, i)), ta * KT);
+            const uint32_t lim = min(static_cast<uint32_t>(__shfl(limit, i)), tb * KT);
+            const uint32_t from = max(static_cast<uint32_t>(__shfl(first, i)), ta * KT);
             uint32_t t, hq;
             row_of(ri, &t, &hq);
             uint32_t found[DP / 64 + 1] = {};                // 1, 2, 4: infinity, -infinity, NaN
@@ -1005,13 +1026,13 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     if (!p.tiles) return p;
     p.row_tiles = static_cast<uint32_t>(most);
     p.grid = static_cast<uint32_t>(most * hkv);
-    // Row tiles that fit at once leave CUs idle at the end, or from the start; where there are more, dealing them gains nothing (660 on 512
-    // places, F32: 393 to 405 us for 355 to 403).  Below 512 keys the join costs what the pieces save.
+    // Row tiles that fit at once leave CUs idle at the end, or from the start; where there are more, dealing them gains nothing (660 on
+    // 512 places, F32: 393 to 405 us for 355 to 403).  Below 512 keys the join costs what the pieces save.
     const int64_t key_tiles = cdiv(cap, k->type == CBX_TYPE_F32 || p.dp > 128 ? 32 : 64);
     if (most > kDealTiles || n_start > kDealTiles || most * key_tiles >= (int64_t{1} << 32) ||
         (!shared && (most * hkv > wide || cap < 512))) return p;
-    // A piece for every workgroup that fits at once (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5 times as many 217, half
-    // 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows: 105 us for 120).
+    // A piece for every workgroup that fits at once (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5 times as many 217,
+    // half 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows: 105 us for 120).
     const int64_t aim = p.pair ? 2 * wide : wide;
     p.deal = static_cast<uint32_t>(aim);
     p.grid = static_cast<uint32_t>(std::min(aim / hkv + most, most * cdiv(key_tiles, kLeast)) * hkv);
@@ -1062,9 +1083,9 @@ void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs&
     else if (i8) launch_dp<float, int8_t, 3>(p, s, a);
     else if (c.k->type == CBX_TYPE_F32) t16 ? launch_dp<uint16_t, float, 2>(p, s, a) : launch_dp<float, float, 2>(p, s, a);
     else if (!t16) launch_dp<float, uint16_t, 2>(p, s, a);
-    // F16 throughout: a probability rounded to one f16 (2^-11 of itself at most) makes the result's error 1.4 times that of its own rounding,
-    // in two parts nothing; two cost a third more products and more conversions.  Where there are many rows, that is time (16000 tokens:
-    // 3.15 ms for 2.27; 48 requests, 25 thousand tokens: 515 us for 391); where there are few, the pages' bytes are, and both take the same.
+    // F16 throughout: a probability rounded to one f16 (2^-11 of itself at most) makes the result's error 1.3 times that of its own
+    // rounding, in two parts nothing; two cost half as many products again and more conversions.  In a call of many rows these are its
+    // time (16000 tokens: 3.15 ms for 2.28; 48 requests, 25 thousand tokens: 515 us for 391), in one of few the pages' bytes are.
     else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p, s, a);
     else launch_dp<uint16_t, uint16_t, 1>(p, s, a);
 }
