@@ -12,30 +12,34 @@ constexpr int kAttnMaxD = 512;
 constexpr float kLowest = -3.0e38f;   // below every score that matters; finite, so that m - m is 0
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// What a small call reads comes first: a launch's arguments are fetched a line at a
+// time, and one line more of them before the keys is half a microsecond.
 struct AttnArgs {
     const char *q, *k, *v, *tables;
-    const char *ks, *vs;             // I8 pages: their rows' scales
     const int32_t* lens;
-    const int32_t* start;            // packed tokens or groups, see PagedAttnCall; null: a row of q a request
     char* y;
     int64_t q_nb1, q_nb2, y_nb1, y_nb2, k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3, t_nb1;
-    int64_t ks_nb0, ks_nb1, ks_nb2, vs_nb0, vs_nb1, vs_nb2;
     uint32_t n_seq, hq, hkv, g, D, page, max_pages, n_pages;
-    uint32_t n_rows;                 // of q: tokens or requests
     int32_t window;
     float scale, softcap;
+    uint32_t own;                    // own_first holds
     uint32_t* err;
     // k_attn_tiles and k_attn_join
     uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
     uint32_t gc, ngr, H;             // heads a run holds (<= 16), runs of heads a group, hkv * ngr
-    bool s_quads;                    // scales can be read four at a time
     uint32_t W;                      // runs; 0: a run a request and key head, none of them split
     float* part_o;                   // [W][2][gc][D]
     float2* part_ml;                 // [W][2][gc]
     uint4* split;                    // [W]: request, first query head, heads and parts of the key head that begins
                                      // in the run and ends in a later one; no parts: none does
-    // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt): own_first, null: all
-    // keys, says where a request's begin, and (o, m, l) go to own_o and own_ml at request * hq + head instead of y
+    // I8 pages: their rows' scales
+    const char *ks, *vs;
+    int64_t ks_nb0, ks_nb1, ks_nb2, vs_nb0, vs_nb1, vs_nb2;
+    bool s_quads;                    // they can be read four at a time
+    const int32_t* start;            // packed tokens or groups, see PagedAttnCall; null: a row of q a request
+    uint32_t n_rows;                 // of q: tokens or requests
+    // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt): own_first says where a
+    // request's begin, and (o, m, l) go to own_o and own_ml at request * hq + head instead of y
     const int32_t* own_first;
     const int32_t* groups;           // own_first holds for the requests [groups[0], groups[n_groups])
     uint32_t n_groups;

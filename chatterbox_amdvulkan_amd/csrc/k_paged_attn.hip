@@ -213,7 +213,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     r.wrong = n < 0 || static_cast<uint32_t>(n) > cap;
     r.len = n < 0 ? 0 : min(static_cast<uint32_t>(n), cap);
     r.first = a.window > 0 && r.len > static_cast<uint32_t>(a.window) ? r.len - a.window : 0;
-    if (a.own_first && static_cast<int32_t>(s) >= a.groups[0] && static_cast<int32_t>(s) < a.groups[a.n_groups]) {
+    if (a.own && static_cast<int32_t>(s) >= a.groups[0] && static_cast<int32_t>(s) < a.groups[a.n_groups]) {
         r.first = max(r.first, min(static_cast<uint32_t>(max(a.own_first[s], 0)), r.len));
     }
     r.tile0 = r.first / KT;
@@ -904,7 +904,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 ll = fmaf(lds_l[w][hh], f, ll);
                 oo = fmaf(lds_o[(w * a.gc + hh) * ld + d], f, oo);
             }
-            if (entire && a.own_first) {
+            if (entire && a.own) {
                 const uint64_t own = static_cast<uint64_t>(s) * a.hq + hq0 + hh;
                 a.own_o[own * a.D + d] = oo;
                 if (d == 0) a.own_ml[own] = make_float2(mm - a.own_up, ll);
@@ -990,11 +990,11 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     __syncthreads();
     l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
     const uint64_t own = static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh;
-    if (a.own_first && tid == 0) a.own_ml[own] = make_float2(m - a.own_up, l);
+    if (a.own && tid == 0) a.own_ml[own] = make_float2(m - a.own_up, l);
     char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
     for (uint32_t d = tid; d < a.D; d += kAttnThreads) {
         const float t = ((lds_o[0][d] + lds_o[1][d]) + lds_o[2][d]) + lds_o[3][d];
-        if (a.own_first) a.own_o[own * a.D + d] = t;
+        if (a.own) a.own_o[own * a.D + d] = t;
         else Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
     }
 }
