@@ -111,19 +111,27 @@ struct Piece {
     uint32_t first = 0, count = 1, at = 0;      // the row tile's first piece, how many it has, which of them
     uint32_t tile0 = 0, tiles = 0;              // key tiles
 
-    template <int KT, int ROWS> __device__ __forceinline__ bool find(const PromptArgs& pa, uint32_t q, uint32_t* lds, uint32_t* x, uint32_t* p) {
+    uint32_t x = 0, p = 0, t0 = 0, t1 = 0;      // the row tile, its request (group), that one's tokens (requests)
+    int32_t keys = 0;                           // and length (shared keys), as given
+
+    // lds: 2 kDealTiles + 2 words
+    template <int KT, int ROWS> __device__ __forceinline__ bool find(const PromptArgs& pa, uint32_t q, uint32_t* lds) {
         const AttnArgs& a = pa.a;
         constexpr int N = kDealTiles / 256;
-        __shared__ uint32_t sums[4], found[6];
+        __shared__ uint32_t sums[4], found[8];
         const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-        for (uint32_t i = tid; i <= pa.n_start; i += 256) lds[i] = start_of(a, i);
+        int32_t* given = reinterpret_cast<int32_t*>(lds) + kDealTiles + 1;
+        for (uint32_t i = tid; i <= pa.n_start; i += 256) {
+            lds[i] = start_of(a, i);
+            if (i < pa.n_start) given[i] = pa.shared ? pa.shared[i] : a.lens[i];
+        }
         if (tid == 0) found[0] = ~0u;
         __syncthreads();
-        uint32_t keys[N], begin[N], whose[N], sum = 0;
+        uint32_t n_tiles[N], begin[N], whose[N], sum = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t xi = tid * N + i;
-            keys[i] = begin[i] = whose[i] = 0;
+        for (int i = 0; i < N; i++) {                        // pieces are numbered by threads, a thread's row tiles lie 256 apart
+            const uint32_t xi = tid + 256 * i;
+            n_tiles[i] = begin[i] = whose[i] = 0;
             if (xi >= pa.tiles) continue;
             uint32_t lo = 0, hi = pa.n_start;                // the last one whose tiles start at or before xi
             while (hi - lo > 1) {
@@ -131,25 +139,24 @@ struct Piece {
                 if (first_tile<ROWS>(a, lds[mid], mid) <= xi) lo = mid;
                 else hi = mid;
             }
-            const uint32_t t0 = lds[lo], t1 = lds[lo + 1], base = first_tile<ROWS>(a, t0, lo);
-            if (xi < base || t1 <= t0 || static_cast<uint64_t>(xi - base) * ROWS >= static_cast<uint64_t>(t1 - t0) * a.g) continue;
-            const uint32_t row0 = (xi - base) * ROWS, row1 = min(row0 + ROWS, (t1 - t0) * a.g) - 1;
-            const int32_t cap = static_cast<int32_t>(a.max_pages * a.page);
-            int32_t first = 0, end;
-            if (pa.shared) {
-                end = min(max(pa.shared[lo], 0), cap);
-            } else {
-                const int32_t len = min(max(a.lens[lo], 0), cap), n = static_cast<int32_t>(t1 - t0);
+            const uint32_t from = lds[lo], to = lds[lo + 1], base = first_tile<ROWS>(a, from, lo);
+            if (xi < base || to <= from || static_cast<uint64_t>(xi - base) * ROWS >= static_cast<uint64_t>(to - from) * a.g) continue;
+            const uint32_t row0 = (xi - base) * ROWS, row1 = min(row0 + ROWS, (to - from) * a.g) - 1;
+            const int32_t len = min(max(given[lo], 0), static_cast<int32_t>(a.max_pages * a.page));
+            int32_t first = 0, end = len;
+            if (!pa.shared) {
                 auto limit = [&](uint32_t row) {
-                    return max(0, len - (n - 1 - static_cast<int32_t>((static_cast<uint64_t>(row) * pa.g_mul) >> pa.g_shift)));
+                    const int32_t j = static_cast<int32_t>((static_cast<uint64_t>(row) * pa.g_mul) >> pa.g_shift);
+                    return max(0, len - (static_cast<int32_t>(to - from) - 1 - j));
                 };
                 end = limit(row1);
                 if (a.window > 0) first = max(0, limit(row0) - a.window);
             }
             begin[i] = first / KT;
-            keys[i] = max(1u, (static_cast<uint32_t>(end) + KT - 1) / KT - min(begin[i], (static_cast<uint32_t>(end) + KT - 1) / KT));
+            const uint32_t behind = (static_cast<uint32_t>(end) + KT - 1) / KT;
+            n_tiles[i] = max(1u, behind - min(begin[i], behind));
             whose[i] = lo;
-            sum += keys[i];
+            sum += n_tiles[i];
         }
         uint32_t all = sum;
 #pragma unroll
@@ -162,7 +169,7 @@ struct Piece {
         const uint32_t size = max(static_cast<uint32_t>(kLeast), static_cast<uint32_t>((static_cast<uint64_t>(all) * a.hkv + pa.deal - 1) / pa.deal));
         sum = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) sum += (keys[i] + size - 1) / size;
+        for (int i = 0; i < N; i++) sum += (n_tiles[i] + size - 1) / size;
         uint32_t before = sum;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -175,13 +182,16 @@ struct Piece {
         for (uint32_t w = 0; w < wid; w++) before += sums[w];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const uint32_t n = (keys[i] + size - 1) / size;
+            const uint32_t n = (n_tiles[i] + size - 1) / size;
             if (q >= before && q - before < n) {
                 found[0] = before;
                 found[1] = n;
                 found[2] = begin[i] + (q - before) * size;
-                found[3] = tid * N + i;
+                found[3] = tid + 256 * i;
                 found[4] = whose[i];
+                found[5] = lds[whose[i]];
+                found[6] = lds[whose[i] + 1];
+                found[7] = static_cast<uint32_t>(given[whose[i]]);
             }
             before += n;
         }
@@ -192,8 +202,11 @@ struct Piece {
         at = q - first;
         tile0 = __builtin_amdgcn_readfirstlane(found[2]);
         tiles = size;
-        *x = __builtin_amdgcn_readfirstlane(found[3]);
-        *p = __builtin_amdgcn_readfirstlane(found[4]);
+        x = __builtin_amdgcn_readfirstlane(found[3]);
+        p = __builtin_amdgcn_readfirstlane(found[4]);
+        t0 = __builtin_amdgcn_readfirstlane(found[5]);
+        t1 = __builtin_amdgcn_readfirstlane(found[6]);
+        keys = __builtin_amdgcn_readfirstlane(static_cast<int>(found[7]));
         return true;
     }
 };
@@ -273,13 +286,15 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     // this workgroup's key head, row tile (undealt: the last rows, which have the most keys, first) and piece of its keys
     const uint32_t hk = blockIdx.x % a.hkv;
     uint32_t x = pa.tiles - 1 - blockIdx.x / a.hkv, p = 0, t0, t1;
-    int32_t given = 0;                                       // the request's length
+    int32_t given = 0;                                       // the request's length, the group's shared keys
     Piece piece;
     if (pa.deal) {
-        if (!piece.find<KT, ROWS>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds0), &x, &p)) return;
-        t0 = start_of(a, p);
-        t1 = start_of(a, p + 1);
-        if (!pa.shared) given = a.lens[p];
+        if (!piece.find<KT, ROWS>(pa, blockIdx.x / a.hkv, reinterpret_cast<uint32_t*>(lds0))) return;
+        x = piece.x;
+        p = piece.p;
+        t0 = piece.t0;
+        t1 = piece.t1;
+        given = piece.keys;
     } else {
         // the request p whose tiles x lies among; what is read with it in one go: where it and the next one start, and its length
         for (uint32_t width = pa.n_start;;) {                // p among [p, p + width)
@@ -319,9 +334,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     if (pa.shared) {
         uint32_t t, hq;
         row_of(lane_row, &t, &hq);
-        given = a.lens[t];
-        wrong = given < 0 || given > cap;
-        const int32_t len = min(max(given, 0), cap), pre = min(max(pa.shared[p], 0), cap);
+        const int32_t all = a.lens[t], len = min(max(all, 0), cap), pre = min(max(given, 0), cap);
+        wrong = all < 0 || all > cap;
         first = first_of(len);
         limit = min(len, pre);
         if (hk == 0 && piece.at == 0 && half == 0 && live_row && wid == row_wave) pa.own_first[t] = limit;
