@@ -167,9 +167,14 @@ struct Piece {
         __syncthreads();
         // key tiles a piece
         const uint32_t size = max(static_cast<uint32_t>(kLeast), static_cast<uint32_t>((static_cast<uint64_t>(all) * a.hkv + pa.deal - 1) / pa.deal));
+        uint32_t pieces[N] = {};
         sum = 0;
 #pragma unroll
-        for (int i = 0; i < N; i++) sum += (n_tiles[i] + size - 1) / size;
+        for (int i = 0; i < N; i++) {
+            if (256u * i >= pa.tiles) break;
+            pieces[i] = (n_tiles[i] + size - 1) / size;
+            sum += pieces[i];
+        }
         uint32_t before = sum;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -182,7 +187,7 @@ struct Piece {
         for (uint32_t w = 0; w < wid; w++) before += sums[w];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const uint32_t n = (n_tiles[i] + size - 1) / size;
+            const uint32_t n = pieces[i];
             if (q >= before && q - before < n) {
                 found[0] = before;
                 found[1] = n;
