@@ -603,6 +603,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 
     // LDS addresses that a lane reads keys and values at
     const uint32_t k_row = n * PITCH;
+    // the swizzle stays within 16 chunks, so that 8 addresses and constants beside them do
+    auto k_at = [&](int c) { return k_row + (T::k_place(n, 2 * (c % 8) + half) + 16 * (c / 8)) * 16; };
     const uint32_t l16 = lane & 15, v_key = 4 * half + l16 / 4, v_c = 2 * (lane >> 4 & 1) + (l16 >> 1 & 1);
     const uint32_t v_at = v_key * PITCH + (l16 & 1) * 8;
 
@@ -616,9 +618,16 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         if constexpr (F32) {
 #pragma unroll
             for (int c = 0; c < DP / 8; c++) {
-                const f4v kf = *reinterpret_cast<const f4v*>(lk + k_row + T::k_place(n, 2 * c + half) * 16);
+                const f4v kf = *reinterpret_cast<const f4v*>(lk + k_at(c));
 #pragma unroll
                 for (int u = 0; u < 4; u++) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[u], qf[4 * c + u], s[0], 0, 0, 0);
+            }
+            constexpr int A = 4;
+            __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+            for (int c = 0; c < DP / 8; c++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                if (c + A < DP / 8) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
         } else {
             f16v low = {};
@@ -628,7 +637,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             for (int i = 0; i < NS; i++) {
 #pragma unroll
                 for (int c = 0; c < QC; c++) {
-                    kf[i][c] = *reinterpret_cast<const h8v*>(lk + i * 32 * PITCH + k_row + T::k_place(n, 2 * c + half) * 16);
+                    kf[i][c] = *reinterpret_cast<const h8v*>(lk + i * 32 * PITCH + k_at(c));
                 }
             }
 #pragma unroll
@@ -743,7 +752,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
                 const uint32_t key = 8 * (e / 4) + 4 * half + e % 4;
 #pragma unroll
                 for (int d = 0; d < DP / 32; d++) {
-                    const char* at = lv + key * PITCH + T::v_place(4 * half, 8 * d + n / 4) * 16 + n % 4 * 4;
+                    const char* at = lv + key * PITCH + (T::v_place(4 * half, 8 * (d % 2) + n / 4) + 16 * (d / 2)) * 16 + n % 4 * 4;
                     const float v = *reinterpret_cast<const float*>(at);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][e], o[d], 0, 0, 0);
                 }
@@ -787,7 +796,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
 #pragma unroll
             for (int d = 0; d < DP / 32; d++) {
                 // place of chunk 4 d + v_c in the lane's rows: these are alike modulo 4
-                const char* at = lv + v_at + T::v_place(v_key, 4 * d + v_c) * 16 + 16 * u * PITCH;
+                const char* at = lv + v_at + (T::v_place(v_key, 4 * (d % 4) + v_c) + 16 * (d / 4)) * 16 + 16 * u * PITCH;
                 const h4v x0 = read_turned(at), x1 = read_turned(at + 8 * PITCH);
                 vf[d] = h8v{x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
             }
