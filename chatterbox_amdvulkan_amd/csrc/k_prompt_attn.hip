@@ -11,10 +11,10 @@
 // the products from some hundred rows on, or rather by what a score takes beside
 // them, an exponential (four issue slots), two to four multiply-adds, a maximum
 // and a conversion for 2 D products of its row.  Measured: 16000 tokens, 32 heads
-// of 128 on 8, F16, 2.28 ms (920 TFLOP/s of the 1156 that a large product
+// of 128 on 8, F16, 2.27 ms (920 TFLOP/s of the 1156 that a large product
 // reaches; without the softmax 1010, without the copies into LDS 1050); 48
 // requests of 1 to 2047 tokens, 16 heads of 64, 0.39 ms (593); 8 requests of 1 to
-// 9 tokens on 900 to 32000 keys in 8 bits, 103 us (2.7 TB/s, latency).
+// 9 tokens on 900 to 32000 keys in 8 bits, 99 us (2.8 TB/s, latency).
 //
 // 32 rows a wave, because a wave's 32 x 32 products then need each key and value
 // once out of LDS for 32 rows (64 rows a wave, one workgroup a CU: 616 TFLOP/s for
