@@ -2,6 +2,7 @@
 rotation), read back, and attended over by one new token a request."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -261,3 +262,29 @@ def test_8_bits_is_no_activation_type(cbx):
     tables = page_tables([4], 4, 1, 1, 0).cuda()
     with pytest.raises(cbx.CbxError, match="unknown type"):
         cbx.paged_attention(x.view(1, 4, 64), x.view(1, 1, 4, 64), x.view(1, 1, 4, 64), tables, ints([4]), 1.0)
+
+
+@pytest.mark.parametrize("d", [64, 60, 512])
+def test_middles_at_every_size(cbx, d):
+    """Elements in the middle of two whole numbers of steps, and the numbers
+    next to these, in rows of every size that f32 has: the largest is 127 * 2^k,
+    so that n + 1/2 steps are a number; and of largest elements that are not."""
+    rows = []
+    for k in range(-126, 121):
+        n = torch.arange(d, dtype=torch.float64) * 5 % 127 + 0.5
+        x = (n * 2.0 ** k).float()
+        near = torch.where(torch.arange(d) % 3 == 0, x, torch.nextafter(x, torch.where(torch.arange(d) % 3 == 1, torch.inf, -torch.inf)))
+        near = torch.where(torch.arange(d) % 2 == 0, near, -near)
+        near[d // 2] = 127 * 2.0 ** k
+        other = near.clone()
+        other[d // 2] = float(np.nextafter(np.float32(127 * 2.0 ** k), np.float32(0)))
+        rows += [near, other]
+    x = torch.stack(rows).cuda()[:, None]
+    t = x.shape[0]
+    kc = torch.zeros(1, 1, t, d, dtype=torch.int8, device="cuda")
+    vc, ks = torch.zeros_like(kc), torch.zeros(1, 1, t, device="cuda")
+    vs = torch.zeros_like(ks)
+    cbx.paged_store(x, -x, torch.arange(t, dtype=torch.int32, device="cuda"), kc, vc, ks, vs)
+    q, s = q8_ref(x[:, 0])
+    assert torch.equal(kc[0, 0], q) and torch.equal(ks[0, 0], s)
+    assert torch.equal(vc[0, 0], -q) and torch.equal(vs[0, 0], s)
