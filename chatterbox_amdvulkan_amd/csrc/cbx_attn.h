@@ -57,7 +57,9 @@ AttnArgs attn_args(const PagedAttnCall& c, const DeviceState* st);
 // A workgroup a row of q and query head, for what no other kernel takes: any
 // sizes, strides and types.
 int launch_attention_rows(const AttnArgs& a, const PagedAttnCall& c, const char* what, hipStream_t s);
-// paged_attention's kernels by tiles over a's tensors: launches them if they take the call; the workspace they need.
+// paged_attention's kernels by tiles over a's tensors: whether they take these shapes; launches them if they take the call; the
+// workspace they need.
+bool attention_tiles(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
 bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, DeviceState* st, hipStream_t s);
 size_t attention_tiles_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st);
 // Whether rows can be read 16 bytes at a time.

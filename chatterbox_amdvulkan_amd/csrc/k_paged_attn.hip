@@ -1148,6 +1148,10 @@ size_t attention_tiles_workspace(const cbx_tensor* q, const cbx_tensor* k, const
     return attn_plan(q, k, tables, st).bytes;
 }
 
+bool attention_tiles(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
+    return attn_plan(q, k, tables, st).tiles;
+}
+
 bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, DeviceState* st, hipStream_t s) {
     const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
     if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return false;

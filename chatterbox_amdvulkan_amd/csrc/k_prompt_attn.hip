@@ -1157,7 +1157,8 @@ SharedPlan shared_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     SharedPlan p{};
     const int64_t n_groups = start->ne[0] - 1, rows = q->ne[1] * q->ne[2];
     p.pre = prompt_plan(q, k, tables, n_groups, true, st);
-    p.tiles = p.pre.tiles && p.pre.deal && n_groups > 0 && n_groups < q->ne[2];
+    // both kernels take it; else paged_attention does, whose scratch is the same
+    p.tiles = p.pre.tiles && p.pre.deal && n_groups > 0 && n_groups < q->ne[2] && attention_tiles(q, k, tables, st);
     p.bytes = attention_tiles_workspace(q, k, tables, st);
     if (!p.tiles) return p;
     p.o_bytes = up16(rows * q->ne[0] * 4);
@@ -1196,7 +1197,9 @@ int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s) 
     b.n_groups = a.n_start;
     b.own_o = own_o;
     b.own_ml = own_ml;
-    launch_attention_tiles(b, own, ws + p.o_bytes + p.ml_bytes + p.first_bytes, st, s);
+    if (!launch_attention_tiles(b, own, ws + p.o_bytes + p.ml_bytes + p.first_bytes, st, s)) {
+        return set_error(CBX_ERR_UNSUPPORTED, "cbx_paged_shared_attention: the requests' own keys have no kernel");
+    }
     launch_join(c, a, s);
     return check_launch(what);
 }

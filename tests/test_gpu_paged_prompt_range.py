@@ -1,0 +1,74 @@
+"""Prompt attention and attention of shared beginnings at the ends of the
+ranges: values near f32's largest, scores of millions, infinite keys that have
+no weight, caps and scales of any size, tables of the largest capacity."""
+import numpy as np
+import pytest
+import torch
+
+from tests._paged import assert_within
+from tests._paged_more import U32, gen, half_step, ints, make_cache, packed, rows_ref
+
+pytestmark = pytest.mark.gpu
+F16, F32, I8 = torch.float16, torch.float32, torch.int8
+TYPES = [(F16, F16), (F32, F16), (F32, F32), (F16, F32), (F16, I8), (F32, I8)]
+TWO_BF16 = 2.0 ** -15                  # of an F16 query over I8 pages: 16 bits of a probability times its value's scale, cut off
+
+
+def test_shared_past_the_tiles_of_one_token(cbx):
+    """32 requests of 4 key heads, tables of 2^31 - 2 keys (one page that all
+    entries repeat): more tiles than the kernel of the requests' own keys
+    counts.  The scratch holds NaN before the call."""
+    n, page, width, d, window = 32, 42966, 49981, 64, 70
+    kc, vc, _, _ = make_cache(1, 4, page, d, F16, gen(4))
+    tables = torch.zeros(1, width, dtype=torch.int32, device="cuda").expand(n, width)
+    q = torch.randn(n, 4, d, device="cuda", generator=gen(5)).half()
+    lens = [page * width - 3 * s for s in range(n)]
+    ws = torch.full((1 << 24,), float("nan"), device="cuda")
+    y = cbx.paged_shared_attention(q, kc, vc, tables, ints(lens), ints([0, n]), ints([page * (width - 1)]), 0.125, window=window, ws=ws)
+    one = torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    short = [c[:, :, page - 200:].contiguous() for c in (kc, vc)]
+    ref, bound = rows_ref(q, *short, None, None, one, [200 - 3 * s for s in range(n)], None, 0.125, window=window)
+    assert_within(y, ref, bound)
+    assert cbx.device_errors(clear=True) == 0
+
+
+def shared_of(groups, own, page, seed=3):
+    """(lens, tables, pages): groups [(first, behind, shared)] of whole pages, own[s] keys behind them."""
+    n = len(own)
+    pre, lead = [0] * n, list(range(n))
+    for a, b, p in groups:
+        assert p % page == 0
+        for s in range(a, b):
+            pre[s], lead[s] = p, a
+    lens = [p + o for p, o in zip(pre, own)]
+    pages = sum(-(-x // page) for x in lens) + 2
+    order = iter(np.random.RandomState(seed).permutation(pages).tolist())
+    tables = np.full((n, max(1, max(-(-x // page) for x in lens))), -1, dtype=np.int32)
+    for s in range(n):
+        whole = pre[s] // page if lead[s] < s else 0
+        tables[s, :whole] = tables[lead[s], :whole]
+        for i in range(whole, -(-lens[s] // page)):
+            tables[s, i] = next(order)
+    return lens, torch.from_numpy(tables).cuda(), pages
+
+
+CALLS = {  # past, new of packed requests: pieces of pairs of waves, of whole row tiles, both undealt; shared beginnings
+    "pieces": ([1500, 40], [3, 2]), "long": ([650, 900], [110, 100]), "pairs": ([0, 40], [50, 33]), "whole": ([0, 70], [130, 200]),
+    "shared": None}
+
+
+def call_of(which, page=16):
+    """(lens, start or None, tables, pages, extra arguments) of one of CALLS."""
+    if CALLS[which]:
+        lens, start, tables, pages = packed(*CALLS[which], page, 3)
+        return lens, start, tables, pages, None
+    groups, own = [(0, 3, 192), (3, 5, 64)], [40, 1, 700, 33, 90]
+    lens, tables, pages = shared_of(groups, own, page)
+    return lens, None, tables, pages, (ints([0, 3, 5]), ints([192, 64]))
+
+
+def attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale, **kw):
+    kw = dict(kw, k_scale=ks, v_scale=vs)
+    if groups:
+        return cbx.paged_shared_attention(q, kc, vc, tables, ints(lens), *groups, scale, **kw)
+    return cbx.paged_prompt_attention(q, kc, vc, tables, ints(lens), ints(start), scale, **kw)
