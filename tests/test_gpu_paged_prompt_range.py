@@ -72,3 +72,44 @@ def attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale, **kw):
     if groups:
         return cbx.paged_shared_attention(q, kc, vc, tables, ints(lens), *groups, scale, **kw)
     return cbx.paged_prompt_attention(q, kc, vc, tables, ints(lens), ints(start), scale, **kw)
+
+
+@pytest.mark.parametrize("which", CALLS)
+@pytest.mark.parametrize("d,g", [(64, 1), (128, 4)])
+@pytest.mark.parametrize("up_k,up_v", [(1e6, 1.0), (1.0, 1e35), (1.0, 1e-33), (1e-30, 1.0)])
+def test_large_and_small_8_bit_scales(cbx, which, d, g, up_k, up_v):
+    """Scores of millions, values near f32's ends, as paged_attention takes them."""
+    lens, start, tables, pages, groups = call_of(which)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, d, I8, gen(19))
+    q = torch.randn(start[-1] if start else len(lens), 2 * g, d, device="cuda", generator=gen(1))
+    k2, v2 = ks * up_k, vs * up_v
+    y = attend(cbx, q, kc, vc, k2, v2, tables, lens, start, groups, 0.125)
+    ref, bound = rows_ref(q, kc, vc, k2, v2, tables, lens, start, 0.125)
+    assert bool(torch.isfinite(y).all())
+    assert_within(y, ref, bound + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("which", CALLS)
+@pytest.mark.parametrize("dt,cdt", [(F32, I8)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_values_behind_a_rising_maximum(cbx, which, dt, cdt, d):
+    """Values of 2^117 (in sum below 2^127 a row) whose scores are 7 powers of
+    two above those of the first 64 keys."""
+    lens, start, tables, pages, groups = call_of(which, 32)
+    kc, vc, ks, vs = make_cache(pages, 2, 32, d, F32, gen(19))
+    vc = vc.abs().clamp(0.25, 1.0) * 2.0 ** 116
+    kc.zero_()
+    rows = tables[:, 2:]
+    kc[rows[rows >= 0].long(), ..., 3] = 1.0
+    if cdt == I8:
+        kc, vc = kc.to(I8), (vc * 2.0 ** -110).to(I8)        # 16 to 64
+        ks, vs = torch.ones(pages, 2, 32, device="cuda"), torch.full((pages, 2, 32), 2.0 ** 110, device="cuda")
+    else:
+        ks = vs = None
+    q = torch.zeros(start[-1] if start else len(lens), 2, d, device="cuda")
+    q[..., 3] = 7.0
+    scale = float(np.log(2.0))
+    y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale)
+    ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, scale)
+    assert bool(torch.isfinite(y).all())
+    assert_within(y, ref, bound)
