@@ -278,9 +278,10 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     constexpr int RPI = 64 / LANES, NI = KT / 4 / RPI;       // rows a wave brings at a time, times
     constexpr int NS = PAIR || KT == 32 || Q2 || DP == 64 ? 1 : 2;   // runs of 32 keys taken together
     // Probabilities are held times 2^kUp, and up to 2^(kUp + kRise), since the sums are rescaled only when a row's maximum has risen by
-    // kRise powers of two.  F16 pages: what f16's 2^15 leaves, values being below 2^16.  A value in I8 may lie anywhere in f32's range:
-    // probabilities up to 1, as in paged_attention.
-    constexpr float kUp = F32 || I8 ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = F32 ? 8.0f : I8 ? 0.0f : PP == 1 ? 6.0f : 1.0f;
+    // kRise powers of two.  F16 pages: what f16's 2^15 leaves, values being below 2^16.  A value in F32 or I8 may lie anywhere in f32's
+    // range: probabilities up to 1, as in paged_attention.
+    constexpr bool WIDE = F32 || I8;
+    constexpr float kUp = WIDE ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = WIDE ? 0.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
     // keys and values of one tile each; two arrays, so that reads of one are known to be apart from what is on its way into the other
     __shared__ __attribute__((aligned(16))) char lds0[2 * BYTES];

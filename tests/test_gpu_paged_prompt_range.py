@@ -90,7 +90,7 @@ def test_large_and_small_8_bit_scales(cbx, which, d, g, up_k, up_v):
 
 
 @pytest.mark.parametrize("which", CALLS)
-@pytest.mark.parametrize("dt,cdt", [(F32, I8)])
+@pytest.mark.parametrize("dt,cdt", [(F32, F32), (F32, I8)])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_large_values_behind_a_rising_maximum(cbx, which, dt, cdt, d):
     """Values of 2^117 (in sum below 2^127 a row) whose scores are 7 powers of
