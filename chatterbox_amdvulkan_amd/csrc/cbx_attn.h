@@ -43,7 +43,7 @@ struct AttnArgs {
     const int32_t* own_first;
     const int32_t* groups;           // own_first holds for the requests [groups[0], groups[n_groups])
     uint32_t n_groups;
-    float own_up;                    // log2 of what the probabilities in o and l are multiplied by
+    float own_down;                  // 1 over what the probabilities in o and l are multiplied by
     float* own_o;
     float2* own_ml;
 };

@@ -906,8 +906,8 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
             }
             if (entire && a.own) {
                 const uint64_t own = static_cast<uint64_t>(s) * a.hq + hq0 + hh;
-                a.own_o[own * a.D + d] = oo;
-                if (d == 0) a.own_ml[own] = make_float2(mm - a.own_up, ll);
+                a.own_o[own * a.D + d] = oo * a.own_down;
+                if (d == 0) a.own_ml[own] = make_float2(mm, ll * a.own_down);
             } else if (entire) {
                 Elt<TQ>::store1(a.y + s * a.y_nb2 + (hq0 + hh) * a.y_nb1 + d * Elt<TQ>::size, ll == 0.0f ? 0.0f : oo / ll);
             } else {
@@ -990,11 +990,11 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     __syncthreads();
     l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
     const uint64_t own = static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh;
-    if (a.own && tid == 0) a.own_ml[own] = make_float2(m - a.own_up, l);
+    if (a.own && tid == 0) a.own_ml[own] = make_float2(m, l * a.own_down);
     char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
     for (uint32_t d = tid; d < a.D; d += kAttnThreads) {
         const float t = ((lds_o[0][d] + lds_o[1][d]) + lds_o[2][d]) + lds_o[3][d];
-        if (a.own) a.own_o[own * a.D + d] = t;
+        if (a.own) a.own_o[own * a.D + d] = t * a.own_down;
         else Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
     }
 }
@@ -1162,7 +1162,7 @@ bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, Device
     a.part_o = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ws) + p.o_bytes);
     a.split = reinterpret_cast<uint4*>(static_cast<char*>(ws) + p.o_bytes + p.ml_bytes);
-    a.own_up = c.k->type == CBX_TYPE_F16 ? 14.0f : 0.0f;         // Core's kUp
+    a.own_down = c.k->type == CBX_TYPE_F16 ? 1.0f / Core<uint16_t, 64>::kUp : 1.0f;
     const bool t16 = c.q->type == CBX_TYPE_F16, c16 = c.k->type == CBX_TYPE_F16, uni = uniform_pages(c.k);
     if (c.k->type == CBX_TYPE_I8) {
         a.s_quads = quad_scales(c.k_scale) && quad_scales(c.v_scale);

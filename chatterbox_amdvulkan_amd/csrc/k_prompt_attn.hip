@@ -872,6 +872,17 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     }
     l += __shfl_xor(l, 32);
     if (__any(wrong) && lane == 0) atomicOr(a.err, DEV_ERR_PAGE);
+    // Parts that are joined: o and l as sums of 2^(s mul - m mul), beside m mul rounded once, as paged_attention's are (the sums of a
+    // group's shared keys meet those).  mc, m mul - kUp rounded, would count a part of scores past 2^22 for another power of two.
+    const bool to_parts = pa.shared || piece.count > 1;
+    if (PAIR || to_parts) {
+        const bool none = m == kLowest;
+        const float down = none ? 1.0f : __builtin_amdgcn_exp2f(far ? -kUp : -fmaf(m, mul, -mc));
+        mc = none ? kLowest : m * mul;
+        l *= down;
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++) o[d] *= down;
+    }
     if constexpr (PAIR) {                                    // the two waves' parts added up, ND runs of 32 dims at a time
         constexpr int ND = 2 * BYTES / 8192 < DP / 32 ? 2 * BYTES / 8192 : DP / 32;
         float* part = reinterpret_cast<float*>(lds0) + row_wave * (ND * 16 * 64) + lane;
@@ -909,7 +920,6 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     if (wid != row_wave) return;
     const_args& late = *args_anew();
     const uint32_t lane1 = anew(lane), n1 = lane1 & 31, half1 = lane1 >> 5, r = row_wave * 32 + n1, D = late.a.D;
-    const bool to_parts = late.shared || piece.count > 1;
     const uint32_t slot = piece.first * late.a.hkv + hk;     // of the row tile's first piece
     const uint64_t part0 = static_cast<uint64_t>(slot + piece.at * late.a.hkv) * late.row_cap;
     if (r < rows) {

@@ -113,3 +113,54 @@ def test_large_values_behind_a_rising_maximum(cbx, which, dt, cdt, d):
     ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, scale)
     assert bool(torch.isfinite(y).all())
     assert_within(y, ref, bound)
+
+
+@pytest.mark.parametrize("which", CALLS)
+@pytest.mark.parametrize("dt,cdt", TYPES)
+@pytest.mark.parametrize("top", [2.0 ** 20, 1.37 * 2 ** 21, 1.83 * 2 ** 21, 1.11 * 2 ** 22, 2.0 ** 25, 1.37 * 2 ** 25, 1.01 * 2 ** 26,
+                                 1.71 * 2 ** 26, 1.99 * 2 ** 28])
+def test_equal_scores_of_millions(cbx, which, dt, cdt, top):
+    """Scores of `top` powers of two, of both signs.  All keys alike: every
+    score is rounded the same way, y is the mean of the row's values: n sums,
+    8 more roundings as of paged_attention, and of the parts that are joined
+    two exponentials, their products and a probability of two f16 parts (16
+    more); 16 bits of a value times its probability under an F16 query over 8
+    bits.  One key ahead of all others by a hundredth: y is its value."""
+    d, page = 64, 16
+    lens, start, tables, pages, groups = call_of(which, page)
+    n = start[-1] if start else len(lens)
+    kc, vc, ks, vs = make_cache(pages, 2, page, d, cdt, gen(7))
+    q = torch.zeros(n, 2, d, dtype=dt, device="cuda")
+    q[..., 3] = 1024.0
+    last = []                                                # request and keys of every row
+    for s, length in enumerate(lens):
+        new = start[s + 1] - start[s] if start else 1
+        last += [(s, length - (new - 1 - j)) for j in range(new)]
+    v = [(vc[tables[s, :-(-x // page)].long()].double()
+          * (1 if vs is None else vs[tables[s, :-(-x // page)].long()].double()[..., None])).transpose(0, 1).reshape(2, -1, d)
+         for s, x in enumerate(lens)]
+    more = (TWO_BF16 if dt == F16 and cdt == I8 else 0.0)
+    for sign in (1.0, -1.0):
+        high, low = (1000.0, 990.0) if sign > 0 else (990.0, 1000.0)
+        unit = 1.0
+        if cdt == I8:
+            high, low, unit = high / 10, low / 10, 10.0
+            ks = torch.full((pages, 2, page), unit, device="cuda")
+        scale = sign * top / (1024.0 * 1000.0) * float(np.log(2.0))
+        kc.zero_()
+        kc[..., 3] = high
+        y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale)
+        ref, size = (torch.stack([f(v[s][:, :x]).mean(1) for s, x in last]) for f in (lambda t: t, torch.abs))
+        ends = torch.tensor([x for _, x in last], device="cuda")[:, None, None]
+        assert_within(y, ref, ((ends + 24) * U32 + more) * size + half_step(dt) * ref.abs(), f"equal scores, sign {sign}")
+        kc[..., 3] = low
+        for s, x in enumerate(lens):
+            best = 0 if start and start[s + 1] - start[s] >= x else x // 2 if start else x - 1
+            kc[tables[s, best // page], :, best % page, 3] = high
+        # of requests with a beginning in common the others' own best keys lie behind it: one key of the highest score each
+        y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale)
+        best = [0 if start and start[s + 1] - start[s] >= lens[s] else lens[s] // 2 if start else lens[s] - 1 for s, _ in last]
+        keep = torch.tensor([b < x for b, (_, x) in zip(best, last)], device="cuda")
+        ref = torch.stack([v[s][:, min(b, x - 1)] for b, (s, x) in zip(best, last)])
+        bound = (8 * U32 + more + half_step(dt)) * ref.abs()
+        assert_within(y[keep], ref[keep], bound[keep], f"one score ahead, sign {sign}")
