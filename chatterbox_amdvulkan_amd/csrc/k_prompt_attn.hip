@@ -517,6 +517,14 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
             if (wid < 2 && lane < KT) lds_s[buf][wid][lane] = rs;
         } else {
             wait_vector_memory();                            // what this wave brings to LDS
+            if (a.D != DP) {                                 // an infinity past D would make NaN of the query's zeros
+                constexpr uint32_t R = KT / 4;               // rows that this wave brings
+                const uint32_t lane1 = anew(lane), row = wid * R + lane1 % R;
+#pragma unroll 1
+                for (uint32_t c = a.D / T::PER + lane1 / R; c < DP / T::PER; c += 64 / R) {
+                    *reinterpret_cast<u4v*>(to + row * PITCH + T::k_place(row, c) * 16) = anew(u4v{});
+                }
+            }
             if (edge) {
 #pragma unroll 1
                 for (int i = 0; i < NI; i++) {

@@ -62,9 +62,10 @@ def call_of(which, page=16):
     if CALLS[which]:
         lens, start, tables, pages = packed(*CALLS[which], page, 3)
         return lens, start, tables, pages, None
-    groups, own = [(0, 3, 192), (3, 5, 64)], [40, 1, 700, 33, 90]
+    one = -(-192 // page) * page
+    groups, own = [(0, 3, one), (3, 5, 4 * page)], [40, 1, 700, 33, 90]
     lens, tables, pages = shared_of(groups, own, page)
-    return lens, None, tables, pages, (ints([0, 3, 5]), ints([192, 64]))
+    return lens, None, tables, pages, (ints([0, 3, 5]), ints([one, 4 * page]))
 
 
 def attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale, **kw):
@@ -164,3 +165,23 @@ def test_equal_scores_of_millions(cbx, which, dt, cdt, top):
         ref = torch.stack([v[s][:, min(b, x - 1)] for b, (s, x) in zip(best, last)])
         bound = (8 * U32 + more + half_step(dt)) * ref.abs()
         assert_within(y[keep], ref[keep], bound[keep], f"one score ahead, sign {sign}")
+
+
+@pytest.mark.parametrize("dt,cdt", [(F16, F16), (F32, F32), (F16, F32)])
+@pytest.mark.parametrize("d", [32, 40, 64, 72, 80, 96, 112, 128, 160, 248, 256, 60])
+@pytest.mark.parametrize("which", ["long", "pairs", "whole", "shared"])
+@pytest.mark.parametrize("page", [16, 10])
+def test_infinite_keys_of_no_weight(cbx, dt, cdt, d, which, page):
+    """A key with an infinity whose score is -inf has no weight, whatever the head_dim: as one that is next to it in f16."""
+    lens, start, tables, pages, groups = call_of(which, page)
+    kc, vc, _, _ = make_cache(pages, 2, page, d, cdt, gen(4))
+    q = torch.randn(start[-1] if start else len(lens), 4, d, device="cuda", generator=gen(5)).to(dt)
+    for dim in (1, d - 1):
+        q[..., dim] = -1.0
+    outs = []
+    for far in (6e4, float("inf")):
+        k2 = kc.clone()
+        for s, key, dim in ((0, 3, 1), (0, 35, d - 1), (1, 20, 1)):
+            k2[tables[s, key // page], :, key % page, dim] = far
+        outs.append(attend(cbx, q, k2, vc, None, None, tables, lens, start, groups, 0.125))
+    assert bool(torch.isfinite(outs[0][2:]).all()) and torch.equal(*outs)
