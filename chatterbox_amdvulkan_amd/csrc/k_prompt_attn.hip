@@ -20,6 +20,8 @@
 // once out of LDS for 32 rows (64 rows a wave, one workgroup a CU: 616 TFLOP/s for
 // 736; 256 rows a workgroup: 570), and 128 rows a workgroup, so that two or three
 // fit a CU and one's products run beside another's softmax.
+#include <cmath>
+
 #include "cbx_attn.h"
 
 namespace cbx {
@@ -1148,6 +1150,12 @@ void launch_join(const PagedAttnCall& c, const PromptArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Numbers that k_prompt's products hold: caps times log2(e), and their share in the scale as a normal number.  The rest, which no model
+// has, is k_attn_rows', or paged_attention's.
+static bool tile_numbers(const PagedAttnCall& c) {
+    return c.softcap <= 0x1p60f && (c.softcap == 0.0f || c.scale == 0.0f || std::fabs(c.scale) / c.softcap >= 0x1p-126f);
+}
+
 size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {
     return prompt_plan(q, k, tables, tables->ne[1], false, st).bytes;
 }
@@ -1155,7 +1163,7 @@ size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cb
 int launch_paged_prompt(const PagedAttnCall& c, DeviceState* st, hipStream_t s) {
     const char* what = "cbx_paged_prompt_attention";
     const PromptPlan p = prompt_plan(c.q, c.k, c.tables, c.tables->ne[1], false, st);
-    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_attention_rows(attn_args(c, st), c, what, s);
+    if (!p.tiles || !tile_numbers(c) || !vector_rows(c.k) || !vector_rows(c.v)) return launch_attention_rows(attn_args(c, st), c, what, s);
     const PromptArgs a = prompt_args(c, p, static_cast<uint32_t>(c.tables->ne[1]), st);
     launch_tiles(c, p, a, s);
     if (p.deal) launch_join(c, a, s);
@@ -1202,7 +1210,7 @@ int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s) 
     const SharedPlan p = shared_plan(c.q, c.k, c.tables, c.start, st);
     PagedAttnCall own = c;
     own.start = own.shared = nullptr;
-    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return launch_paged_attention(own, st, s);
+    if (!p.tiles || !tile_numbers(c) || !vector_rows(c.k) || !vector_rows(c.v)) return launch_paged_attention(own, st, s);
     PromptArgs a = prompt_args(c, p.pre, static_cast<uint32_t>(c.start->ne[0] - 1), st);
     char* ws = static_cast<char*>(c.ws) + p.pre.bytes;
     float* own_o = reinterpret_cast<float*>(ws);

@@ -185,3 +185,19 @@ def test_infinite_keys_of_no_weight(cbx, dt, cdt, d, which, page):
             k2[tables[s, key // page], :, key % page, dim] = far
         outs.append(attend(cbx, q, k2, vc, None, None, tables, lens, start, groups, 0.125))
     assert bool(torch.isfinite(outs[0][2:]).all()) and torch.equal(*outs)
+
+
+@pytest.mark.parametrize("which", CALLS)
+@pytest.mark.parametrize("dt,cdt", TYPES)
+@pytest.mark.parametrize("cap", [2.0 ** 61, 2.0 ** 100, 3.3e38])
+def test_caps_next_to_the_largest(cbx, which, dt, cdt, cap):
+    """cap * tanh(s / cap) of a cap so far above the scores is s: the quotient
+    is held to 2^-150 or 2^-24 of itself (2^-150 times the cap: at most 4
+    U32), the tanh, products and the exponent's parts to 8 roundings of s."""
+    lens, start, tables, pages, groups = call_of(which)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, 64, cdt, gen(4))
+    q = torch.randn(start[-1] if start else len(lens), 4, 64, device="cuda", generator=gen(5)).to(dt)
+    y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, 0.125, softcap=cap)
+    top = 0.125 * 64 * float(q.abs().max()) * 6              # above every |s|
+    ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, 0.125, p_err=U32 * (8 * top + 4) + half_step(dt))
+    assert_within(y, ref, bound)
