@@ -609,7 +609,7 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
         cap_in = fminf(mul / kLog2e / a.softcap, 0x1p127f);  // finite: 0 stays 0
         mul = 1.0f;
     }
-    mul = fmaxf(mul, 0x1p-126f);                             // -inf, the score of a key that a row does not have, stays that
+    mul = fmaxf(mul, 0x1p-149f);                             // -inf, the score of a key that a row does not have, stays that
 
     f16v o[DP / 32];
     float m, mc, l;

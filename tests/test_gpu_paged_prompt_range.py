@@ -201,3 +201,21 @@ def test_caps_next_to_the_largest(cbx, which, dt, cdt, cap):
     top = 0.125 * 64 * float(q.abs().max()) * 6              # above every |s|
     ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, 0.125, p_err=U32 * (8 * top + 4) + half_step(dt))
     assert_within(y, ref, bound)
+
+
+@pytest.mark.parametrize("which", CALLS)
+@pytest.mark.parametrize("cdt", [F32, I8])
+@pytest.mark.parametrize("scale,up", [(0.0, 2.0 ** 62), (2.0 ** -140, 2.0 ** 62), (-(2.0 ** -130), 2.0 ** 62)])
+def test_scales_next_to_nothing(cbx, which, cdt, scale, up):
+    """Scales of 0 and below the smallest normal number, under products of up to 2^125."""
+    lens, start, tables, pages, groups = call_of(which)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, 64, cdt, gen(4))
+    if cdt == I8:
+        ks = ks * up
+    else:
+        kc = kc * up
+    q = torch.randn(start[-1] if start else len(lens), 2, 64, device="cuda", generator=gen(5)).clamp(-2, 2) * 2.0 ** 56
+    y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale)
+    # |q . k| < 2^126; the scale times log2(e) is off by at most 2^-149 of its own: 2^-23, 2 U32, of the exponent
+    ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, scale, p_err=4 * U32)
+    assert_within(y, ref, bound)
