@@ -26,6 +26,8 @@
 // a workgroup a request and query head, a key's elements over the lanes: 64
 // requests of 1 to 2048 keys, 16 heads of 60 703 us (of 64, by tiles, 50; of 64 off
 // their alignment 784).
+#include <cmath>
+
 #include "cbx_attn.h"
 
 namespace cbx {
@@ -1154,7 +1156,7 @@ bool attention_tiles(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor*
 
 bool launch_attention_tiles(AttnArgs a, const PagedAttnCall& c, void* ws, DeviceState* st, hipStream_t s) {
     const AttnPlan p = attn_plan(c.q, c.k, c.tables, st);
-    if (!p.tiles || !vector_rows(c.k) || !vector_rows(c.v)) return false;
+    if (!p.tiles || !std::isfinite(c.scale * kLog2e) || !vector_rows(c.k) || !vector_rows(c.v)) return false;
     a.gc = p.gc;
     a.ngr = p.ngr;
     a.H = p.H;

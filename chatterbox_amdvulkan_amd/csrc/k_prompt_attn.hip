@@ -1150,10 +1150,10 @@ void launch_join(const PagedAttnCall& c, const PromptArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Numbers that k_prompt's products hold: caps times log2(e), and their share in the scale as a normal number.  The rest, which no model
-// has, is k_attn_rows', or paged_attention's.
+// Numbers that k_prompt's products hold: scales and caps times log2(e), and a cap's share in the scale as a normal number.  The rest,
+// which no model has, is k_attn_rows', or paged_attention's.
 static bool tile_numbers(const PagedAttnCall& c) {
-    return c.softcap <= 0x1p60f && (c.softcap == 0.0f || c.scale == 0.0f || std::fabs(c.scale) / c.softcap >= 0x1p-126f);
+    return std::isfinite(c.scale * kLog2e) && c.softcap <= 0x1p60f && (c.softcap == 0.0f || c.scale == 0.0f || std::fabs(c.scale) / c.softcap >= 0x1p-126f);
 }
 
 size_t paged_prompt_workspace(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* tables, const DeviceState* st) {

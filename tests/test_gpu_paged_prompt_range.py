@@ -219,3 +219,34 @@ def test_scales_next_to_nothing(cbx, which, cdt, scale, up):
     # |q . k| < 2^126; the scale times log2(e) is off by at most 2^-149 of its own: 2^-23, 2 U32, of the exponent
     ref, bound = rows_ref(q, kc, vc, ks, vs, tables, lens, start, scale, p_err=4 * U32)
     assert_within(y, ref, bound)
+
+
+@pytest.mark.parametrize("which", list(CALLS) + ["one"])
+@pytest.mark.parametrize("dt,cdt", TYPES)
+@pytest.mark.parametrize("scale", [3e38, -2.5e38])
+def test_scales_next_to_the_largest(cbx, which, dt, cdt, scale):
+    """Scales that log2(e) would take past f32: the query's elements times the
+    scale lie below 2^126, and so do the scores."""
+    lens, start, tables, pages, groups = call_of("shared" if which == "one" else which)
+    kc, vc, ks, vs = make_cache(pages, 2, 16, 64, cdt, gen(4))
+    # q 2^-14 to 2^-10; of the keys, 2^-24 to 2^-20 in F16, one element is not 0: scores of 2^90 and more are 0 or far apart
+    q = torch.zeros(start[-1] if start else len(lens), 2, 64, dtype=dt, device="cuda")
+    q[..., 5] = 2.0 ** -12
+    kc.zero_()
+    best = []
+    for s, x in enumerate(lens):
+        first = x - (start[s + 1] - start[s]) if start else x - 1
+        best.append(first if start else x - 1)
+        kc[tables[s, best[s] // 16], :, best[s] % 16, 5] = (1 if cdt == I8 else 2.0 ** -20) * (1 if scale > 0 else -1)
+    if cdt == I8:
+        ks = torch.full_like(ks, 2.0 ** -20)
+    if which == "one":
+        y = cbx.paged_attention(q, kc, vc, tables, ints(lens), scale, k_scale=ks, v_scale=vs)
+    else:
+        y = attend(cbx, q, kc, vc, ks, vs, tables, lens, start, groups, scale)
+    of = [s for s in range(len(lens)) for _ in range(start[s + 1] - start[s] if start else 1)]
+    page = [tables[s, best[s] // 16].long() for s in of]
+    ref = torch.stack([vc[p, :, best[s] % 16].double() * (1 if vs is None else vs[p, :, best[s] % 16].double()[:, None])
+                       for p, s in zip(page, of)])
+    more = TWO_BF16 if dt == F16 and cdt == I8 else 0.0
+    assert_within(y, ref, (8 * U32 + more + half_step(dt)) * ref.abs())
