@@ -22,7 +22,6 @@ struct AttnArgs {
     uint32_t n_seq, hq, hkv, g, D, page, max_pages, n_pages;
     int32_t window;
     float scale, softcap;
-    uint32_t own;                    // own_first holds
     uint32_t* err;
     // k_attn_tiles and k_attn_join
     uint32_t page_mul, page_shift;   // key / page = (key * page_mul) >> page_shift for key < 2^31
@@ -38,7 +37,7 @@ struct AttnArgs {
     bool s_quads;                    // they can be read four at a time
     const int32_t* start;            // packed tokens or groups, see PagedAttnCall; null: a row of q a request
     uint32_t n_rows;                 // of q: tokens or requests
-    // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt): own_first says where a
+    // the keys behind the shared ones of a group (k_attn_tiles and k_attn_join after k_prompt; else null): own_first says where a
     // request's begin, and (o, m, l) go to own_o and own_ml at request * hq + head instead of y
     const int32_t* own_first;
     const int32_t* groups;           // own_first holds for the requests [groups[0], groups[n_groups])

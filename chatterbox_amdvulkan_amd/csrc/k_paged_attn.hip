@@ -207,7 +207,7 @@ struct Span {
     uint32_t first, len, tile0, tiles;
     bool wrong;
 };
-template <int KT>
+template <int KT, bool OWN>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     const uint32_t cap = a.max_pages * a.page;
     const int32_t n = a.lens[s];
@@ -215,7 +215,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     r.wrong = n < 0 || static_cast<uint32_t>(n) > cap;
     r.len = n < 0 ? 0 : min(static_cast<uint32_t>(n), cap);
     r.first = a.window > 0 && r.len > static_cast<uint32_t>(a.window) ? r.len - a.window : 0;
-    if (a.own && static_cast<int32_t>(s) >= a.groups[0] && static_cast<int32_t>(s) < a.groups[a.n_groups]) {
+    if (OWN && static_cast<int32_t>(s) >= a.groups[0] && static_cast<int32_t>(s) < a.groups[a.n_groups]) {
         r.first = max(r.first, min(static_cast<uint32_t>(max(a.own_first[s], 0)), r.len));
     }
     r.tile0 = r.first / KT;
@@ -239,11 +239,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // The exclusive prefix over the requests of their tiles, as every workgroup
 // needs it: each thread sums c neighbouring requests.  *total the sum.
-template <int KT>
+template <int KT, bool OWN>
 __device__ __forceinline__ uint32_t tiles_before(const AttnArgs& a, uint32_t c, uint32_t* lds, uint32_t* mine, uint32_t* total) {
     const uint32_t tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
     uint32_t sum = 0;
-    for (uint32_t s = tid * c; s < min(a.n_seq, (tid + 1) * c); s++) sum += span_of<KT>(a, s).tiles;
+    for (uint32_t s = tid * c; s < min(a.n_seq, (tid + 1) * c); s++) sum += span_of<KT, OWN>(a, s).tiles;
     const uint32_t x = wave_scan(sum);
     if (lane == 63) lds[wid] = x;
     __syncthreads();
@@ -623,8 +623,11 @@ template <int DP> struct Core<float, DP> {
 constexpr int per_cu(int dp, bool uni) { return dp <= 64 ? (uni ? 4 : 3) : dp <= 96 ? (uni ? 3 : 2) : dp <= 128 ? 2 : 1; }
 
 // UNI: a page holds whole runs of 16 keys, looked up once a wave and half;
-// else every lane looks its key up and passes the page on.
-template <typename TQ, typename TC, int DP, bool UNI>
+// else every lane looks its key up and passes the page on.  OWN: the keys
+// behind a group's shared ones, as parts (a form of its own: asked for at run
+// time, it cost every other call 0.15 us and 23 requests of up to 7001 F32 keys
+// 39.2 us for 38.4).
+template <typename TQ, typename TC, int DP, bool UNI, bool OWN>
 __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(AttnArgs a) {
     using C = Core<TC, DP>;
     constexpr int NK = C::NK, NH = C::NH, NE = C::NE, W4 = kAttnThreads / 64, KT = NK * W4;
@@ -641,13 +644,13 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
     if (a.W == 0) {
         s = blockIdx.x / a.H;
         base = 0;
-        const uint32_t tiles = span_of<KT>(a, s).tiles;
+        const uint32_t tiles = span_of<KT, OWN>(a, s).tiles;
         at = (blockIdx.x - s * a.H) * tiles;
         end = at + tiles;
     } else {
         const uint32_t c = (a.n_seq + kAttnThreads - 1) / kAttnThreads;
         uint32_t mine, total;
-        uint32_t before = tiles_before<KT>(a, c, lds_scan, &mine, &total);
+        uint32_t before = tiles_before<KT, OWN>(a, c, lds_scan, &mine, &total);
         T = total * a.H;
         W = min(a.W, T);                                 // runs, each of a tile at least
         if (blockIdx.x >= W) {
@@ -660,7 +663,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
         if (before * a.H <= at && at < (before + mine) * a.H) {
             uint32_t i = tid * c;
             for (;; i++) {
-                const uint32_t t = span_of<KT>(a, i).tiles;
+                const uint32_t t = span_of<KT, OWN>(a, i).tiles;
                 if (at < (before + t) * a.H) break;
                 before += t;
             }
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
     C core;
     core.offsets(n, grp, a.D);
     while (at < end) {
-        const Span sp = span_of<KT>(a, s);
+        const Span sp = span_of<KT, OWN>(a, s);
         wrong |= sp.wrong;
         const uint32_t h = (at - base) / sp.tiles, t0 = at - base - h * sp.tiles;
         const uint32_t n_tiles = min(end - at, sp.tiles - t0);
@@ -906,7 +909,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
                 ll = fmaf(lds_l[w][hh], f, ll);
                 oo = fmaf(lds_o[(w * a.gc + hh) * ld + d], f, oo);
             }
-            if (entire && a.own) {
+            if (entire && OWN) {
                 const uint64_t own = static_cast<uint64_t>(s) * a.hq + hq0 + hh;
                 a.own_o[own * a.D + d] = oo * a.own_down;
                 if (d == 0) a.own_ml[own] = make_float2(mm, ll * a.own_down);
@@ -933,7 +936,7 @@ __global__ __launch_bounds__(kAttnThreads, per_cu(DP, UNI)) void k_attn_tiles(At
 // Part 0 lies in its run's second place (the run ends with it), the others in
 // the first.  A wave adds every fourth part, a part's dims over its lanes, 8
 // parts in flight (of the first 32 already while their maxima are read).
-template <typename TQ, int DP>
+template <typename TQ, int DP, bool OWN>
 __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     constexpr int N = DP / 64, U = 8;
     __shared__ float lds_m[kAttnThreads / 64], lds_l[kAttnThreads / 64], lds_f[kAttnThreads];
@@ -992,11 +995,11 @@ __global__ __launch_bounds__(kAttnThreads) void k_attn_join(AttnArgs a) {
     __syncthreads();
     l = ((lds_l[0] + lds_l[1]) + lds_l[2]) + lds_l[3];
     const uint64_t own = static_cast<uint64_t>(sp.x) * a.hq + sp.y + hh;
-    if (a.own && tid == 0) a.own_ml[own] = make_float2(m, l * a.own_down);
+    if (OWN && tid == 0) a.own_ml[own] = make_float2(m, l * a.own_down);
     char* yr = a.y + sp.x * a.y_nb2 + (sp.y + hh) * a.y_nb1;
     for (uint32_t d = tid; d < a.D; d += kAttnThreads) {
         const float t = ((lds_o[0][d] + lds_o[1][d]) + lds_o[2][d]) + lds_o[3][d];
-        if (a.own) a.own_o[own * a.D + d] = t * a.own_down;
+        if (OWN) a.own_o[own * a.D + d] = t * a.own_down;
         else Elt<TQ>::store1(yr + d * Elt<TQ>::size, l == 0.0f ? 0.0f : t / l);
     }
 }
@@ -1049,28 +1052,33 @@ AttnPlan attn_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tensor* t
     return p;
 }
 
-template <typename TQ, typename TC, int DP>
+template <typename TQ, typename TC, int DP, bool OWN>
 void tiles_uni(bool uni, dim3 grid, size_t lds, hipStream_t s, const AttnArgs& a) {
-    if (uni) hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, true>), grid, dim3(kAttnThreads), lds, s, a);
-    else hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, false>), grid, dim3(kAttnThreads), lds, s, a);
+    if (uni) hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, true, OWN>), grid, dim3(kAttnThreads), lds, s, a);
+    else hipLaunchKernelGGL((k_attn_tiles<TQ, TC, DP, false, OWN>), grid, dim3(kAttnThreads), lds, s, a);
 }
 
-template <typename TQ, typename TC>
+template <typename TQ, typename TC, bool OWN>
 void launch_tiles(const AttnPlan& p, bool uni, AttnArgs& a, hipStream_t s) {
     if (!p.join) a.W = 0;
     const dim3 grid(p.join ? p.W : a.n_seq * a.H);
     const size_t lds = static_cast<size_t>(kAttnThreads / 64) * p.gc * (p.dp + 4) * sizeof(float);
-    if (p.dp == 64) tiles_uni<TQ, TC, 64>(uni, grid, lds, s, a);
+    if (p.dp == 64) tiles_uni<TQ, TC, 64, OWN>(uni, grid, lds, s, a);
     else if (p.dp == 96) {
-        if constexpr (sizeof(TC) > 1) tiles_uni<TQ, TC, 96>(uni, grid, lds, s, a);
+        if constexpr (sizeof(TC) > 1) tiles_uni<TQ, TC, 96, OWN>(uni, grid, lds, s, a);
     }
-    else if (p.dp == 128) tiles_uni<TQ, TC, 128>(uni, grid, lds, s, a);
-    else tiles_uni<TQ, TC, 256>(uni, grid, lds, s, a);
+    else if (p.dp == 128) tiles_uni<TQ, TC, 128, OWN>(uni, grid, lds, s, a);
+    else tiles_uni<TQ, TC, 256, OWN>(uni, grid, lds, s, a);
     if (!p.join) return;
     const dim3 parts(p.W * p.gc);
-    if (p.dp == 64) hipLaunchKernelGGL((k_attn_join<TQ, 64>), parts, dim3(kAttnThreads), 0, s, a);
-    else if (p.dp <= 128) hipLaunchKernelGGL((k_attn_join<TQ, 128>), parts, dim3(kAttnThreads), 0, s, a);
-    else hipLaunchKernelGGL((k_attn_join<TQ, 256>), parts, dim3(kAttnThreads), 0, s, a);
+    if (p.dp == 64) hipLaunchKernelGGL((k_attn_join<TQ, 64, OWN>), parts, dim3(kAttnThreads), 0, s, a);
+    else if (p.dp <= 128) hipLaunchKernelGGL((k_attn_join<TQ, 128, OWN>), parts, dim3(kAttnThreads), 0, s, a);
+    else hipLaunchKernelGGL((k_attn_join<TQ, 256, OWN>), parts, dim3(kAttnThreads), 0, s, a);
+}
+
+template <typename TQ, typename TC> void launch_tiles(const AttnPlan& p, bool uni, AttnArgs& a, hipStream_t s) {
+    if (a.own_first) launch_tiles<TQ, TC, true>(p, uni, a, s);
+    else launch_tiles<TQ, TC, false>(p, uni, a, s);
 }
 
 }  // namespace

@@ -1221,7 +1221,6 @@ int launch_paged_shared(const PagedAttnCall& c, DeviceState* st, hipStream_t s) 
     a.own_first = reinterpret_cast<int32_t*>(ws + p.o_bytes + p.ml_bytes);
     launch_tiles(c, p.pre, a, s);
     AttnArgs b = attn_args(own, st);
-    b.own = 1;
     b.own_first = a.own_first;
     b.groups = a.a.start;
     b.n_groups = a.n_start;
