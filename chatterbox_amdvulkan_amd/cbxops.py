@@ -1035,7 +1035,7 @@ def paged_shared_attention(q, k_cache, v_cache, block_tables, seq_lens, group_st
     """paged_attention for requests that begin with the same keys, which are
     read once a group: the requests [group_start[p], group_start[p + 1]) have
     their first shared_lens[p] keys in the same pages (their tables begin
-    alike).  group_start int32 [n_groups + 1], shared_lens int32 [n_groups];
+    alike, also those of requests that are shorter or sit out).  group_start int32 [n_groups + 1], shared_lens int32 [n_groups];
     ws of paged_shared_attention_workspace bytes."""
     return _call("paged_shared_attention", q, k_cache, v_cache, block_tables, seq_lens, group_start, shared_lens, scale, softcap,
                  window, out, ws, k_scale, v_scale)

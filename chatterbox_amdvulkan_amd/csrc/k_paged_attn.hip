@@ -433,12 +433,13 @@ template <int DP> struct Core<uint16_t, DP> {
 // f16 products as above, times the keys' scales in f32.  A probability times its
 // value's scale may lie anywhere in f32's range, so it is split into bf16 parts
 // for products of bf16: three under an F32 query (all 24 bits), two under an F16
-// one (held to 2^-16).  A lane reads 16 dims of a key at once: MFMA c takes dims
+// one (its upper 16 bits: up to 2^-15 of it are cut off, a sixteenth of what the
+// F16 result is rounded by).  A lane reads 16 dims of a key at once: MFMA c takes dims
 // 64 (c / 2) + 16 (lane / 16) + 8 (c % 2) + [0, 8).  Half the bytes of F16 pages;
 // 8 requests of 1500 to 65000 keys, 32 heads of 128 on 8: 108 us (561 MB, 5.2
 // TB/s), of which the bytes take 104.  Short requests are bound by the widening,
 // 320 instructions for 32 keys of a head: 64 of 1 to 2048 keys, 16 heads of 64
-// under an F32 query, 42 us (143 MB, 3.4 TB/s).
+// under an F32 query, 43.5 us (143 MB, 3.3 TB/s).
 template <int DP> struct Core<int8_t, DP> {
     static constexpr bool SCALED = true;
     static constexpr int NK = 32, NH = 2, NE = 8;

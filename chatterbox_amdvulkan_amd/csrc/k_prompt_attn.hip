@@ -14,7 +14,7 @@
 // of 128 on 8, F16, 2.27 ms (920 TFLOP/s of the 1156 that a large product
 // reaches; without the softmax 1010, without the copies into LDS 1050); 48
 // requests of 1 to 2047 tokens, 16 heads of 64, 0.39 ms (593); 8 requests of 1 to
-// 9 tokens on 900 to 32000 keys in 8 bits, 99 us (2.8 TB/s, latency).
+// 9 tokens on 900 to 32000 keys in 8 bits, 101 us (2.8 TB/s, latency).
 //
 // 32 rows a wave, because a wave's 32 x 32 products then need each key and value
 // once out of LDS for 32 rows (64 rows a wave, one workgroup a CU: 616 TFLOP/s for
@@ -281,7 +281,8 @@ __global__ __launch_bounds__(256, waves_per_simd(DP, sizeof(TC) == 4)) void k_pr
     constexpr int NS = PAIR || KT == 32 || Q2 || DP == 64 ? 1 : 2;   // runs of 32 keys taken together
     // Probabilities are held times 2^kUp, and up to 2^(kUp + kRise), since the sums are rescaled only when a row's maximum has risen by
     // kRise powers of two.  F16 pages: what f16's 2^15 leaves, values being below 2^16.  A value in F32 or I8 may lie anywhere in f32's
-    // range: probabilities up to 1, as in paged_attention.
+    // range: probabilities up to 1, as in paged_attention.  Rescaling at every rise costs 1 to 6 % (F32, at 8 powers of two: 5 requests of
+    // 300 to 1301 tokens, heads of 80, 356 us for 363, 1522 tokens, heads of 256, 755 for 801; I8, at one, drafts 99.6 for 100.8).
     constexpr bool WIDE = F32 || I8;
     constexpr float kUp = WIDE ? 0.0f : PP == 1 ? 9.0f : 14.0f, kRise = WIDE ? 0.0f : PP == 1 ? 6.0f : 1.0f;
     const AttnArgs& a = pa.a;
@@ -1083,8 +1084,9 @@ PromptPlan prompt_plan(const cbx_tensor* q, const cbx_tensor* k, const cbx_tenso
     const int64_t key_tiles = cdiv(cap, k->type == CBX_TYPE_F32 || p.dp > 128 ? 32 : 64);
     if (most > kDealTiles || n_start > kDealTiles || most * key_tiles >= (int64_t{1} << 32) ||
         (!shared && (most * hkv > wide || cap < 512))) return p;
-    // A piece for every workgroup that fits at once (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5 times as many 217,
-    // half 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows: 105 us for 120).
+    // Two pieces a CU, as many as fit it at once at head_dim 65 to 128 (documents of 5000 to 30000 keys, 96 rows a head: 193 us; 1.5
+    // times as many 217, half 234); of pairs twice as many, which evens out the last pieces (8 requests of up to 32000 keys, 36 rows:
+    // 105 us for 120).
     const int64_t aim = p.pair ? 2 * wide : wide;
     p.deal = static_cast<uint32_t>(aim);
     p.grid = static_cast<uint32_t>(std::min(aim / hkv + most, most * cdiv(key_tiles, kLeast)) * hkv);
@@ -1137,7 +1139,9 @@ void launch_tiles(const PagedAttnCall& c, const PromptPlan& p, const PromptArgs&
     else if (!t16) launch_dp<float, uint16_t, 2>(p, s, a);
     // F16 throughout: a probability rounded to one f16 (2^-11 of itself at most) makes the result's error 1.3 times that of its own
     // rounding, in two parts nothing; two cost half as many products again and more conversions.  In a call of many rows these are its
-    // time (16000 tokens: 3.15 ms for 2.28; 48 requests, 25 thousand tokens: 515 us for 391), in one of few the pages' bytes are.
+    // time (16000 tokens: 3.15 ms for 2.28; 48 requests, 25 thousand tokens: 515 us for 391; 4096 rows, of 256 tokens of 16 heads of 64:
+    // 14.3 for 12.1, behind 2000 others 30.4 for 27.8, of 16 x 8 drafts of 32 heads on 8 64.0 for 61.5), in one of few the pages' bytes
+    // and latency are, and it keeps its precision.
     else if (c.shared || c.q->ne[1] * c.q->ne[2] < 4096) launch_dp<uint16_t, uint16_t, 2>(p, s, a);
     else launch_dp<uint16_t, uint16_t, 1>(p, s, a);
 }

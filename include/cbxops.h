@@ -667,8 +667,9 @@ int cbx_qk_norm_rope_store_q8(const cbx_tensor* q, const cbx_tensor* gq,
  * n_head_kv, query head h reads key head h / (n_head / n_head_kv).  A request
  * without keys gets zeros; keys past its length are never looked at, whatever
  * the page holds there; an infinity among those looked at may give NaN.
- * q . k_i, s_i and the elements of scale * q lie below 2^126 in size (past it
- * they may count as infinite).  head_dim <= 512, n_head * n_seq < 2^24.
+ * q . k_i, s_i, the elements of scale * q and, of each dim, the sum of |v_i|
+ * over the keys lie below 2^126 in size (past it they may count as infinite).
+ * head_dim <= 512, n_head * n_seq < 2^24.
  * Scores and sums are held in f32, also between the parts that a long request
  * is split into; where the parts begin depends on all of the call's lengths.
  * Over F16 caches the elements of an F32 query and the probabilities are
@@ -689,8 +690,10 @@ int cbx_paged_attention(const cbx_tensor* q, const cbx_tensor* k_cache,
                         float softcap, int32_t window, cbx_tensor* y,
                         void* ws, size_t ws_bytes, cbx_stream stream);
 /* ... over an 8-bit cache: k_i and v_i are scale * element.  The scales
- * multiply the products' sums and the probabilities in f32.  Workspace as
- * above, of the I8 k_cache.                                                */
+ * multiply the products' sums and the probabilities in f32; of a probability
+ * times its value's scale an F16 query's call takes the upper 16 bits (up to
+ * 2^-15 of it are cut off), an F32 query's all.  Workspace as above, of the
+ * I8 k_cache.                                                              */
 int cbx_paged_attention_q8(const cbx_tensor* q, const cbx_tensor* k_cache,
                            const cbx_tensor* k_scale,
                            const cbx_tensor* v_cache,
@@ -717,10 +720,10 @@ int cbx_paged_attention_q8(const cbx_tensor* q, const cbx_tensor* k_cache,
  * reaches its row, infinities and NaN included.  k_scale, v_scale: of an I8
  * cache, NULL for F32 and F16.  The rest as for cbx_paged_attention, with
  * n_head * n_tok < 2^24 and one choice more: where the matrix cores are the
- * bound (an F16 query in a call of many rows), probabilities are rounded to F16
- * for their products, by up to 2^-11 of themselves (small ones by 2^-34 of
- * their row's largest), and the sums they are divided by are sums of the
- * rounded ones.                                                            */
+ * bound (an F16 query over F16 pages, n_head * n_tok of 4096 or more),
+ * probabilities are rounded to F16 for their products, by up to 2^-11 of
+ * themselves (small ones by 2^-34 of their row's largest), and the sums they
+ * are divided by are sums of the rounded ones.                             */
 int cbx_paged_prompt_attention_workspace(const cbx_tensor* q,
                                          const cbx_tensor* k_cache,
                                          const cbx_tensor* block_tables,
@@ -743,7 +746,8 @@ int cbx_paged_prompt_attention(const cbx_tensor* q,
  *                [group_start[p], group_start[p + 1]), never falling; requests
  *                outside share nothing
  *   shared_lens  I32 (n_groups): so many keys at the beginning of the group's
- *                requests lie in the same pages, by each one's table
+ *                requests lie in the same pages, by each one's table: also a
+ *                request that sits out or is shorter still names these pages
  * block_tables and seq_lens are as cbx_paged_attention's, the shared keys
  * among them (a request may be shorter than its group's shared keys), and so
  * are the results, up to the rounding of sums that are split elsewhere.    */
